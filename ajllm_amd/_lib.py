@@ -270,7 +270,53 @@ DENSE_SIGNATURES: dict[str, tuple] = {
     "ajqd_scan_step": (c_int, [ctypes.POINTER(ScanStepArgs), _P]),
 }
 
+SERVE_LIBRARY_PATH = LIBRARY_PATH.with_name("libajq_serve.so")
+
+AJQS_F32 = 0
+AJQS_BF16 = 1
+
+
+class NormRopeArgs(ctypes.Structure):
+    """``ajqs_norm_rope_args``"""
+
+    _fields_ = ([(n, c_void_p) for n in ("qkv", "cosine", "sine", "q_gain", "k_gain", "rows", "positions", "counts", "offset", "keys",
+                                         "values", "q")]
+                + [(n, c_int64) for n in ("ld", "cache_batch", "cache_head")]
+                + [(n, c_int) for n in ("batch", "tokens", "heads", "kv_heads", "dim", "max_len", "table_rows", "in_dtype", "q_dtype",
+                                        "cache_dtype")]
+                + [("eps", c_float)])
+
+
+class SharedAttentionArgs(ctypes.Structure):
+    """``ajqs_shared_attention_args``"""
+
+    _fields_ = ([(n, c_void_p) for n in ("q", "prefix_keys", "prefix_values", "keys", "values", "prefix_lengths", "rows", "counts",
+                                         "offset", "out")]
+                + [(n, c_int64) for n in ("prefix_group", "prefix_head", "cache_batch", "cache_head")]
+                + [(n, c_int) for n in ("groups", "batch", "tokens", "heads", "kv_heads", "dim", "prefix_cap", "max_len", "q_dtype",
+                                        "cache_dtype")])
+
+
+class AdjustLogitsArgs(ctypes.Structure):
+    """``ajqs_adjust_logits_args``"""
+
+    _fields_ = ([(n, c_void_p) for n in ("logits", "out", "tokens", "token_counts", "prompt", "prompt_counts", "repetition", "frequency",
+                                         "presence", "bias_ids", "bias", "allowed", "allowed_rows")]
+                + [(n, c_int64) for n in ("ld", "out_ld", "tokens_ld", "prompt_ld", "bias_ld", "allowed_ld")]
+                + [(n, c_int) for n in ("batch", "vocab", "max_tokens", "max_prompt", "biases", "masks", "token_count_stride",
+                                        "prompt_count_stride", "dtype")])
+
+
+SERVE_SIGNATURES: dict[str, tuple] = {
+    "ajqs_last_error": (c_char_p, []),
+    "ajqs_norm_rope": (c_int, [ctypes.POINTER(NormRopeArgs), _P]),
+    "ajqs_shared_attention_workspace": (c_size_t, [ctypes.POINTER(SharedAttentionArgs)]),
+    "ajqs_shared_attention": (c_int, [ctypes.POINTER(SharedAttentionArgs), _P, c_size_t, _P]),
+    "ajqs_adjust_logits": (c_int, [ctypes.POINTER(AdjustLogitsArgs), _P]),
+}
+
 _lib: ctypes.CDLL | None = None
+_serve_lib: ctypes.CDLL | None = None
 _dense_lib: ctypes.CDLL | None = None
 _bench_lib: ctypes.CDLL | None = None
 _native = None
@@ -346,6 +392,31 @@ def load_dense() -> ctypes.CDLL:
         fn.argtypes = argtypes
     _dense_lib = lib
     return lib
+
+
+def load_serve() -> ctypes.CDLL:
+    """The operators of decoding many continuations of one prompt, bound on first use (built by ``python -m ajllm_amd.build``)."""
+    global _serve_lib
+    if _serve_lib is not None:
+        return _serve_lib
+    if not SERVE_LIBRARY_PATH.exists():
+        raise RuntimeError(f"{SERVE_LIBRARY_PATH} is missing: build it with `python -m ajllm_amd.build` "
+                           "(these operators have no fallback path)")
+    lib = ctypes.CDLL(str(SERVE_LIBRARY_PATH))
+    for name, (restype, argtypes) in SERVE_SIGNATURES.items():
+        fn = getattr(lib, name)
+        fn.restype = restype
+        fn.argtypes = argtypes
+    _serve_lib = lib
+    return lib
+
+
+def check_serve(status: int, what: str) -> None:
+    """``check`` for a status of libajq_serve.so."""
+    if status == 0:
+        return
+    message = f"{what}: {load_serve().ajqs_last_error().decode()}"
+    raise ValueError(message) if status in _ARGUMENT_ERRORS else RuntimeError(message)
 
 
 def check_dense(status: int, what: str) -> None:

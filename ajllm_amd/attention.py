@@ -1,6 +1,7 @@
-"""Host side of the library's causal prefill attention (``ajq_attn_prefill``).
+"""Host side of the library's causal prefill attention (``ajq_attn_prefill``), and of attention for sequences that share a prefix
+(``norm_rope``, ``shared_prefix_attention``).
 
-Stands where the reference switches to its FlashAttention under ``use_flash_attention``
+The first stands where the reference switches to its FlashAttention under ``use_flash_attention``
 (src/ajllm/modeling/attention.py:106-117; its own kernels, flash_attention.py:44-108,194-298, need
 CUDA/Triton).  Same contract as there: the arithmetic is flash attention's (bf16 products, fp32
 online softmax), not bit-for-bit the eager fp32 one, so it is opt-in.
@@ -8,6 +9,7 @@ online softmax), not bit-for-bit the eager fp32 one, so it is opt-in.
 
 from __future__ import annotations
 
+import ctypes
 from contextlib import nullcontext
 
 import torch
@@ -64,3 +66,120 @@ def prefill_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor,
                                            hd, out.data_ptr(), out_flag, room.data_ptr(), size, stream)
     return lib.ajq_attn_prefill(q.data_ptr(), keys.data_ptr(), values.data_ptr(), flag, batch, heads, kv_heads, seq, start, max_len, hd,
                                 out.data_ptr(), out_flag, stream)
+
+
+_TYPES = {torch.float32: _lib.AJQS_F32, torch.bfloat16: _lib.AJQS_BF16}
+
+
+def _on(device: torch.device):
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _pointer(t: torch.Tensor | None) -> int | None:
+    return None if t is None else t.data_ptr()
+
+
+def _check_caches(what: str, keys: torch.Tensor, values: torch.Tensor, device: torch.device) -> None:
+    if keys.dim() != 4 or keys.shape != values.shape or keys.stride() != values.stride() or keys.shape[3] not in (128, 64, 32):
+        raise ValueError(f"{what}: caches [.., Hkv, rows, hd] of one shape and layout with hd 128, 64 or 32 expected")
+    if keys.stride(3) != 1 or keys.stride(2) != keys.shape[3]:
+        raise ValueError(f"{what}: the rows of a cache head must lie one behind the other")
+    if keys.dtype not in _TYPES or values.dtype != keys.dtype:
+        raise ValueError(f"{what}: the caches must be float32 or bfloat16")
+    if keys.device != device or values.device != device:
+        raise ValueError(f"{what}: all tensors must be on one device")
+
+
+def _whole_numbers(what: str, name: str, t: torch.Tensor | None, count: int, device: torch.device) -> None:
+    if t is not None and (t.dtype != torch.int64 or t.numel() != count or not t.is_contiguous() or t.device != device):
+        raise ValueError(f"{what}: {name} must be {count} contiguous int64 on the device of the others")
+
+
+def _floats(what: str, name: str, t: torch.Tensor | None, shape: tuple, device: torch.device) -> None:
+    if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != shape or not t.is_contiguous() or t.device != device):
+        raise ValueError(f"{what}: {name} must be contiguous float32 {list(shape)} on the device of the others")
+
+
+def norm_rope(qkv: torch.Tensor, cosine: torch.Tensor, sine: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, rows: torch.Tensor, *,
+              heads: int, tokens: int = 1, q_gain: torch.Tensor | None = None, k_gain: torch.Tensor | None = None, epsilon: float = 1e-5,
+              positions: torch.Tensor | None = None, counts: torch.Tensor | None = None, offset: torch.Tensor | None = None,
+              out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """Queries and keys of a projection's output, each head RMS-normed (``q_gain``, ``k_gain`` fp32 ``[hd]``; None: as it is) and rotated,
+    keys and values written into the caches, in one launch: for sequences at positions of their own.
+
+    ``qkv`` fp32 or bf16 ``[B * tokens, (heads + 2 Hkv) * hd]`` (query heads, key heads, value heads; rows may be further apart); ``cosine`` /
+    ``sine`` fp32 ``[positions, hd / 2]``; ``keys`` / ``values`` ``[B, Hkv, max_len, hd]`` fp32 or bf16.  Token t of sequence b goes to row
+    ``rows[b] + offset + t`` of its caches and turns by position ``positions[b] + offset + t`` (``positions`` None: the row); ``rows``,
+    ``positions`` and ``counts`` int64 ``[B]``, ``offset`` one int64, all on the device.  Of the tokens of sequence b the first
+    ``counts[b]`` are there (None: all); the others write no row, and zeros for queries.  A row outside the caches is not written, a
+    position is held inside the tables.  Returns the queries ``[B, heads, tokens, hd]`` in ``out_dtype``
+    (RMSNorm.forward, src/ajllm/modeling/layers.py:70-74, on every head, then attention.py:36-60)."""
+    what = "norm_rope"
+    if not qkv.is_cuda:
+        raise ValueError("norm_rope needs tensors on a ROCm device (there is no CPU path)")
+    device = qkv.device
+    _check_caches(what, keys, values, device)
+    batch, kv_heads, max_len, hd = keys.shape
+    if qkv.dim() != 2 or tokens < 1 or qkv.shape[0] != batch * tokens or qkv.shape[1] != (heads + 2 * kv_heads) * hd or qkv.stride(1) != 1:
+        raise ValueError("norm_rope: qkv [B * tokens, (heads + 2 Hkv) * hd] expected")
+    if qkv.dtype not in _TYPES or out_dtype not in _TYPES:
+        raise ValueError("norm_rope: qkv and out_dtype must be float32 or bfloat16")
+    _floats(what, "cosine", cosine, (cosine.shape[0], hd // 2), device)
+    _floats(what, "sine", sine, tuple(cosine.shape), device)
+    _floats(what, "q_gain", q_gain, (hd,), device)
+    _floats(what, "k_gain", k_gain, (hd,), device)
+    _whole_numbers(what, "rows", rows, batch, device)
+    _whole_numbers(what, "positions", positions, batch, device)
+    _whole_numbers(what, "counts", counts, batch, device)
+    _whole_numbers(what, "offset", offset, 1, device)
+    q = torch.empty((batch, heads, tokens, hd), dtype=out_dtype, device=device)
+    args = _lib.NormRopeArgs(
+        qkv.data_ptr(), cosine.data_ptr(), sine.data_ptr(), _pointer(q_gain), _pointer(k_gain), rows.data_ptr(), _pointer(positions),
+        _pointer(counts), _pointer(offset), keys.data_ptr(), values.data_ptr(), q.data_ptr(), qkv.stride(0), keys.stride(0), keys.stride(1),
+        batch, tokens, heads, kv_heads, hd, max_len, cosine.shape[0], _TYPES[qkv.dtype], _TYPES[out_dtype], _TYPES[keys.dtype], epsilon)
+    with _on(device):
+        status = _lib.load_serve().ajqs_norm_rope(ctypes.byref(args), torch.cuda.current_stream().cuda_stream)
+    _lib.check_serve(status, what)
+    return q
+
+
+def shared_prefix_attention(q: torch.Tensor, prefix_keys: torch.Tensor, prefix_values: torch.Tensor, prefix_lengths: torch.Tensor,
+                            keys: torch.Tensor, values: torch.Tensor, rows: torch.Tensor, *, counts: torch.Tensor | None = None,
+                            offset: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of ``B`` sequences in groups that share a prefix, whose rows lie and are read once for the whole group.
+
+    ``q`` fp32 or bf16 ``[B, H, T, hd]`` (rotated); ``prefix_keys`` / ``prefix_values`` ``[G, Hkv, capacity, hd]``, the first
+    ``prefix_lengths[g]`` rows filled, for sequences ``g * B / G ..``; ``keys`` / ``values`` ``[B, Hkv, max_len, hd]`` with each sequence's own
+    rows, the T new tokens' (``norm_rope`` writes them) included.  Token t of sequence b sees its group's prefix and its own rows up to ``rows[b]
+    + offset + t``.  Caches fp32 or bf16; ``prefix_lengths`` int64 ``[G]``, ``rows`` and ``counts`` int64 ``[B]``, ``offset`` one int64, on
+    the device, as in ``norm_rope``.  Returns bf16 ``[B, T, H * hd]`` (what the output projection takes); zeros for a token that is not there
+    or sees nothing."""
+    what = "shared_prefix_attention"
+    if not q.is_cuda:
+        raise ValueError("shared_prefix_attention needs tensors on a ROCm device (there is no CPU path)")
+    device = q.device
+    _check_caches(what, prefix_keys, prefix_values, device)
+    _check_caches(what, keys, values, device)
+    if q.dim() != 4 or q.dtype not in _TYPES:
+        raise ValueError("shared_prefix_attention: q [B, H, T, hd] in float32 or bfloat16 expected")
+    batch, heads, seq, hd = q.shape
+    groups, kv_heads, capacity, _ = prefix_keys.shape
+    if keys.shape[0] != batch or keys.shape[1] != kv_heads or keys.shape[3] != hd or prefix_keys.shape[3] != hd or keys.dtype != prefix_keys.dtype:
+        raise ValueError("shared_prefix_attention: caches [B, Hkv, max_len, hd] and prefix caches [G, Hkv, capacity, hd] of one type expected")
+    _whole_numbers(what, "prefix_lengths", prefix_lengths, groups, device)
+    _whole_numbers(what, "rows", rows, batch, device)
+    _whole_numbers(what, "counts", counts, batch, device)
+    _whole_numbers(what, "offset", offset, 1, device)
+    q = q.contiguous()
+    out = torch.empty((batch, seq, heads * hd), dtype=torch.bfloat16, device=device)
+    args = _lib.SharedAttentionArgs(
+        q.data_ptr(), prefix_keys.data_ptr(), prefix_values.data_ptr(), keys.data_ptr(), values.data_ptr(), prefix_lengths.data_ptr(),
+        rows.data_ptr(), _pointer(counts), _pointer(offset), out.data_ptr(), prefix_keys.stride(0), prefix_keys.stride(1), keys.stride(0),
+        keys.stride(1), groups, batch, seq, heads, kv_heads, hd, capacity, keys.shape[2], _TYPES[q.dtype], _TYPES[keys.dtype])
+    lib = _lib.load_serve()
+    with _on(device):
+        size = lib.ajqs_shared_attention_workspace(ctypes.byref(args))
+        room = torch.empty(size, dtype=torch.uint8, device=device) if size else None
+        status = lib.ajqs_shared_attention(ctypes.byref(args), _pointer(room), size, torch.cuda.current_stream().cuda_stream)
+    _lib.check_serve(status, what)
+    return out

@@ -1,5 +1,5 @@
-"""Compile the HIP sources in ``csrc/`` into ``libajq.so`` and ``libajq_dense.so`` next to this file, and the extension module
-``_native.so``.
+"""Compile the HIP sources in ``csrc/`` into ``libajq.so``, ``libajq_dense.so`` and ``libajq_serve.so`` next to this file, and the
+extension module ``_native.so``.
 
 Cross-compiles for gfx950 with hipcc; needs no GPU.  Run as
 ``python -m ajllm_amd.build`` or call :func:`build_library`, which makes all that a quantized layer needs
@@ -21,6 +21,9 @@ LIBRARY = PACKAGE_DIR / "libajq.so"
 # without waiting for the quantized matmuls to compile
 DENSE_SOURCE = PACKAGE_DIR / "csrc" / "ajq_dense.hip"
 DENSE_LIBRARY = PACKAGE_DIR / "libajq_dense.so"
+# operators of decoding many continuations of one prompt (include/ajq_serve.h)
+SERVE_SOURCE = PACKAGE_DIR / "csrc" / "ajq_serve.hip"
+SERVE_LIBRARY = PACKAGE_DIR / "libajq_serve.so"
 # a quantized layer's forward without the interpreter: an extension module that calls the operator library
 NATIVE_SOURCE = PACKAGE_DIR / "csrc" / "native_linear.cpp"
 NATIVE_MODULE = PACKAGE_DIR / "_native.so"
@@ -64,6 +67,10 @@ def build_dense_library(verbose: bool = False) -> Path:
     return build_library(verbose, DENSE_SOURCE, DENSE_LIBRARY)
 
 
+def build_serve_library(verbose: bool = False) -> Path:
+    return build_library(verbose, SERVE_SOURCE, SERVE_LIBRARY)
+
+
 def ensure_dense_library() -> Path:
     """The dense library, compiled now if it is not there yet."""
     if not DENSE_LIBRARY.exists():
@@ -102,5 +109,6 @@ def build_bench_library(verbose: bool = False) -> Path:
 if __name__ == "__main__":
     print(build_library(verbose=True))
     print(build_dense_library(verbose=True))
+    print(build_serve_library(verbose=True))
     print(build_native_module(verbose=True))
     print(build_bench_library(verbose=True))

@@ -6,6 +6,7 @@
 // memory, so a recorded HIP graph can be replayed for every token.
 #pragma once
 #include "ajq_common.h"
+#include "lane_rows.h"
 
 namespace ajq {
 
@@ -174,64 +175,6 @@ __global__ __launch_bounds__(256) void rope_prefill_kernel(const float* __restri
 // sums start on a 16-byte boundary so that a GEMV prologue can fetch them with 128-bit loads.
 constexpr int attn_partial_stride(int hd) { return 4 + hd; }
 constexpr int kAttnPartialStride = attn_partial_stride(128);
-// Which HD / 16 of a row's dimensions lane c of a team holds (DPL of them: 8, 4 or 2), and how it fetches them.
-// 8 per lane, bf16 rows (256 B): 8c .. 8c+7, one 128-bit load.  8 per lane, fp32 rows (512 B): 4c .. 4c+3
-// and 64+4c .. 64+4c+3, so each of a team's two 128-bit loads covers 256 contiguous bytes.  4 per lane:
-// 4c .. 4c+3, one 128-bit (fp32) or 64-bit (bf16) load.  2 per lane: 2c, 2c+1, one 64-bit or 32-bit load.
-template <typename CacheT, int HD> struct LaneDims {
-  static_assert(HD == 128 || HD == 64 || HD == 32, "head_dim 128, 64 or 32");
-  static constexpr int DPL = HD / 16;
-  static constexpr bool split = sizeof(CacheT) == 4 && DPL == 8;
-  static constexpr int per_lane = split ? 4 : DPL;   // the lane's first dimension = per_lane * c
-  static constexpr int second = split ? 64 : 4;      // DPL == 8: its second four start this many dimensions later
-  __device__ static __forceinline__ int dim(int c, int i) { return per_lane * c + (i < 4 ? i : second + i - 4); }
-};
-template <int DPL> struct KvRow {
-  float v[DPL];
-};
-template <bool kStream, typename T>
-__device__ __forceinline__ T load_kv(const T* p) {
-  if constexpr (kStream) return __builtin_nontemporal_load(p);
-  return *p;
-}
-__device__ __forceinline__ void widen2(uint32_t w, float& lo, float& hi) {  // two bf16 -> two fp32
-  lo = __uint_as_float(w << 16);
-  hi = __uint_as_float(w & 0xFFFF0000u);
-}
-// A row of the cache as loaded (the lane's dimensions; p: the first of them) and widened to fp32 when it is used, so that a row
-// on its way from memory costs no more registers than its bytes.
-template <typename CacheT, int HD> struct RawRow {
-  static constexpr int words = (HD / 16) * (int)sizeof(CacheT) / 4;  // 8, 4, 2 (fp32) or 4, 2, 1 (bf16)
-  uint32_t w[words];
-};
-template <bool kStream, int HD, typename CacheT>
-__device__ __forceinline__ RawRow<CacheT, HD> load_raw(const CacheT* p) {
-  constexpr int words = RawRow<CacheT, HD>::words;
-  RawRow<CacheT, HD> r;
-  if constexpr (words >= 4) {
-#pragma unroll
-    for (int h = 0; h < words / 4; ++h) {
-      const u32x4_t a = load_kv<kStream>(reinterpret_cast<const u32x4_t*>(p + h * LaneDims<CacheT, HD>::second));
-      r.w[4 * h] = a.x; r.w[4 * h + 1] = a.y; r.w[4 * h + 2] = a.z; r.w[4 * h + 3] = a.w;
-    }
-  } else if constexpr (words == 2) {
-    const u32x2_t a = load_kv<kStream>(reinterpret_cast<const u32x2_t*>(p));
-    r.w[0] = a.x; r.w[1] = a.y;
-  } else {
-    r.w[0] = load_kv<kStream>(reinterpret_cast<const uint32_t*>(p));
-  }
-  return r;
-}
-template <typename CacheT, int HD>
-__device__ __forceinline__ KvRow<HD / 16> widen_row(const RawRow<CacheT, HD>& raw) {
-  KvRow<HD / 16> r;
-#pragma unroll
-  for (int i = 0; i < RawRow<CacheT, HD>::words; ++i) {
-    if constexpr (sizeof(CacheT) == 4) r.v[i] = __uint_as_float(raw.w[i]);
-    else widen2(raw.w[i], r.v[2 * i], r.v[2 * i + 1]);
-  }
-  return r;
-}
 // the step's own key / value row into the cache; a bf16 cache rounds and hands the rounded values back (what a
 // later read of the cache would give)
 template <int HD>
@@ -271,11 +214,6 @@ __device__ __forceinline__ void store_row(uint16_t* p, KvRow<HD / 16>& r) {
 // into the caches and attends to them from registers.  (Merging the S partial results in the
 // workgroup that finishes last was tried and lost: the device-scope fences it needs write back
 // and invalidate the XCD's L2, several microseconds per launch; the merge stays a launch.)
-
-// 2^x by the hardware instruction (1 ulp); the softmax below keeps its running maximum and
-// scores in the base-2 domain, scores pre-multiplied by log2(e)
-__device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
-constexpr float kLog2e = 1.4426950408889634f;
 
 template <int R, typename CacheT, bool kStep, bool kStream, int kWaves, int HD>
 __global__ __launch_bounds__(64 * kWaves) void attn_decode_kernel(const float* __restrict__ q, CacheT* __restrict__ kcache,
