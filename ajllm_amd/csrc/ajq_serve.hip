@@ -75,11 +75,92 @@ int check_shared(const ajqs_shared_attention_args* a) {
   return check_caches(what, a->keys, a->values, a->cache_batch, a->cache_head);
 }
 
-SharedAttention shared_of(const ajqs_shared_attention_args* a) {
-  return SharedAttention{a->q, a->prefix_keys, a->prefix_values, a->keys, a->values, int64s(a->prefix_lengths), int64s(a->rows),
-                         int64s(a->counts), int64s(a->offset), reinterpret_cast<uint16_t*>(a->out), a->prefix_group, a->prefix_head,
-                         a->cache_batch, a->cache_head, a->groups, a->batch, a->tokens, a->heads, a->kv_heads, a->prefix_cap, a->max_len,
-                         kLog2e / sqrtf((float)a->dim)};
+constexpr int kLdsLimit = 160 * 1024;
+template <typename K>
+int allow_lds(K kernel, int bytes, const char* what) {
+  if (bytes > kLdsLimit) return fail(AJQ_ERR_UNSUPPORTED, "%s: %d bytes of LDS needed", what, bytes);
+  if (bytes > 64 * 1024) {
+    hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != hipSuccess) return fail(AJQ_ERR_HIP, "%s: %s", what, hipGetErrorString(e));
+  }
+  return AJQ_OK;
+}
+
+long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
+
+// How an attention call is cut up: tiles of queries, parts of the rows.  The device's lengths are not known here; the capacities are what they
+// can be.
+struct SharedPlan {
+  int prefix_rt, own_rt;            // tiles of 16 queries a wave
+  int prefix_tiles, own_tiles, prefix_parts, own_parts;
+  long long prefix_blocks, own_blocks, queries;
+  size_t bytes;
+};
+constexpr int kMostParts = 64;      // a lane each in the merge
+SharedPlan shared_plan(const ajqs_shared_attention_args* a) {
+  SharedPlan p;
+  const long long share = a->heads / a->kv_heads, mine = a->tokens * share, all = a->batch / a->groups * mine;
+  p.own_rt = mine > 16 ? 2 : 1;
+  p.prefix_rt = all > 16 ? 2 : 1;
+  p.own_tiles = (int)ceil_div(mine, 16 * p.own_rt);
+  p.prefix_tiles = (int)ceil_div(all, 16 * p.prefix_rt);
+  const long long own_units = (long long)a->batch * a->kv_heads, prefix_units = (long long)a->groups * a->kv_heads;
+  auto parts = [](long long workgroups, long long rows, long long most) {
+    return (int)std::max(1ll, std::min({512 / workgroups, ceil_div(rows, 128), most}));
+  };
+  p.own_parts = parts(own_units * p.own_tiles, a->max_len, 16);
+  p.prefix_parts = parts(prefix_units * p.prefix_tiles, a->prefix_cap, kMostParts - 16);
+  p.prefix_blocks = ceil_div(prefix_units * p.prefix_parts, 8) * 8 * p.prefix_tiles;
+  p.own_blocks = ceil_div(own_units * p.own_parts, 8) * 8 * p.own_tiles;
+  p.queries = (long long)a->batch * a->heads * a->tokens;
+  p.bytes = (size_t)(p.prefix_parts + p.own_parts) * p.queries * (8 + 4 * (size_t)a->dim);
+  return p;
+}
+
+SharedAttention shared_of(const ajqs_shared_attention_args* a, const SharedPlan& p, void* workspace) {
+  SharedAttention s{};
+  s.q = a->q;
+  s.prefix_keys = a->prefix_keys;
+  s.prefix_values = a->prefix_values;
+  s.keys = a->keys;
+  s.values = a->values;
+  s.prefix_lengths = int64s(a->prefix_lengths);
+  s.rows = int64s(a->rows);
+  s.counts = int64s(a->counts);
+  s.offset = int64s(a->offset);
+  s.out = reinterpret_cast<uint16_t*>(a->out);
+  s.part_sums = reinterpret_cast<float*>(workspace);
+  s.part_ml = reinterpret_cast<float2*>(s.part_sums + (size_t)(p.prefix_parts + p.own_parts) * p.queries * a->dim);
+  s.prefix_group = a->prefix_group;
+  s.prefix_head = a->prefix_head;
+  s.cache_batch = a->cache_batch;
+  s.cache_head = a->cache_head;
+  s.queries = p.queries;
+  s.groups = a->groups;
+  s.batch = a->batch;
+  s.tokens = a->tokens;
+  s.heads = a->heads;
+  s.kv_heads = a->kv_heads;
+  s.prefix_cap = a->prefix_cap;
+  s.max_len = a->max_len;
+  s.prefix_blocks = (int)p.prefix_blocks;
+  s.prefix_parts = p.prefix_parts;
+  s.prefix_tiles = p.prefix_tiles;
+  s.own_parts = p.own_parts;
+  s.own_tiles = p.own_tiles;
+  s.scale2 = kLog2e / sqrtf((float)a->dim);
+  return s;
+}
+
+template <int HD, typename QT, typename CacheT, int RTP, int RTO>
+int launch_few(const SharedAttention& s, const SharedPlan& p, hipStream_t stream, const char* what) {
+  constexpr int bytes = std::max(few_lds_bytes<HD, CacheT, RTP>(), few_lds_bytes<HD, CacheT, RTO>());
+  auto kernel = shared_attention_few_kernel<HD, QT, CacheT, RTP, RTO>;
+  if (int e = allow_lds(kernel, bytes, what)) return e;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)(p.prefix_blocks + p.own_blocks)), dim3(256), bytes, stream, s);
+  if (int e = check_launch(what)) return e;
+  hipLaunchKernelGGL(shared_attention_merge_kernel<HD>, dim3((unsigned)ceil_div(p.queries, 4)), dim3(256), 0, stream, s);
+  return check_launch(what);
 }
 
 }  // namespace
@@ -125,26 +206,32 @@ int ajqs_norm_rope(const ajqs_norm_rope_args* a, void* stream) {
   return check_launch(what);
 }
 
-size_t ajqs_shared_attention_workspace(const ajqs_shared_attention_args* a) { return check_shared(a) ? 0 : 0; }
+size_t ajqs_shared_attention_workspace(const ajqs_shared_attention_args* a) { return check_shared(a) ? 0 : shared_plan(a).bytes; }
 
 int ajqs_shared_attention(const ajqs_shared_attention_args* a, void* workspace, size_t workspace_bytes, void* stream) {
   const char* what = "ajqs_shared_attention";
   if (int e = check_shared(a)) return e;
-  const size_t need = ajqs_shared_attention_workspace(a);
-  if (need && (!workspace || workspace_bytes < need))
-    return fail(AJQ_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, %zu given", what, need, workspace_bytes);
+  const SharedPlan p = shared_plan(a);
+  if (p.prefix_blocks + p.own_blocks > 0x7FFFFFFFLL) return fail(AJQ_ERR_SHAPE, "%s: too many tiles of queries", what);
+  if (!workspace || workspace_bytes < p.bytes)
+    return fail(AJQ_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, %zu given", what, p.bytes, workspace_bytes);
   if (!aligned16(workspace)) return fail(AJQ_ERR_ALIGN, "%s: the workspace must be 16-byte aligned", what);
-  const SharedAttention s = shared_of(a);
-  const long long queries = (long long)a->batch * a->heads * a->tokens;
+  const SharedAttention s = shared_of(a, p, workspace);
+  int status = AJQ_OK;
   with_dim(a->dim, [&](auto dim) {
     with_type(a->q_dtype, [&](auto q) {
       with_type(a->cache_dtype, [&](auto cache) {
-        hipLaunchKernelGGL((shared_attention_plain_kernel<decltype(q), decltype(cache), decltype(dim)::value>), dim3((unsigned)((queries + 3) / 4)),
-                           dim3(256), 0, (hipStream_t)stream, s);
+        constexpr int HD = decltype(dim)::value;
+        using QT = decltype(q);
+        using CacheT = decltype(cache);
+        const auto launch = p.own_rt == 2      ? launch_few<HD, QT, CacheT, 2, 2>
+                            : p.prefix_rt == 2 ? launch_few<HD, QT, CacheT, 2, 1>
+                                               : launch_few<HD, QT, CacheT, 1, 1>;
+        status = launch(s, p, (hipStream_t)stream, what);
       });
     });
   });
-  return check_launch(what);
+  return status;
 }
 
 int ajqs_adjust_logits(const ajqs_adjust_logits_args* a, void* stream) {

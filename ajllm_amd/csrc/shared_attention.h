@@ -1,6 +1,20 @@
 // Attention of sequences that share a prefix: token t of sequence b sees its group's prefix rows and its own rows up to its own.
+//
+//   out[b, t, h] = sum_j p_j v_j / sum_j p_j,   p_j = 2^(c q . k_j - m),  c = log2(e) / sqrt(HD),  m a number near the largest exponent
+//
+// The keys fall into two sets, and a softmax over both is put together from the (m, sum p, sum p v) of any parts of them.  The prefix's
+// rows are met by the queries of ALL sequences of the group, as a matrix product's rows; a sequence's own rows by its own queries.
+//
+// Products run on bf16 MFMA, transposed so that no operand changes its layout between them (as in prefill_attention.h):
+//   S^T = K Q^T    A = 16 keys x 32 dims from row-major key rows in LDS, B = queries; lane (g = l / 16, r = l % 16) gets keys 4 g .. 4 g + 3 of
+//                  query r;
+//   O^T += V^T P^T the lane's probabilities of 32 keys are its B fragment as they are; V^T by transposing reads of row-major rows.
+// A key's 16-byte chunks (a value row's 32-byte segments) sit in slots permuted by the row, so that these reads spread over the banks.
+// fp32 queries and fp32 rows are taken as two bf16 each (x = hi + lo, 16 bits): one product more for each; probabilities are
+// rounded to bf16, whose 2^-9 at most a weight is what the bf16 result's own rounding is.  Everything else is fp32.
 #pragma once
 #include "lane_rows.h"
+#include "prefill_attention.h"  // dma16, the fragment reads, pack8_bf16
 
 namespace ajq {
 
@@ -8,61 +22,392 @@ struct SharedAttention {
   const void *q, *prefix_keys, *prefix_values, *keys, *values;
   const long long *prefix_lengths, *rows, *counts, *offset;
   uint16_t* out;
+  float2* part_ml;      // [parts, queries] (m, sum p)
+  float* part_sums;     // [parts, queries, HD] sum p v
   long long prefix_group, prefix_head, cache_batch, cache_head;
+  long long queries;    // batch * heads * tokens, in the order of q
   int groups, batch, tokens, heads, kv_heads, prefix_cap, max_len;
-  float scale2;   // log2(e) / sqrt(dim)
+  int prefix_blocks, prefix_parts, prefix_tiles, own_parts, own_tiles;
+  float scale2;         // log2(e) / sqrt(HD)
 };
 
 __device__ __forceinline__ int held(long long n, int most) { return (int)min(max(n, 0ll), (long long)most); }
 
-// A wave a query: four teams of sixteen lanes take rows in turn, the prefix's and then the sequence's own.
-template <typename QT, typename CacheT, int HD>
-__global__ __launch_bounds__(256) void shared_attention_plain_kernel(SharedAttention a) {
-  using LD = LaneDims<float, HD>;
-  constexpr int DPL = LD::DPL;
-  const long long id = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);   // (b, h, t)
-  if (id >= (long long)a.batch * a.heads * a.tokens) return;
-  const int t = (int)(id % a.tokens), h = (int)(id / a.tokens % a.heads), b = (int)(id / a.tokens / a.heads);
-  const int lane = threadIdx.x & 63, team = lane >> 4, c = lane & 15, d0 = LD::per_lane * c;
-  const int hk = h / (a.heads / a.kv_heads), g = b / (a.batch / a.groups);
-  const bool there = a.counts == nullptr || t < a.counts[b];
-  const int before = there ? held(a.prefix_lengths[g], a.prefix_cap) : 0;
-  const int own = there ? held(a.rows[b] + (a.offset ? *a.offset : 0ll) + t + 1, a.max_len) : 0;
-  const KvRow<DPL> q = load_lane<HD>(reinterpret_cast<const QT*>(a.q) + (size_t)id * HD + d0);
-  float m = -INFINITY, l = 0.f, acc[DPL] = {};
-  auto walk = [&](const CacheT* keys, const CacheT* values, int rows) {
-    for (int i = team; i < rows; i += 4) {
-      const KvRow<DPL> k = load_lane<HD>(keys + (size_t)i * HD + d0), v = load_lane<HD>(values + (size_t)i * HD + d0);
-      float s = 0.f;
+// What a workgroup works on: a tile of the queries that meet one run of rows.
+template <typename CacheT> struct Meeting {
+  const CacheT *keys, *values;   // of the (group or sequence, key head)
+  int key_head, first_sequence;  // the queries are those of `sequences` sequences from here on and of the key head's heads
+  int queries;                   // sequences * tokens * share
+  int first;                     // the tile's first query
+  int begin, end;                // rows
+  bool own;
+  long long before;              // own rows a sequence's first new token sees ahead of its own row
+};
+
+// query number n of a meeting -> its place in q (and of its partial results), the token
+__device__ __forceinline__ long long query_place(const SharedAttention& a, int key_head, int first_sequence, int n, int& token) {
+  const int share = a.heads / a.kv_heads, each = a.tokens * share;
+  const int sequence = n / each, rest = n - sequence * each;
+  token = rest / share;
+  const int head = key_head * share + (rest - token * share);
+  return ((long long)(first_sequence + sequence) * a.heads + head) * a.tokens + token;
+}
+
+// 8 query components at p as bf16: hi (and lo, what fp32 has beyond it)
+__device__ __forceinline__ void split8(const float* v, u32x4_t& hi, u32x4_t& lo) {
+  hi = pack8_bf16(v);
+  float rest[8];
 #pragma unroll
-      for (int j = 0; j < DPL; ++j) s += q.v[j] * k.v[j];
-      s = team_sum16(s) * a.scale2;
-      const float m_new = fmaxf(m, s), corr = exp2_hw(m - m_new), w = exp2_hw(s - m_new);
-      l = l * corr + w;
+  for (int i = 0; i < 4; ++i) {
+    float a, b;
+    widen2(hi[i], a, b);
+    rest[2 * i] = v[2 * i] - a;
+    rest[2 * i + 1] = v[2 * i + 1] - b;
+  }
+  lo = pack8_bf16(rest);
+}
+template <typename T> constexpr int kHalves = sizeof(T) == 4 ? 2 : 1;   // bf16 numbers that stand for one
+__device__ __forceinline__ void load8_halves(const float* p, u32x4_t* to) {
+  const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+  const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+  split8(v, to[0], to[1]);
+}
+__device__ __forceinline__ void load8_halves(const uint16_t* p, u32x4_t* to) { to[0] = *reinterpret_cast<const u32x4_t*>(p); }
+
+// The running softmax of 16 queries, one a lane & 15: m, the lane's own part of the sum, and HD / 16 accumulators of O^T.
+template <int HD> struct RunningRow {
+  f32x4_t o[HD / 16];
+  float m, l;
+  bool fresh;   // no visible row met yet
+};
+
+// N exponents' products (N 16-key tiles of scores, scaled here) -> probabilities.  The reference point m moves where a lane's sum passes
+// kPfTrigger, to the largest exponent where that is past the slack (prefill_attention.h).
+template <int HD, int N>
+__device__ __forceinline__ void to_probabilities(RunningRow<HD>& row, const f32x4_t (&sc)[N], float scale2, float (&p)[4 * N]) {
+  float x[4 * N], sum = 0.f;
 #pragma unroll
-      for (int j = 0; j < DPL; ++j) acc[j] = acc[j] * corr + w * v.v[j];
-      m = m_new;
+  for (int e = 0; e < 4 * N; ++e) {
+    x[e] = __builtin_fmaf(sc[e >> 2][e & 3], scale2, -row.m);
+    p[e] = exp2_hw(x[e]);
+    sum += p[e];
+  }
+  if (__builtin_amdgcn_ballot_w64(row.fresh || sum > kPfTrigger) != 0) {
+    float mx = x[0];
+#pragma unroll
+    for (int e = 1; e < 4 * N; ++e) mx = fmaxf(mx, x[e]);
+    mx = quad_max(mx);
+    const bool move = row.fresh ? mx > -INFINITY : mx > kPfSlack;
+    const float shift = move ? mx : 0.f;
+    const float corr = move && !row.fresh ? exp2_hw(-shift) : 1.0f;
+    sum = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4 * N; ++e) {
+      p[e] = exp2_hw(x[e] - shift);
+      sum += p[e];
+    }
+    row.m += shift;
+    row.l *= corr;
+    row.fresh = row.fresh && !move;
+#pragma unroll
+    for (int t = 0; t < HD / 16; ++t) row.o[t] *= corr;
+  }
+  row.l += sum;
+}
+
+// ---- Few queries: the four waves of a workgroup take blocks of 32 rows in turn, each for itself (no barrier until the end), and RT tiles of 16
+// queries meet every row fetched.  What bounds it is memory: a wave asks for the next block's keys as soon as it has used this block's, and for
+// its values likewise; eight waves a CU (bf16) then have 64 to 128 KB on their way.
+// LDS of a wave: keys, then values, 32 rows each; fp32 rows as two planes of bf16, through registers.
+template <int HD, typename CacheT> constexpr int few_wave_bytes() { return 2 * 32 * 2 * HD * kHalves<CacheT>; }
+template <int HD, typename CacheT, int RT> constexpr int few_lds_bytes() {
+  constexpr int walk = 4 * few_wave_bytes<HD, CacheT>(), join = 4 * RT * 16 * HD * 4;
+  return (walk > join ? walk : join) + 4 * RT * 16 * 8;
+}
+
+template <int HD, typename QT, typename CacheT, int RT>
+__device__ __forceinline__ void meet_few(const SharedAttention& a, const Meeting<CacheT>& w, int part, unsigned char* lds, uint32_t lds0) {
+  constexpr int RB = 2 * HD, C = HD / 8, KS = HD / 32, TT = HD / 16, KH = kHalves<CacheT>, QH = kHalves<QT>;
+  constexpr int kPlane = 32 * RB;                 // 32 rows of bf16
+  constexpr bool kDma = KH == 1;
+  constexpr int kRows = 1024 / RB;                // rows of one wave-wide request
+  constexpr int kAsk = 32 / kRows;                // requests a block of keys (or values)
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r = lane & 15, g = lane >> 4;
+  const uint32_t mine = lds0 + (uint32_t)(wave * few_wave_bytes<HD, CacheT>());
+  unsigned char* mine_p = lds + wave * few_wave_bytes<HD, CacheT>();
+
+  // ---- queries: fragments of RT tiles, and how many of the meeting's rows each sees
+  u32x4_t qf[RT][KS][QH];
+  int limit[RT];
+#pragma unroll
+  for (int u = 0; u < RT; ++u) {
+    int token;
+    const long long place = query_place(a, w.key_head, w.first_sequence, min(w.first + 16 * u + r, w.queries - 1), token);
+    limit[u] = w.own ? held(w.before + token + 1, w.end) : w.end;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) load8_halves(reinterpret_cast<const QT*>(a.q) + place * HD + 32 * s + 8 * g, qf[u][s]);
+  }
+  RunningRow<HD> row[RT];
+#pragma unroll
+  for (int u = 0; u < RT; ++u) {
+    row[u].m = row[u].l = 0.f;
+    row[u].fresh = true;
+#pragma unroll
+    for (int t = 0; t < TT; ++t) row[u].o[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  }
+
+  // ---- rows on their way (past the last: the last again, which is there and finite)
+  const int ask_row = lane / C, slot = lane % C;
+  auto ask = [&](const CacheT* from, int at, uint32_t to, bool values) {
+    const CacheT* base = from + (size_t)at * HD;
+#pragma unroll
+    for (int i = 0; i < kAsk; ++i) {
+      const int k = kRows * i + ask_row;
+      const uint32_t chunk = values ? (uint32_t)((((slot >> 1) ^ (k & (TT - 1))) << 1) | (slot & 1)) : (uint32_t)(slot ^ (k & (C - 1)));
+      dma16(base, (uint32_t)(min(k, w.end - 1 - at) * RB) + chunk * 16u, to + (uint32_t)(i * 1024));
     }
   };
-  const size_t at = (size_t)g * a.prefix_group + (size_t)hk * a.prefix_head, mine = (size_t)b * a.cache_batch + (size_t)hk * a.cache_head;
-  walk(reinterpret_cast<const CacheT*>(a.prefix_keys) + at, reinterpret_cast<const CacheT*>(a.prefix_values) + at, before);
-  walk(reinterpret_cast<const CacheT*>(a.keys) + mine, reinterpret_cast<const CacheT*>(a.values) + mine, own);
+  constexpr int kPieces = kDma ? 1 : 32 * C / 64;   // 8 components each, a lane
+  Raw8F32 kraw[kPieces], vraw[kPieces];
+  auto fetch = [&](int at) {
+    if constexpr (!kDma) {
 #pragma unroll
-  for (int off = 16; off <= 32; off <<= 1) {
-    const float mo = __shfl_xor(m, off), lo = __shfl_xor(l, off), top = fmaxf(m, mo);
-    const float cm = m == -INFINITY ? 0.f : exp2_hw(m - top), co = mo == -INFINITY ? 0.f : exp2_hw(mo - top);
-    l = l * cm + lo * co;
+      for (int i = 0; i < kPieces; ++i) {
+        const int piece = lane + 64 * i, k = min(at + piece / C, w.end - 1);
+        kraw[i] = load8_raw(w.keys + (size_t)k * HD + 8 * (piece % C));
+        vraw[i] = load8_raw(w.values + (size_t)k * HD + 8 * (piece % C));
+      }
+    }
+  };
+  auto lay_down = [&]() {
+    if constexpr (!kDma) {
 #pragma unroll
-    for (int j = 0; j < DPL; ++j) acc[j] = acc[j] * cm + __shfl_xor(acc[j], off) * co;
-    m = top;
+      for (int i = 0; i < kPieces; ++i) {
+        const int piece = lane + 64 * i, k = piece / C, c = piece % C;
+        u32x4_t hi, lo;
+        auto put = [&](const Raw8F32& x, unsigned char* to) {
+          const float v[8] = {x.a.x, x.a.y, x.a.z, x.a.w, x.b.x, x.b.y, x.b.z, x.b.w};
+          split8(v, hi, lo);
+          *reinterpret_cast<u32x4_t*>(to) = hi;
+          *reinterpret_cast<u32x4_t*>(to + kPlane) = lo;
+        };
+        put(kraw[i], mine_p + k * RB + 16 * (c ^ (k & (C - 1))));
+        put(vraw[i], mine_p + 2 * kPlane + k * RB + 16 * ((((c >> 1) ^ (k & (TT - 1))) << 1) | (c & 1)));
+      }
+    }
+  };
+  const uint32_t values0 = mine + (uint32_t)(KH * kPlane);
+  uint32_t k_rd[KS], v_rd[TT];
+#pragma unroll
+  for (int s = 0; s < KS; ++s) k_rd[s] = mine + (uint32_t)(r * RB + 16 * ((4 * s + g) ^ (r & (C - 1))));
+  const int vkey = 4 * g + (r >> 2);
+#pragma unroll
+  for (int t = 0; t < TT; ++t) v_rd[t] = values0 + (uint32_t)(vkey * RB + 32 * (t ^ (vkey & (TT - 1))) + 8 * (r & 3));
+
+  int at = w.begin + 32 * wave;
+  if (at < w.end) {
+    if constexpr (kDma) {
+      ask(w.keys, at, mine, false);
+      ask(w.values, at, values0, true);
+    } else {
+      fetch(at);
+    }
   }
-  if (team != 0) return;
-  KvRow<DPL> o{};
-  if (l != 0.f) {
+  for (; at < w.end; at += 128) {
+    const bool more = at + 128 < w.end;
+    if constexpr (kDma) {
+      // (behind this block's keys only its values are on their way)
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kAsk) : "memory");
+    } else {
+      lay_down();
+      if (more) fetch(at + 128);
+      wave_lds_order();
+    }
+    f32x4_t sc[RT][2];
 #pragma unroll
-    for (int j = 0; j < DPL; ++j) o.v[j] = acc[j] / l;
+    for (int u = 0; u < RT; ++u) sc[u][0] = sc[u][1] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+#pragma unroll
+      for (int jb = 0; jb < 2; ++jb) {
+#pragma unroll
+        for (int kh = 0; kh < KH; ++kh) {
+          const u32x4_t k = pf_read128(k_rd[s] + (uint32_t)(kh * kPlane + jb * 16 * RB));
+#pragma unroll
+          for (int u = 0; u < RT; ++u)
+#pragma unroll
+            for (int qh = 0; qh < QH; ++qh)
+              if (kh + qh < 2) sc[u][jb] = mfma16(k, qf[u][s][qh], sc[u][jb]);   // (lo times lo is beyond what is kept)
+        }
+      }
+    }
+    if constexpr (kDma) {
+      if (more) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        ask(w.keys, at + 128, mine, false);
+      }
+    }
+    u32x4_t pf[RT];
+#pragma unroll
+    for (int u = 0; u < RT; ++u) {
+      if (__builtin_amdgcn_ballot_w64(at + 32 > limit[u]) != 0) {
+#pragma unroll
+        for (int jb = 0; jb < 2; ++jb)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (at + 16 * jb + 4 * g + i >= limit[u]) sc[u][jb][i] = -INFINITY;
+      }
+      float p[8];
+      to_probabilities<HD, 2>(row[u], sc[u], a.scale2, p);
+      pf[u] = pack8_bf16(p);
+    }
+    if constexpr (kDma) {
+      if (more) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kAsk) : "memory");
+      else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
+#pragma unroll
+    for (int t = 0; t < TT; ++t) {
+#pragma unroll
+      for (int kh = 0; kh < KH; ++kh) {
+        const u32x2_t lo = pf_read_tr(v_rd[t] + (uint32_t)(kh * kPlane)), hi = pf_read_tr(v_rd[t] + (uint32_t)(kh * kPlane + 16 * RB));
+        const u32x4_t v = {lo.x, lo.y, hi.x, hi.y};
+#pragma unroll
+        for (int u = 0; u < RT; ++u) row[u].o[t] = mfma16(v, pf[u], row[u].o[t]);
+      }
+    }
+    if constexpr (kDma) {
+      if (more) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        ask(w.values, at + 128, values0, true);
+      }
+    } else {
+      wave_lds_order();
+    }
   }
-  store_lane<HD>(a.out + ((size_t)b * a.tokens + t) * ((size_t)a.heads * HD) + (size_t)h * HD + d0, o);
+
+  // ---- the four waves' results meet in LDS
+  __syncthreads();
+  constexpr int kJoin = RT * 16;   // queries
+  float* sums = reinterpret_cast<float*>(lds);
+  float2* ml = reinterpret_cast<float2*>(lds + few_lds_bytes<HD, CacheT, RT>() - 4 * RT * 16 * 8);
+#pragma unroll
+  for (int u = 0; u < RT; ++u) {
+    const float l = quad_sum(row[u].l);
+    if (g == 0) ml[wave * kJoin + 16 * u + r] = float2{row[u].fresh && l == 0.f ? -INFINITY : row[u].m, l};   // (NaN stays)
+#pragma unroll
+    for (int t = 0; t < TT; ++t)
+      *reinterpret_cast<f32x4_t*>(sums + ((size_t)(wave * kJoin + 16 * u + r)) * HD + 16 * t + 4 * g) = row[u].o[t];
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < kJoin * (HD / 4); i += 256) {
+    const int n = i / (HD / 4), d = 4 * (i % (HD / 4));
+    if (w.first + n >= w.queries) break;   // (n only grows)
+    float2 e[4];
+    float m = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      e[k] = ml[k * kJoin + n];
+      m = fmaxf(m, e[k].x);
+    }
+    float l = 0.f;
+    f32x4_t o = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float weight = e[k].x == -INFINITY ? 0.f : exp2_hw(e[k].x - m);
+      l += e[k].y * weight;
+      o += *reinterpret_cast<const f32x4_t*>(sums + (size_t)(k * kJoin + n) * HD + d) * weight;
+    }
+    int token;
+    const long long place = query_place(a, w.key_head, w.first_sequence, w.first + n, token) + part * a.queries;
+    if (d == 0) a.part_ml[place] = float2{m, l};
+    *reinterpret_cast<f32x4_t*>(a.part_sums + place * HD + d) = o;
+  }
+}
+
+// A launch's workgroups: first the prefix's (a part of a (group, key head)'s rows and a tile of queries each; those that share rows are next
+// to each other on one XCD), then the sequences' own likewise.
+template <typename CacheT, int HD>
+__device__ __forceinline__ bool find_meeting(const SharedAttention& a, int tile_queries_prefix, int tile_queries_own, Meeting<CacheT>& w, int& part) {
+  const int share = a.heads / a.kv_heads;
+  w.own = (int)blockIdx.x >= a.prefix_blocks;
+  const int id = (int)blockIdx.x - (w.own ? a.prefix_blocks : 0);
+  const int tiles = w.own ? a.own_tiles : a.prefix_tiles, parts = w.own ? a.own_parts : a.prefix_parts;
+  const int runs = (w.own ? a.batch : a.groups) * a.kv_heads * parts;      // of rows
+  const int run = (id & 7) + 8 * (id / (8 * tiles)), tile = (id >> 3) % tiles;
+  if (run >= runs) return false;
+  part = run % parts;
+  const int unit = run / parts;
+  w.key_head = unit % a.kv_heads;
+  const int outer = unit / a.kv_heads, each = a.batch / a.groups;
+  const long long off = a.offset ? *a.offset : 0ll;
+  int there = a.tokens, rows;
+  if (w.own) {
+    w.first_sequence = outer;
+    w.queries = a.tokens * share;
+    w.before = a.rows[outer] + off;
+    if (a.counts) there = held(a.counts[outer], a.tokens);
+    rows = held(w.before + there, a.max_len);
+    const size_t at = (size_t)outer * a.cache_batch + (size_t)w.key_head * a.cache_head;
+    w.keys = reinterpret_cast<const CacheT*>(a.keys) + at;
+    w.values = reinterpret_cast<const CacheT*>(a.values) + at;
+  } else {
+    w.first_sequence = outer * each;
+    w.queries = each * a.tokens * share;
+    w.before = 0;
+    rows = held(a.prefix_lengths[outer], a.prefix_cap);
+    const size_t at = (size_t)outer * a.prefix_group + (size_t)w.key_head * a.prefix_head;
+    w.keys = reinterpret_cast<const CacheT*>(a.prefix_keys) + at;
+    w.values = reinterpret_cast<const CacheT*>(a.prefix_values) + at;
+  }
+  w.first = tile * (w.own ? tile_queries_own : tile_queries_prefix);
+  // parts of whole blocks of 32 rows
+  const int per = ((rows + parts - 1) / parts + 31) & ~31;
+  w.begin = min(rows, part * per);
+  w.end = min(rows, w.begin + per);
+  if (w.own) part += a.prefix_parts;
+  return true;
+}
+
+template <int HD, typename QT, typename CacheT, int RTP, int RTO>
+__global__ __launch_bounds__(256, sizeof(CacheT) == 4 ? 1 : 2) void shared_attention_few_kernel(SharedAttention a) {
+  extern __shared__ __attribute__((aligned(1024))) unsigned char shared_lds[];
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(pf_lds_char_t*)shared_lds;
+  Meeting<CacheT> w;
+  int part;
+  if (!find_meeting<CacheT, HD>(a, 16 * RTP, 16 * RTO, w, part)) return;
+  if (RTP == RTO || !w.own) meet_few<HD, QT, CacheT, RTP>(a, w, part, shared_lds, lds0);
+  else meet_few<HD, QT, CacheT, RTO>(a, w, part, shared_lds, lds0);
+}
+
+// ---- the parts of a query put together: a wave a query, lane p holding part p's (m, sum)
+template <int HD>
+__global__ __launch_bounds__(256) void shared_attention_merge_kernel(SharedAttention a) {
+  const long long place = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (place >= a.queries) return;
+  const int lane = threadIdx.x & 63, parts = a.prefix_parts + a.own_parts;
+  const int t = (int)(place % a.tokens), h = (int)(place / a.tokens % a.heads), b = (int)(place / a.tokens / a.heads);
+  const float2 ml = a.part_ml[min(lane, parts - 1) * a.queries + place];
+  constexpr int kLanes = HD / 2;                   // that hold two components
+  const int dl = min(lane, kLanes - 1);
+  const bool there = a.counts == nullptr || t < a.counts[b];
+  const float mine = lane < parts && there ? ml.x : -INFINITY;
+  float top = mine;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) top = fmaxf(top, __shfl_xor(top, off));
+  const float weight = mine == -INFINITY ? 0.f : exp2_hw(mine - top);
+  const float l = wave_sum(lane < parts && weight != 0.f ? ml.y * weight : 0.f);
+  float2 o = float2{0.f, 0.f};
+#pragma unroll 8
+  for (int p = 0; p < parts; ++p) {
+    const float c = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(weight), p));
+    const float2 x = *reinterpret_cast<const float2*>(a.part_sums + (p * a.queries + place) * HD + 2 * dl);
+    o.x += x.x * c;
+    o.y += x.y * c;
+  }
+  if (lane >= kLanes) return;
+  const uint32_t to = l > 0.f || l != l ? pack2_bf16(o.x / l, o.y / l) : 0u;
+  reinterpret_cast<uint32_t*>(a.out + (((size_t)b * a.tokens + t) * a.heads + h) * HD)[lane] = to;
 }
 
 }  // namespace ajq
