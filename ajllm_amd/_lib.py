@@ -8,6 +8,7 @@ CPU or PyTorch fallback behind any of these calls.
 from __future__ import annotations
 
 import ctypes
+import warnings
 from ctypes import c_char_p, c_float, c_int, c_int64, c_size_t, c_void_p
 from pathlib import Path
 
@@ -320,6 +321,33 @@ _serve_lib: ctypes.CDLL | None = None
 _dense_lib: ctypes.CDLL | None = None
 _bench_lib: ctypes.CDLL | None = None
 _native = None
+
+
+_serve_native: dict = {}
+
+
+def serve_native(name: str):
+    """The extension module's function of that name (``norm_rope``, ``shared_prefix_attention``, ``adjust_logits``), bound to the library on first
+    use.  Without the module every call is left to the general path: the function says None."""
+    function = _serve_native.get(name)
+    if function is None:
+        lib = load_serve()
+        try:
+            module = load_native()
+        except NativeModuleMissing as error:
+            warnings.warn(f"{error}; until then these calls take the longer way through the interpreter", RuntimeWarning, stacklevel=3)
+            module = None
+        else:
+            module.bind_serve(*(ctypes.cast(getattr(lib, entry), c_void_p).value for entry in (
+                "ajqs_norm_rope", "ajqs_shared_attention_workspace", "ajqs_shared_attention", "ajqs_adjust_logits")))
+        for each in ("norm_rope", "shared_prefix_attention", "adjust_logits"):
+            _serve_native[each] = getattr(module, each, _leave)
+        function = _serve_native[name]
+    return function
+
+
+def _leave(*args) -> None:
+    """In a native function's place."""
 
 
 def load_bench() -> ctypes.CDLL:

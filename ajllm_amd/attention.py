@@ -117,6 +117,11 @@ def norm_rope(qkv: torch.Tensor, cosine: torch.Tensor, sine: torch.Tensor, keys:
     what = "norm_rope"
     if not qkv.is_cuda:
         raise ValueError("norm_rope needs tensors on a ROCm device (there is no CPU path)")
+    # tensors as the kernel takes them: one call of native code, which leaves everything else to the lines below it
+    q = (_lib._serve_native.get(what) or _lib.serve_native(what))(
+        qkv, cosine, sine, keys, values, rows, heads, tokens, q_gain, k_gain, epsilon, positions, counts, offset, out_dtype)
+    if q is not None:
+        return q
     device = qkv.device
     _check_caches(what, keys, values, device)
     batch, kv_heads, max_len, hd = keys.shape
@@ -157,6 +162,9 @@ def shared_prefix_attention(q: torch.Tensor, prefix_keys: torch.Tensor, prefix_v
     what = "shared_prefix_attention"
     if not q.is_cuda:
         raise ValueError("shared_prefix_attention needs tensors on a ROCm device (there is no CPU path)")
+    out = (_lib._serve_native.get(what) or _lib.serve_native(what))(q, prefix_keys, prefix_values, prefix_lengths, keys, values, rows, counts, offset)
+    if out is not None:
+        return out
     device = q.device
     _check_caches(what, prefix_keys, prefix_values, device)
     _check_caches(what, keys, values, device)

@@ -24,8 +24,8 @@ DENSE_LIBRARY = PACKAGE_DIR / "libajq_dense.so"
 # operators of decoding many continuations of one prompt (include/ajq_serve.h)
 SERVE_SOURCE = PACKAGE_DIR / "csrc" / "ajq_serve.hip"
 SERVE_LIBRARY = PACKAGE_DIR / "libajq_serve.so"
-# a quantized layer's forward without the interpreter: an extension module that calls the operator library
-NATIVE_SOURCE = PACKAGE_DIR / "csrc" / "native_linear.cpp"
+# a quantized layer's forward (and the operators above) without the interpreter: an extension module that calls the libraries
+NATIVE_SOURCES = [PACKAGE_DIR / "csrc" / "native_linear.cpp", PACKAGE_DIR / "csrc" / "native_serve.cpp"]
 NATIVE_MODULE = PACKAGE_DIR / "_native.so"
 # measurement probes for bench.py (include/ajq_bench.h); the operator library does not depend on it
 BENCH_SOURCE = PACKAGE_DIR / "csrc" / "ajq_bench.hip"
@@ -90,7 +90,7 @@ def build_native_module(verbose: bool = False) -> Path:
     tmp = NATIVE_MODULE.with_suffix(".so.tmp%d" % os.getpid())
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-I{p}" for p in include_paths()),
-           f"-I{rocm / 'include'}", "-I/opt/rocm/include", f"-I{sysconfig.get_paths()['include']}", str(NATIVE_SOURCE), "-o", str(tmp),
+           f"-I{rocm / 'include'}", "-I/opt/rocm/include", f"-I{sysconfig.get_paths()['include']}", *(str(p) for p in NATIVE_SOURCES), "-o", str(tmp),
            f"-L{libraries}", "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_hip"]
     if verbose:
         print(" ".join(cmd), flush=True)

@@ -4,18 +4,11 @@
 // ordinary (another dtype or layout, a subclass, a mode or a transform that wants to see the operators, another device, an error
 // status): the caller then goes through its general path, which converts, refuses or reports.  What bounds a decode step's call is
 // the host: 8.8 us through ctypes, where the kernel takes 3.6.
-#include <Python.h>
-
-#include <ATen/ATen.h>
-#include <ATen/PythonTorchFunctionTLS.h>
-#include <c10/core/impl/TorchDispatchModeTLS.h>
-#include <c10/hip/HIPFunctions.h>
-#include <c10/hip/HIPStream.h>
-#include <torch/csrc/Dtype.h>
-#include <torch/csrc/Exceptions.h>
-#include <torch/csrc/autograd/python_variable.h>
+#include "native_common.h"
 
 #include "../../include/ajq.h"
+
+using native::plain, native::watched, native::WithoutInterpreter;
 
 namespace {
 
@@ -28,22 +21,6 @@ decltype(&ajq_w4a16_matmul) w4_matmul;
 decltype(&ajq_w8a16_matmul) w8_matmul;
 decltype(&ajq_matmul_scratch_bytes) scratch_bytes;
 
-// a tensor (or parameter) of the plain kind on the current device, or null
-const at::Tensor* plain(PyObject* object) {
-  if (!THPVariable_CheckExact(object)) return nullptr;
-  const at::Tensor& t = THPVariable_Unpack(object);
-  const c10::DispatchKeySet special({c10::DispatchKey::Python, c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::FuncTorchGradWrapper,
-                                     c10::DispatchKey::Functionalize, c10::DispatchKey::Conjugate, c10::DispatchKey::Negative,
-                                     c10::DispatchKey::ZeroTensor, c10::DispatchKey::Named});
-  return t.is_cuda() && t.layout() == at::kStrided && !t.key_set().has_any(special) ? &t : nullptr;
-}
-
-// other threads run while the allocator and the runtime do (a full queue makes a launch wait)
-struct WithoutInterpreter {
-  PyThreadState* state = PyEval_SaveThread();
-  ~WithoutInterpreter() { PyEval_RestoreThread(state); }
-};
-
 PyObject* linear(PyObject*, PyObject* const* args, Py_ssize_t count) {
   HANDLE_TH_ERRORS
   if (count != 7 || !scratch_bytes) {
@@ -51,7 +28,7 @@ PyObject* linear(PyObject*, PyObject* const* args, Py_ssize_t count) {
     return nullptr;
   }
   const at::Tensor *x = plain(args[0]), *wq = x ? plain(args[1]) : nullptr, *meta = wq ? plain(args[2]) : nullptr;
-  if (!meta || c10::impl::TorchDispatchModeTLS::any_modes_set() || at::impl::torch_function_mode_enabled()) Py_RETURN_NONE;
+  if (!meta || watched()) Py_RETURN_NONE;
   const bool w4 = args[3] == Py_True;
   const int64_t k = PyLong_AsLongLong(args[4]), columns = PyLong_AsLongLong(args[5]);
   if (PyErr_Occurred()) return nullptr;
@@ -124,6 +101,11 @@ PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t count) {
 
 PyMethodDef methods[] = {{"linear", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&linear)), METH_FASTCALL, nullptr},
                          {"bind", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&bind)), METH_FASTCALL, nullptr},
+                         {"norm_rope", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&native::norm_rope)), METH_FASTCALL, nullptr},
+                         {"shared_prefix_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&native::shared_prefix_attention)),
+                          METH_FASTCALL, nullptr},
+                         {"adjust_logits", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&native::adjust_logits)), METH_FASTCALL, nullptr},
+                         {"bind_serve", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&native::bind_serve)), METH_FASTCALL, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

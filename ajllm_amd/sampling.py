@@ -63,6 +63,10 @@ def adjust_logits(logits: torch.Tensor, *, tokens: torch.Tensor | None = None, l
     on 16-byte boundaries, as ``ajq_sample_pick`` wants them."""
     if not logits.is_cuda:
         raise ValueError("adjust_logits needs tensors on a ROCm device (there is no CPU path)")
+    made = (_lib._serve_native.get("adjust_logits") or _lib.serve_native("adjust_logits"))(
+        logits, tokens, lengths, prompt, prompt_lengths, repetition, frequency, presence, bias_ids, bias, allowed, allowed_rows, out)
+    if made is not None:
+        return made if out is None else out
     if logits.dim() != 2 or logits.dtype not in _TYPES or logits.stride(1) != 1 or 0 in logits.shape:
         raise ValueError("adjust_logits: logits [B, V] in float32 or bfloat16 expected")
     device = logits.device

@@ -458,3 +458,33 @@ def test_two_captured_steps_replay_as_eager_ones(cuda):
             _step(_fresh(cuda, 3))
     for s, e in zip(states, eager):
         assert torch.equal(s["out"], e["out"]) and torch.equal(s["keys"], e["keys"])
+
+
+def test_general_path_gives_the_same_bits(cuda, monkeypatch):
+    """Without the extension module, under a mode that looks on, and where its functions leave a call to the lines behind them."""
+    from ajllm_amd import _lib
+
+    def everything():
+        s = _fresh(cuda, 5)
+        q = attention.norm_rope(s["qkv"], s["cosine"], s["sine"], s["keys"], s["values"], s["rows"], heads=8, k_gain=s["gain"], offset=s["step"],
+                                out_dtype=BF16)
+        out = attention.shared_prefix_attention(q, s["pk"], s["pv"], s["lengths"], s["keys"], s["values"], s["rows"])
+        logits = sampling.adjust_logits(out.view(6, 512)[:, 1:], tokens=s["out"], lengths=s["step"], presence=s["penalty"])
+        into = torch.zeros((6, 511), device=cuda)
+        assert sampling.adjust_logits(out.view(6, 512)[:, 1:], out=into, bias_ids=s["out"], bias=torch.ones((6, 32), device=cuda)) is into
+        return q, s["keys"], s["values"], out, logits, into
+
+    def same(a, b):
+        return all(torch.equal(x, y) for x, y in zip(a, b))
+
+    fast = everything()
+    strided = torch.zeros((6, 8, 2, 64), dtype=BF16, device=cuda)[:, :, :1]
+    strided.copy_(fast[0])
+    s = _fresh(cuda, 5)
+    assert torch.equal(attention.shared_prefix_attention(strided, s["pk"], s["pv"], s["lengths"], fast[1], fast[2], s["rows"]), fast[3])
+    with torch.overrides.BaseTorchFunctionMode():
+        assert same(fast, everything())
+    calls = []
+    for name in ("norm_rope", "shared_prefix_attention", "adjust_logits"):
+        monkeypatch.setitem(_lib._serve_native, name, lambda *a, name=name: calls.append(name))
+    assert same(fast, everything()) and calls == ["norm_rope", "shared_prefix_attention", "adjust_logits", "adjust_logits"]
