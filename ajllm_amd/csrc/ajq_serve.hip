@@ -57,6 +57,7 @@ int check_caches(const char* what, const void* keys, const void* values, long lo
   return AJQ_OK;
 }
 
+constexpr int kMostRows = 1 << 30;   // of a cache head
 int check_shared(const ajqs_shared_attention_args* a) {
   const char* what = "ajqs_shared_attention";
   if (!a) return fail(AJQ_ERR_NULL, "%s: null arguments", what);
@@ -64,7 +65,7 @@ int check_shared(const ajqs_shared_attention_args* a) {
     return fail(AJQ_ERR_NULL, "%s: null pointer argument", what);
   if (!built_dim(a->dim)) return fail(AJQ_ERR_UNSUPPORTED, "%s: head size %d (128, 64 and 32 are built)", what, a->dim);
   if (a->batch < 1 || a->tokens < 1 || a->groups < 1 || a->batch % a->groups != 0 || a->kv_heads < 1 || a->heads < 1 ||
-      a->heads % a->kv_heads != 0 || a->prefix_cap < 1 || a->max_len < 1)
+      a->heads % a->kv_heads != 0 || a->prefix_cap < 1 || a->max_len < 1 || a->prefix_cap > kMostRows || a->max_len > kMostRows)
     return fail(AJQ_ERR_SHAPE, "%s: unsupported shape (groups=%d batch=%d tokens=%d heads=%d kv_heads=%d prefix_cap=%d max_len=%d)", what,
                 a->groups, a->batch, a->tokens, a->heads, a->kv_heads, a->prefix_cap, a->max_len);
   if ((long long)a->batch * a->heads * a->tokens > 0x1FFFFFFFLL)
@@ -90,7 +91,9 @@ long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 
 // How an attention call is cut up: tiles of queries, parts of the rows.  The device's lengths are not known here; the capacities are what they
 // can be.
+enum class SharedForm { few, many, walk };   // (the prefix by meet_few, by meet_many; everything in one walk)
 struct SharedPlan {
+  SharedForm form;
   int prefix_rt, own_rt;            // tiles of 16 queries a wave
   int prefix_tiles, own_tiles, prefix_parts, own_parts;
   long long prefix_blocks, own_blocks, queries;
@@ -98,22 +101,32 @@ struct SharedPlan {
 };
 constexpr int kMostParts = 64;      // a lane each in the merge
 SharedPlan shared_plan(const ajqs_shared_attention_args* a) {
-  SharedPlan p;
+  SharedPlan p{};
   const long long share = a->heads / a->kv_heads, mine = a->tokens * share, all = a->batch / a->groups * mine;
-  p.own_rt = mine > 16 ? 2 : 1;
-  p.prefix_rt = all > 16 ? 2 : 1;
-  p.own_tiles = (int)ceil_div(mine, 16 * p.own_rt);
-  p.prefix_tiles = (int)ceil_div(all, 16 * p.prefix_rt);
   const long long own_units = (long long)a->batch * a->kv_heads, prefix_units = (long long)a->groups * a->kv_heads;
+  const bool bf16 = a->cache_dtype == AJQS_BF16;
   auto parts = [](long long workgroups, long long rows, long long most) {
     return (int)std::max(1ll, std::min({512 / workgroups, ceil_div(rows, 128), most}));
   };
-  p.own_parts = parts(own_units * p.own_tiles, a->max_len, 16);
-  p.prefix_parts = parts(prefix_units * p.prefix_tiles, a->prefix_cap, kMostParts - 16);
-  p.prefix_blocks = ceil_div(prefix_units * p.prefix_parts, 8) * 8 * p.prefix_tiles;
-  p.own_blocks = ceil_div(own_units * p.own_parts, 8) * 8 * p.own_tiles;
   p.queries = (long long)a->batch * a->heads * a->tokens;
-  p.bytes = (size_t)(p.prefix_parts + p.own_parts) * p.queries * (8 + 4 * (size_t)a->dim);
+  if (bf16 && mine > 64) {
+    p.form = SharedForm::walk;
+    p.own_tiles = (int)ceil_div(mine, 128);
+    p.own_parts = parts(own_units * p.own_tiles, (long long)a->prefix_cap + a->max_len, kMostParts);
+    p.own_blocks = ceil_div(own_units, 8) * 8 * p.own_tiles * p.own_parts;
+  } else {
+    p.form = bf16 && all > 64 ? SharedForm::many : SharedForm::few;
+    p.own_rt = mine > 16 ? 2 : 1;
+    p.prefix_rt = all > 16 ? 2 : 1;
+    p.own_tiles = (int)ceil_div(mine, 16 * p.own_rt);
+    p.prefix_tiles = (int)ceil_div(all, p.form == SharedForm::many ? 128 : 16 * p.prefix_rt);
+    p.own_parts = parts(own_units * p.own_tiles, a->max_len, 16);
+    p.prefix_parts = parts(prefix_units * p.prefix_tiles, a->prefix_cap, kMostParts - 16);
+    p.prefix_blocks = ceil_div(prefix_units * p.prefix_parts, 8) * 8 * p.prefix_tiles;
+    p.own_blocks = ceil_div(own_units * p.own_parts, 8) * 8 * p.own_tiles;
+  }
+  const int all_parts = p.prefix_parts + p.own_parts;
+  p.bytes = all_parts > 1 ? (size_t)all_parts * p.queries * (8 + 4 * (size_t)a->dim) : 0;
   return p;
 }
 
@@ -152,15 +165,32 @@ SharedAttention shared_of(const ajqs_shared_attention_args* a, const SharedPlan&
   return s;
 }
 
+template <int HD>
+int merge_parts(const SharedAttention& s, const SharedPlan& p, hipStream_t stream, const char* what) {
+  if (int e = check_launch(what)) return e;
+  hipLaunchKernelGGL(shared_attention_merge_kernel<HD>, dim3((unsigned)ceil_div(p.queries, 4)), dim3(256), 0, stream, s);
+  return check_launch(what);
+}
 template <int HD, typename QT, typename CacheT, int RTP, int RTO>
 int launch_few(const SharedAttention& s, const SharedPlan& p, hipStream_t stream, const char* what) {
   constexpr int bytes = std::max(few_lds_bytes<HD, CacheT, RTP>(), few_lds_bytes<HD, CacheT, RTO>());
   auto kernel = shared_attention_few_kernel<HD, QT, CacheT, RTP, RTO>;
   if (int e = allow_lds(kernel, bytes, what)) return e;
   hipLaunchKernelGGL(kernel, dim3((unsigned)(p.prefix_blocks + p.own_blocks)), dim3(256), bytes, stream, s);
-  if (int e = check_launch(what)) return e;
-  hipLaunchKernelGGL(shared_attention_merge_kernel<HD>, dim3((unsigned)ceil_div(p.queries, 4)), dim3(256), 0, stream, s);
-  return check_launch(what);
+  return merge_parts<HD>(s, p, stream, what);
+}
+template <int HD, typename QT, int RTO>
+int launch_many(const SharedAttention& s, const SharedPlan& p, hipStream_t stream, const char* what) {
+  constexpr int bytes = std::max(many_lds_bytes<HD>(), few_lds_bytes<HD, uint16_t, RTO>());
+  auto kernel = shared_attention_many_kernel<HD, QT, RTO>;
+  if (int e = allow_lds(kernel, bytes, what)) return e;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)(p.prefix_blocks + p.own_blocks)), dim3(256), bytes, stream, s);
+  return merge_parts<HD>(s, p, stream, what);
+}
+template <int HD, typename QT>
+int launch_walk(const SharedAttention& s, const SharedPlan& p, hipStream_t stream, const char* what) {
+  hipLaunchKernelGGL((shared_attention_walk_kernel<HD, QT>), dim3((unsigned)p.own_blocks), dim3(256), many_lds_bytes<HD>(), stream, s);
+  return p.own_parts > 1 ? merge_parts<HD>(s, p, stream, what) : check_launch(what);
 }
 
 }  // namespace
@@ -213,7 +243,7 @@ int ajqs_shared_attention(const ajqs_shared_attention_args* a, void* workspace, 
   if (int e = check_shared(a)) return e;
   const SharedPlan p = shared_plan(a);
   if (p.prefix_blocks + p.own_blocks > 0x7FFFFFFFLL) return fail(AJQ_ERR_SHAPE, "%s: too many tiles of queries", what);
-  if (!workspace || workspace_bytes < p.bytes)
+  if (p.bytes && (!workspace || workspace_bytes < p.bytes))
     return fail(AJQ_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, %zu given", what, p.bytes, workspace_bytes);
   if (!aligned16(workspace)) return fail(AJQ_ERR_ALIGN, "%s: the workspace must be 16-byte aligned", what);
   const SharedAttention s = shared_of(a, p, workspace);
@@ -224,6 +254,17 @@ int ajqs_shared_attention(const ajqs_shared_attention_args* a, void* workspace, 
         constexpr int HD = decltype(dim)::value;
         using QT = decltype(q);
         using CacheT = decltype(cache);
+        if constexpr (sizeof(CacheT) == 2) {
+          if (p.form == SharedForm::walk) {
+            status = launch_walk<HD, QT>(s, p, (hipStream_t)stream, what);
+            return;
+          }
+          if (p.form == SharedForm::many) {
+            const auto launch = p.own_rt == 2 ? launch_many<HD, QT, 2> : launch_many<HD, QT, 1>;
+            status = launch(s, p, (hipStream_t)stream, what);
+            return;
+          }
+        }
         const auto launch = p.own_rt == 2      ? launch_few<HD, QT, CacheT, 2, 2>
                             : p.prefix_rt == 2 ? launch_few<HD, QT, CacheT, 2, 1>
                                                : launch_few<HD, QT, CacheT, 1, 1>;

@@ -325,6 +325,165 @@ __device__ __forceinline__ void meet_few(const SharedAttention& a, const Meeting
   }
 }
 
+// ---- Many queries on bf16 rows: 128 to a workgroup, 32 to each wave, all four walking the same blocks of 64 rows (LDS, two stages, one barrier a
+// block, as attn_prefill_kernel).  Bound by MFMA.  The walk goes over a run of the group's prefix and, behind it, of one sequence's own
+// rows; either may be empty.
+template <typename CacheT> struct Walk {
+  const CacheT *keys[2], *values[2];   // prefix, own
+  int rows[2];                         // of which so many are there
+  int first_block, blocks;             // the walk's part of the blocks of both
+  int key_head, first_sequence, queries, first;
+  long long before;
+};
+template <int HD> constexpr int many_lds_bytes() { return 4 * 64 * 2 * HD; }
+
+template <int HD, typename QT>
+__device__ __forceinline__ void meet_many(const SharedAttention& a, const Walk<uint16_t>& w, RunningRow<HD> (&row)[2], uint32_t lds0) {
+  constexpr int RB = 2 * HD, C = HD / 8, KS = HD / 32, TT = HD / 16, QH = kHalves<QT>;
+  constexpr int kTile = 64 * RB;
+  constexpr int kReqRows = 1024 / RB;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r = lane & 15, g = lane >> 4;
+  const int prefix_blocks = (w.rows[0] + 63) >> 6;
+
+  const int krow = kReqRows * wave + lane / C, slot = lane % C;
+  const uint32_t k_chunk = (uint32_t)(slot ^ (krow & (C - 1)));
+  const uint32_t v_chunk = (uint32_t)((((slot >> 1) ^ (krow & (TT - 1))) << 1) | (slot & 1));
+  // part i (of KS) of block j: this wave's kReqRows rows of the i-th group of 4 kReqRows
+  auto ask = [&](int j, int i) {
+    const int own = w.first_block + j >= prefix_blocks, kb0 = (w.first_block + j - (own ? prefix_blocks : 0)) * 64;
+    const uint32_t to = lds0 + (uint32_t)((j & 1) * 2 * kTile + (wave + 4 * i) * 1024);
+    const uint32_t at = (uint32_t)(min(4 * kReqRows * i + krow, w.rows[own] - 1 - kb0) * RB);
+    dma16(w.keys[own] + (size_t)kb0 * HD, at + k_chunk * 16u, to);
+    dma16(w.values[own] + (size_t)kb0 * HD, at + v_chunk * 16u, to + (uint32_t)kTile);
+  };
+  uint32_t k_rd[KS], v_rd[TT];
+#pragma unroll
+  for (int s = 0; s < KS; ++s) k_rd[s] = lds0 + (uint32_t)(r * RB + 16 * ((4 * s + g) ^ (r & (C - 1))));
+  const int vkey = 4 * g + (r >> 2);
+#pragma unroll
+  for (int t = 0; t < TT; ++t) v_rd[t] = lds0 + (uint32_t)(kTile + vkey * RB + 32 * (t ^ (vkey & (TT - 1))) + 8 * (r & 3));
+
+#pragma unroll
+  for (int i = 0; i < KS; ++i) ask(0, i);
+  u32x4_t qf[2][KS][QH];
+  int limit[2], nearest, farthest;   // own rows that a lane's queries see, that the wave's first and last one see
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    int token;
+    const long long place = query_place(a, w.key_head, w.first_sequence, min(w.first + 32 * wave + 16 * u + r, w.queries - 1), token);
+    limit[u] = held(w.before + token + 1, w.rows[1]);
+#pragma unroll
+    for (int s = 0; s < KS; ++s) load8_halves(reinterpret_cast<const QT*>(a.q) + place * HD + 32 * s + 8 * g, qf[u][s]);
+    row[u].m = row[u].l = 0.f;
+    row[u].fresh = true;
+#pragma unroll
+    for (int t = 0; t < TT; ++t) row[u].o[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  }
+  nearest = __builtin_amdgcn_readlane(limit[0], 0);
+  farthest = __builtin_amdgcn_readlane(limit[1], 63);
+  const bool idle = w.first + 32 * wave >= w.queries;
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  for (int j = 0; j < w.blocks; ++j) {
+    const bool own = w.first_block + j >= prefix_blocks;
+    const int kb0 = (w.first_block + j - (own ? prefix_blocks : 0)) * 64;
+    const bool more = j + 1 < w.blocks;
+    if (idle || (own && kb0 >= farthest)) {
+      if (more) {
+#pragma unroll
+        for (int i = 0; i < KS; ++i) ask(j + 1, i);
+      }
+    } else {
+      f32x4_t sc[2][4];
+      u32x4_t ka[4];
+#pragma unroll
+      for (int jb = 0; jb < 4; ++jb) ka[jb] = pf_read128(k_rd[0] + (uint32_t)(jb * 16 * RB));
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        u32x4_t kn[4];
+        if (s < KS - 1) {
+#pragma unroll
+          for (int jb = 0; jb < 4; ++jb) kn[jb] = pf_read128(k_rd[s + 1] + (uint32_t)(jb * 16 * RB));
+        }
+#pragma unroll
+        for (int qh = 0; qh < QH; ++qh)
+#pragma unroll
+          for (int jb = 0; jb < 4; ++jb)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) sc[u][jb] = mfma16(ka[jb], qf[u][s][qh], s + qh == 0 ? f32x4_t{0.f, 0.f, 0.f, 0.f} : sc[u][jb]);
+        if (more) ask(j + 1, s);
+        if (s < KS - 1) {
+#pragma unroll
+          for (int jb = 0; jb < 4; ++jb) ka[jb] = kn[jb];
+        }
+      }
+      const int seen = own ? nearest : w.rows[0];
+      if (kb0 + 64 > seen) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int last = own ? limit[u] : w.rows[0];
+#pragma unroll
+          for (int jb = 0; jb < 4; ++jb)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (kb0 + 16 * jb + 4 * g + i >= last) sc[u][jb][i] = -INFINITY;
+        }
+      }
+      u32x4_t pf[2][2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        float p[16];
+        to_probabilities<HD, 4>(row[u], sc[u], a.scale2, p);
+        pf[u][0] = pack8_bf16(&p[0]);
+        pf[u][1] = pack8_bf16(&p[8]);
+      }
+      constexpr int kRing = TT < 8 ? TT : 8;
+      auto v_lo = [&](int i) { return pf_read_tr(v_rd[i % TT] + (uint32_t)((i / TT) * 32 * RB)); };
+      auto v_hi = [&](int i) { return pf_read_tr(v_rd[i % TT] + (uint32_t)((i / TT) * 32 * RB + 16 * RB)); };
+      u32x2_t vlo[kRing], vhi[kRing];
+#pragma unroll
+      for (int i = 0; i < kRing; ++i) {
+        vlo[i] = v_lo(i);
+        vhi[i] = v_hi(i);
+      }
+#pragma unroll
+      for (int i = 0; i < 2 * TT; ++i) {
+        const u32x4_t vf = {vlo[i % kRing].x, vlo[i % kRing].y, vhi[i % kRing].x, vhi[i % kRing].y};
+#pragma unroll
+        for (int u = 0; u < 2; ++u) row[u].o[i % TT] = mfma16(vf, pf[u][i / TT], row[u].o[i % TT]);
+        if (i + kRing < 2 * TT) {
+          vlo[i % kRing] = v_lo(i + kRing);
+          vhi[i % kRing] = v_hi(i + kRing);
+        }
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < KS; ++s) k_rd[s] ^= (uint32_t)(2 * kTile);
+#pragma unroll
+    for (int t = 0; t < TT; ++t) v_rd[t] ^= (uint32_t)(2 * kTile);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+  }
+}
+
+// a lane's queries of meet_many as partial results
+template <int HD>
+__device__ __forceinline__ void leave_part(const SharedAttention& a, const Walk<uint16_t>& w, const RunningRow<HD> (&row)[2], int part) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const float l = quad_sum(row[u].l);
+    const int n = w.first + 32 * wave + 16 * u + r;
+    if (n >= w.queries) continue;
+    int token;
+    const long long place = query_place(a, w.key_head, w.first_sequence, n, token) + part * a.queries;
+    if (g == 0) a.part_ml[place] = float2{row[u].fresh && l == 0.f ? -INFINITY : row[u].m, l};
+#pragma unroll
+    for (int t = 0; t < HD / 16; ++t) *reinterpret_cast<f32x4_t*>(a.part_sums + place * HD + 16 * t + 4 * g) = row[u].o[t];
+  }
+}
+
 // A launch's workgroups: first the prefix's (a part of a (group, key head)'s rows and a tile of queries each; those that share rows are next
 // to each other on one XCD), then the sequences' own likewise.
 template <typename CacheT, int HD>
@@ -363,7 +522,7 @@ __device__ __forceinline__ bool find_meeting(const SharedAttention& a, int tile_
   w.first = tile * (w.own ? tile_queries_own : tile_queries_prefix);
   // parts of whole blocks of 32 rows
   const int per = ((rows + parts - 1) / parts + 31) & ~31;
-  w.begin = min(rows, part * per);
+  w.begin = (int)min((long long)rows, (long long)part * per);
   w.end = min(rows, w.begin + per);
   if (w.own) part += a.prefix_parts;
   return true;
@@ -378,6 +537,111 @@ __global__ __launch_bounds__(256, sizeof(CacheT) == 4 ? 1 : 2) void shared_atten
   if (!find_meeting<CacheT, HD>(a, 16 * RTP, 16 * RTO, w, part)) return;
   if (RTP == RTO || !w.own) meet_few<HD, QT, CacheT, RTP>(a, w, part, shared_lds, lds0);
   else meet_few<HD, QT, CacheT, RTO>(a, w, part, shared_lds, lds0);
+}
+
+// The prefix by meet_many, the sequences' own rows by meet_few.
+template <int HD, typename QT, int RTO>
+__global__ __launch_bounds__(256, 2) void shared_attention_many_kernel(SharedAttention a) {
+  extern __shared__ __attribute__((aligned(1024))) unsigned char shared_lds[];
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(pf_lds_char_t*)shared_lds;
+  Meeting<uint16_t> w;
+  int part;
+  if (!find_meeting<uint16_t, HD>(a, 128, 16 * RTO, w, part)) return;
+  if (w.own) {
+    meet_few<HD, QT, uint16_t, RTO>(a, w, part, shared_lds, lds0);
+    return;
+  }
+  Walk<uint16_t> walk;
+  walk.keys[0] = w.keys + (size_t)w.begin * HD;
+  walk.values[0] = w.values + (size_t)w.begin * HD;
+  walk.keys[1] = walk.values[1] = nullptr;
+  walk.rows[0] = w.end - w.begin;
+  walk.rows[1] = 0;
+  walk.first_block = 0;
+  walk.blocks = (walk.rows[0] + 63) >> 6;
+  walk.key_head = w.key_head;
+  walk.first_sequence = w.first_sequence;
+  walk.queries = w.queries;
+  walk.first = w.first;
+  walk.before = 0;
+  RunningRow<HD> row[2];
+  if (walk.blocks > 0) {
+    meet_many<HD, QT>(a, walk, row, lds0);
+  } else {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      row[u].m = row[u].l = 0.f;
+      row[u].fresh = true;
+#pragma unroll
+      for (int t = 0; t < HD / 16; ++t) row[u].o[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    }
+  }
+  leave_part<HD>(a, walk, row, part);
+}
+
+// Sequences with many new tokens each: 128 queries of one sequence walk the prefix and then its own rows, and what comes out is the result.  With
+// own_parts > 1 the walk is cut up and leaves parts for the merge.
+template <int HD, typename QT>
+__global__ __launch_bounds__(256, 2) void shared_attention_walk_kernel(SharedAttention a) {
+  extern __shared__ __attribute__((aligned(1024))) unsigned char shared_lds[];
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(pf_lds_char_t*)shared_lds;
+  const int share = a.heads / a.kv_heads, parts = a.own_parts, tiles = a.own_tiles;
+  const int id = (int)blockIdx.x, run = (id & 7) + 8 * (id / (8 * tiles * parts)), rest = (id >> 3) % (tiles * parts);
+  if (run >= a.batch * a.kv_heads) return;
+  const int tile = tiles - 1 - rest / parts, part = rest % parts;
+  const int b = run / a.kv_heads, hk = run % a.kv_heads, group = b / (a.batch / a.groups);
+  Walk<uint16_t> w;
+  w.key_head = hk;
+  w.first_sequence = b;
+  w.queries = a.tokens * share;
+  w.first = 128 * tile;
+  w.before = a.rows[b] + (a.offset ? *a.offset : 0ll);
+  const int there = a.counts ? held(a.counts[b], a.tokens) : a.tokens;
+  const int last = min((w.first + 127) / share, there - 1);          // the tile's last token that is there
+  const size_t at = (size_t)group * a.prefix_group + (size_t)hk * a.prefix_head, own = (size_t)b * a.cache_batch + (size_t)hk * a.cache_head;
+  w.keys[0] = reinterpret_cast<const uint16_t*>(a.prefix_keys) + at;
+  w.values[0] = reinterpret_cast<const uint16_t*>(a.prefix_values) + at;
+  w.keys[1] = reinterpret_cast<const uint16_t*>(a.keys) + own;
+  w.values[1] = reinterpret_cast<const uint16_t*>(a.values) + own;
+  const bool none = w.first >= there * share;
+  w.rows[0] = none ? 0 : held(a.prefix_lengths[group], a.prefix_cap);
+  w.rows[1] = none ? 0 : held(w.before + last + 1, a.max_len);
+  const int blocks = ((w.rows[0] + 63) >> 6) + ((w.rows[1] + 63) >> 6), per = (blocks + parts - 1) / parts;
+  w.first_block = min(blocks, part * per);
+  w.blocks = min(blocks - w.first_block, per);
+  RunningRow<HD> row[2];
+  if (w.blocks > 0) {
+    meet_many<HD, QT>(a, w, row, lds0);
+  } else {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      row[u].m = row[u].l = 0.f;
+      row[u].fresh = true;
+#pragma unroll
+      for (int t = 0; t < HD / 16; ++t) row[u].o[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    }
+  }
+  if (parts > 1) {
+    leave_part<HD>(a, w, row, part);
+    return;
+  }
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const float l = quad_sum(row[u].l);
+    const int n = w.first + 32 * wave + 16 * u + r;
+    if (n >= w.queries) continue;
+    const int token = n / share, head = hk * share + (n - token * share);
+    const float inv = token < there && (l > 0.f || l != l) ? 1.0f / l : 0.f;
+    const bool zero = inv == 0.f;
+    uint16_t* to = a.out + (((size_t)b * a.tokens + token) * a.heads + head) * HD + 4 * g;
+#pragma unroll
+    for (int t = 0; t < HD / 16; ++t) {
+      const f32x4_t o = row[u].o[t];
+      *reinterpret_cast<u32x2_t*>(to + 16 * t) =
+          zero ? u32x2_t{0u, 0u} : u32x2_t{pack2_bf16(o[0] * inv, o[1] * inv), pack2_bf16(o[2] * inv, o[3] * inv)};
+    }
+  }
 }
 
 // ---- the parts of a query put together: a wave a query, lane p holding part p's (m, sum)
