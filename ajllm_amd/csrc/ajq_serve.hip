@@ -105,23 +105,28 @@ SharedPlan shared_plan(const ajqs_shared_attention_args* a) {
   const long long share = a->heads / a->kv_heads, mine = a->tokens * share, all = a->batch / a->groups * mine;
   const long long own_units = (long long)a->batch * a->kv_heads, prefix_units = (long long)a->groups * a->kv_heads;
   const bool bf16 = a->cache_dtype == AJQS_BF16;
-  auto parts = [](long long workgroups, long long rows, long long most) {
-    return (int)std::max(1ll, std::min({512 / workgroups, ceil_div(rows, 128), most}));
+  // parts of at least `least` rows, until there are `wanted` workgroups
+  auto parts = [](long long workgroups, long long wanted, long long rows, long long least, long long most) {
+    return (int)std::max(1ll, std::min({wanted / workgroups, ceil_div(rows, least), most}));
   };
   p.queries = (long long)a->batch * a->heads * a->tokens;
   if (bf16 && mine > 64) {
     p.form = SharedForm::walk;
-    p.own_tiles = (int)ceil_div(mine, 128);
-    p.own_parts = parts(own_units * p.own_tiles, (long long)a->prefix_cap + a->max_len, kMostParts);
+    p.own_rt = a->q_dtype == AJQS_F32 ? 1 : 2;   // (two bf16 for a query component leave no registers for two tiles)
+    p.own_tiles = (int)ceil_div(mine, 64 * p.own_rt);
+    p.own_parts = parts(own_units * p.own_tiles, 512, (long long)a->prefix_cap + a->max_len, 128, kMostParts);
     p.own_blocks = ceil_div(own_units, 8) * 8 * p.own_tiles * p.own_parts;
   } else {
     p.form = bf16 && all > 64 ? SharedForm::many : SharedForm::few;
     p.own_rt = mine > 16 ? 2 : 1;
     p.prefix_rt = all > 16 ? 2 : 1;
+    // tiles of 128 queries, 64 where those times 128 rows are less than two a CU
+    if (p.form == SharedForm::many) p.prefix_rt = prefix_units * ceil_div(all, 128) * ceil_div(a->prefix_cap, 128) < 512 ? 1 : 2;
     p.own_tiles = (int)ceil_div(mine, 16 * p.own_rt);
-    p.prefix_tiles = (int)ceil_div(all, p.form == SharedForm::many ? 128 : 16 * p.prefix_rt);
-    p.own_parts = parts(own_units * p.own_tiles, a->max_len, 16);
-    p.prefix_parts = parts(prefix_units * p.prefix_tiles, a->prefix_cap, kMostParts - 16);
+    p.prefix_tiles = (int)ceil_div(all, (p.form == SharedForm::many ? 64 : 16) * p.prefix_rt);
+    p.prefix_parts = parts(prefix_units * p.prefix_tiles, 256, a->prefix_cap, bf16 || p.prefix_rt > 1 ? 128 : 64, kMostParts - 16);
+    const long long others = std::min(256ll, prefix_units * p.prefix_tiles * p.prefix_parts);
+    p.own_parts = parts(own_units * p.own_tiles, 512 - others, a->max_len, bf16 || p.own_rt > 1 ? 128 : 64, 16);
     p.prefix_blocks = ceil_div(prefix_units * p.prefix_parts, 8) * 8 * p.prefix_tiles;
     p.own_blocks = ceil_div(own_units * p.own_parts, 8) * 8 * p.own_tiles;
   }
@@ -162,6 +167,16 @@ SharedAttention shared_of(const ajqs_shared_attention_args* a, const SharedPlan&
   s.own_parts = p.own_parts;
   s.own_tiles = p.own_tiles;
   s.scale2 = kLog2e / sqrtf((float)a->dim);
+  s.by_share = divide_by(a->heads / a->kv_heads);
+  s.by_each = divide_by((long long)a->tokens * (a->heads / a->kv_heads));
+  s.by_tokens = divide_by(a->tokens);
+  s.by_heads = divide_by(a->heads);
+  s.by_kv_heads = divide_by(a->kv_heads);
+  s.by_group = divide_by(a->batch / a->groups);
+  s.by_prefix_tiles = divide_by(p.prefix_tiles);
+  s.by_prefix_parts = divide_by(p.prefix_parts);
+  s.by_own_tiles = divide_by(p.own_tiles);
+  s.by_own_parts = divide_by(p.own_parts);
   return s;
 }
 
@@ -173,23 +188,25 @@ int merge_parts(const SharedAttention& s, const SharedPlan& p, hipStream_t strea
 }
 template <int HD, typename QT, typename CacheT, int RTP, int RTO>
 int launch_few(const SharedAttention& s, const SharedPlan& p, hipStream_t stream, const char* what) {
-  constexpr int bytes = std::max(few_lds_bytes<HD, CacheT, RTP>(), few_lds_bytes<HD, CacheT, RTO>());
+  constexpr int bytes = std::max(some_lds_bytes<HD, CacheT, RTP>(), some_lds_bytes<HD, CacheT, RTO>());
   auto kernel = shared_attention_few_kernel<HD, QT, CacheT, RTP, RTO>;
   if (int e = allow_lds(kernel, bytes, what)) return e;
   hipLaunchKernelGGL(kernel, dim3((unsigned)(p.prefix_blocks + p.own_blocks)), dim3(256), bytes, stream, s);
   return merge_parts<HD>(s, p, stream, what);
 }
-template <int HD, typename QT, int RTO>
+template <int HD, typename QT, int U, int RTO>
 int launch_many(const SharedAttention& s, const SharedPlan& p, hipStream_t stream, const char* what) {
   constexpr int bytes = std::max(many_lds_bytes<HD>(), few_lds_bytes<HD, uint16_t, RTO>());
-  auto kernel = shared_attention_many_kernel<HD, QT, RTO>;
+  auto kernel = shared_attention_many_kernel<HD, QT, U, RTO>;
   if (int e = allow_lds(kernel, bytes, what)) return e;
   hipLaunchKernelGGL(kernel, dim3((unsigned)(p.prefix_blocks + p.own_blocks)), dim3(256), bytes, stream, s);
   return merge_parts<HD>(s, p, stream, what);
 }
-template <int HD, typename QT>
+template <int HD, typename QT, int U>
 int launch_walk(const SharedAttention& s, const SharedPlan& p, hipStream_t stream, const char* what) {
-  hipLaunchKernelGGL((shared_attention_walk_kernel<HD, QT>), dim3((unsigned)p.own_blocks), dim3(256), many_lds_bytes<HD>(), stream, s);
+  auto kernel = shared_attention_walk_kernel<HD, QT, U>;
+  if (int e = allow_lds(kernel, many_lds_bytes<HD>(), what)) return e;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)p.own_blocks), dim3(256), many_lds_bytes<HD>(), stream, s);
   return p.own_parts > 1 ? merge_parts<HD>(s, p, stream, what) : check_launch(what);
 }
 
@@ -256,11 +273,12 @@ int ajqs_shared_attention(const ajqs_shared_attention_args* a, void* workspace, 
         using CacheT = decltype(cache);
         if constexpr (sizeof(CacheT) == 2) {
           if (p.form == SharedForm::walk) {
-            status = launch_walk<HD, QT>(s, p, (hipStream_t)stream, what);
+            status = launch_walk<HD, QT, sizeof(QT) == 4 ? 1 : 2>(s, p, (hipStream_t)stream, what);
             return;
           }
           if (p.form == SharedForm::many) {
-            const auto launch = p.own_rt == 2 ? launch_many<HD, QT, 2> : launch_many<HD, QT, 1>;
+            const auto launch = p.prefix_rt == 2 ? (p.own_rt == 2 ? launch_many<HD, QT, 2, 2> : launch_many<HD, QT, 2, 1>)
+                                                 : (p.own_rt == 2 ? launch_many<HD, QT, 1, 2> : launch_many<HD, QT, 1, 1>);
             status = launch(s, p, (hipStream_t)stream, what);
             return;
           }

@@ -14,9 +14,28 @@
 // rounded to bf16, whose 2^-9 at most a weight is what the bf16 result's own rounding is.  Everything else is fp32.
 #pragma once
 #include "lane_rows.h"
-#include "prefill_attention.h"  // dma16, the fragment reads, pack8_bf16
+#include <type_traits>
+
+#include "gemm_turns_kernels.h"  // turn_barrier
+#include "prefill_attention.h"   // the fragment reads, pack8_bf16; dma16
 
 namespace ajq {
+
+// Division by a number that the host knows: the product with 2^32 / d rounded down is the quotient or one less for every 32-bit n.  (A division of
+// its own is some forty instructions, at the start of a kernel that runs for a few microseconds a third of its instructions.)
+struct Divide {
+  uint32_t d, m;
+};
+__host__ inline Divide divide_by(long long d) { return Divide{(uint32_t)d, (uint32_t)((d > 1 ? (1ll << 32) / d : 0xFFFFFFFFll))}; }
+__device__ __forceinline__ int divide(int n, const Divide& by, int& rest) {
+  int q = (int)__umulhi((uint32_t)n, by.m);
+  rest = n - q * (int)by.d;
+  if (rest >= (int)by.d) {
+    rest -= (int)by.d;
+    ++q;
+  }
+  return q;
+}
 
 struct SharedAttention {
   const void *q, *prefix_keys, *prefix_values, *keys, *values;
@@ -29,6 +48,8 @@ struct SharedAttention {
   int groups, batch, tokens, heads, kv_heads, prefix_cap, max_len;
   int prefix_blocks, prefix_parts, prefix_tiles, own_parts, own_tiles;
   float scale2;         // log2(e) / sqrt(HD)
+  Divide by_share, by_each, by_tokens, by_heads, by_kv_heads, by_group;   // heads / kv_heads, that times tokens, .., batch / groups
+  Divide by_prefix_tiles, by_prefix_parts, by_own_tiles, by_own_parts;
 };
 
 __device__ __forceinline__ int held(long long n, int most) { return (int)min(max(n, 0ll), (long long)most); }
@@ -39,6 +60,7 @@ template <typename CacheT> struct Meeting {
   int key_head, first_sequence;  // the queries are those of `sequences` sequences from here on and of the key head's heads
   int queries;                   // sequences * tokens * share
   int first;                     // the tile's first query
+  int part, parts, outer;        // part of the rows of sequence or group `outer`
   int begin, end;                // rows
   bool own;
   long long before;              // own rows a sequence's first new token sees ahead of its own row
@@ -46,11 +68,10 @@ template <typename CacheT> struct Meeting {
 
 // query number n of a meeting -> its place in q (and of its partial results), the token
 __device__ __forceinline__ long long query_place(const SharedAttention& a, int key_head, int first_sequence, int n, int& token) {
-  const int share = a.heads / a.kv_heads, each = a.tokens * share;
-  const int sequence = n / each, rest = n - sequence * each;
-  token = rest / share;
-  const int head = key_head * share + (rest - token * share);
-  return ((long long)(first_sequence + sequence) * a.heads + head) * a.tokens + token;
+  int rest, head;
+  const int sequence = divide(n, a.by_each, rest);
+  token = divide(rest, a.by_share, head);
+  return ((long long)(first_sequence + sequence) * a.heads + (key_head * (int)a.by_share.d + head)) * a.tokens + token;
 }
 
 // 8 query components at p as bf16: hi (and lo, what fp32 has beyond it)
@@ -67,12 +88,12 @@ __device__ __forceinline__ void split8(const float* v, u32x4_t& hi, u32x4_t& lo)
   lo = pack8_bf16(rest);
 }
 template <typename T> constexpr int kHalves = sizeof(T) == 4 ? 2 : 1;   // bf16 numbers that stand for one
-__device__ __forceinline__ void load8_halves(const float* p, u32x4_t* to) {
-  const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-  const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+template <typename T> using Raw8 = decltype(load8_raw(static_cast<const T*>(nullptr)));
+__device__ __forceinline__ void to_halves(const Raw8F32& x, u32x4_t* to) {
+  const float v[8] = {x.a.x, x.a.y, x.a.z, x.a.w, x.b.x, x.b.y, x.b.z, x.b.w};
   split8(v, to[0], to[1]);
 }
-__device__ __forceinline__ void load8_halves(const uint16_t* p, u32x4_t* to) { to[0] = *reinterpret_cast<const u32x4_t*>(p); }
+__device__ __forceinline__ void to_halves(const u32x4_t& x, u32x4_t* to) { to[0] = x; }
 
 // The running softmax of 16 queries, one a lane & 15: m, the lane's own part of the sum, and HD / 16 accumulators of O^T.
 template <int HD> struct RunningRow {
@@ -115,18 +136,100 @@ __device__ __forceinline__ void to_probabilities(RunningRow<HD>& row, const f32x
   row.l += sum;
 }
 
+// A launch's workgroups: first the prefix's (a part of a (group, key head)'s rows and a tile of queries each; those that share rows are next
+// to each other on one XCD), then the sequences' own likewise.  What this takes is known without the lengths on the device.
+template <typename CacheT, int HD>
+__device__ __forceinline__ bool find_meeting(const SharedAttention& a, int tile_queries_prefix, int tile_queries_own, Meeting<CacheT>& w) {
+  w.own = (int)blockIdx.x >= a.prefix_blocks;
+  const int id = (int)blockIdx.x - (w.own ? a.prefix_blocks : 0);
+  w.parts = w.own ? a.own_parts : a.prefix_parts;
+  int tile;
+  const int run = (id & 7) + 8 * divide(id >> 3, w.own ? a.by_own_tiles : a.by_prefix_tiles, tile);
+  if (run >= (w.own ? a.batch : a.groups) * a.kv_heads * w.parts) return false;
+  const int unit = divide(run, w.own ? a.by_own_parts : a.by_prefix_parts, w.part);
+  w.outer = divide(unit, a.by_kv_heads, w.key_head);
+  const int each = (int)a.by_group.d;
+  w.first_sequence = w.own ? w.outer : w.outer * each;
+  w.queries = (w.own ? 1 : each) * (int)a.by_each.d;
+  w.first = tile * (w.own ? tile_queries_own : tile_queries_prefix);
+  const size_t at = w.own ? (size_t)w.outer * a.cache_batch + (size_t)w.key_head * a.cache_head
+                          : (size_t)w.outer * a.prefix_group + (size_t)w.key_head * a.prefix_head;
+  w.keys = reinterpret_cast<const CacheT*>(w.own ? a.keys : a.prefix_keys) + at;
+  w.values = reinterpret_cast<const CacheT*>(w.own ? a.values : a.prefix_values) + at;
+  return true;
+}
+// Its rows: a part of whole blocks of 32.
+template <typename CacheT>
+__device__ __forceinline__ void find_rows(const SharedAttention& a, Meeting<CacheT>& w) {
+  int rows;
+  w.before = 0;
+  if (w.own) {
+    w.before = a.rows[w.outer] + (a.offset ? *a.offset : 0ll);
+    rows = held(w.before + (a.counts ? held(a.counts[w.outer], a.tokens) : a.tokens), a.max_len);
+  } else {
+    rows = held(a.prefix_lengths[w.outer], a.prefix_cap);
+  }
+  const int per = ((rows + w.parts - 1) / w.parts + 31) & ~31;
+  w.begin = (int)min((long long)rows, (long long)w.part * per);
+  w.end = min(rows, w.begin + per);
+}
+
 // ---- Few queries: the four waves of a workgroup take blocks of 32 rows in turn, each for itself (no barrier until the end), and RT tiles of 16
 // queries meet every row fetched.  What bounds it is memory: a wave asks for the next block's keys as soon as it has used this block's, and for
 // its values likewise; eight waves a CU (bf16) then have 64 to 128 KB on their way.
 // LDS of a wave: keys, then values, 32 rows each; fp32 rows as two planes of bf16, through registers.
 template <int HD, typename CacheT> constexpr int few_wave_bytes() { return 2 * 32 * 2 * HD * kHalves<CacheT>; }
+template <int HD, int RT> constexpr int few_join_bytes() { return 4 * RT * 16 * (HD + 4) * 4; }
 template <int HD, typename CacheT, int RT> constexpr int few_lds_bytes() {
-  constexpr int walk = 4 * few_wave_bytes<HD, CacheT>(), join = 4 * RT * 16 * HD * 4;
-  return (walk > join ? walk : join) + 4 * RT * 16 * 8;
+  constexpr int walk = 4 * few_wave_bytes<HD, CacheT>(), join = few_join_bytes<HD, RT>() + 4 * RT * 16 * 8;
+  return walk > join ? walk : join;
 }
 
-template <int HD, typename QT, typename CacheT, int RT>
-__device__ __forceinline__ void meet_few(const SharedAttention& a, const Meeting<CacheT>& w, int part, unsigned char* lds, uint32_t lds0) {
+// The four waves' results meet in LDS (rows of HD + 4 numbers: sixteen queries' pieces fall on different banks) and become the workgroup's part.
+// put(u, to): a lane's sums of its query of tile u, to the query's row.
+template <int HD, int RT, int kMl, typename CacheT, typename Put>
+__device__ __forceinline__ void join_waves(const SharedAttention& a, const Meeting<CacheT>& w, unsigned char* lds, const RunningRow<HD> (&row)[RT], Put put) {
+  constexpr int kJoin = RT * 16, kPitch = HD + 4, kHelpers = 256 / kJoin;   // queries, lanes that put one together
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
+  float* sums = reinterpret_cast<float*>(lds);
+  float2* ml = reinterpret_cast<float2*>(lds + kMl);
+  __syncthreads();
+#pragma unroll
+  for (int u = 0; u < RT; ++u) {
+    const float l = quad_sum(row[u].l);
+    if (g == 0) ml[wave * kJoin + 16 * u + r] = float2{row[u].fresh && l == 0.f ? -INFINITY : row[u].m, l};   // (NaN stays)
+    put(u, sums + (wave * kJoin + 16 * u + r) * kPitch);
+  }
+  __syncthreads();
+  const int n = (int)threadIdx.x / kHelpers, d0 = 4 * ((int)threadIdx.x % kHelpers);
+  if (w.first + n >= w.queries) return;
+  float2 e[4];
+  float m = -INFINITY, l = 0.f, weight[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    e[k] = ml[k * kJoin + n];
+    m = fmaxf(m, e[k].x);
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    weight[k] = e[k].x == -INFINITY ? 0.f : exp2_hw(e[k].x - m);
+    l += e[k].y * weight[k];
+  }
+  int unused;
+  const long long place = query_place(a, w.key_head, w.first_sequence, w.first + n, unused) + (w.part + (w.own ? a.prefix_parts : 0)) * a.queries;
+  if (d0 == 0) a.part_ml[place] = float2{m, l};
+#pragma unroll
+  for (int d = 0; d < HD; d += 4 * kHelpers) {
+    if (d + d0 >= HD) break;
+    f32x4_t o = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) o += *reinterpret_cast<const f32x4_t*>(sums + (k * kJoin + n) * kPitch + d + d0) * weight[k];
+    *reinterpret_cast<f32x4_t*>(a.part_sums + place * HD + d + d0) = o;
+  }
+}
+
+template <int HD, typename QT, typename CacheT, int RT, int W = 4>
+__device__ __forceinline__ void meet_few(const SharedAttention& a, Meeting<CacheT>& w, unsigned char* lds, uint32_t lds0) {
   constexpr int RB = 2 * HD, C = HD / 8, KS = HD / 32, TT = HD / 16, KH = kHalves<CacheT>, QH = kHalves<QT>;
   constexpr int kPlane = 32 * RB;                 // 32 rows of bf16
   constexpr bool kDma = KH == 1;
@@ -137,20 +240,22 @@ __device__ __forceinline__ void meet_few(const SharedAttention& a, const Meeting
   const uint32_t mine = lds0 + (uint32_t)(wave * few_wave_bytes<HD, CacheT>());
   unsigned char* mine_p = lds + wave * few_wave_bytes<HD, CacheT>();
 
-  // ---- queries: fragments of RT tiles, and how many of the meeting's rows each sees
-  u32x4_t qf[RT][KS][QH];
-  int limit[RT];
+  // ---- queries: fragments of RT tiles (asked for ahead of the lengths, of which nothing in them depends)
+  Raw8<QT> raw[RT][KS];
+  int token[RT];
 #pragma unroll
   for (int u = 0; u < RT; ++u) {
-    int token;
-    const long long place = query_place(a, w.key_head, w.first_sequence, min(w.first + 16 * u + r, w.queries - 1), token);
-    limit[u] = w.own ? held(w.before + token + 1, w.end) : w.end;
+    const long long place = query_place(a, w.key_head, w.first_sequence, min(w.first + 16 * u + r, w.queries - 1), token[u]);
 #pragma unroll
-    for (int s = 0; s < KS; ++s) load8_halves(reinterpret_cast<const QT*>(a.q) + place * HD + 32 * s + 8 * g, qf[u][s]);
+    for (int s = 0; s < KS; ++s) raw[u][s] = load8_raw(reinterpret_cast<const QT*>(a.q) + place * HD + 32 * s + 8 * g);
   }
+  __builtin_amdgcn_sched_barrier(0);
+  find_rows(a, w);
   RunningRow<HD> row[RT];
+  int limit[RT];   // how many of the meeting's rows a lane's queries see
 #pragma unroll
   for (int u = 0; u < RT; ++u) {
+    limit[u] = w.own ? held(w.before + token[u] + 1, w.end) : w.end;
     row[u].m = row[u].l = 0.f;
     row[u].fresh = true;
 #pragma unroll
@@ -185,12 +290,11 @@ __device__ __forceinline__ void meet_few(const SharedAttention& a, const Meeting
 #pragma unroll
       for (int i = 0; i < kPieces; ++i) {
         const int piece = lane + 64 * i, k = piece / C, c = piece % C;
-        u32x4_t hi, lo;
         auto put = [&](const Raw8F32& x, unsigned char* to) {
-          const float v[8] = {x.a.x, x.a.y, x.a.z, x.a.w, x.b.x, x.b.y, x.b.z, x.b.w};
-          split8(v, hi, lo);
-          *reinterpret_cast<u32x4_t*>(to) = hi;
-          *reinterpret_cast<u32x4_t*>(to + kPlane) = lo;
+          u32x4_t halves[2];
+          to_halves(x, halves);
+          *reinterpret_cast<u32x4_t*>(to) = halves[0];
+          *reinterpret_cast<u32x4_t*>(to + kPlane) = halves[1];
         };
         put(kraw[i], mine_p + k * RB + 16 * (c ^ (k & (C - 1))));
         put(vraw[i], mine_p + 2 * kPlane + k * RB + 16 * ((((c >> 1) ^ (k & (TT - 1))) << 1) | (c & 1)));
@@ -206,6 +310,7 @@ __device__ __forceinline__ void meet_few(const SharedAttention& a, const Meeting
   for (int t = 0; t < TT; ++t) v_rd[t] = values0 + (uint32_t)(vkey * RB + 32 * (t ^ (vkey & (TT - 1))) + 8 * (r & 3));
 
   int at = w.begin + 32 * wave;
+  if (wave >= W) at = w.end;
   if (at < w.end) {
     if constexpr (kDma) {
       ask(w.keys, at, mine, false);
@@ -214,14 +319,19 @@ __device__ __forceinline__ void meet_few(const SharedAttention& a, const Meeting
       fetch(at);
     }
   }
-  for (; at < w.end; at += 128) {
-    const bool more = at + 128 < w.end;
+  u32x4_t qf[RT][KS][QH];
+#pragma unroll
+  for (int u = 0; u < RT; ++u)
+#pragma unroll
+    for (int s = 0; s < KS; ++s) to_halves(raw[u][s], qf[u][s]);
+  for (; at < w.end; at += 32 * W) {
+    const bool more = at + 32 * W < w.end;
     if constexpr (kDma) {
       // (behind this block's keys only its values are on their way)
       asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kAsk) : "memory");
     } else {
       lay_down();
-      if (more) fetch(at + 128);
+      if (more) fetch(at + 32 * W);
       wave_lds_order();
     }
     f32x4_t sc[RT][2];
@@ -245,7 +355,7 @@ __device__ __forceinline__ void meet_few(const SharedAttention& a, const Meeting
     if constexpr (kDma) {
       if (more) {
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        ask(w.keys, at + 128, mine, false);
+        ask(w.keys, at + 32 * W, mine, false);
       }
     }
     u32x4_t pf[RT];
@@ -279,83 +389,160 @@ __device__ __forceinline__ void meet_few(const SharedAttention& a, const Meeting
     if constexpr (kDma) {
       if (more) {
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        ask(w.values, at + 128, values0, true);
+        ask(w.values, at + 32 * W, values0, true);
       }
     } else {
       wave_lds_order();
     }
   }
 
-  // ---- the four waves' results meet in LDS
-  __syncthreads();
-  constexpr int kJoin = RT * 16;   // queries
-  float* sums = reinterpret_cast<float*>(lds);
-  float2* ml = reinterpret_cast<float2*>(lds + few_lds_bytes<HD, CacheT, RT>() - 4 * RT * 16 * 8);
+  join_waves<HD, RT, few_join_bytes<HD, RT>()>(a, w, lds, row, [&](int u, float* to) {
 #pragma unroll
-  for (int u = 0; u < RT; ++u) {
-    const float l = quad_sum(row[u].l);
-    if (g == 0) ml[wave * kJoin + 16 * u + r] = float2{row[u].fresh && l == 0.f ? -INFINITY : row[u].m, l};   // (NaN stays)
-#pragma unroll
-    for (int t = 0; t < TT; ++t)
-      *reinterpret_cast<f32x4_t*>(sums + ((size_t)(wave * kJoin + 16 * u + r)) * HD + 16 * t + 4 * g) = row[u].o[t];
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < kJoin * (HD / 4); i += 256) {
-    const int n = i / (HD / 4), d = 4 * (i % (HD / 4));
-    if (w.first + n >= w.queries) break;   // (n only grows)
-    float2 e[4];
-    float m = -INFINITY;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      e[k] = ml[k * kJoin + n];
-      m = fmaxf(m, e[k].x);
-    }
-    float l = 0.f;
-    f32x4_t o = f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float weight = e[k].x == -INFINITY ? 0.f : exp2_hw(e[k].x - m);
-      l += e[k].y * weight;
-      o += *reinterpret_cast<const f32x4_t*>(sums + (size_t)(k * kJoin + n) * HD + d) * weight;
-    }
-    int token;
-    const long long place = query_place(a, w.key_head, w.first_sequence, w.first + n, token) + part * a.queries;
-    if (d == 0) a.part_ml[place] = float2{m, l};
-    *reinterpret_cast<f32x4_t*>(a.part_sums + place * HD + d) = o;
-  }
+    for (int t = 0; t < TT; ++t) *reinterpret_cast<f32x4_t*>(to + 16 * t + 4 * g) = row[u].o[t];
+  });
 }
 
-// ---- Many queries on bf16 rows: 128 to a workgroup, 32 to each wave, all four walking the same blocks of 64 rows (LDS, two stages, one barrier a
-// block, as attn_prefill_kernel).  Bound by MFMA.  The walk goes over a run of the group's prefix and, behind it, of one sequence's own
-// rows; either may be empty.
-template <typename CacheT> struct Walk {
-  const CacheT *keys[2], *values[2];   // prefix, own
-  int rows[2];                         // of which so many are there
-  int first_block, blocks;             // the walk's part of the blocks of both
-  int key_head, first_sequence, queries, first;
-  long long before;
-};
-template <int HD> constexpr int many_lds_bytes() { return 4 * 64 * 2 * HD; }
-
+// ---- At most 16 queries on fp32 rows, in fp32 throughout (v_mfma_f32_16x16x4_f32: 32 cycles for 16 rows x 4 components, where the memory's share of a CU
+// brings them in more).  Rows go from memory to registers as the products take them; nothing passes LDS.  A wave takes 16 rows at a time.
+//   S^T: lane (g, r) holds components 16 c + 4 g .. + 3 of key r and of query r; step (c, e) multiplies the e-th of each.
+//   O^T: lane (g, r) has the weights of keys 4 g .. 4 g + 3; step i takes key 4 g + i and, of its values, components P r .. P r + P - 1 of every
+//   16 P (P = 4, or 2 where there are 32): tile (v, e) is then components 16 P v + P m + e, m = 0 .. 15.
+__device__ __forceinline__ float4 query4(const float* p) { return *reinterpret_cast<const float4*>(p); }
+__device__ __forceinline__ float4 query4(const uint16_t* p) {
+  const u32x2_t w = *reinterpret_cast<const u32x2_t*>(p);
+  float4 v;
+  widen2(w.x, v.x, v.y);
+  widen2(w.y, v.z, v.w);
+  return v;
+}
+template <int HD> constexpr int few_f32_lds_bytes() { return few_join_bytes<HD, 1>() + 4 * 16 * 8; }
 template <int HD, typename QT>
-__device__ __forceinline__ void meet_many(const SharedAttention& a, const Walk<uint16_t>& w, RunningRow<HD> (&row)[2], uint32_t lds0) {
-  constexpr int RB = 2 * HD, C = HD / 8, KS = HD / 32, TT = HD / 16, QH = kHalves<QT>;
+__device__ __forceinline__ void meet_few_f32(const SharedAttention& a, Meeting<float>& w, unsigned char* lds) {
+  constexpr int KC = HD / 16, P = HD == 32 ? 2 : 4, VC = HD / (16 * P);
+  typedef float part_t __attribute__((ext_vector_type(P)));
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r = lane & 15, g = lane >> 4;
+  int token;
+  const QT* from = reinterpret_cast<const QT*>(a.q) + query_place(a, w.key_head, w.first_sequence, min(w.first + r, w.queries - 1), token) * HD + 4 * g;
+  float4 q[KC];
+#pragma unroll
+  for (int c = 0; c < KC; ++c) q[c] = query4(from + 16 * c);
+  __builtin_amdgcn_sched_barrier(0);
+  find_rows(a, w);
+  const int limit = w.own ? held(w.before + token + 1, w.end) : w.end;
+  RunningRow<HD> row[1];
+  row[0].m = row[0].l = 0.f;
+  row[0].fresh = true;
+#pragma unroll
+  for (int t = 0; t < HD / 16; ++t) row[0].o[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  float4 k[KC];
+  part_t v[4][VC];
+  auto ask = [&](int at) __attribute__((always_inline)) {   // (past the last row: that one again)
+    const float* keys = w.keys + (size_t)min(at + r, w.end - 1) * HD + 4 * g;
+#pragma unroll
+    for (int c = 0; c < KC; ++c) k[c] = *reinterpret_cast<const float4*>(keys + 16 * c);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float* values = w.values + (size_t)min(at + 4 * g + i, w.end - 1) * HD + P * r;
+#pragma unroll
+      for (int c = 0; c < VC; ++c) v[i][c] = *reinterpret_cast<const part_t*>(values + 16 * P * c);
+    }
+  };
+  int at = w.begin + 16 * wave;
+  if (at < w.end) ask(at);
+  for (; at < w.end; at += 64) {
+    f32x4_t even = f32x4_t{0.f, 0.f, 0.f, 0.f}, odd = even;
+#pragma unroll
+    for (int c = 0; c < KC; ++c) {
+      even = __builtin_amdgcn_mfma_f32_16x16x4f32(k[c].x, q[c].x, even, 0, 0, 0);
+      odd = __builtin_amdgcn_mfma_f32_16x16x4f32(k[c].y, q[c].y, odd, 0, 0, 0);
+      even = __builtin_amdgcn_mfma_f32_16x16x4f32(k[c].z, q[c].z, even, 0, 0, 0);
+      odd = __builtin_amdgcn_mfma_f32_16x16x4f32(k[c].w, q[c].w, odd, 0, 0, 0);
+    }
+    f32x4_t sc[1] = {even + odd};
+    part_t values[4][VC];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int c = 0; c < VC; ++c) values[i][c] = v[i][c];
+    if (at + 64 < w.end) ask(at + 64);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (at + 4 * g + i >= limit) sc[0][i] = -INFINITY;
+    float p[4];
+    to_probabilities<HD, 1>(row[0], sc, a.scale2, p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int c = 0; c < VC; ++c)
+#pragma unroll
+        for (int e = 0; e < P; ++e) row[0].o[c * P + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(values[i][c][e], p[i], row[0].o[c * P + e], 0, 0, 0);
+  }
+  // a lane has components 16 P v + P (4 g + i) + e of query r: of each v 4 P of them one behind the other
+  join_waves<HD, 1, few_join_bytes<HD, 1>()>(a, w, lds, row, [&](int, float* to) {
+#pragma unroll
+    for (int c = 0; c < VC; ++c)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        part_t x;
+#pragma unroll
+        for (int e = 0; e < P; ++e) x[e] = row[0].o[c * P + e][i];
+        *reinterpret_cast<part_t*>(to + 16 * P * c + P * (4 * g + i)) = x;
+      }
+  });
+}
+
+// ---- Many queries on bf16 rows: 64 U to a workgroup, 16 U to each wave, all four walking the same blocks of 64 rows (LDS, two stages of a key and a
+// value tile, one barrier a block).  Bound by MFMA.  The walk goes over a run of the group's prefix and, behind it, of one sequence's own
+// rows; either may be empty.  It goes in steps of 32 rows; step t holds the exponents of step t + 1, the softmax of step t and the values of step t - 1
+// times their probabilities, laid out in HD / 16 pieces of either product with their share of the exponentials, in that order for good, so that a
+// wave has MFMAs and vector work to issue side by side (attn_prefill_steps_kernel).
+//
+// Keys of block j + 2 and values of block j + 1 are asked for in the second step of block j.  A prefix that few tiles of queries walk at a time comes from
+// HBM, whose latency is longer than a block: the lines of block j + 4 are touched then as well (four bytes each, into a corner of
+// LDS that nobody reads), so that the requests themselves find them in L2.
+template <typename CacheT> struct Walk {
+  const CacheT *keys[2], *values[2];   // the part's first rows: prefix, own
+  int rows[2];                         // how many there are
+  int key_head, first_sequence, queries, first;
+  long long before;                    // own rows ahead of a sequence's first new token, counted from the part's first own row
+};
+template <int HD> constexpr int many_lds_bytes() { return 4 * 64 * 2 * HD + 4 * 256; }
+
+template <int HD, typename QT, int U>
+__device__ __forceinline__ void meet_many(const SharedAttention& a, const Walk<uint16_t>& w, RunningRow<HD> (&row)[U], uint32_t lds0) {
+  constexpr int RB = 2 * HD, C = HD / 8, KS = HD / 32, TT = HD / 16, QH = kHalves<QT>, kAhead = TT < 3 ? TT : 3;
   constexpr int kTile = 64 * RB;
   constexpr int kReqRows = 1024 / RB;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 15, g = lane >> 4;
-  const int prefix_blocks = (w.rows[0] + 63) >> 6;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    row[u].m = row[u].l = 0.f;
+    row[u].fresh = true;
+#pragma unroll
+    for (int t = 0; t < TT; ++t) row[u].o[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  }
+  const int prefix_blocks = (w.rows[0] + 63) >> 6, blocks = prefix_blocks + ((w.rows[1] + 63) >> 6);
+  if (blocks == 0) return;
 
+  // ---- requests: 1 KiB of rows each; wave w takes rows kReqRows w .. of every group of 4 kReqRows.  Rows past a run's last: that one again.
   const int krow = kReqRows * wave + lane / C, slot = lane % C;
-  const uint32_t k_chunk = (uint32_t)(slot ^ (krow & (C - 1)));
-  const uint32_t v_chunk = (uint32_t)((((slot >> 1) ^ (krow & (TT - 1))) << 1) | (slot & 1));
-  // part i (of KS) of block j: this wave's kReqRows rows of the i-th group of 4 kReqRows
-  auto ask = [&](int j, int i) {
-    const int own = w.first_block + j >= prefix_blocks, kb0 = (w.first_block + j - (own ? prefix_blocks : 0)) * 64;
-    const uint32_t to = lds0 + (uint32_t)((j & 1) * 2 * kTile + (wave + 4 * i) * 1024);
-    const uint32_t at = (uint32_t)(min(4 * kReqRows * i + krow, w.rows[own] - 1 - kb0) * RB);
-    dma16(w.keys[own] + (size_t)kb0 * HD, at + k_chunk * 16u, to);
-    dma16(w.values[own] + (size_t)kb0 * HD, at + v_chunk * 16u, to + (uint32_t)kTile);
+  const uint32_t k_chunk = (uint32_t)(slot ^ (krow & (C - 1))) * 16u;
+  const uint32_t v_chunk = (uint32_t)((((slot >> 1) ^ (krow & (TT - 1))) << 1) | (slot & 1)) * 16u;
+  const uint32_t k_lane = (uint32_t)(krow * RB) + k_chunk, v_lane = (uint32_t)(krow * RB) + v_chunk;
+  auto place = [&](bool values, int i, int stage) __attribute__((always_inline)) {
+    return lds0 + (uint32_t)(stage * 2 * kTile + (values ? kTile : 0) + (wave + 4 * i) * 1024);
+  };
+  auto request = [&](int j, bool values) __attribute__((always_inline)) {
+    const bool own = j >= prefix_blocks;
+    const int at = 64 * (own ? j - prefix_blocks : j), there = own ? w.rows[1] : w.rows[0];
+    const uint16_t* from = (values ? (own ? w.values[1] : w.values[0]) : (own ? w.keys[1] : w.keys[0])) + (size_t)at * HD;
+#pragma unroll
+    for (int i = 0; i < KS; ++i) {
+      const uint32_t k = (uint32_t)min(4 * kReqRows * i + krow, there - 1 - at) * (uint32_t)RB;
+      dma16(from, k + (values ? v_chunk : k_chunk), place(values, i, j & 1));
+    }
   };
   uint32_t k_rd[KS], v_rd[TT];
 #pragma unroll
@@ -364,117 +551,212 @@ __device__ __forceinline__ void meet_many(const SharedAttention& a, const Walk<u
 #pragma unroll
   for (int t = 0; t < TT; ++t) v_rd[t] = lds0 + (uint32_t)(kTile + vkey * RB + 32 * (t ^ (vkey & (TT - 1))) + 8 * (r & 3));
 
+  request(0, false);
+  request(0, true);
+  u32x4_t qf[U][KS][QH];
+  int limit[U];   // own rows that a lane's queries see
 #pragma unroll
-  for (int i = 0; i < KS; ++i) ask(0, i);
-  u32x4_t qf[2][KS][QH];
-  int limit[2], nearest, farthest;   // own rows that a lane's queries see, that the wave's first and last one see
-#pragma unroll
-  for (int u = 0; u < 2; ++u) {
+  for (int u = 0; u < U; ++u) {
     int token;
-    const long long place = query_place(a, w.key_head, w.first_sequence, min(w.first + 32 * wave + 16 * u + r, w.queries - 1), token);
+    const long long at = query_place(a, w.key_head, w.first_sequence, min(w.first + 16 * (U * wave + u) + r, w.queries - 1), token);
     limit[u] = held(w.before + token + 1, w.rows[1]);
 #pragma unroll
-    for (int s = 0; s < KS; ++s) load8_halves(reinterpret_cast<const QT*>(a.q) + place * HD + 32 * s + 8 * g, qf[u][s]);
-    row[u].m = row[u].l = 0.f;
-    row[u].fresh = true;
-#pragma unroll
-    for (int t = 0; t < TT; ++t) row[u].o[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < KS; ++s) to_halves(load8_raw(reinterpret_cast<const QT*>(a.q) + at * HD + 32 * s + 8 * g), qf[u][s]);
   }
-  nearest = __builtin_amdgcn_readlane(limit[0], 0);
-  farthest = __builtin_amdgcn_readlane(limit[1], 63);
-  const bool idle = w.first + 32 * wave >= w.queries;
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int h = 0; h < QH; ++h) asm volatile("" : "+v"(qf[u][s][h]));
+  const int nearest = __builtin_amdgcn_readlane(limit[0], 0), farthest = __builtin_amdgcn_readlane(limit[U - 1], 63);  // of the wave's queries
+  // steps of this wave
+  const int steps = w.first + 16 * U * wave >= w.queries ? 0 : farthest > 0 ? 2 * prefix_blocks + ((farthest + 31) >> 5) : (w.rows[0] + 31) >> 5;
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  __syncthreads();
-  for (int j = 0; j < w.blocks; ++j) {
-    const bool own = w.first_block + j >= prefix_blocks;
-    const int kb0 = (w.first_block + j - (own ? prefix_blocks : 0)) * 64;
-    const bool more = j + 1 < w.blocks;
-    if (idle || (own && kb0 >= farthest)) {
-      if (more) {
+  if (blocks > 1) request(1, false);
+  turn_barrier();
+
+  f32x4_t sn[U][2];  // products of the step ahead
+  u32x4_t pf[U];     // probabilities of the step behind
+  auto key_frag = [&](int at, int i) __attribute__((always_inline)) { return pf_read128(k_rd[i >> 1] + (uint32_t)(at + (i & 1) * 16 * RB)); };
+  auto score = [&](const u32x4_t& kf, int i) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < KS; ++i) ask(j + 1, i);
+    for (int h = 0; h < QH; ++h)
+#pragma unroll
+      for (int u = 0; u < U; ++u) sn[u][i & 1] = mfma16(kf, qf[u][i >> 1][h], i < 2 && h == 0 ? f32x4_t{0.f, 0.f, 0.f, 0.f} : sn[u][i & 1]);
+  };
+  // Step t: products from the keys at k_at, values at v_at (kV: not in the very first), and req(piece)
+  auto step = [&](int t, auto values, auto masked, int k_at, int v_at, auto req) __attribute__((always_inline)) {
+    constexpr bool kV = decltype(values)::value;
+    f32x4_t sc[U][2];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int jb = 0; jb < 2; ++jb) sc[u][jb] = sn[u][jb];
+    u32x4_t kf[TT];
+    u32x2_t vl[TT], vh[TT];
+    auto fetch = [&](int i) __attribute__((always_inline)) {
+      kf[i] = key_frag(k_at, i);
+      if (kV) {
+        vl[i] = pf_read_tr(v_rd[i] + (uint32_t)v_at);
+        vh[i] = pf_read_tr(v_rd[i] + (uint32_t)(v_at + 16 * RB));
       }
-    } else {
-      f32x4_t sc[2][4];
-      u32x4_t ka[4];
+    };
 #pragma unroll
-      for (int jb = 0; jb < 4; ++jb) ka[jb] = pf_read128(k_rd[0] + (uint32_t)(jb * 16 * RB));
+    for (int i = 0; i < kAhead; ++i) fetch(i);
+    if (decltype(masked)::value) {
+      const bool own = (t >> 1) >= prefix_blocks;
+      const int at = 32 * (t - (own ? 2 * prefix_blocks : 0));
+      if (at + 32 > (own ? nearest : w.rows[0])) {
 #pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        u32x4_t kn[4];
-        if (s < KS - 1) {
+        for (int u = 0; u < U; ++u) {
+          const int last = (own ? limit[u] : w.rows[0]) - at - 4 * g;
 #pragma unroll
-          for (int jb = 0; jb < 4; ++jb) kn[jb] = pf_read128(k_rd[s + 1] + (uint32_t)(jb * 16 * RB));
-        }
-#pragma unroll
-        for (int qh = 0; qh < QH; ++qh)
-#pragma unroll
-          for (int jb = 0; jb < 4; ++jb)
-#pragma unroll
-            for (int u = 0; u < 2; ++u) sc[u][jb] = mfma16(ka[jb], qf[u][s][qh], s + qh == 0 ? f32x4_t{0.f, 0.f, 0.f, 0.f} : sc[u][jb]);
-        if (more) ask(j + 1, s);
-        if (s < KS - 1) {
-#pragma unroll
-          for (int jb = 0; jb < 4; ++jb) ka[jb] = kn[jb];
-        }
-      }
-      const int seen = own ? nearest : w.rows[0];
-      if (kb0 + 64 > seen) {
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const int last = own ? limit[u] : w.rows[0];
-#pragma unroll
-          for (int jb = 0; jb < 4; ++jb)
+          for (int jb = 0; jb < 2; ++jb)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-              if (kb0 + 16 * jb + 4 * g + i >= last) sc[u][jb][i] = -INFINITY;
-        }
-      }
-      u32x4_t pf[2][2];
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        float p[16];
-        to_probabilities<HD, 4>(row[u], sc[u], a.scale2, p);
-        pf[u][0] = pack8_bf16(&p[0]);
-        pf[u][1] = pack8_bf16(&p[8]);
-      }
-      constexpr int kRing = TT < 8 ? TT : 8;
-      auto v_lo = [&](int i) { return pf_read_tr(v_rd[i % TT] + (uint32_t)((i / TT) * 32 * RB)); };
-      auto v_hi = [&](int i) { return pf_read_tr(v_rd[i % TT] + (uint32_t)((i / TT) * 32 * RB + 16 * RB)); };
-      u32x2_t vlo[kRing], vhi[kRing];
-#pragma unroll
-      for (int i = 0; i < kRing; ++i) {
-        vlo[i] = v_lo(i);
-        vhi[i] = v_hi(i);
-      }
-#pragma unroll
-      for (int i = 0; i < 2 * TT; ++i) {
-        const u32x4_t vf = {vlo[i % kRing].x, vlo[i % kRing].y, vhi[i % kRing].x, vhi[i % kRing].y};
-#pragma unroll
-        for (int u = 0; u < 2; ++u) row[u].o[i % TT] = mfma16(vf, pf[u][i / TT], row[u].o[i % TT]);
-        if (i + kRing < 2 * TT) {
-          vlo[i % kRing] = v_lo(i + kRing);
-          vhi[i % kRing] = v_hi(i + kRing);
+              if (16 * jb + i >= last) sc[u][jb][i] = -INFINITY;
         }
       }
     }
+    u32x4_t pn[U];
+    float p[U][8], psum[U] = {};
+    constexpr int kPer = 8 * U / TT;  // exponentials of a piece
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int s = 0; s < KS; ++s) k_rd[s] ^= (uint32_t)(2 * kTile);
+    for (int i = 0; i < TT; ++i) {
+      if (i + kAhead < TT) fetch(i + kAhead);
+      req(i);
+      score(kf[i], i);
 #pragma unroll
-    for (int t = 0; t < TT; ++t) v_rd[t] ^= (uint32_t)(2 * kTile);
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
+      for (int x = 0; x < kPer; ++x) {
+        const int u = (i * kPer + x) >> 3, e = (i * kPer + x) & 7;
+        p[u][e] = exp2_hw(__builtin_fmaf(sc[u][e >> 2][e & 3], a.scale2, -row[u].m));
+        psum[u] += p[u][e];
+      }
+      if (U * (i + 1) % TT == 0) {  // a group of rows is through (pinned: the compiler would sink it behind the branches below)
+        const int u = U * i / TT;
+        pn[u] = pack8_bf16(p[u]);
+        asm volatile("" : "+v"(pn[u]), "+v"(psum[u]));
+      }
+      if (kV) {
+        const u32x4_t vf = {vl[i].x, vl[i].y, vh[i].x, vh[i].y};
+#pragma unroll
+        for (int u = 0; u < U; ++u) row[u].o[i] = mfma16(vf, pf[u], row[u].o[i]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (__builtin_amdgcn_ballot_w64(row[u].fresh || psum[u] > kPfTrigger) != 0) {
+        float x[8], mx = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          x[e] = __builtin_fmaf(sc[u][e >> 2][e & 3], a.scale2, -row[u].m);
+          mx = fmaxf(mx, x[e]);
+        }
+        mx = quad_max(mx);
+        const bool move = row[u].fresh ? mx > -INFINITY : mx > kPfSlack;
+        const float shift = move ? mx : 0.f;
+        const float corr = move && !row[u].fresh ? exp2_hw(-shift) : 1.0f;
+        psum[u] = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          p[u][e] = exp2_hw(x[e] - shift);
+          psum[u] += p[u][e];
+        }
+        pn[u] = pack8_bf16(p[u]);
+        row[u].m += shift;
+        row[u].fresh = row[u].fresh && !move;
+        row[u].l *= corr;
+        if (kV) {
+#pragma unroll
+          for (int tt = 0; tt < TT; ++tt) row[u].o[tt] *= corr;
+        }
+      }
+      row[u].l += psum[u];
+      pf[u] = pn[u];
+    }
+  };
+  auto last_values = [&](int v_at) __attribute__((always_inline)) {
+    u32x2_t vl[TT], vh[TT];
+#pragma unroll
+    for (int i = 0; i < TT; ++i) {
+      vl[i] = pf_read_tr(v_rd[i] + (uint32_t)v_at);
+      vh[i] = pf_read_tr(v_rd[i] + (uint32_t)(v_at + 16 * RB));
+    }
+#pragma unroll
+    for (int i = 0; i < TT; ++i) {
+      const u32x4_t vf = {vl[i].x, vl[i].y, vh[i].x, vh[i].y};
+#pragma unroll
+      for (int u = 0; u < U; ++u) row[u].o[i] = mfma16(vf, pf[u], row[u].o[i]);
+    }
+  };
+  constexpr std::integral_constant<bool, true> yes{};
+  constexpr std::integral_constant<bool, false> no{};
+  auto none = [](int) {};
+  if (steps > 0) {
+    u32x4_t kf[TT];
+#pragma unroll
+    for (int i = 0; i < TT; ++i) kf[i] = key_frag(0, i);
+#pragma unroll
+    for (int i = 0; i < TT; ++i) score(kf[i], i);
+    step(0, no, yes, 32 * RB, 0, none);
   }
+  // The prefix's blocks j (even) and j + 1 at places known to the compiler: the second step of j, both of j + 1, the first of j + 2, while what they ask for and
+  // multiply is whole blocks.
+  int j = 0;
+  const int whole = w.rows[0] >> 6;
+  const char* k_from = reinterpret_cast<const char*>(w.keys[0]) + 2 * kTile;
+  const char* v_from = reinterpret_cast<const char*>(w.values[0]) + kTile;
+  if (2 * j + 5 < steps && j + 4 <= whole) {
+    // lines: of the keys waves 0 and 1, of the values 2 and 3, of block j + 4 (of the last whole one, at most)
+    const uint32_t corner = lds0 + (uint32_t)(4 * kTile + 256 * wave);
+    const uint32_t line = (uint32_t)((64 * (wave & 1) + lane) * (RB / 2));
+    const char* lines = reinterpret_cast<const char*>(wave < 2 ? w.keys[0] : w.values[0]);
+    auto touch = [&](int block) __attribute__((always_inline)) { dma4(lines + (size_t)min(block, whole - 1) * kTile, line, corner); };
+    touch(4);
+    do {
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        asm volatile("s_waitcnt vmcnt(1)" ::: "memory");   // (all but the touch)
+        turn_barrier();
+        step(2 * j + 2 * x + 1, yes, no, (x ^ 1) * 2 * kTile, x * 2 * kTile, [&](int i) __attribute__((always_inline)) {
+          if (i < KS) dma16(k_from + i * 4096, k_lane, place(false, i, x));
+          else dma16(v_from + (i - KS) * 4096, v_lane, place(true, i - KS, x ^ 1));
+          if (i == TT - 1) touch(j + x + 5);
+        });
+        k_from += kTile;
+        v_from += kTile;
+        step(2 * j + 2 * x + 2, yes, no, (x ^ 1) * 2 * kTile + 32 * RB, x * 2 * kTile + 32 * RB, none);
+      }
+      j += 2;
+    } while (2 * j + 5 < steps && j + 4 <= whole);
+  }
+  for (int t = 2 * j + 1; t < 2 * blocks; ++t) {
+    const int block = t >> 1;
+    if (t & 1) {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      turn_barrier();
+      if (block + 2 < blocks) request(block + 2, false);
+      if (block + 1 < blocks) request(block + 1, true);
+    }
+    auto half = [&](int n) { return ((n >> 1) & 1) * 2 * kTile + (n & 1) * 32 * RB; };  // where step n's keys (values) lie
+    // (the last step's products of the one behind it are of no use, whatever lies there)
+    if (t < steps) step(t, yes, yes, half(t + 1), half(t - 1), none);
+    else if (t == steps) last_values(half(t - 1));
+  }
+  if (steps == 2 * blocks) last_values(((blocks - 1) & 1) * 2 * kTile + 32 * RB);
 }
 
 // a lane's queries of meet_many as partial results
-template <int HD>
-__device__ __forceinline__ void leave_part(const SharedAttention& a, const Walk<uint16_t>& w, const RunningRow<HD> (&row)[2], int part) {
+template <int HD, int U>
+__device__ __forceinline__ void leave_part(const SharedAttention& a, const Walk<uint16_t>& w, const RunningRow<HD> (&row)[U], int part) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
 #pragma unroll
-  for (int u = 0; u < 2; ++u) {
+  for (int u = 0; u < U; ++u) {
     const float l = quad_sum(row[u].l);
-    const int n = w.first + 32 * wave + 16 * u + r;
+    const int n = w.first + 16 * (U * wave + u) + r;
     if (n >= w.queries) continue;
     int token;
     const long long place = query_place(a, w.key_head, w.first_sequence, n, token) + part * a.queries;
@@ -484,154 +766,102 @@ __device__ __forceinline__ void leave_part(const SharedAttention& a, const Walk<
   }
 }
 
-// A launch's workgroups: first the prefix's (a part of a (group, key head)'s rows and a tile of queries each; those that share rows are next
-// to each other on one XCD), then the sequences' own likewise.
-template <typename CacheT, int HD>
-__device__ __forceinline__ bool find_meeting(const SharedAttention& a, int tile_queries_prefix, int tile_queries_own, Meeting<CacheT>& w, int& part) {
-  const int share = a.heads / a.kv_heads;
-  w.own = (int)blockIdx.x >= a.prefix_blocks;
-  const int id = (int)blockIdx.x - (w.own ? a.prefix_blocks : 0);
-  const int tiles = w.own ? a.own_tiles : a.prefix_tiles, parts = w.own ? a.own_parts : a.prefix_parts;
-  const int runs = (w.own ? a.batch : a.groups) * a.kv_heads * parts;      // of rows
-  const int run = (id & 7) + 8 * (id / (8 * tiles)), tile = (id >> 3) % tiles;
-  if (run >= runs) return false;
-  part = run % parts;
-  const int unit = run / parts;
-  w.key_head = unit % a.kv_heads;
-  const int outer = unit / a.kv_heads, each = a.batch / a.groups;
-  const long long off = a.offset ? *a.offset : 0ll;
-  int there = a.tokens, rows;
-  if (w.own) {
-    w.first_sequence = outer;
-    w.queries = a.tokens * share;
-    w.before = a.rows[outer] + off;
-    if (a.counts) there = held(a.counts[outer], a.tokens);
-    rows = held(w.before + there, a.max_len);
-    const size_t at = (size_t)outer * a.cache_batch + (size_t)w.key_head * a.cache_head;
-    w.keys = reinterpret_cast<const CacheT*>(a.keys) + at;
-    w.values = reinterpret_cast<const CacheT*>(a.values) + at;
-  } else {
-    w.first_sequence = outer * each;
-    w.queries = each * a.tokens * share;
-    w.before = 0;
-    rows = held(a.prefix_lengths[outer], a.prefix_cap);
-    const size_t at = (size_t)outer * a.prefix_group + (size_t)w.key_head * a.prefix_head;
-    w.keys = reinterpret_cast<const CacheT*>(a.prefix_keys) + at;
-    w.values = reinterpret_cast<const CacheT*>(a.prefix_values) + at;
-  }
-  w.first = tile * (w.own ? tile_queries_own : tile_queries_prefix);
-  // parts of whole blocks of 32 rows
-  const int per = ((rows + parts - 1) / parts + 31) & ~31;
-  w.begin = (int)min((long long)rows, (long long)part * per);
-  w.end = min(rows, w.begin + per);
-  if (w.own) part += a.prefix_parts;
-  return true;
+template <int HD, typename QT, typename CacheT, int RT>
+__device__ __forceinline__ void meet_some(const SharedAttention& a, Meeting<CacheT>& w, unsigned char* lds, uint32_t lds0) {
+  if constexpr (sizeof(CacheT) == 4 && RT == 1) meet_few_f32<HD, QT>(a, w, lds);
+  else meet_few<HD, QT, CacheT, RT>(a, w, lds, lds0);
 }
-
+template <int HD, typename CacheT, int RT> constexpr int some_lds_bytes() {
+  return sizeof(CacheT) == 4 && RT == 1 ? few_f32_lds_bytes<HD>() : few_lds_bytes<HD, CacheT, RT>();
+}
 template <int HD, typename QT, typename CacheT, int RTP, int RTO>
-__global__ __launch_bounds__(256, sizeof(CacheT) == 4 ? 1 : 2) void shared_attention_few_kernel(SharedAttention a) {
+__global__ __launch_bounds__(256, sizeof(CacheT) == 4 && RTP == 2 ? 1 : 2) void shared_attention_few_kernel(SharedAttention a) {
   extern __shared__ __attribute__((aligned(1024))) unsigned char shared_lds[];
   const uint32_t lds0 = (uint32_t)(uintptr_t)(pf_lds_char_t*)shared_lds;
   Meeting<CacheT> w;
-  int part;
-  if (!find_meeting<CacheT, HD>(a, 16 * RTP, 16 * RTO, w, part)) return;
-  if (RTP == RTO || !w.own) meet_few<HD, QT, CacheT, RTP>(a, w, part, shared_lds, lds0);
-  else meet_few<HD, QT, CacheT, RTO>(a, w, part, shared_lds, lds0);
+  if (!find_meeting<CacheT, HD>(a, 16 * RTP, 16 * RTO, w)) return;
+  if (RTP == RTO || !w.own) meet_some<HD, QT, CacheT, RTP>(a, w, shared_lds, lds0);
+  else meet_some<HD, QT, CacheT, RTO>(a, w, shared_lds, lds0);
 }
 
 // The prefix by meet_many, the sequences' own rows by meet_few.
-template <int HD, typename QT, int RTO>
+template <int HD, typename QT, int U, int RTO>
 __global__ __launch_bounds__(256, 2) void shared_attention_many_kernel(SharedAttention a) {
   extern __shared__ __attribute__((aligned(1024))) unsigned char shared_lds[];
   const uint32_t lds0 = (uint32_t)(uintptr_t)(pf_lds_char_t*)shared_lds;
   Meeting<uint16_t> w;
-  int part;
-  if (!find_meeting<uint16_t, HD>(a, 128, 16 * RTO, w, part)) return;
+  if (!find_meeting<uint16_t, HD>(a, 64 * U, 16 * RTO, w)) return;
   if (w.own) {
-    meet_few<HD, QT, uint16_t, RTO>(a, w, part, shared_lds, lds0);
+    meet_few<HD, QT, uint16_t, RTO, U == 2 ? 2 : 4>(a, w, shared_lds, lds0);
     return;
   }
+  find_rows(a, w);
   Walk<uint16_t> walk;
   walk.keys[0] = w.keys + (size_t)w.begin * HD;
   walk.values[0] = w.values + (size_t)w.begin * HD;
   walk.keys[1] = walk.values[1] = nullptr;
   walk.rows[0] = w.end - w.begin;
   walk.rows[1] = 0;
-  walk.first_block = 0;
-  walk.blocks = (walk.rows[0] + 63) >> 6;
   walk.key_head = w.key_head;
   walk.first_sequence = w.first_sequence;
   walk.queries = w.queries;
   walk.first = w.first;
   walk.before = 0;
-  RunningRow<HD> row[2];
-  if (walk.blocks > 0) {
-    meet_many<HD, QT>(a, walk, row, lds0);
-  } else {
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      row[u].m = row[u].l = 0.f;
-      row[u].fresh = true;
-#pragma unroll
-      for (int t = 0; t < HD / 16; ++t) row[u].o[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    }
-  }
-  leave_part<HD>(a, walk, row, part);
+  RunningRow<HD> row[U];
+  meet_many<HD, QT, U>(a, walk, row, lds0);
+  leave_part<HD, U>(a, walk, row, w.part);
 }
 
 // Sequences with many new tokens each: 128 queries of one sequence walk the prefix and then its own rows, and what comes out is the result.  With
 // own_parts > 1 the walk is cut up and leaves parts for the merge.
-template <int HD, typename QT>
+template <int HD, typename QT, int U>
 __global__ __launch_bounds__(256, 2) void shared_attention_walk_kernel(SharedAttention a) {
   extern __shared__ __attribute__((aligned(1024))) unsigned char shared_lds[];
   const uint32_t lds0 = (uint32_t)(uintptr_t)(pf_lds_char_t*)shared_lds;
-  const int share = a.heads / a.kv_heads, parts = a.own_parts, tiles = a.own_tiles;
-  const int id = (int)blockIdx.x, run = (id & 7) + 8 * (id / (8 * tiles * parts)), rest = (id >> 3) % (tiles * parts);
+  const int share = (int)a.by_share.d, parts = a.own_parts;
+  int part, hk, unused, tile;
+  const int id = (int)blockIdx.x, run = (id & 7) + 8 * divide(divide(id >> 3, a.by_own_parts, part), a.by_own_tiles, tile);
   if (run >= a.batch * a.kv_heads) return;
-  const int tile = tiles - 1 - rest / parts, part = rest % parts;
-  const int b = run / a.kv_heads, hk = run % a.kv_heads, group = b / (a.batch / a.groups);
+  tile = a.own_tiles - 1 - tile;
+  const int b = divide(run, a.by_kv_heads, hk), group = divide(b, a.by_group, unused);
   Walk<uint16_t> w;
   w.key_head = hk;
   w.first_sequence = b;
   w.queries = a.tokens * share;
-  w.first = 128 * tile;
+  w.first = 64 * U * tile;
   w.before = a.rows[b] + (a.offset ? *a.offset : 0ll);
   const int there = a.counts ? held(a.counts[b], a.tokens) : a.tokens;
-  const int last = min((w.first + 127) / share, there - 1);          // the tile's last token that is there
+  const int last = min(divide(w.first + 64 * U - 1, a.by_share, unused), there - 1);          // the tile's last token that is there
   const size_t at = (size_t)group * a.prefix_group + (size_t)hk * a.prefix_head, own = (size_t)b * a.cache_batch + (size_t)hk * a.cache_head;
-  w.keys[0] = reinterpret_cast<const uint16_t*>(a.prefix_keys) + at;
-  w.values[0] = reinterpret_cast<const uint16_t*>(a.prefix_values) + at;
-  w.keys[1] = reinterpret_cast<const uint16_t*>(a.keys) + own;
-  w.values[1] = reinterpret_cast<const uint16_t*>(a.values) + own;
   const bool none = w.first >= there * share;
-  w.rows[0] = none ? 0 : held(a.prefix_lengths[group], a.prefix_cap);
-  w.rows[1] = none ? 0 : held(w.before + last + 1, a.max_len);
-  const int blocks = ((w.rows[0] + 63) >> 6) + ((w.rows[1] + 63) >> 6), per = (blocks + parts - 1) / parts;
-  w.first_block = min(blocks, part * per);
-  w.blocks = min(blocks - w.first_block, per);
-  RunningRow<HD> row[2];
-  if (w.blocks > 0) {
-    meet_many<HD, QT>(a, w, row, lds0);
-  } else {
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      row[u].m = row[u].l = 0.f;
-      row[u].fresh = true;
-#pragma unroll
-      for (int t = 0; t < HD / 16; ++t) row[u].o[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    }
-  }
+  const int prefix_rows = none ? 0 : held(a.prefix_lengths[group], a.prefix_cap), own_rows = none ? 0 : held(w.before + last + 1, a.max_len);
+  // this part's blocks: first .. first + many - 1 of the prefix's and the sequence's own
+  const int prefix_blocks = (prefix_rows + 63) >> 6, blocks = prefix_blocks + ((own_rows + 63) >> 6), per = (blocks + parts - 1) / parts;
+  const int first = min(blocks, part * per), many = min(blocks - first, per);
+  const int skip = min(first, prefix_blocks), own_skip = first - skip, of_prefix = min(many, prefix_blocks - skip);
+  w.keys[0] = reinterpret_cast<const uint16_t*>(a.prefix_keys) + at + (size_t)skip * 64 * HD;
+  w.values[0] = reinterpret_cast<const uint16_t*>(a.prefix_values) + at + (size_t)skip * 64 * HD;
+  w.keys[1] = reinterpret_cast<const uint16_t*>(a.keys) + own + (size_t)own_skip * 64 * HD;
+  w.values[1] = reinterpret_cast<const uint16_t*>(a.values) + own + (size_t)own_skip * 64 * HD;
+  w.rows[0] = min(prefix_rows - skip * 64, of_prefix * 64);
+  w.rows[0] = max(w.rows[0], 0);
+  w.rows[1] = max(min(own_rows - own_skip * 64, (many - of_prefix) * 64), 0);
+  w.before -= (long long)own_skip * 64;
+  RunningRow<HD> row[U];
+  meet_many<HD, QT, U>(a, w, row, lds0);
   if (parts > 1) {
-    leave_part<HD>(a, w, row, part);
+    leave_part<HD, U>(a, w, row, part);
     return;
   }
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
 #pragma unroll
-  for (int u = 0; u < 2; ++u) {
+  for (int u = 0; u < U; ++u) {
     const float l = quad_sum(row[u].l);
-    const int n = w.first + 32 * wave + 16 * u + r;
+    const int n = w.first + 16 * (U * wave + u) + r;
     if (n >= w.queries) continue;
-    const int token = n / share, head = hk * share + (n - token * share);
+    int head;
+    const int token = divide(n, a.by_share, head);
+    head += hk * share;
     const float inv = token < there && (l > 0.f || l != l) ? 1.0f / l : 0.f;
     const bool zero = inv == 0.f;
     uint16_t* to = a.out + (((size_t)b * a.tokens + token) * a.heads + head) * HD + 4 * g;
@@ -644,34 +874,61 @@ __global__ __launch_bounds__(256, 2) void shared_attention_walk_kernel(SharedAtt
   }
 }
 
-// ---- the parts of a query put together: a wave a query, lane p holding part p's (m, sum)
+// ---- the parts of a query put together: a wave a query, lane p holding part p's (m, sum).  The first kFirst parts' sums are asked for beside them.
+__device__ __forceinline__ float wave_max(float v) {
+  v = quad_max(v);   // over lanes l, l ^ 16, l ^ 32, l ^ 48
+  v = fmaxf(v, row_ror<8>(v));
+  v = fmaxf(v, row_ror<4>(v));
+  v = fmaxf(v, row_ror<2>(v));
+  return fmaxf(v, row_ror<1>(v));
+}
 template <int HD>
 __global__ __launch_bounds__(256) void shared_attention_merge_kernel(SharedAttention a) {
+  constexpr int kEach = HD == 128 ? 2 : 1, kLanes = HD / kEach, kFirst = 8;   // components of a lane, lanes that hold some
   const long long place = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (place >= a.queries) return;
   const int lane = threadIdx.x & 63, parts = a.prefix_parts + a.own_parts;
-  const int t = (int)(place % a.tokens), h = (int)(place / a.tokens % a.heads), b = (int)(place / a.tokens / a.heads);
   const float2 ml = a.part_ml[min(lane, parts - 1) * a.queries + place];
-  constexpr int kLanes = HD / 2;                   // that hold two components
-  const int dl = min(lane, kLanes - 1);
+  const float* from = a.part_sums + place * HD + kEach * min(lane, kLanes - 1);
+  const size_t apart = (size_t)a.queries * HD;
+  float x[kFirst][kEach];
+  auto ask = [&](int first) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < kFirst; ++i) {
+      const float* at = from + min(first + i, parts - 1) * apart;
+      if constexpr (kEach == 2) {
+        const float2 v = *reinterpret_cast<const float2*>(at);
+        x[i][0] = v.x;
+        x[i][kEach - 1] = v.y;
+      } else {
+        x[i][0] = *at;
+      }
+    }
+  };
+  ask(0);
+  int t, h;
+  const int b = divide(divide((int)place, a.by_tokens, t), a.by_heads, h);
   const bool there = a.counts == nullptr || t < a.counts[b];
   const float mine = lane < parts && there ? ml.x : -INFINITY;
-  float top = mine;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) top = fmaxf(top, __shfl_xor(top, off));
+  const float top = wave_max(mine);
   const float weight = mine == -INFINITY ? 0.f : exp2_hw(mine - top);
-  const float l = wave_sum(lane < parts && weight != 0.f ? ml.y * weight : 0.f);
-  float2 o = float2{0.f, 0.f};
-#pragma unroll 8
-  for (int p = 0; p < parts; ++p) {
-    const float c = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(weight), p));
-    const float2 x = *reinterpret_cast<const float2*>(a.part_sums + (p * a.queries + place) * HD + 2 * dl);
-    o.x += x.x * c;
-    o.y += x.y * c;
+  const float l = wave_sum(weight != 0.f ? ml.y * weight : 0.f);
+  float o[kEach] = {};
+  for (int first = 0; first < parts; first += kFirst) {
+    if (first > 0) ask(first);
+#pragma unroll
+    for (int i = 0; i < kFirst; ++i) {
+      // (a lane behind the parts weighs nothing)
+      const float c = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(weight), first + i));
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) o[e] += x[i][e] * c;
+    }
   }
   if (lane >= kLanes) return;
-  const uint32_t to = l > 0.f || l != l ? pack2_bf16(o.x / l, o.y / l) : 0u;
-  reinterpret_cast<uint32_t*>(a.out + (((size_t)b * a.tokens + t) * a.heads + h) * HD)[lane] = to;
+  const bool some = l > 0.f || l != l;
+  uint16_t* to = a.out + (((size_t)b * a.tokens + t) * a.heads + h) * HD + kEach * lane;
+  if constexpr (kEach == 2) *reinterpret_cast<uint32_t*>(to) = some ? pack2_bf16(o[0] / l, o[kEach - 1] / l) : 0u;
+  else *to = some ? f32_to_bf16_rne(o[0] / l) : (uint16_t)0;
 }
 
 }  // namespace ajq
