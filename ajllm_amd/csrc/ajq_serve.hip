@@ -317,20 +317,35 @@ int ajqs_adjust_logits(const ajqs_adjust_logits_args* a, void* stream) {
     return fail(AJQ_ERR_SHAPE, "%s: %d masks for %d rows", what, a->masks, a->batch);
   if (!aligned4(a->out) || !aligned4(a->allowed) || (a->dtype == AJQS_F32 && !aligned4(a->logits)) || (reinterpret_cast<uintptr_t>(a->logits) & 1u))
     return fail(AJQ_ERR_ALIGN, "%s: logits, out and the masks must be aligned to their elements", what);
-  const int slice = 8192;
-  AdjustLogits n{a->logits, a->out, int64s(a->tokens), int64s(a->token_counts), int64s(a->prompt), int64s(a->prompt_counts), a->repetition,
-                 a->frequency, a->presence, int64s(a->bias_ids), a->bias, a->allowed, int64s(a->allowed_rows), a->ld, a->out_ld, a->tokens_ld,
-                 a->prompt_ld, a->bias_ld, a->allowed_ld, a->vocab, a->max_tokens, a->max_prompt, a->bias_ids ? a->biases : 0, a->masks,
-                 a->token_count_stride, a->prompt_count_stride, slice};
-  const long long slices = ((long long)a->vocab + slice - 1) / slice;
-  if (slices > 65535) return fail(AJQ_ERR_SHAPE, "%s: vocabulary of %d", what, a->vocab);
-  const bool words = (a->tokens && a->max_tokens) || (a->prompt && a->max_prompt) || n.biases;
+  const bool words = (a->tokens && a->max_tokens) || (a->prompt && a->max_prompt) || (a->bias_ids && a->biases);
+  // slices of 16384 tokens (two workgroups of 1024 lanes a CU then), smaller ones until there are two workgroups a CU
+  int slice = 4 * kSliceThreads * kSlicePieces;
+  while (slice > 1024 && (long long)a->batch * ceil_div(a->vocab, slice) < 512) slice /= 2;
+  const int threads = std::min(slice / 4, std::max(256, slice / (4 * kSlicePieces))), slices = (int)ceil_div(a->vocab, slice);
+  const long long blocks = ceil_div(a->batch, 8) * 8 * slices;
+  if (blocks > 0x7FFFFFFFLL) return fail(AJQ_ERR_SHAPE, "%s: %d rows of %d", what, a->batch, a->vocab);
+  const AdjustLogits n{a->logits, a->out, a->max_tokens ? int64s(a->tokens) : nullptr, int64s(a->token_counts), a->max_prompt ? int64s(a->prompt) : nullptr, int64s(a->prompt_counts),
+                       a->repetition, a->frequency, a->presence, int64s(a->bias_ids), a->bias, a->allowed, int64s(a->allowed_rows), a->ld, a->out_ld, a->tokens_ld,
+                       a->prompt_ld, a->bias_ld, a->allowed_ld, a->vocab, a->max_tokens, a->max_prompt, a->bias_ids ? a->biases : 0, a->masks,
+                       a->token_count_stride, a->prompt_count_stride, a->batch, slice, slices};
+  int status = AJQ_OK;
   with_type(a->dtype, [&](auto type) {
-    if (words)
-      hipLaunchKernelGGL((adjust_logits_kernel<decltype(type), true>), dim3(a->batch, (unsigned)slices), dim3(1024), slice * 4, (hipStream_t)stream, n);
-    else
-      hipLaunchKernelGGL((adjust_logits_kernel<decltype(type), false>), dim3(a->batch, (unsigned)slices), dim3(1024), 0, (hipStream_t)stream, n);
+    using T = decltype(type);
+    auto launch = [&](auto with_words, auto in_place) {
+      auto kernel = adjust_logits_kernel<T, decltype(with_words)::value, decltype(in_place)::value>;
+      const int bytes = decltype(with_words)::value ? slice * 4 : 0;
+      if ((status = allow_lds(kernel, bytes, what)) == AJQ_OK)
+        hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(threads), bytes, (hipStream_t)stream, n);
+    };
+    const std::integral_constant<bool, true> yes;
+    const std::integral_constant<bool, false> no;
+    auto for_words = [&](auto in_place) { words ? launch(yes, in_place) : launch(no, in_place); };
+    if constexpr (sizeof(T) == 4) {
+      if (a->logits == a->out) return for_words(yes);
+    }
+    for_words(no);
   });
+  if (status) return status;
   return check_launch(what);
 }
 

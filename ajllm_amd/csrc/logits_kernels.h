@@ -1,10 +1,12 @@
 // Logits ahead of the choice of a token: penalties for tokens that a row holds already, biases, masks of allowed tokens.
 //
-// A workgroup takes a slice of one row's vocabulary.  It keeps a word per token of the slice in LDS,
+// A workgroup takes a slice of one row's vocabulary.  It asks for its logits, then keeps a word per token of the slice in LDS,
 //   bits 0 .. 19  how often the token is among the row's tokens,   bit 20  whether it is in the prompt,   bits 21 .. 31  its bias slot + 1,
-// fills them from the row's lists (whole numbers: no result depends on the order of the atomics), then walks the slice once.
+// fills them from the row's lists (whole numbers: no result depends on the order of the atomics) while the logits are on their way, and
+// puts both together, four tokens a lane at a time.  What bounds it is memory: a row is read and written once; its lists are read by
+// every slice, from L2 (slices of a row run next to each other on one XCD).
 #pragma once
-#include "ajq_common.h"
+#include "lane_rows.h"
 
 namespace ajq {
 
@@ -22,86 +24,192 @@ struct AdjustLogits {
   const long long* allowed_rows;
   long long ld, out_ld, tokens_ld, prompt_ld, bias_ld, allowed_ld;
   int vocab, max_tokens, max_prompt, biases, masks, token_count_stride, prompt_count_stride;
-  int slice;
+  int batch, slice, slices;
 };
 
-__device__ __forceinline__ float logit_of(const float* p) { return *p; }
-__device__ __forceinline__ float logit_of(const uint16_t* p) { return __uint_as_float((uint32_t)*p << 16); }
+constexpr int kSliceThreads = 1024, kSlicePieces = 4;   // lanes, and pieces of four tokens a lane: slices of up to 16384 tokens
 
-// Grid (rows, slices); `words` are a.slice words of LDS (none where the row has neither lists nor biases: kWords false).
-template <typename T, bool kWords>
-__global__ __launch_bounds__(1024) void adjust_logits_kernel(AdjustLogits a) {
+// Four logits by one load, wherever they lie (rows of an odd vocabulary begin anywhere; the hardware takes any address); fewer at a row's end.
+__device__ __forceinline__ void load_logits(const float* p, int there, float (&x)[4]) {
+  if (there >= 4) {
+    __builtin_memcpy(x, p, 16);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = i < there ? p[i] : 0.f;
+  }
+}
+__device__ __forceinline__ void load_logits(const uint16_t* p, int there, float (&x)[4]) {
+  u32x2_t v = u32x2_t{0u, 0u};
+  if (there >= 4) {
+    __builtin_memcpy(&v, p, 8);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 3; ++i)
+      if (i < there) v[i >> 1] |= (uint32_t)p[i] << (16 * (i & 1));
+  }
+  widen2(v.x, x[0], x[1]);
+  widen2(v.y, x[2], x[3]);
+}
+__device__ __forceinline__ void store_logits(float* p, int there, const float (&x)[4]) {
+  if (there >= 4) {
+    __builtin_memcpy(p, x, 16);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < there) p[i] = x[i];
+  }
+}
+// fn(id) for the first n of a list of `most`.  The first ids are asked for before n is known (ask), four a lane.
+struct Ids {
+  static constexpr int kAtOnce = 4;
+  long long id[kAtOnce];
+};
+__device__ __forceinline__ void ask_ids(const long long* ids, int first, int most, Ids& got) {
+#pragma unroll
+  for (int i = 0; i < Ids::kAtOnce; ++i) got.id[i] = ids[min(first + i * (int)blockDim.x, most - 1)];
+}
+template <typename F>
+__device__ __forceinline__ void each_id(const long long* ids, int n, Ids& got, F&& fn) {
+  for (int first = threadIdx.x;;) {
+#pragma unroll
+    for (int i = 0; i < Ids::kAtOnce; ++i)
+      if (first + i * (int)blockDim.x < n) fn(got.id[i]);
+    first += Ids::kAtOnce * (int)blockDim.x;
+    if (first >= n) break;
+    ask_ids(ids, first, n, got);
+  }
+}
+
+// kWords: rows have lists or biases (a.slice words of LDS); kInPlace: logits are the results, and only what changes is read and written.
+template <typename T, bool kWords, bool kInPlace>
+__global__ __launch_bounds__(kSliceThreads, 8) void adjust_logits_kernel(AdjustLogits a) {
   extern __shared__ __attribute__((aligned(16))) uint32_t words[];
   __shared__ float sums[kWords ? kMaxBiases : 1];
   __shared__ int bias_at[kWords ? kMaxBiases : 1];
-  const int b = blockIdx.x, t = threadIdx.x, threads = blockDim.x;
-  const int base = blockIdx.y * a.slice, count = min(a.slice, a.vocab - base);
-  if (kWords) {
-    for (int i = t; i < count; i += threads) words[i] = 0u;
-    __syncthreads();
-    auto held = [&](const long long* counts, int stride, int most) {
-      return counts ? (int)min(max(counts[(size_t)b * stride], 0ll), (long long)most) : most;
-    };
-    if (a.tokens) {
-      const int n = held(a.token_counts, a.token_count_stride, a.max_tokens);
-      for (int i = t; i < n; i += threads) {
-        const long long at = a.tokens[(size_t)b * a.tokens_ld + i] - base;
-        if (at >= 0 && at < count) atomicAdd(&words[at], 1u);
-      }
+  __shared__ int again;   // whether a token is biased twice
+  const int t = threadIdx.x, threads = blockDim.x;
+  const int turn = (int)(blockIdx.x >> 3) / a.slices;
+  const int b = 8 * turn + (int)(blockIdx.x & 7), base = ((int)(blockIdx.x >> 3) - turn * a.slices) * a.slice;
+  if (b >= a.batch) return;
+  const int count = min(a.slice, a.vocab - base);
+  const T* row = reinterpret_cast<const T*>(a.logits) + (size_t)b * a.ld + base;
+  float x[kSlicePieces][4];
+  if (!kInPlace) {
+#pragma unroll
+    for (int i = 0; i < kSlicePieces; ++i) {
+      const int at = 4 * (t + i * threads);
+      if (at < count) load_logits(row + at, count - at, x[i]);
     }
-    if (a.prompt) {
-      const int n = held(a.prompt_counts, a.prompt_count_stride, a.max_prompt);
-      for (int i = t; i < n; i += threads) {
-        const long long at = a.prompt[(size_t)b * a.prompt_ld + i] - base;
-        if (at >= 0 && at < count) atomicOr(&words[at], kInPrompt);
-      }
-    }
-    for (int i = t; i < a.biases; i += threads) {
-      const long long at = a.bias_ids[(size_t)b * a.bias_ld + i] - base;
-      bias_at[i] = at >= 0 && at < count ? (int)at : -1;
-      sums[i] = a.bias[(size_t)b * a.bias_ld + i];
-    }
-    __syncthreads();
-    // the first of a token's entries takes the sum of all of them, in their order
-    float mine = 0.f;
-    bool first = false;
-    if (t < a.biases && bias_at[t] >= 0) {
-      first = true;
-      for (int j = 0; j < a.biases; ++j) {
-        if (bias_at[j] != bias_at[t]) continue;
-        if (j < t) first = false;
-        mine += sums[j];
-      }
-    }
-    __syncthreads();
-    if (first) {
-      sums[t] = mine;
-      atomicOr(&words[bias_at[t]], (uint32_t)(t + 1) << 21);
-    }
-    __syncthreads();
   }
-  const float repeat = a.repetition ? a.repetition[b] : 1.f, frequency = a.frequency ? a.frequency[b] : 0.f,
-              presence = a.presence ? a.presence[b] : 0.f;
+  const long long *tokens = nullptr, *prompt = nullptr, *bias_ids = nullptr;
+  const float* bias = nullptr;
+  Ids mine, given;
+  long long bias_id = -1;
+  float bias_by = 0.f;
+  if (kWords) {
+    if (a.tokens) ask_ids(tokens = a.tokens + (size_t)b * a.tokens_ld, t, a.max_tokens, mine);
+    if (a.prompt) ask_ids(prompt = a.prompt + (size_t)b * a.prompt_ld, t, a.max_prompt, given);
+    if (a.biases) {
+      bias_ids = a.bias_ids + (size_t)b * a.bias_ld;
+      bias = a.bias + (size_t)b * a.bias_ld;
+      bias_id = bias_ids[min(t, a.biases - 1)];
+      bias_by = bias[min(t, a.biases - 1)];
+    }
+  }
   const uint32_t* mask = nullptr;
   if (a.allowed) {
     const long long which = a.allowed_rows ? a.allowed_rows[b] : (long long)b;
     if (which >= 0 && which < a.masks) mask = a.allowed + which * a.allowed_ld;
   }
-  const T* row = reinterpret_cast<const T*>(a.logits) + (size_t)b * a.ld + base;
-  float* to = a.out + (size_t)b * a.out_ld + base;
-  for (int i = t; i < count; i += threads) {
-    float x = logit_of(row + i);
-    if (kWords) {
-      const uint32_t w = words[i];
-      if (w) {
-        const uint32_t n = w & (kInPrompt - 1);
-        if (w & (kInPrompt | (kInPrompt - 1))) x = x > 0.f ? x / repeat : x * repeat;
-        if (n) x -= frequency * (float)n + presence;
-        if (w >> 21) x += sums[(w >> 21) - 1];
+  uint32_t allowed[kSlicePieces];
+#pragma unroll
+  for (int i = 0; i < kSlicePieces; ++i) {
+    const int at = 4 * (t + i * threads);
+    allowed[i] = mask && at < count ? mask[(base + at) >> 5] >> (at & 31) : 15u;   // (slices begin on boundaries of 32)
+  }
+  const float repeat = a.repetition ? a.repetition[b] : 1.f, frequency = a.frequency ? a.frequency[b] : 0.f,
+              presence = a.presence ? a.presence[b] : 0.f;
+  if (kWords) {
+    for (int i = 4 * t; i < a.slice; i += 4 * threads) *reinterpret_cast<u32x4_t*>(words + i) = u32x4_t{0u, 0u, 0u, 0u};
+    if (t == 0) again = 0;
+    __syncthreads();
+    auto held = [&](const long long* counts, int stride, int most) {
+      return counts ? (int)min(max(counts[(size_t)b * stride], 0ll), (long long)most) : most;
+    };
+    if (tokens)
+      each_id(tokens, held(a.token_counts, a.token_count_stride, a.max_tokens), mine, [&](long long id) {
+        const long long at = id - base;
+        if (at >= 0 && at < count) atomicAdd(&words[at], 1u);
+      });
+    if (prompt)
+      each_id(prompt, held(a.prompt_counts, a.prompt_count_stride, a.max_prompt), given, [&](long long id) {
+        const long long at = id - base;
+        if (at >= 0 && at < count) atomicOr(&words[at], kInPrompt);
+      });
+    __syncthreads();
+    if (a.biases) {
+      // a token's slot is that of its first entry, which takes the sum of all of them, in their order.  (Slot kMaxBiases - i for entry i: the largest is the
+      // first.  The low bits are settled by now.)
+      for (int i = t; i < a.biases; i += threads) {
+        const long long at = (i == t ? bias_id : bias_ids[i]) - base;
+        const bool here = at >= 0 && at < count;
+        bias_at[i] = here ? (int)at : -1;
+        sums[i] = i == t ? bias_by : bias[i];
+        if (here) atomicMax(&words[at], (words[at] & ((1u << 21) - 1)) | ((uint32_t)(kMaxBiases - i) << 21));
+      }
+      __syncthreads();
+      for (int i = t; i < a.biases; i += threads)
+        if (bias_at[i] >= 0 && words[bias_at[i]] >> 21 != (uint32_t)(kMaxBiases - i)) again = 1;
+      __syncthreads();
+      if (again) {
+        for (int first = 0; first < a.biases; first += threads) {
+          const int i = first + t;
+          const bool take = i < a.biases && bias_at[i] >= 0 && words[bias_at[i]] >> 21 == (uint32_t)(kMaxBiases - i);
+          float sum = 0.f;
+          if (take) {
+            for (int j = i; j < a.biases; ++j)
+              if (bias_at[j] == bias_at[i]) sum += sums[j];
+          }
+          __syncthreads();
+          if (take) sums[i] = sum;   // (no entry of a later round reads it)
+          __syncthreads();
+        }
       }
     }
-    if (mask && !((mask[(base + i) >> 5] >> ((base + i) & 31)) & 1u)) x = -INFINITY;
-    to[i] = x;
+  }
+  float* to = a.out + (size_t)b * a.out_ld + base;
+#pragma unroll
+  for (int i = 0; i < kSlicePieces; ++i) {
+    const int at = 4 * (t + i * threads);
+    if (at >= count) break;
+    u32x4_t w = u32x4_t{0u, 0u, 0u, 0u};
+    if (kWords) w = *reinterpret_cast<const u32x4_t*>(words + at);
+    if (kInPlace) {
+      if (!(w.x | w.y | w.z | w.w) && (allowed[i] & 15u) == 15u) continue;
+      load_logits(row + at, count - at, x[i]);
+    }
+    if (kWords) {
+      // (few of a wave's tokens have a word: one after the other, a lane its next one)
+      uint32_t todo = (w.x != 0u ? 1u : 0u) | (w.y != 0u ? 2u : 0u) | (w.z != 0u ? 4u : 0u) | (w.w != 0u ? 8u : 0u);
+      while (todo) {
+        const bool second = (todo & 1u) == 0u, upper = (todo & 3u) == 0u, last = (todo & 7u) == 0u;
+        const uint32_t word = upper ? (last ? w.w : w.z) : (second ? w.y : w.x);
+        float v = upper ? (last ? x[i][3] : x[i][2]) : (second ? x[i][1] : x[i][0]);
+        const uint32_t n = word & (kInPrompt - 1);
+        if (word & (kInPrompt | (kInPrompt - 1))) v = v > 0.f ? v / repeat : v * repeat;
+        if (n) v -= frequency * (float)n + presence;
+        if (word >> 21) v += sums[kMaxBiases - (word >> 21)];
+        x[i][0] = !second ? v : x[i][0];
+        x[i][1] = second && !upper ? v : x[i][1];
+        x[i][2] = upper && !last ? v : x[i][2];
+        x[i][3] = last ? v : x[i][3];
+        todo &= todo - 1;
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (!((allowed[i] >> e) & 1u)) x[i][e] = -INFINITY;
+    store_logits(to + at, count - at, x[i]);
   }
 }
 
