@@ -30,33 +30,26 @@ struct AdjustLogits {
 constexpr int kSliceThreads = 1024, kSlicePieces = 4;   // lanes, and pieces of four tokens a lane: slices of up to 16384 tokens
 
 // Four logits by one load, wherever they lie (rows of an odd vocabulary begin anywhere; the hardware takes any address); fewer at a row's end.
-__device__ __forceinline__ void load_logits(const float* p, int there, float (&x)[4]) {
-  if (there >= 4) {
-    __builtin_memcpy(x, p, 16);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = i < there ? p[i] : 0.f;
-  }
+// A row goes past L2, which the lists are read from.
+typedef float f32x4u_t __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t u32x2u_t __attribute__((ext_vector_type(2), aligned(2)));
+__device__ __forceinline__ f32x4_t load_logits(const float* p, int there) {
+  if (there >= 4) return __builtin_nontemporal_load(reinterpret_cast<const f32x4u_t*>(p));
+  return f32x4_t{p[0], there > 1 ? p[1] : 0.f, there > 2 ? p[2] : 0.f, 0.f};
 }
-__device__ __forceinline__ void load_logits(const uint16_t* p, int there, float (&x)[4]) {
-  u32x2_t v = u32x2_t{0u, 0u};
-  if (there >= 4) {
-    __builtin_memcpy(&v, p, 8);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 3; ++i)
-      if (i < there) v[i >> 1] |= (uint32_t)p[i] << (16 * (i & 1));
-  }
-  widen2(v.x, x[0], x[1]);
-  widen2(v.y, x[2], x[3]);
+__device__ __forceinline__ f32x4_t load_logits(const uint16_t* p, int there) {
+  u32x2_t v;
+  if (there >= 4) v = __builtin_nontemporal_load(reinterpret_cast<const u32x2u_t*>(p));
+  else v = u32x2_t{p[0] | (there > 1 ? (uint32_t)p[1] << 16 : 0u), there > 2 ? p[2] : 0u};
+  return f32x4_t{__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xFFFF0000u), __uint_as_float(v.y << 16), __uint_as_float(v.y & 0xFFFF0000u)};
 }
-__device__ __forceinline__ void store_logits(float* p, int there, const float (&x)[4]) {
+__device__ __forceinline__ void store_logits(float* p, int there, f32x4_t x) {
   if (there >= 4) {
-    __builtin_memcpy(p, x, 16);
+    __builtin_nontemporal_store(x, reinterpret_cast<f32x4u_t*>(p));
   } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (i < there) p[i] = x[i];
+    p[0] = x[0];
+    if (there > 1) p[1] = x[1];
+    if (there > 2) p[2] = x[2];
   }
 }
 // fn(id) for the first n of a list of `most`.  The first ids are asked for before n is known (ask), four a lane.
@@ -93,12 +86,12 @@ __global__ __launch_bounds__(kSliceThreads, 8) void adjust_logits_kernel(AdjustL
   if (b >= a.batch) return;
   const int count = min(a.slice, a.vocab - base);
   const T* row = reinterpret_cast<const T*>(a.logits) + (size_t)b * a.ld + base;
-  float x[kSlicePieces][4];
+  f32x4_t x[kSlicePieces] = {};
   if (!kInPlace) {
 #pragma unroll
     for (int i = 0; i < kSlicePieces; ++i) {
       const int at = 4 * (t + i * threads);
-      if (at < count) load_logits(row + at, count - at, x[i]);
+      x[i] = at < count ? load_logits(row + at, count - at) : f32x4_t{0.f, 0.f, 0.f, 0.f};
     }
   }
   const long long *tokens = nullptr, *prompt = nullptr, *bias_ids = nullptr;
@@ -181,35 +174,36 @@ __global__ __launch_bounds__(kSliceThreads, 8) void adjust_logits_kernel(AdjustL
 #pragma unroll
   for (int i = 0; i < kSlicePieces; ++i) {
     const int at = 4 * (t + i * threads);
-    if (at >= count) break;
-    u32x4_t w = u32x4_t{0u, 0u, 0u, 0u};
-    if (kWords) w = *reinterpret_cast<const u32x4_t*>(words + at);
-    if (kInPlace) {
-      if (!(w.x | w.y | w.z | w.w) && (allowed[i] & 15u) == 15u) continue;
-      load_logits(row + at, count - at, x[i]);
-    }
-    if (kWords) {
-      // (few of a wave's tokens have a word: one after the other, a lane its next one)
-      uint32_t todo = (w.x != 0u ? 1u : 0u) | (w.y != 0u ? 2u : 0u) | (w.z != 0u ? 4u : 0u) | (w.w != 0u ? 8u : 0u);
-      while (todo) {
-        const bool second = (todo & 1u) == 0u, upper = (todo & 3u) == 0u, last = (todo & 7u) == 0u;
-        const uint32_t word = upper ? (last ? w.w : w.z) : (second ? w.y : w.x);
-        float v = upper ? (last ? x[i][3] : x[i][2]) : (second ? x[i][1] : x[i][0]);
-        const uint32_t n = word & (kInPrompt - 1);
-        if (word & (kInPrompt | (kInPrompt - 1))) v = v > 0.f ? v / repeat : v * repeat;
-        if (n) v -= frequency * (float)n + presence;
-        if (word >> 21) v += sums[kMaxBiases - (word >> 21)];
-        x[i][0] = !second ? v : x[i][0];
-        x[i][1] = second && !upper ? v : x[i][1];
-        x[i][2] = upper && !last ? v : x[i][2];
-        x[i][3] = last ? v : x[i][3];
-        todo &= todo - 1;
+    if (at < count) {
+      u32x4_t w = u32x4_t{0u, 0u, 0u, 0u};
+      if (kWords) w = *reinterpret_cast<const u32x4_t*>(words + at);
+      const bool changed = (w.x | w.y | w.z | w.w) != 0u || (allowed[i] & 15u) != 15u;
+      f32x4_t v = x[i];
+      if (kInPlace && changed) v = load_logits(row + at, count - at);
+      if (kWords) {
+        // (few of a wave's tokens have a word: one after the other, a lane its next one)
+        uint32_t todo = (w.x != 0u ? 1u : 0u) | (w.y != 0u ? 2u : 0u) | (w.z != 0u ? 4u : 0u) | (w.w != 0u ? 8u : 0u);
+        while (todo) {
+          const bool second = (todo & 1u) == 0u, upper = (todo & 3u) == 0u, last = (todo & 7u) == 0u;
+          const uint32_t word = upper ? (last ? w.w : w.z) : (second ? w.y : w.x);
+          float y = upper ? (last ? v.w : v.z) : (second ? v.y : v.x);
+          const uint32_t n = word & (kInPrompt - 1);
+          if (word & (kInPrompt | (kInPrompt - 1))) y = y > 0.f ? y / repeat : y * repeat;
+          if (n) y -= frequency * (float)n + presence;
+          if (word >> 21) y += sums[kMaxBiases - (word >> 21)];
+          v.x = second ? v.x : y;
+          v.y = second && !upper ? y : v.y;
+          v.z = upper && !last ? y : v.z;
+          v.w = last ? y : v.w;
+          todo &= todo - 1;
+        }
       }
+      v.x = allowed[i] & 1u ? v.x : -INFINITY;
+      v.y = allowed[i] & 2u ? v.y : -INFINITY;
+      v.z = allowed[i] & 4u ? v.z : -INFINITY;
+      v.w = allowed[i] & 8u ? v.w : -INFINITY;
+      if (!kInPlace || changed) store_logits(to + at, count - at, v);
     }
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (!((allowed[i] >> e) & 1u)) x[i][e] = -INFINITY;
-    store_logits(to + at, count - at, x[i]);
   }
 }
 
