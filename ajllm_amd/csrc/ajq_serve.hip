@@ -237,15 +237,24 @@ int ajqs_norm_rope(const ajqs_norm_rope_args* a, void* stream) {
     return fail(AJQ_ERR_SHAPE, "%s: cache heads that overlap cannot be written", what);
   const NormRope n{a->qkv, a->cosine, a->sine, a->q_gain, a->k_gain, int64s(a->rows), int64s(a->positions), int64s(a->counts),
                    int64s(a->offset), a->keys, a->values, a->q, a->ld, a->cache_batch, a->cache_head, a->tokens, a->heads, a->kv_heads,
-                   a->max_len, a->table_rows, a->eps};
+                   a->max_len, a->table_rows, a->eps, divide_by(a->tokens)};
   with_dim(a->dim, [&](auto dim) {
     with_type(a->in_dtype, [&](auto in) {
       with_type(a->q_dtype, [&](auto q) {
         with_type(a->cache_dtype, [&](auto cache) {
-          constexpr int U = 1;
-          const dim3 grid((unsigned)(a->batch * a->tokens), (unsigned)((all + 16 * U - 1) / (16 * U)));
-          hipLaunchKernelGGL((norm_rope_kernel<decltype(in), decltype(q), decltype(cache), decltype(dim)::value, U>), grid, dim3(256), 0,
-                             (hipStream_t)stream, n);
+          auto launch = [&](auto each, auto many) {
+            constexpr int U = decltype(each)::value;
+            const dim3 grid((unsigned)(a->batch * a->tokens), (unsigned)ceil_div(all, 16 * U));
+            hipLaunchKernelGGL((norm_rope_kernel<decltype(in), decltype(q), decltype(cache), decltype(dim)::value, U, decltype(many)::value>), grid,
+                               dim3(256), 0, (hipStream_t)stream, n);
+          };
+          const std::integral_constant<bool, true> yes;
+          const std::integral_constant<bool, false> no;
+          // one head a team until there are workgroups enough, then as many as a token has for its sixteen teams
+          const bool full = (long long)a->batch * a->tokens >= 1024;
+          if (a->tokens == 1) full && all > 16 ? launch(Size<2>{}, no) : launch(Size<1>{}, no);
+          else if (!full || all <= 16) launch(Size<1>{}, yes);
+          else all <= 32 || all > 48 ? launch(Size<2>{}, yes) : launch(Size<3>{}, yes);
         });
       });
     });

@@ -1,4 +1,4 @@
-// Rows of a key / value cache dealt to teams of sixteen lanes.
+// Rows of a key / value cache dealt to teams of sixteen lanes, and what else small kernels share.
 #pragma once
 #include "ajq_common.h"
 
@@ -122,6 +122,22 @@ __device__ __forceinline__ void store_lane(uint16_t* p, const KvRow<HD / 16>& r)
     *reinterpret_cast<u32x2_t*>(p) = u32x2_t{pack2_bf16(r.v[0], r.v[1]), pack2_bf16(r.v[2], r.v[3])};
     if constexpr (LD::DPL == 8) *reinterpret_cast<u32x2_t*>(p + LD::second) = u32x2_t{pack2_bf16(r.v[4], r.v[5]), pack2_bf16(r.v[6], r.v[7])};
   }
+}
+
+// Division by a number that the host knows: the product with 2^32 / d rounded down is the quotient or one less for every 32-bit n.  (A division of
+// its own is some forty instructions, at the start of a kernel that runs for a few microseconds a third of its instructions.)
+struct Divide {
+  uint32_t d, m;
+};
+__host__ inline Divide divide_by(long long d) { return Divide{(uint32_t)d, (uint32_t)((d > 1 ? (1ll << 32) / d : 0xFFFFFFFFll))}; }
+__device__ __forceinline__ int divide(int n, const Divide& by, int& rest) {
+  int q = (int)__umulhi((uint32_t)n, by.m);
+  rest = n - q * (int)by.d;
+  if (rest >= (int)by.d) {
+    rest -= (int)by.d;
+    ++q;
+  }
+  return q;
 }
 
 }  // namespace ajq

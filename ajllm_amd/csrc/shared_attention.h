@@ -21,22 +21,6 @@
 
 namespace ajq {
 
-// Division by a number that the host knows: the product with 2^32 / d rounded down is the quotient or one less for every 32-bit n.  (A division of
-// its own is some forty instructions, at the start of a kernel that runs for a few microseconds a third of its instructions.)
-struct Divide {
-  uint32_t d, m;
-};
-__host__ inline Divide divide_by(long long d) { return Divide{(uint32_t)d, (uint32_t)((d > 1 ? (1ll << 32) / d : 0xFFFFFFFFll))}; }
-__device__ __forceinline__ int divide(int n, const Divide& by, int& rest) {
-  int q = (int)__umulhi((uint32_t)n, by.m);
-  rest = n - q * (int)by.d;
-  if (rest >= (int)by.d) {
-    rest -= (int)by.d;
-    ++q;
-  }
-  return q;
-}
-
 struct SharedAttention {
   const void *q, *prefix_keys, *prefix_values, *keys, *values;
   const long long *prefix_lengths, *rows, *counts, *offset;
