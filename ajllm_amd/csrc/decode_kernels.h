@@ -801,7 +801,9 @@ __global__ __launch_bounds__(1024) void sample_pick_kernel(const float* __restri
     __syncthreads();
   }
   // ---- the token inside the block, the same way: thread i holds token 1024 block + i
-  {
+  if (m == -INFINITY) {   // a row that allows nothing: the first token, as in greedy_pick_kernel (its weights are no numbers)
+    if (t == 0) chosen = 0;
+  } else {
     const int j = (sh_block << 10) + t;
     unsigned long long mine = 0ull;
     if (j < V) {
