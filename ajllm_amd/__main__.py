@@ -21,6 +21,9 @@ def main(argv: list[str] | None = None) -> int:
     gen.add_argument("--temperature", type=float, default=0.0, help="0: the most probable token")
     gen.add_argument("--top-p", type=float, default=None)
     gen.add_argument("--seed", type=int, default=0)
+    gen.add_argument("--repetition-penalty", type=float, default=1.0, help="divides the positive logits of tokens that are there already")
+    gen.add_argument("--frequency-penalty", type=float, default=0.0, help="off a token's logit for each time it has been produced")
+    gen.add_argument("--presence-penalty", type=float, default=0.0, help="off the logit of a token that has been produced")
     gen.add_argument("--eos", type=int, default=None, help="stop once every prompt has produced this id")
     args = ap.parse_args(argv)
     prompts = [[int(t) for t in text.split(",")] for text in args.tokens]
@@ -37,6 +40,8 @@ def main(argv: list[str] | None = None) -> int:
     decoder = decoding.decoder_for(model)(model, len(prompts), len(prompts[0]) + args.max_new_tokens)
     if args.temperature > 0:
         decoder.set_sampling(args.temperature, args.top_p, args.seed)
+    if args.repetition_penalty != 1.0 or args.frequency_penalty or args.presence_penalty:
+        decoder.set_penalties(args.repetition_penalty, args.frequency_penalty, args.presence_penalty)
     decoder.prefill(torch.tensor(prompts))
     for row in decoder.generate(args.max_new_tokens, args.eos).tolist():
         print(",".join(str(t) for t in row))

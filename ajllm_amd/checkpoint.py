@@ -52,6 +52,7 @@ def model_config(model: modeling.TransformerLM) -> dict[str, Any]:
         "norm_placement": first.norm_placement,
         "feed_forward": "swiglu" if isinstance(first.feed_forward, modeling.SwiGLU) else "silu",
         "tie_embeddings": model.tie_embeddings,
+        **({"head_norm": True} if first.attention.q_norm is not None else {}),
     }
 
 

@@ -15,8 +15,9 @@ import ctypes
 import torch
 
 from . import _lib, dense, modeling
-from .attention import prefill_attention
+from .attention import norm_rope, prefill_attention, shared_prefix_attention
 from .quant import QuantLinear, repack_w4, repack_w8, w4a16_matmul, w8a16_matmul
+from .sampling import adjust_logits
 
 
 class GraphDecoder:
@@ -47,6 +48,10 @@ class GraphDecoder:
         self.temperature = 0.0
         self.top_p: float | None = None
         self.uniforms: torch.Tensor | None = None
+        # what ``set_penalties`` asks for (``sampling.adjust_logits``' arguments), and the prompts it may count
+        self.adjustments: dict[str, torch.Tensor] = {}
+        self.prompt_ids = torch.full((batch, max_len), -1, dtype=torch.long, device=device)
+        self.prompt_count = torch.zeros(1, dtype=torch.long, device=device)
 
     def set_sampling(self, temperature: float, top_p: float | None = None, seed: int = 0) -> None:
         """Choose tokens as the reference's ``sample_next_token`` does (src/ajllm/generation/sampling.py:8-22):
@@ -62,8 +67,52 @@ class GraphDecoder:
         if self.temperature > 0:
             generator = torch.Generator(device=self.device).manual_seed(int(seed))
             self.uniforms = torch.rand((self.max_len, self.batch), generator=generator, device=self.device)
+        self._drop_graphs()
+
+    def _drop_graphs(self) -> None:
         self.graph = self.graph_many = None
         self.graph_many_steps = 0
+
+    def set_penalties(self, repetition: float = 1.0, frequency: float = 0.0, presence: float = 0.0,
+                      bias: dict[int, float] | None = None, allowed: torch.Tensor | None = None,
+                      allowed_rows: torch.Tensor | None = None) -> None:
+        """What happens to the logits ahead of every choice (``sampling.adjust_logits``): ``repetition`` for tokens of the prompt and of what has been
+        produced, ``frequency`` and ``presence`` for the latter's, ``bias`` for tokens of its own, and masks of allowed tokens (bit v % 32 of word
+        v // 32; int32 ``[masks, words]``, row b's mask ``allowed_rows[b]`` or, without it, the b-th).  The masks are read where they are: a program that
+        follows a grammar writes the next ones into ``allowed`` or ``allowed_rows`` between calls of ``generate``.  Call it before ``prefill``; graphs
+        recorded so far are dropped.  Without arguments nothing happens to the logits any more."""
+        if not repetition > 0:
+            raise ValueError("repetition must be positive")
+        if allowed_rows is not None and allowed is None:
+            raise ValueError("allowed_rows without allowed")
+        if bias and not all(0 <= v < self.model.vocab_size for v in bias):
+            raise ValueError(f"biased tokens must be in [0, {self.model.vocab_size})")
+        rows = lambda value: torch.full((self.batch,), float(value), device=self.device)  # noqa: E731
+        self.adjustments = {}
+        if repetition != 1.0:
+            self.adjustments["repetition"] = rows(repetition)
+        if frequency != 0.0 or presence != 0.0:
+            self.adjustments["frequency"], self.adjustments["presence"] = rows(frequency), rows(presence)
+        if bias:
+            ids = torch.tensor([list(bias)], dtype=torch.long, device=self.device)
+            by = torch.tensor([list(bias.values())], dtype=torch.float32, device=self.device)
+            self.adjustments["bias_ids"], self.adjustments["bias"] = ids.repeat(self.batch, 1), by.repeat(self.batch, 1)
+        if allowed is not None:
+            self.adjustments["allowed"] = allowed
+            if allowed_rows is not None:
+                self.adjustments["allowed_rows"] = allowed_rows
+        self._drop_graphs()
+
+    def _adjusted(self, logits: torch.Tensor, in_place: bool = False) -> torch.Tensor:
+        """``logits`` ``[B, V]`` as ``set_penalties`` asks for them (``in_place``: fp32 ones that nobody else reads)."""
+        if not self.adjustments:
+            return logits
+        lists = {}
+        if "repetition" in self.adjustments or "frequency" in self.adjustments:
+            lists = dict(tokens=self.out, lengths=self.step_index)
+            if "repetition" in self.adjustments:
+                lists.update(prompt=self.prompt_ids, prompt_lengths=self.prompt_count)
+        return adjust_logits(logits, out=logits if in_place else None, **lists, **self.adjustments)
 
     def _sample(self, logits: torch.Tensor, embedding: torch.Tensor | None = None, hidden: torch.Tensor | None = None,
                 counters: torch.Tensor | None = None, ticket: torch.Tensor | None = None, vocab: int | None = None) -> None:
@@ -81,6 +130,7 @@ class GraphDecoder:
     def _choose(self, logits: torch.Tensor) -> None:
         """The next token of every row from ``logits`` ``[B, V]`` into ``self.token`` and ``self.out[:, step_index]``
         (greedy: the first maximum; otherwise ``_sample``)."""
+        logits = self._adjusted(logits)
         if self.temperature > 0:
             vocab = logits.shape[1]
             self._sample(torch.nn.functional.pad(logits.float(), (0, -vocab % 4)).contiguous(), vocab=vocab)
@@ -107,12 +157,18 @@ class GraphDecoder:
             raise ValueError("prompt must be [batch, T] with T < max_len")
         self.cache.static = False
         prompt = prompt.to(self.device)
+        self._remember(prompt)
         step = rows_per_pass or self.batch
         parts = []
         for start in range(0, self.batch, step):
             rows = self.cache.rows(start, min(start + step, self.batch))
             parts.append(self.model(prompt[start:start + step], rows, last_token_only=True)[:, -1, :])
         self._prefilled(torch.cat(parts, dim=0), prompt.shape[1])
+
+    def _remember(self, prompt: torch.Tensor) -> None:
+        """The prompts' tokens, for ``set_penalties``."""
+        self.prompt_ids[:, :prompt.shape[1]].copy_(prompt)
+        self.prompt_count.fill_(prompt.shape[1])
 
     def _prefilled(self, logits: torch.Tensor, prompt_len: int) -> None:
         """The prompt is in the cache, ``logits`` are its last position's: choose the first new token, go static."""
@@ -444,6 +500,11 @@ class FusedDecoder(GraphDecoder):
                 "w2": _FusedLinear([ff.w2]),
                 "cos": att.rope.cosine.float().contiguous(), "sin": att.rope.sine.float().contiguous(),
             })
+            if att.q_norm is not None:
+                self.layers[-1].update(gq=att.q_norm.weight.detach().float().contiguous(), gk=att.k_norm.weight.detach().float().contiguous(),
+                                       eps_heads=att.q_norm.epsilon)
+        self.head_norm = first.attention.q_norm is not None
+        self.zero_rows = torch.zeros(batch, dtype=torch.long, device=dev)
         self.final_gain = model.final_norm.weight.detach().float().contiguous()
         self.final_eps = model.final_norm.epsilon
         self.head = _FusedLinear([model.lm_head])
@@ -474,7 +535,7 @@ class FusedDecoder(GraphDecoder):
         # 0.314 ms per step at batch 1, 0.364 against 0.398 at batch 2, 0.386 against 0.469 at batch 3).  Set it to
         # True (where ``merge_splits`` > 0) before the first ``generate`` to have the merging projection.
         self.merge_splits = (self.layers[0]["o"].merge_splits(batch)
-                             if self.layers[0]["o"].in_features == d and self.head_dim == 128 else 0)
+                             if self.layers[0]["o"].in_features == d and self.head_dim == 128 and not self.head_norm else 0)
         self.fuse_merge = False
         # Larger batches (every workgroup would re-read the fp32 sources of all rows): the norm's row scale
         # is applied to the OUTPUTS of q|k|v, w1|w3 and the head instead, the output projection and w2 add
@@ -532,6 +593,7 @@ class FusedDecoder(GraphDecoder):
             if prompt.shape[0] != self.batch or prompt.shape[1] >= self.max_len:
                 raise ValueError("prompt must be [batch, T] with T < max_len")
             prompt = prompt.to(self.device)
+            self._remember(prompt)
             step = rows_per_pass or self.batch
             logits = torch.cat([self._prefill_rows(prompt[i:i + step], i) for i in range(0, self.batch, step)], dim=0)
             self._prefilled(logits, prompt.shape[1])
@@ -540,12 +602,44 @@ class FusedDecoder(GraphDecoder):
     def _prefill_rows(self, prompt: torch.Tensor, first: int) -> torch.Tensor:
         """Sequences ``first .. first + rows - 1`` of the batch through the layer stack on library
         kernels, from an empty cache; returns the last position's logits ``[rows, V]``."""
+        rows = prompt.shape[0]
+        return self._run_prompt(prompt, [k[first:first + rows] for k in self.cache.keys], [v[first:first + rows] for v in self.cache.values])
+
+    def _run_prompt(self, prompt: torch.Tensor, cache_keys: list[torch.Tensor], cache_values: list[torch.Tensor],
+                    last: torch.Tensor | None = None) -> torch.Tensor:
+        """Prompts ``[rows, T]`` through the layer stack into caches ``[rows, Hkv, .., hd]`` of each layer, from their first row on."""
         lib, st = _lib.load(), _stream()
         rows, seq = prompt.shape
-        d, m = self.model.d_model, rows * seq
-        hidden = self.embedding[prompt.reshape(-1)]  # [rows * seq, d] fp32, row b * seq + t
-        normed = torch.empty((m, d), dtype=torch.bfloat16, device=self.device)
+        max_len = cache_keys[0].shape[2]
         q_rot = torch.empty((rows, self.heads, seq, self.head_dim), dtype=torch.float32, device=self.device)
+        start = torch.zeros(rows, dtype=torch.long, device=self.device) if self.head_norm else None
+
+        def attend(index: int, w: dict, normed: torch.Tensor) -> torch.Tensor:
+            qkv = w["qkv"](normed)
+            keys, values, q = cache_keys[index], cache_values[index], q_rot
+            if self.head_norm:
+                q = norm_rope(qkv[:, :w["qkv"].out_features], w["cos"], w["sin"], keys, values, start, heads=self.heads, tokens=seq,
+                              q_gain=w["gq"], k_gain=w["gk"], epsilon=w["eps_heads"])
+            else:
+                _lib.check(lib.ajq_rope_prefill(qkv.data_ptr(), w["cos"].data_ptr(), w["sin"].data_ptr(), q.data_ptr(),
+                                                keys.data_ptr(), values.data_ptr(), self.kv_flag, rows, seq, self.heads,
+                                                self.kv_heads, self.head_dim, 0, max_len, st), "rope_prefill")
+            del qkv
+            attended = torch.empty((rows * seq, self.model.d_model), dtype=torch.bfloat16, device=self.device)
+            _lib.check(prefill_attention(q, keys, values, self.kv_flag, rows, self.heads, self.kv_heads, seq, 0, max_len, self.head_dim,
+                                         attended, _lib.AJQ_OUT_BF16, st), "attn_prefill")
+            return attended
+
+        return self._layers(prompt, attend, last)
+
+    def _layers(self, tokens: torch.Tensor, attend, last: torch.Tensor | None = None) -> torch.Tensor:
+        """``tokens`` ``[rows, T]`` through the layer stack on library kernels, ``attend(layer's number, its weights, normed rows)`` for q|k|v and
+        attention; the logits ``[rows, V]`` of the last position, or of position ``last[row]``."""
+        lib, st = _lib.load(), _stream()
+        rows, seq = tokens.shape
+        d, m = self.model.d_model, rows * seq
+        hidden = self.embedding[tokens.reshape(-1)]  # [rows * seq, d] fp32, row b * seq + t
+        normed = torch.empty((m, d), dtype=torch.bfloat16, device=self.device)
         w13 = self.layers[0]["w13"]
         gate_in_gemm = w13.rows16 == 2 * self.d_ff and w13.gate_fusable(m)
         gated = None if gate_in_gemm else torch.empty((m, self.d_ff), dtype=torch.bfloat16, device=self.device)
@@ -553,17 +647,7 @@ class FusedDecoder(GraphDecoder):
         for index, w in enumerate(self.layers):
             _lib.check(lib.ajq_add_rmsnorm(hidden.data_ptr(), delta.data_ptr() if delta is not None else None,
                                            w["g1"].data_ptr(), w["eps1"], normed.data_ptr(), m, d, st), "add_rmsnorm")
-            qkv = w["qkv"](normed)
-            keys, values = self.cache.keys[index][first:first + rows], self.cache.values[index][first:first + rows]
-            _lib.check(lib.ajq_rope_prefill(qkv.data_ptr(), w["cos"].data_ptr(), w["sin"].data_ptr(), q_rot.data_ptr(),
-                                            keys.data_ptr(), values.data_ptr(), self.kv_flag, rows, seq, self.heads,
-                                            self.kv_heads, self.head_dim, 0, self.max_len, st), "rope_prefill")
-            del qkv
-            attended = torch.empty((m, d), dtype=torch.bfloat16, device=self.device)
-            _lib.check(prefill_attention(q_rot, keys, values, self.kv_flag, rows, self.heads, self.kv_heads, seq, 0, self.max_len, self.head_dim,
-                                         attended, _lib.AJQ_OUT_BF16, st), "attn_prefill")
-            delta = w["o"](attended)
-            del attended
+            delta = w["o"](attend(index, w, normed))
             _lib.check(lib.ajq_add_rmsnorm(hidden.data_ptr(), delta.data_ptr(), w["g2"].data_ptr(), w["eps2"],
                                            normed.data_ptr(), m, d, st), "add_rmsnorm")
             if gate_in_gemm:
@@ -573,10 +657,14 @@ class FusedDecoder(GraphDecoder):
                 _lib.check(lib.ajq_swiglu(ab.data_ptr(), gated.data_ptr(), m, self.d_ff, st), "swiglu")
                 del ab
             delta = w["w2"](gated)
-        last = hidden.view(rows, seq, d)[:, -1, :].contiguous()
-        last_delta = delta.view(rows, seq, -1)[:, -1, :d].contiguous()
+        if last is None:
+            last_hidden = hidden.view(rows, seq, d)[:, -1, :].contiguous()
+            last_delta = delta.view(rows, seq, -1)[:, -1, :d].contiguous()
+        else:
+            at = torch.arange(rows, device=self.device) * seq + last
+            last_hidden, last_delta = hidden[at], delta[at][:, :d].contiguous()
         last_normed = torch.empty((rows, d), dtype=torch.bfloat16, device=self.device)
-        _lib.check(lib.ajq_add_rmsnorm(last.data_ptr(), last_delta.data_ptr(), self.final_gain.data_ptr(), self.final_eps,
+        _lib.check(lib.ajq_add_rmsnorm(last_hidden.data_ptr(), last_delta.data_ptr(), self.final_gain.data_ptr(), self.final_eps,
                                        last_normed.data_ptr(), rows, d, st), "add_rmsnorm")
         return self.head(last_normed)[:, : self.vocab]
 
@@ -586,6 +674,7 @@ class FusedDecoder(GraphDecoder):
         input) and the two counters in one launch."""
         self._logits()
         full = self.logits_full
+        self._adjusted(full[:, : self.vocab], in_place=True)
         if self.temperature > 0:
             self._sample(full, self.embedding, self.embedded, self.counters, self.ticket, self.vocab)
             return
@@ -602,19 +691,22 @@ class FusedDecoder(GraphDecoder):
         chunks = _lib.load().ajq_attn_row_chunks(self.batch, self.kv_heads, self.max_len)
         return not self.fuse_merge and chunks > 1
 
+    @property
+    def attention_launches(self) -> int:
+        """Launches of a layer's attention: the norm of the heads with rotation and cache write where there is one, attention, its merge."""
+        return int(self.head_norm) + 1 + int(self.merge_launch)
+
     def launches_per_step(self) -> int:
         """Kernel launches of one decode step as this decoder is configured."""
         lib = _lib.load()
         if self.fuse_epilogue:
             # q|k|v, attention (+ merge), output projection, w1|w3 with the gate, w2; the first norm, head, pick
-            per_layer = 6 if self.merge_launch else 5
+            per_layer = 4 + self.attention_launches
             if self.norm_launch:  # both norms of a layer and the final one as launches
                 return (per_layer + 2) * len(self.layers) + 3
             return per_layer * len(self.layers) + (2 if self.first_norm_fused else 3)
         per_layer = 2 if self.fuse_norm else 4           # q|k|v and w1|w3, each with or without its norm launch
-        per_layer += 1                                   # attention
-        if self.merge_launch:                            # merge of its row chunks (none if there is one chunk)
-            per_layer += 1
+        per_layer += self.attention_launches             # attention and the merge of its row chunks (none if there is one chunk)
         per_layer += 1                                   # output projection
         per_layer += 1 if self.fuse_gate else 2          # w2 with or without the gate launch
         head = 1 if self.fuse_norm else 2
@@ -668,11 +760,7 @@ class FusedDecoder(GraphDecoder):
                                                      self.attn_ws_bytes, st), "attn_step_partial")
                 delta = w["o"].after_merge(self.attn_ws, splits.value, b)
             else:
-                _lib.check(lib.ajq_attn_step(qkv.data_ptr(), w["cos"].data_ptr(), w["sin"].data_ptr(), pos.data_ptr(),
-                                             self.cache.keys[index].data_ptr(), self.cache.values[index].data_ptr(),
-                                             self.kv_flag, b, self.heads, self.kv_heads, self.head_dim, self.max_len,
-                                             self.attended.data_ptr(), self.attn_ws.data_ptr(), self.attn_ws_bytes, st),
-                           "attn_step")
+                self._attention(index, w, qkv)
                 delta = w["o"](self.attended)
             ab = normed_linear(w["w13"], w["g2"], w["eps2"])
             if self.fuse_gate:
@@ -686,6 +774,14 @@ class FusedDecoder(GraphDecoder):
 
     def _attention(self, index: int, w: dict, qkv: torch.Tensor) -> None:
         """RoPE, cache write and single-query attention of layer ``index`` into ``self.attended``."""
+        if self.head_norm:   # (the norm needs a whole head ahead of the rotation: a launch of its own)
+            keys, values = self.cache.keys[index], self.cache.values[index]
+            q = norm_rope(qkv[:, :w["qkv"].out_features], w["cos"], w["sin"], keys, values, self.zero_rows, heads=self.heads, q_gain=w["gq"],
+                          k_gain=w["gk"], epsilon=w["eps_heads"], offset=self.cache.position)
+            _lib.check(_lib.load().ajq_attn_decode(q.data_ptr(), keys.data_ptr(), values.data_ptr(), self.kv_flag, self.cache.position.data_ptr(),
+                                                   self.batch, self.heads, self.kv_heads, self.head_dim, self.max_len, self.attended.data_ptr(),
+                                                   self.attn_ws.data_ptr(), self.attn_ws_bytes, _stream()), "attn_decode")
+            return
         _lib.check(_lib.load().ajq_attn_step(qkv.data_ptr(), w["cos"].data_ptr(), w["sin"].data_ptr(),
                                              self.cache.position.data_ptr(), self.cache.keys[index].data_ptr(),
                                              self.cache.values[index].data_ptr(), self.kv_flag, self.batch, self.heads,
@@ -748,6 +844,97 @@ class FusedDecoder(GraphDecoder):
         return self.logits_full[:, : self.vocab]
 
 
+class SharedPrefixDecoder(FusedDecoder):
+    """FusedDecoder for ``completions`` continuations of each of ``prompts`` prompts, whose keys and values lie once for all of them (the reference's
+    ``lm generate`` decodes each completion by itself, workflows/lm_generate.py:61-69), or for questions of different lengths behind a common text.
+
+    A prompt's rows (up to ``prefix_len``) are in caches ``[prompts, Hkv, prefix_len, hd]``; every sequence has ``max_len`` rows of its own behind them, at
+    positions of its own.  A step is FusedDecoder's with ``attention.norm_rope`` and ``attention.shared_prefix_attention`` in the attention's place,
+    replayed from a graph like it.  Sequence ``b`` continues prompt ``b // completions``."""
+
+    def __init__(self, model: modeling.TransformerLM, prompts: int, completions: int, prefix_len: int, max_len: int,
+                 kv_dtype: torch.dtype | None = None, activation_rounding: str = "reference") -> None:
+        if prompts < 1 or completions < 1 or prefix_len < 1:
+            raise ValueError("prompts, completions and prefix_len must be positive")
+        if prefix_len + max_len > model.context_length:
+            raise ValueError(f"prefix_len + max_len {prefix_len + max_len} exceeds the model's context length {model.context_length}")
+        super().__init__(model, prompts * completions, max_len, kv_dtype, activation_rounding)
+        self.prompts, self.completions = prompts, completions
+        self.prefix = model.new_cache(prompts, prefix_len, dtype=kv_dtype)
+        self.prefix_lengths = torch.zeros(prompts, dtype=torch.long, device=self.device)
+        # row and position of a sequence's token of a step, less the step's number (``step_index`` counts on the device)
+        self.rows = torch.zeros(self.batch, dtype=torch.long, device=self.device)
+        self.positions = torch.zeros(self.batch, dtype=torch.long, device=self.device)
+        self.prompt_ids = torch.full((self.batch, prefix_len + max_len), -1, dtype=torch.long, device=self.device)
+        self.merge_splits = 0
+
+    @property
+    def attention_launches(self) -> int:
+        return 3   # (norm and rotation, attention of the prefix's and the own rows, what puts them together)
+
+    @staticmethod
+    def _padded(prompts: torch.Tensor | list[list[int]], count: int, longest: int, what: str) -> tuple[torch.Tensor, torch.Tensor]:
+        """Token lists as ``[count, T]``, padded with zeros, and their lengths."""
+        if isinstance(prompts, torch.Tensor):
+            if prompts.dim() != 2:
+                raise ValueError(f"{what}: a tensor [n, T] or a list of token lists expected")
+            prompts = prompts.tolist()
+        lengths = [len(p) for p in prompts]
+        if len(prompts) != count or min(lengths) < 1 or max(lengths) > longest:
+            raise ValueError(f"{what}: {count} of 1 to {longest} tokens each expected")
+        return torch.tensor([list(p) + [0] * (max(lengths) - len(p)) for p in prompts]), torch.tensor(lengths)
+
+    @torch.no_grad()
+    def prefill(self, prompt: torch.Tensor | list[list[int]], questions: list[list[int]] | None = None) -> None:
+        """``prompt``: ``[prompts, T]``, or a list of token lists of any lengths.  ``questions``: the tokens that follow it in each of the ``prompts *
+        completions`` sequences (None: none, all continue the prompt itself).  Chooses each sequence's first new token."""
+        tokens, lengths = self._padded(prompt, self.prompts, self.prefix.max_len, "prompt")
+        asked = None if questions is None else self._padded(questions, self.batch, self.max_len - 1, "questions")
+        tokens, lengths = tokens.to(self.device), lengths.to(self.device)
+        each = torch.arange(self.batch, device=self.device) // self.completions
+        logits = self._run_prompt(tokens, self.prefix.keys, self.prefix.values, lengths - 1)[each]
+        self.prefix_lengths.copy_(lengths)
+        before = lengths[each]
+        self.prompt_ids.fill_(-1)   # (no token: the places between the lists)
+        place = torch.arange(tokens.shape[1], device=self.device)
+        self.prompt_ids[:, :tokens.shape[1]] = torch.where(place < before[:, None], tokens[each], -1)
+        width, own = tokens.shape[1], torch.zeros_like(before)
+        if asked is not None:
+            more, own = (t.to(self.device) for t in asked)
+            self.prompt_ids[:, width:width + more.shape[1]] = torch.where(torch.arange(more.shape[1], device=self.device) < own[:, None], more, -1)
+            width += more.shape[1]
+            logits = self._ask(more, own, before)
+        self.prompt_count.fill_(width)
+        self.rows.copy_(own - 1)
+        self.positions.copy_(before + own - 1)
+        self._prefilled(logits, 0 if asked is None else asked[0].shape[1])
+        torch.index_select(self.embedding, 0, self.token.view(-1), out=self.embedded)
+
+    def _ask(self, questions: torch.Tensor, counts: torch.Tensor, before: torch.Tensor) -> torch.Tensor:
+        """Questions ``[B, T]`` behind the prompts, into the sequences' own rows; the logits of each one's last token."""
+        seq = questions.shape[1]
+
+        def attend(index: int, w: dict, normed: torch.Tensor) -> torch.Tensor:
+            qkv = w["qkv"](normed)
+            keys, values = self.cache.keys[index], self.cache.values[index]
+            q = norm_rope(qkv[:, :w["qkv"].out_features], w["cos"], w["sin"], keys, values, self.zero_rows, heads=self.heads, tokens=seq,
+                          q_gain=w.get("gq"), k_gain=w.get("gk"), epsilon=w.get("eps_heads", 0.0), positions=before, counts=counts,
+                          out_dtype=torch.bfloat16)
+            del qkv
+            return shared_prefix_attention(q, self.prefix.keys[index], self.prefix.values[index], self.prefix_lengths, keys, values, self.zero_rows,
+                                           counts=counts).view(self.batch * seq, -1)
+
+        return self._layers(questions, attend, counts - 1)
+
+    def _attention(self, index: int, w: dict, qkv: torch.Tensor) -> None:
+        """Rotation, cache write and attention of layer ``index`` behind the prompts, into ``self.attended``."""
+        keys, values = self.cache.keys[index], self.cache.values[index]
+        q = norm_rope(qkv[:, :w["qkv"].out_features], w["cos"], w["sin"], keys, values, self.rows, heads=self.heads, q_gain=w.get("gq"),
+                      k_gain=w.get("gk"), epsilon=w.get("eps_heads", 0.0), positions=self.positions, offset=self.step_index)
+        self.attended = shared_prefix_attention(q, self.prefix.keys[index], self.prefix.values[index], self.prefix_lengths, keys, values, self.rows,
+                                                offset=self.step_index).view(self.batch, -1)
+
+
 class DenseDecoder(GraphDecoder):
     """GraphDecoder for a ``dense.DenseLM``, whose step is this library's kernels already: the choice of the token
     and the step's two counters are one launch as well (``ajq_greedy_pick`` / ``ajq_sample_pick``), and eight steps make
@@ -771,6 +958,7 @@ class DenseDecoder(GraphDecoder):
             raise ValueError("prompt must be [batch, T] with T < max_len")
         self.cache.static = False
         prompt = prompt.to(self.device)
+        self._remember(prompt)
         step, seq, parts = rows_per_pass or self.batch, prompt.shape[1], []
         for first in range(0, self.batch, step):
             rows = self.cache.rows(first, min(first + step, self.batch))
@@ -782,7 +970,7 @@ class DenseDecoder(GraphDecoder):
 
     @torch.no_grad()
     def _step(self) -> None:
-        logits = self._logits()
+        logits = self._adjusted(self._logits())
         if self.temperature > 0:
             _lib.check(_lib.load().ajq_sample_pick(
                 logits.data_ptr(), self.batch, logits.shape[1], logits.stride(0), self.temperature,

@@ -304,10 +304,11 @@ class RingCache:
 
 class MultiHeadSelfAttention(nn.Module):
     """Causal self-attention.  ``num_kv_heads < num_heads`` gives grouped-query attention (the
-    reference has multi-head only; with ``num_kv_heads == num_heads`` this is the reference layer)."""
+    reference has multi-head only; with ``num_kv_heads == num_heads`` this is the reference layer).  ``head_norm``: every
+    query and key head is RMS-normed ahead of its rotation (``q_norm``, ``k_norm``; the reference has none)."""
 
     def __init__(self, d_model: int, num_heads: int, context_length: int, position_encoding: str,
-                 rope_theta: float, num_kv_heads: int | None = None) -> None:
+                 rope_theta: float, num_kv_heads: int | None = None, head_norm: bool = False) -> None:
         super().__init__()
         if d_model % num_heads != 0:
             raise ValueError("d_model must be divisible by num_heads")
@@ -324,6 +325,8 @@ class MultiHeadSelfAttention(nn.Module):
         self.output_proj = Linear(d_model, d_model)
         self.rope = (RotaryPositionalEmbedding(rope_theta, self.head_dimension, context_length)
                      if position_encoding == "rope" else None)
+        self.q_norm = RMSNorm(self.head_dimension) if head_norm else None
+        self.k_norm = RMSNorm(self.head_dimension) if head_norm else None
         # as the reference's flag (attention.py:106-117): on a GPU, multi-token calls go to the
         # library's flash-attention kernel instead of the masked softmax below (head_dim 128, 64 or 32)
         self.use_flash_attention = False
@@ -335,6 +338,8 @@ class MultiHeadSelfAttention(nn.Module):
         q = self.q_proj(inputs).view(batch, seq, self.num_heads, hd).transpose(1, 2)
         k = self.k_proj(inputs).view(batch, seq, self.num_kv_heads, hd).transpose(1, 2)
         v = self.v_proj(inputs).view(batch, seq, self.num_kv_heads, hd).transpose(1, 2)
+        if self.q_norm is not None:
+            q, k = self.q_norm(q), self.k_norm(k)
         if self.rope is not None:
             q = self.rope(q, positions[:, None, :].expand(batch, self.num_heads, seq))
             k = self.rope(k, positions[:, None, :].expand(batch, self.num_kv_heads, seq))
@@ -389,7 +394,7 @@ class MultiHeadSelfAttention(nn.Module):
 class TransformerBlock(nn.Module):
     def __init__(self, d_model: int, num_heads: int, d_ff: int, context_length: int, position_encoding: str,
                  rope_theta: float, normalization: str, norm_placement: str, feed_forward: str,
-                 num_kv_heads: int | None = None) -> None:
+                 num_kv_heads: int | None = None, head_norm: bool = False) -> None:
         super().__init__()
         if norm_placement not in {"pre", "post"}:
             raise ValueError("normalization.placement must be 'pre' or 'post'")
@@ -397,7 +402,7 @@ class TransformerBlock(nn.Module):
         self.norm1 = build_norm(normalization, d_model)
         self.norm2 = build_norm(normalization, d_model)
         self.attention = MultiHeadSelfAttention(d_model, num_heads, context_length, position_encoding,
-                                                rope_theta, num_kv_heads)
+                                                rope_theta, num_kv_heads, head_norm)
         self.feed_forward = build_feed_forward(feed_forward, d_model, d_ff)
 
     def forward(self, inputs: torch.Tensor, positions: torch.Tensor, cache: KVCache | None = None,
@@ -416,7 +421,7 @@ class TransformerLM(nn.Module):
     def __init__(self, vocab_size: int, context_length: int, d_model: int, num_layers: int, num_heads: int,
                  d_ff: int, position_encoding: str = "rope", rope_theta: float = 10_000.0,
                  normalization: str = "rmsnorm", norm_placement: str = "pre", feed_forward: str = "swiglu",
-                 tie_embeddings: bool = False, num_kv_heads: int | None = None) -> None:
+                 tie_embeddings: bool = False, num_kv_heads: int | None = None, head_norm: bool = False) -> None:
         super().__init__()
         if position_encoding not in {"rope", "none", "learned"}:
             raise ValueError("position encoding must be rope, none, or learned")
@@ -433,7 +438,7 @@ class TransformerLM(nn.Module):
         self.position_embeddings = Embedding(context_length, d_model) if position_encoding == "learned" else None
         self.layers = nn.ModuleList([
             TransformerBlock(d_model, num_heads, d_ff, context_length, position_encoding, rope_theta,
-                             normalization, norm_placement, feed_forward, num_kv_heads)
+                             normalization, norm_placement, feed_forward, num_kv_heads, head_norm)
             for _ in range(num_layers)
         ])
         self.final_norm = build_norm(normalization if norm_placement == "pre" else "none", d_model)
@@ -523,6 +528,7 @@ def build_model(config: dict[str, Any], vocab_size: int | None = None) -> nn.Mod
         feed_forward=ff_type,
         tie_embeddings=bool(config.get("tie_embeddings", False)),
         num_kv_heads=(int(config["num_kv_heads"]) if "num_kv_heads" in config else None),
+        head_norm=bool(normalization.get("heads", False)),
     )
 
 
