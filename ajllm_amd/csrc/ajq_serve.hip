@@ -91,7 +91,7 @@ long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 
 // How an attention call is cut up: tiles of queries, parts of the rows.  The device's lengths are not known here; the capacities are what they
 // can be.
-enum class SharedForm { few, many, walk };   // (the prefix by meet_few, by meet_many; everything in one walk)
+enum class SharedForm { few, many, walk, each };   // (the prefix by meet_few, by meet_many; everything in one walk of many, of few queries)
 struct SharedPlan {
   SharedForm form;
   int prefix_rt, own_rt;            // tiles of 16 queries a wave
@@ -100,6 +100,14 @@ struct SharedPlan {
   size_t bytes;
 };
 constexpr int kMostParts = 64;      // a lane each in the merge
+// Whether one launch in which every sequence walks the prefix by itself is the faster (sum of kernel times, against those of two launches; 32 / 8 heads of 128,
+// bf16, rows of prefix + own): 8 sequences of 64 rows 4.7 and 9.0 us, of 512 6.7 and 9.4, of 768 7.7 and 9.2, of 1536 11.5 and 11.5; 128 sequences of 64 9.0 and
+// 14.2, of 768 22.3 and 23.5, of 1536 49 and 39.  fp32 rows take longer in fp32: 8 of 64 6.3 and 11.2, of 192 8.5 and 11.5, of 512 14.4 and 12.9; 128 of 192 27.0
+// and 28.8.
+bool shared_each(const ajqs_shared_attention_args* a, long long workgroups) {
+  const long long rows = (long long)a->prefix_cap + a->max_len;
+  return workgroups <= 1024 && rows <= (a->cache_dtype == AJQS_BF16 ? 768 : 192);
+}
 SharedPlan shared_plan(const ajqs_shared_attention_args* a) {
   SharedPlan p{};
   const long long share = a->heads / a->kv_heads, mine = a->tokens * share, all = a->batch / a->groups * mine;
@@ -116,6 +124,12 @@ SharedPlan shared_plan(const ajqs_shared_attention_args* a) {
     p.own_tiles = (int)ceil_div(mine, 64 * p.own_rt);
     p.own_parts = parts(own_units * p.own_tiles, 512, (long long)a->prefix_cap + a->max_len, 128, kMostParts);
     p.own_blocks = ceil_div(own_units, 8) * 8 * p.own_tiles * p.own_parts;
+  } else if (shared_each(a, own_units * ceil_div(mine, mine > 16 ? 32 : 16))) {
+    p.form = SharedForm::each;
+    p.own_rt = mine > 16 ? 2 : 1;
+    p.own_tiles = (int)ceil_div(mine, 16 * p.own_rt);
+    p.own_parts = 1;
+    p.own_blocks = ceil_div(own_units, 8) * 8 * p.own_tiles;
   } else {
     p.form = bf16 && all > 64 ? SharedForm::many : SharedForm::few;
     p.own_rt = mine > 16 ? 2 : 1;
@@ -193,6 +207,14 @@ int launch_few(const SharedAttention& s, const SharedPlan& p, hipStream_t stream
   if (int e = allow_lds(kernel, bytes, what)) return e;
   hipLaunchKernelGGL(kernel, dim3((unsigned)(p.prefix_blocks + p.own_blocks)), dim3(256), bytes, stream, s);
   return merge_parts<HD>(s, p, stream, what);
+}
+template <int HD, typename QT, typename CacheT, int RT>
+int launch_each(const SharedAttention& s, const SharedPlan& p, hipStream_t stream, const char* what) {
+  constexpr int bytes = some_lds_bytes<HD, CacheT, RT>();
+  auto kernel = shared_attention_each_kernel<HD, QT, CacheT, RT>;
+  if (int e = allow_lds(kernel, bytes, what)) return e;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)p.own_blocks), dim3(256), bytes, stream, s);
+  return check_launch(what);
 }
 template <int HD, typename QT, int U, int RTO>
 int launch_many(const SharedAttention& s, const SharedPlan& p, hipStream_t stream, const char* what) {
@@ -291,6 +313,11 @@ int ajqs_shared_attention(const ajqs_shared_attention_args* a, void* workspace, 
             status = launch(s, p, (hipStream_t)stream, what);
             return;
           }
+        }
+        if (p.form == SharedForm::each) {
+          const auto launch = p.own_rt == 2 ? launch_each<HD, QT, CacheT, 2> : launch_each<HD, QT, CacheT, 1>;
+          status = launch(s, p, (hipStream_t)stream, what);
+          return;
         }
         const auto launch = p.own_rt == 2      ? launch_few<HD, QT, CacheT, 2, 2>
                             : p.prefix_rt == 2 ? launch_few<HD, QT, CacheT, 2, 1>

@@ -46,6 +46,8 @@ template <typename CacheT> struct Meeting {
   int first;                     // the tile's first query
   int part, parts, outer;        // part of the rows of sequence or group `outer`
   int begin, end;                // rows
+  const CacheT *own_keys, *own_values;   // a second run of rows, from its first on (only where a workgroup walks both: `own` is then false and
+  int own_end;                           // the queries are one sequence's)
   bool own;
   long long before;              // own rows a sequence's first new token sees ahead of its own row
 };
@@ -158,6 +160,23 @@ __device__ __forceinline__ void find_rows(const SharedAttention& a, Meeting<Cach
   w.end = min(rows, w.begin + per);
 }
 
+// Both runs of one sequence's queries: its group's prefix, and its own rows.
+template <int HD, typename CacheT>
+__device__ __forceinline__ void find_both(const SharedAttention& a, Meeting<CacheT>& w) {
+  int unused;
+  const int group = divide(w.outer, a.by_group, unused);
+  w.own_keys = w.keys;
+  w.own_values = w.values;
+  w.own = false;
+  w.before = a.rows[w.outer] + (a.offset ? *a.offset : 0ll);
+  w.own_end = held(w.before + (a.counts ? held(a.counts[w.outer], a.tokens) : a.tokens), a.max_len);
+  w.begin = 0;
+  w.end = held(a.prefix_lengths[group], a.prefix_cap);
+  const size_t at = (size_t)group * a.prefix_group + (size_t)w.key_head * a.prefix_head;
+  w.keys = reinterpret_cast<const CacheT*>(a.prefix_keys) + at;
+  w.values = reinterpret_cast<const CacheT*>(a.prefix_values) + at;
+}
+
 // ---- Few queries: the four waves of a workgroup take blocks of 32 rows in turn, each for itself (no barrier until the end), and RT tiles of 16
 // queries meet every row fetched.  What bounds it is memory: a wave asks for the next block's keys as soon as it has used this block's, and for
 // its values likewise; eight waves a CU (bf16) then have 64 to 128 KB on their way.
@@ -169,9 +188,9 @@ template <int HD, typename CacheT, int RT> constexpr int few_lds_bytes() {
   return walk > join ? walk : join;
 }
 
-// The four waves' results meet in LDS (rows of HD + 4 numbers: sixteen queries' pieces fall on different banks) and become the workgroup's part.
-// put(u, to): a lane's sums of its query of tile u, to the query's row.
-template <int HD, int RT, int kMl, typename CacheT, typename Put>
+// The four waves' results meet in LDS (rows of HD + 4 numbers: sixteen queries' pieces fall on different banks) and become the workgroup's part, or
+// (kWhole) the result.  put(u, to): a lane's sums of its query of tile u, to the query's row.
+template <int HD, int RT, int kMl, bool kWhole, typename CacheT, typename Put>
 __device__ __forceinline__ void join_waves(const SharedAttention& a, const Meeting<CacheT>& w, unsigned char* lds, const RunningRow<HD> (&row)[RT], Put put) {
   constexpr int kJoin = RT * 16, kPitch = HD + 4, kHelpers = 256 / kJoin;   // queries, lanes that put one together
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
@@ -199,20 +218,54 @@ __device__ __forceinline__ void join_waves(const SharedAttention& a, const Meeti
     weight[k] = e[k].x == -INFINITY ? 0.f : exp2_hw(e[k].x - m);
     l += e[k].y * weight[k];
   }
-  int unused;
-  const long long place = query_place(a, w.key_head, w.first_sequence, w.first + n, unused) + (w.part + (w.own ? a.prefix_parts : 0)) * a.queries;
-  if (d0 == 0) a.part_ml[place] = float2{m, l};
+  int token;
+  const long long in_q = query_place(a, w.key_head, w.first_sequence, w.first + n, token);
+  const long long place = in_q + (kWhole ? 0 : (w.part + (w.own ? a.prefix_parts : 0)) * a.queries);
+  if (!kWhole && d0 == 0) a.part_ml[place] = float2{m, l};
+  float scale = 1.f;   // (zeros where a token is not there or saw nothing)
+  uint16_t* out = nullptr;
+  if constexpr (kWhole) {
+    int rest, share;
+    divide(w.first + n, a.by_each, rest);
+    divide(rest, a.by_share, share);
+    const bool there = a.counts == nullptr || token < a.counts[w.outer];
+    scale = there && (l > 0.f || l != l) ? 1.f / l : 0.f;
+    out = a.out + (((size_t)w.outer * a.tokens + token) * a.heads + (w.key_head * (int)a.by_share.d + share)) * HD;
+  }
 #pragma unroll
   for (int d = 0; d < HD; d += 4 * kHelpers) {
     if (d + d0 >= HD) break;
     f32x4_t o = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int k = 0; k < 4; ++k) o += *reinterpret_cast<const f32x4_t*>(sums + (k * kJoin + n) * kPitch + d + d0) * weight[k];
-    *reinterpret_cast<f32x4_t*>(a.part_sums + place * HD + d + d0) = o;
+    if constexpr (kWhole)
+      *reinterpret_cast<u32x2_t*>(out + d + d0) =
+          scale == 0.f ? u32x2_t{0u, 0u} : u32x2_t{pack2_bf16(o[0] * scale, o[1] * scale), pack2_bf16(o[2] * scale, o[3] * scale)};
+    else *reinterpret_cast<f32x4_t*>(a.part_sums + place * HD + d + d0) = o;
   }
 }
 
-template <int HD, typename QT, typename CacheT, int RT, int W = 4>
+// Block n (of N rows) of a meeting's rows: of the second run's behind the first's (kBoth).
+template <int HD, int N, bool kBoth, typename CacheT> struct Block {
+  const CacheT *keys, *values;   // its first row
+  int rows;                      // from there on in its run
+  int at;                        // its first row's number there
+  bool second;
+  __device__ __forceinline__ Block(const Meeting<CacheT>& w, int n) {
+    const int of_first = (w.end - w.begin + N - 1) / N;
+    second = kBoth && n >= of_first;
+    at = second ? N * (n - of_first) : w.begin + N * n;
+    rows = (second ? w.own_end : w.end) - at;
+    keys = (second ? w.own_keys : w.keys) + (size_t)at * HD;
+    values = (second ? w.own_values : w.values) + (size_t)at * HD;
+  }
+};
+template <int N, bool kBoth, typename CacheT>
+__device__ __forceinline__ int blocks_of(const Meeting<CacheT>& w) {
+  return (w.end - w.begin + N - 1) / N + (kBoth ? (w.own_end + N - 1) / N : 0);
+}
+
+template <int HD, typename QT, typename CacheT, int RT, int W = 4, bool kBoth = false>
 __device__ __forceinline__ void meet_few(const SharedAttention& a, Meeting<CacheT>& w, unsigned char* lds, uint32_t lds0) {
   constexpr int RB = 2 * HD, C = HD / 8, KS = HD / 32, TT = HD / 16, KH = kHalves<CacheT>, QH = kHalves<QT>;
   constexpr int kPlane = 32 * RB;                 // 32 rows of bf16
@@ -234,12 +287,12 @@ __device__ __forceinline__ void meet_few(const SharedAttention& a, Meeting<Cache
     for (int s = 0; s < KS; ++s) raw[u][s] = load8_raw(reinterpret_cast<const QT*>(a.q) + place * HD + 32 * s + 8 * g);
   }
   __builtin_amdgcn_sched_barrier(0);
-  find_rows(a, w);
+  kBoth ? find_both<HD>(a, w) : find_rows(a, w);
   RunningRow<HD> row[RT];
-  int limit[RT];   // how many of the meeting's rows a lane's queries see
+  int limit[RT];   // how many of the meeting's rows (kBoth: of the second run's) a lane's queries see
 #pragma unroll
   for (int u = 0; u < RT; ++u) {
-    limit[u] = w.own ? held(w.before + token[u] + 1, w.end) : w.end;
+    limit[u] = kBoth ? held(w.before + token[u] + 1, w.own_end) : w.own ? held(w.before + token[u] + 1, w.end) : w.end;
     row[u].m = row[u].l = 0.f;
     row[u].fresh = true;
 #pragma unroll
@@ -248,24 +301,24 @@ __device__ __forceinline__ void meet_few(const SharedAttention& a, Meeting<Cache
 
   // ---- rows on their way (past the last: the last again, which is there and finite)
   const int ask_row = lane / C, slot = lane % C;
-  auto ask = [&](const CacheT* from, int at, uint32_t to, bool values) {
-    const CacheT* base = from + (size_t)at * HD;
+  using Rows = Block<HD, 32, kBoth, CacheT>;
+  auto ask = [&](const CacheT* from, int rows, uint32_t to, bool values) {
 #pragma unroll
     for (int i = 0; i < kAsk; ++i) {
       const int k = kRows * i + ask_row;
       const uint32_t chunk = values ? (uint32_t)((((slot >> 1) ^ (k & (TT - 1))) << 1) | (slot & 1)) : (uint32_t)(slot ^ (k & (C - 1)));
-      dma16(base, (uint32_t)(min(k, w.end - 1 - at) * RB) + chunk * 16u, to + (uint32_t)(i * 1024));
+      dma16(from, (uint32_t)(min(k, rows - 1) * RB) + chunk * 16u, to + (uint32_t)(i * 1024));
     }
   };
   constexpr int kPieces = kDma ? 1 : 32 * C / 64;   // 8 components each, a lane
   Raw8F32 kraw[kPieces], vraw[kPieces];
-  auto fetch = [&](int at) {
+  auto fetch = [&](const Rows& from) {
     if constexpr (!kDma) {
 #pragma unroll
       for (int i = 0; i < kPieces; ++i) {
-        const int piece = lane + 64 * i, k = min(at + piece / C, w.end - 1);
-        kraw[i] = load8_raw(w.keys + (size_t)k * HD + 8 * (piece % C));
-        vraw[i] = load8_raw(w.values + (size_t)k * HD + 8 * (piece % C));
+        const int piece = lane + 64 * i, k = min(piece / C, from.rows - 1);
+        kraw[i] = load8_raw(from.keys + k * HD + 8 * (piece % C));
+        vraw[i] = load8_raw(from.values + k * HD + 8 * (piece % C));
       }
     }
   };
@@ -293,14 +346,14 @@ __device__ __forceinline__ void meet_few(const SharedAttention& a, Meeting<Cache
 #pragma unroll
   for (int t = 0; t < TT; ++t) v_rd[t] = values0 + (uint32_t)(vkey * RB + 32 * (t ^ (vkey & (TT - 1))) + 8 * (r & 3));
 
-  int at = w.begin + 32 * wave;
-  if (wave >= W) at = w.end;
-  if (at < w.end) {
+  const int blocks = wave < W ? blocks_of<32, kBoth>(w) : 0;
+  if (wave < blocks) {
+    const Rows first(w, wave);
     if constexpr (kDma) {
-      ask(w.keys, at, mine, false);
-      ask(w.values, at, values0, true);
+      ask(first.keys, first.rows, mine, false);
+      ask(first.values, first.rows, values0, true);
     } else {
-      fetch(at);
+      fetch(first);
     }
   }
   u32x4_t qf[RT][KS][QH];
@@ -308,14 +361,15 @@ __device__ __forceinline__ void meet_few(const SharedAttention& a, Meeting<Cache
   for (int u = 0; u < RT; ++u)
 #pragma unroll
     for (int s = 0; s < KS; ++s) to_halves(raw[u][s], qf[u][s]);
-  for (; at < w.end; at += 32 * W) {
-    const bool more = at + 32 * W < w.end;
+  for (int n = wave; n < blocks; n += W) {
+    const bool more = n + W < blocks;
+    const Rows now(w, n), next(w, more ? n + W : n);
     if constexpr (kDma) {
       // (behind this block's keys only its values are on their way)
       asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kAsk) : "memory");
     } else {
       lay_down();
-      if (more) fetch(at + 32 * W);
+      if (more) fetch(next);
       wave_lds_order();
     }
     f32x4_t sc[RT][2];
@@ -339,18 +393,19 @@ __device__ __forceinline__ void meet_few(const SharedAttention& a, Meeting<Cache
     if constexpr (kDma) {
       if (more) {
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        ask(w.keys, at + 32 * W, mine, false);
+        ask(next.keys, next.rows, mine, false);
       }
     }
     u32x4_t pf[RT];
 #pragma unroll
     for (int u = 0; u < RT; ++u) {
-      if (__builtin_amdgcn_ballot_w64(at + 32 > limit[u]) != 0) {
+      const int seen = (kBoth && !now.second ? w.end : limit[u]) - now.at;   // of the block's rows
+      if (__builtin_amdgcn_ballot_w64(seen < 32) != 0) {
 #pragma unroll
         for (int jb = 0; jb < 2; ++jb)
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            if (at + 16 * jb + 4 * g + i >= limit[u]) sc[u][jb][i] = -INFINITY;
+            if (16 * jb + 4 * g + i >= seen) sc[u][jb][i] = -INFINITY;
       }
       float p[8];
       to_probabilities<HD, 2>(row[u], sc[u], a.scale2, p);
@@ -373,14 +428,14 @@ __device__ __forceinline__ void meet_few(const SharedAttention& a, Meeting<Cache
     if constexpr (kDma) {
       if (more) {
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        ask(w.values, at + 32 * W, values0, true);
+        ask(next.values, next.rows, values0, true);
       }
     } else {
       wave_lds_order();
     }
   }
 
-  join_waves<HD, RT, few_join_bytes<HD, RT>()>(a, w, lds, row, [&](int u, float* to) {
+  join_waves<HD, RT, few_join_bytes<HD, RT>(), kBoth>(a, w, lds, row, [&](int u, float* to) {
 #pragma unroll
     for (int t = 0; t < TT; ++t) *reinterpret_cast<f32x4_t*>(to + 16 * t + 4 * g) = row[u].o[t];
   });
@@ -400,7 +455,7 @@ __device__ __forceinline__ float4 query4(const uint16_t* p) {
   return v;
 }
 template <int HD> constexpr int few_f32_lds_bytes() { return few_join_bytes<HD, 1>() + 4 * 16 * 8; }
-template <int HD, typename QT>
+template <int HD, typename QT, bool kBoth = false>
 __device__ __forceinline__ void meet_few_f32(const SharedAttention& a, Meeting<float>& w, unsigned char* lds) {
   constexpr int KC = HD / 16, P = HD == 32 ? 2 : 4, VC = HD / (16 * P);
   typedef float part_t __attribute__((ext_vector_type(P)));
@@ -412,8 +467,9 @@ __device__ __forceinline__ void meet_few_f32(const SharedAttention& a, Meeting<f
 #pragma unroll
   for (int c = 0; c < KC; ++c) q[c] = query4(from + 16 * c);
   __builtin_amdgcn_sched_barrier(0);
-  find_rows(a, w);
-  const int limit = w.own ? held(w.before + token + 1, w.end) : w.end;
+  kBoth ? find_both<HD>(a, w) : find_rows(a, w);
+  const int limit = kBoth ? held(w.before + token + 1, w.own_end) : w.own ? held(w.before + token + 1, w.end) : w.end;
+  using Rows = Block<HD, 16, kBoth, float>;
   RunningRow<HD> row[1];
   row[0].m = row[0].l = 0.f;
   row[0].fresh = true;
@@ -421,20 +477,22 @@ __device__ __forceinline__ void meet_few_f32(const SharedAttention& a, Meeting<f
   for (int t = 0; t < HD / 16; ++t) row[0].o[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   float4 k[KC];
   part_t v[4][VC];
-  auto ask = [&](int at) __attribute__((always_inline)) {   // (past the last row: that one again)
-    const float* keys = w.keys + (size_t)min(at + r, w.end - 1) * HD + 4 * g;
+  auto ask = [&](const Rows& from) __attribute__((always_inline)) {   // (past the last row: that one again)
+    const float* keys = from.keys + min(r, from.rows - 1) * HD + 4 * g;
 #pragma unroll
     for (int c = 0; c < KC; ++c) k[c] = *reinterpret_cast<const float4*>(keys + 16 * c);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float* values = w.values + (size_t)min(at + 4 * g + i, w.end - 1) * HD + P * r;
+      const float* values = from.values + min(4 * g + i, from.rows - 1) * HD + P * r;
 #pragma unroll
       for (int c = 0; c < VC; ++c) v[i][c] = *reinterpret_cast<const part_t*>(values + 16 * P * c);
     }
   };
-  int at = w.begin + 16 * wave;
-  if (at < w.end) ask(at);
-  for (; at < w.end; at += 64) {
+  const int blocks = blocks_of<16, kBoth>(w);
+  if (wave < blocks) ask(Rows(w, wave));
+  for (int n = wave; n < blocks; n += 4) {
+    const Rows now(w, n);
+    const int seen = (kBoth && !now.second ? w.end : limit) - now.at;   // of the block's rows
     f32x4_t even = f32x4_t{0.f, 0.f, 0.f, 0.f}, odd = even;
 #pragma unroll
     for (int c = 0; c < KC; ++c) {
@@ -449,10 +507,10 @@ __device__ __forceinline__ void meet_few_f32(const SharedAttention& a, Meeting<f
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int c = 0; c < VC; ++c) values[i][c] = v[i][c];
-    if (at + 64 < w.end) ask(at + 64);
+    if (n + 4 < blocks) ask(Rows(w, n + 4));
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      if (at + 4 * g + i >= limit) sc[0][i] = -INFINITY;
+      if (4 * g + i >= seen) sc[0][i] = -INFINITY;
     float p[4];
     to_probabilities<HD, 1>(row[0], sc, a.scale2, p);
 #pragma unroll
@@ -463,7 +521,7 @@ __device__ __forceinline__ void meet_few_f32(const SharedAttention& a, Meeting<f
         for (int e = 0; e < P; ++e) row[0].o[c * P + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(values[i][c][e], p[i], row[0].o[c * P + e], 0, 0, 0);
   }
   // a lane has components 16 P v + P (4 g + i) + e of query r: of each v 4 P of them one behind the other
-  join_waves<HD, 1, few_join_bytes<HD, 1>()>(a, w, lds, row, [&](int, float* to) {
+  join_waves<HD, 1, few_join_bytes<HD, 1>(), kBoth>(a, w, lds, row, [&](int, float* to) {
 #pragma unroll
     for (int c = 0; c < VC; ++c)
 #pragma unroll
@@ -750,10 +808,10 @@ __device__ __forceinline__ void leave_part(const SharedAttention& a, const Walk<
   }
 }
 
-template <int HD, typename QT, typename CacheT, int RT>
+template <int HD, typename QT, typename CacheT, int RT, bool kBoth = false>
 __device__ __forceinline__ void meet_some(const SharedAttention& a, Meeting<CacheT>& w, unsigned char* lds, uint32_t lds0) {
-  if constexpr (sizeof(CacheT) == 4 && RT == 1) meet_few_f32<HD, QT>(a, w, lds);
-  else meet_few<HD, QT, CacheT, RT>(a, w, lds, lds0);
+  if constexpr (sizeof(CacheT) == 4 && RT == 1) meet_few_f32<HD, QT, kBoth>(a, w, lds);
+  else meet_few<HD, QT, CacheT, RT, 4, kBoth>(a, w, lds, lds0);
 }
 template <int HD, typename CacheT, int RT> constexpr int some_lds_bytes() {
   return sizeof(CacheT) == 4 && RT == 1 ? few_f32_lds_bytes<HD>() : few_lds_bytes<HD, CacheT, RT>();
@@ -766,6 +824,17 @@ __global__ __launch_bounds__(256, sizeof(CacheT) == 4 && RTP == 2 ? 1 : 2) void 
   if (!find_meeting<CacheT, HD>(a, 16 * RTP, 16 * RTO, w)) return;
   if (RTP == RTO || !w.own) meet_some<HD, QT, CacheT, RTP>(a, w, shared_lds, lds0);
   else meet_some<HD, QT, CacheT, RTO>(a, w, shared_lds, lds0);
+}
+
+// Few rows in all: a workgroup walks the prefix and then a sequence's own rows with that sequence's queries alone, and what comes out is the result, in
+// one launch.  Each sequence reads the prefix again (from L2), which two launches cost more than.
+template <int HD, typename QT, typename CacheT, int RT>
+__global__ __launch_bounds__(256, sizeof(CacheT) == 4 && RT == 2 ? 1 : 2) void shared_attention_each_kernel(SharedAttention a) {
+  extern __shared__ __attribute__((aligned(1024))) unsigned char shared_lds[];
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(pf_lds_char_t*)shared_lds;
+  Meeting<CacheT> w;
+  if (!find_meeting<CacheT, HD>(a, 16 * RT, 16 * RT, w)) return;
+  meet_some<HD, QT, CacheT, RT, true>(a, w, shared_lds, lds0);
 }
 
 // The prefix by meet_many, the sequences' own rows by meet_few.

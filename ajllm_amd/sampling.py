@@ -60,9 +60,12 @@ def adjust_logits(logits: torch.Tensor, *, tokens: torch.Tensor | None = None, l
     ``tokens`` and ``prompt`` are int64 ``[B, n]``, of which the first ``lengths`` (``prompt_lengths``) count: int64 on the device, one a row or
     one for all (a decoder's step counter), None: all of them.  Ids outside ``[0, V)`` are passed over.  ``repetition``, ``frequency`` and
     ``presence`` are numbers or fp32 ``[B]``.  ``out`` may be ``logits`` itself where they are fp32; without it the rows of the result begin
-    on 16-byte boundaries, as ``ajq_sample_pick`` wants them."""
+    on 16-byte boundaries, as ``ajq_sample_pick`` wants them (fp32 logits that nothing is to happen to are returned as they are)."""
     if not logits.is_cuda:
         raise ValueError("adjust_logits needs tensors on a ROCm device (there is no CPU path)")
+    if (tokens is lengths is prompt is prompt_lengths is repetition is frequency is presence is bias_ids is bias is allowed is allowed_rows is out is None
+            and logits.dtype == torch.float32 and logits.dim() == 2 and logits.stride(1) == 1 and 0 not in logits.shape):
+        return logits   # (nothing to do)
     made = (_lib._serve_native.get("adjust_logits") or _lib.serve_native("adjust_logits"))(
         logits, tokens, lengths, prompt, prompt_lengths, repetition, frequency, presence, bias_ids, bias, allowed, allowed_rows, out)
     if made is not None:
