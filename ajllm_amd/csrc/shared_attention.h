@@ -475,39 +475,34 @@ __device__ __forceinline__ void meet_few_f32(const SharedAttention& a, Meeting<f
   row[0].fresh = true;
 #pragma unroll
   for (int t = 0; t < HD / 16; ++t) row[0].o[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  float4 k[KC];
-  part_t v[4][VC];
-  auto ask = [&](const Rows& from) __attribute__((always_inline)) {   // (past the last row: that one again)
+  struct Fetched {
+    float4 k[KC];
+    part_t v[4][VC];
+  };
+  auto ask = [&](const Rows& from, Fetched& to) __attribute__((always_inline)) {   // (past the last row: that one again)
     const float* keys = from.keys + min(r, from.rows - 1) * HD + 4 * g;
 #pragma unroll
-    for (int c = 0; c < KC; ++c) k[c] = *reinterpret_cast<const float4*>(keys + 16 * c);
+    for (int c = 0; c < KC; ++c) to.k[c] = *reinterpret_cast<const float4*>(keys + 16 * c);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float* values = from.values + min(4 * g + i, from.rows - 1) * HD + P * r;
 #pragma unroll
-      for (int c = 0; c < VC; ++c) v[i][c] = *reinterpret_cast<const part_t*>(values + 16 * P * c);
+      for (int c = 0; c < VC; ++c) to.v[i][c] = *reinterpret_cast<const part_t*>(values + 16 * P * c);
     }
+    __builtin_amdgcn_sched_barrier(0);
   };
-  const int blocks = blocks_of<16, kBoth>(w);
-  if (wave < blocks) ask(Rows(w, wave));
-  for (int n = wave; n < blocks; n += 4) {
+  auto meet = [&](int n, const Fetched& rows) __attribute__((always_inline)) {
     const Rows now(w, n);
     const int seen = (kBoth && !now.second ? w.end : limit) - now.at;   // of the block's rows
     f32x4_t even = f32x4_t{0.f, 0.f, 0.f, 0.f}, odd = even;
 #pragma unroll
     for (int c = 0; c < KC; ++c) {
-      even = __builtin_amdgcn_mfma_f32_16x16x4f32(k[c].x, q[c].x, even, 0, 0, 0);
-      odd = __builtin_amdgcn_mfma_f32_16x16x4f32(k[c].y, q[c].y, odd, 0, 0, 0);
-      even = __builtin_amdgcn_mfma_f32_16x16x4f32(k[c].z, q[c].z, even, 0, 0, 0);
-      odd = __builtin_amdgcn_mfma_f32_16x16x4f32(k[c].w, q[c].w, odd, 0, 0, 0);
+      even = __builtin_amdgcn_mfma_f32_16x16x4f32(rows.k[c].x, q[c].x, even, 0, 0, 0);
+      odd = __builtin_amdgcn_mfma_f32_16x16x4f32(rows.k[c].y, q[c].y, odd, 0, 0, 0);
+      even = __builtin_amdgcn_mfma_f32_16x16x4f32(rows.k[c].z, q[c].z, even, 0, 0, 0);
+      odd = __builtin_amdgcn_mfma_f32_16x16x4f32(rows.k[c].w, q[c].w, odd, 0, 0, 0);
     }
     f32x4_t sc[1] = {even + odd};
-    part_t values[4][VC];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int c = 0; c < VC; ++c) values[i][c] = v[i][c];
-    if (n + 4 < blocks) ask(Rows(w, n + 4));
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       if (4 * g + i >= seen) sc[0][i] = -INFINITY;
@@ -518,7 +513,18 @@ __device__ __forceinline__ void meet_few_f32(const SharedAttention& a, Meeting<f
 #pragma unroll
       for (int c = 0; c < VC; ++c)
 #pragma unroll
-        for (int e = 0; e < P; ++e) row[0].o[c * P + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(values[i][c][e], p[i], row[0].o[c * P + e], 0, 0, 0);
+        for (int e = 0; e < P; ++e) row[0].o[c * P + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(rows.v[i][c][e], p[i], row[0].o[c * P + e], 0, 0, 0);
+  };
+  // two blocks' registers in turn, the next one's rows on their way while one is worked on
+  const int blocks = blocks_of<16, kBoth>(w);
+  Fetched even_rows, odd_rows;
+  if (wave < blocks) ask(Rows(w, wave), even_rows);
+  for (int n = wave; n < blocks; n += 8) {
+    if (n + 4 < blocks) ask(Rows(w, n + 4), odd_rows);
+    meet(n, even_rows);
+    if (n + 4 >= blocks) break;
+    if (n + 8 < blocks) ask(Rows(w, n + 8), even_rows);
+    meet(n + 4, odd_rows);
   }
   // a lane has components 16 P v + P (4 g + i) + e of query r: of each v 4 P of them one behind the other
   join_waves<HD, 1, few_join_bytes<HD, 1>(), kBoth>(a, w, lds, row, [&](int, float* to) {
