@@ -36,6 +36,12 @@ struct SharedAttention {
   Divide by_prefix_tiles, by_prefix_parts, by_own_tiles, by_own_parts;
 };
 
+// a number that every lane of a workgroup reads, kept where such numbers are
+__device__ __forceinline__ long long read_uniform(const long long* p) {
+  const unsigned long long v = (unsigned long long)*p;
+  return (long long)((unsigned long long)(uint32_t)__builtin_amdgcn_readfirstlane((int)v) |
+                     (unsigned long long)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32);
+}
 __device__ __forceinline__ int held(long long n, int most) { return (int)min(max(n, 0ll), (long long)most); }
 
 // What a workgroup works on: a tile of the queries that meet one run of rows.
@@ -84,41 +90,50 @@ __device__ __forceinline__ void to_halves(const u32x4_t& x, u32x4_t* to) { to[0]
 // The running softmax of 16 queries, one a lane & 15: m, the lane's own part of the sum, and HD / 16 accumulators of O^T.
 template <int HD> struct RunningRow {
   f32x4_t o[HD / 16];
-  float m, l;
-  bool fresh;   // no visible row met yet
-};
-
-// N exponents' products (N 16-key tiles of scores, scaled here) -> probabilities.  The reference point m moves where a lane's sum passes
-// kPfTrigger, to the largest exponent where that is past the slack (prefill_attention.h).
-template <int HD, int N>
-__device__ __forceinline__ void to_probabilities(RunningRow<HD>& row, const f32x4_t (&sc)[N], float scale2, float (&p)[4 * N]) {
-  float x[4 * N], sum = 0.f;
+  float m, l;   // (m: -inf while no visible row has been met)
+  // as a part's: nothing met weighs nothing, unless it was no number
+  __device__ __forceinline__ float2 part(float all) const { return float2{m == -INFINITY && all != 0.f ? 0.f : m, all}; }
+  __device__ __forceinline__ void clear() {
+    m = -INFINITY;
+    l = 0.f;
 #pragma unroll
-  for (int e = 0; e < 4 * N; ++e) {
-    x[e] = __builtin_fmaf(sc[e >> 2][e & 3], scale2, -row.m);
-    p[e] = exp2_hw(x[e]);
+    for (int t = 0; t < HD / 16; ++t) o[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  }
+};
+// Where a lane's sum of new probabilities has outgrown the reference point (or is no number: there is none yet): it moves to the largest of a query's scores if
+// that is past the slack, and what has been summed up follows.  sc: N scores not scaled yet -> p and their sum.
+template <int HD, int N, bool kSums>
+__device__ __forceinline__ void move_point(RunningRow<HD>& row, const f32x4_t* sc, float scale2, float* p, float& sum) {
+  float top = sc[0][0];
+#pragma unroll
+  for (int e = 1; e < N; ++e) top = fmaxf(top, sc[e >> 2][e & 3]);
+  top = quad_max(top) * scale2;
+  const float m = top > row.m + kPfSlack ? top : row.m;   // (nothing is more than -inf by no number)
+  const float corr = m == row.m ? 1.0f : exp2_hw(row.m - m);
+  sum = 0.f;
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    p[e] = exp2_hw(m == -INFINITY ? sc[e >> 2][e & 3] : __builtin_fmaf(sc[e >> 2][e & 3], scale2, -m));   // (0, or NaN, while there is none)
     sum += p[e];
   }
-  if (__builtin_amdgcn_ballot_w64(row.fresh || sum > kPfTrigger) != 0) {
-    float mx = x[0];
-#pragma unroll
-    for (int e = 1; e < 4 * N; ++e) mx = fmaxf(mx, x[e]);
-    mx = quad_max(mx);
-    const bool move = row.fresh ? mx > -INFINITY : mx > kPfSlack;
-    const float shift = move ? mx : 0.f;
-    const float corr = move && !row.fresh ? exp2_hw(-shift) : 1.0f;
-    sum = 0.f;
-#pragma unroll
-    for (int e = 0; e < 4 * N; ++e) {
-      p[e] = exp2_hw(x[e] - shift);
-      sum += p[e];
-    }
-    row.m += shift;
-    row.l *= corr;
-    row.fresh = row.fresh && !move;
+  row.m = m;
+  row.l *= corr;
+  if (kSums) {
 #pragma unroll
     for (int t = 0; t < HD / 16; ++t) row.o[t] *= corr;
   }
+}
+
+// N 16-key tiles of scores, scaled here -> probabilities.  (The test of the sum: prefill_attention.h.)
+template <int HD, int N>
+__device__ __forceinline__ void to_probabilities(RunningRow<HD>& row, const f32x4_t (&sc)[N], float scale2, float (&p)[4 * N]) {
+  float sum = 0.f;
+#pragma unroll
+  for (int e = 0; e < 4 * N; ++e) {
+    p[e] = exp2_hw(__builtin_fmaf(sc[e >> 2][e & 3], scale2, -row.m));
+    sum += p[e];
+  }
+  if (__builtin_amdgcn_ballot_w64(!(sum <= kPfTrigger)) != 0) move_point<HD, 4 * N, true>(row, sc, scale2, p, sum);
   row.l += sum;
 }
 
@@ -150,10 +165,10 @@ __device__ __forceinline__ void find_rows(const SharedAttention& a, Meeting<Cach
   int rows;
   w.before = 0;
   if (w.own) {
-    w.before = a.rows[w.outer] + (a.offset ? *a.offset : 0ll);
-    rows = held(w.before + (a.counts ? held(a.counts[w.outer], a.tokens) : a.tokens), a.max_len);
+    w.before = read_uniform(a.rows + w.outer) + (a.offset ? read_uniform(a.offset) : 0ll);
+    rows = held(w.before + (a.counts ? held(read_uniform(a.counts + w.outer), a.tokens) : a.tokens), a.max_len);
   } else {
-    rows = held(a.prefix_lengths[w.outer], a.prefix_cap);
+    rows = held(read_uniform(a.prefix_lengths + w.outer), a.prefix_cap);
   }
   const int per = ((rows + w.parts - 1) / w.parts + 31) & ~31;
   w.begin = (int)min((long long)rows, (long long)w.part * per);
@@ -168,10 +183,10 @@ __device__ __forceinline__ void find_both(const SharedAttention& a, Meeting<Cach
   w.own_keys = w.keys;
   w.own_values = w.values;
   w.own = false;
-  w.before = a.rows[w.outer] + (a.offset ? *a.offset : 0ll);
-  w.own_end = held(w.before + (a.counts ? held(a.counts[w.outer], a.tokens) : a.tokens), a.max_len);
+  w.before = read_uniform(a.rows + w.outer) + (a.offset ? read_uniform(a.offset) : 0ll);
+  w.own_end = held(w.before + (a.counts ? held(read_uniform(a.counts + w.outer), a.tokens) : a.tokens), a.max_len);
   w.begin = 0;
-  w.end = held(a.prefix_lengths[group], a.prefix_cap);
+  w.end = held(read_uniform(a.prefix_lengths + group), a.prefix_cap);
   const size_t at = (size_t)group * a.prefix_group + (size_t)w.key_head * a.prefix_head;
   w.keys = reinterpret_cast<const CacheT*>(a.prefix_keys) + at;
   w.values = reinterpret_cast<const CacheT*>(a.prefix_values) + at;
@@ -200,7 +215,7 @@ __device__ __forceinline__ void join_waves(const SharedAttention& a, const Meeti
 #pragma unroll
   for (int u = 0; u < RT; ++u) {
     const float l = quad_sum(row[u].l);
-    if (g == 0) ml[wave * kJoin + 16 * u + r] = float2{row[u].fresh && l == 0.f ? -INFINITY : row[u].m, l};   // (NaN stays)
+    if (g == 0) ml[wave * kJoin + 16 * u + r] = row[u].part(l);
     put(u, sums + (wave * kJoin + 16 * u + r) * kPitch);
   }
   __syncthreads();
@@ -293,10 +308,7 @@ __device__ __forceinline__ void meet_few(const SharedAttention& a, Meeting<Cache
 #pragma unroll
   for (int u = 0; u < RT; ++u) {
     limit[u] = kBoth ? held(w.before + token[u] + 1, w.own_end) : w.own ? held(w.before + token[u] + 1, w.end) : w.end;
-    row[u].m = row[u].l = 0.f;
-    row[u].fresh = true;
-#pragma unroll
-    for (int t = 0; t < TT; ++t) row[u].o[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    row[u].clear();
   }
 
   // ---- rows on their way (past the last: the last again, which is there and finite)
@@ -471,10 +483,7 @@ __device__ __forceinline__ void meet_few_f32(const SharedAttention& a, Meeting<f
   const int limit = kBoth ? held(w.before + token + 1, w.own_end) : w.own ? held(w.before + token + 1, w.end) : w.end;
   using Rows = Block<HD, 16, kBoth, float>;
   RunningRow<HD> row[1];
-  row[0].m = row[0].l = 0.f;
-  row[0].fresh = true;
-#pragma unroll
-  for (int t = 0; t < HD / 16; ++t) row[0].o[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  row[0].clear();
   struct Fetched {
     float4 k[KC];
     part_t v[4][VC];
@@ -566,19 +575,15 @@ __device__ __forceinline__ void meet_many(const SharedAttention& a, const Walk<u
   const int r = lane & 15, g = lane >> 4;
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    row[u].m = row[u].l = 0.f;
-    row[u].fresh = true;
-#pragma unroll
-    for (int t = 0; t < TT; ++t) row[u].o[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    row[u].clear();
   }
   const int prefix_blocks = (w.rows[0] + 63) >> 6, blocks = prefix_blocks + ((w.rows[1] + 63) >> 6);
   if (blocks == 0) return;
 
   // ---- requests: 1 KiB of rows each; wave w takes rows kReqRows w .. of every group of 4 kReqRows.  Rows past a run's last: that one again.
   const int krow = kReqRows * wave + lane / C, slot = lane % C;
-  const uint32_t k_chunk = (uint32_t)(slot ^ (krow & (C - 1))) * 16u;
-  const uint32_t v_chunk = (uint32_t)((((slot >> 1) ^ (krow & (TT - 1))) << 1) | (slot & 1)) * 16u;
-  const uint32_t k_lane = (uint32_t)(krow * RB) + k_chunk, v_lane = (uint32_t)(krow * RB) + v_chunk;
+  const uint32_t k_lane = (uint32_t)(krow * RB) + (uint32_t)(slot ^ (krow & (C - 1))) * 16u;
+  const uint32_t v_lane = (uint32_t)(krow * RB) + (uint32_t)((((slot >> 1) ^ (krow & (TT - 1))) << 1) | (slot & 1)) * 16u;
   auto place = [&](bool values, int i, int stage) __attribute__((always_inline)) {
     return lds0 + (uint32_t)(stage * 2 * kTile + (values ? kTile : 0) + (wave + 4 * i) * 1024);
   };
@@ -586,28 +591,35 @@ __device__ __forceinline__ void meet_many(const SharedAttention& a, const Walk<u
     const bool own = j >= prefix_blocks;
     const int at = 64 * (own ? j - prefix_blocks : j), there = own ? w.rows[1] : w.rows[0];
     const uint16_t* from = (values ? (own ? w.values[1] : w.values[0]) : (own ? w.keys[1] : w.keys[0])) + (size_t)at * HD;
+    int l = lane;   // (formed again from the lane's number: no register of its own beside the steps)
+    asm volatile("" : "+v"(l));
+    const int row = kReqRows * wave + l / C, to = l % C;
+    const uint32_t chunk = values ? (uint32_t)((((to >> 1) ^ (row & (TT - 1))) << 1) | (to & 1)) * 16u : (uint32_t)(to ^ (row & (C - 1))) * 16u;
 #pragma unroll
     for (int i = 0; i < KS; ++i) {
-      const uint32_t k = (uint32_t)min(4 * kReqRows * i + krow, there - 1 - at) * (uint32_t)RB;
-      dma16(from, k + (values ? v_chunk : k_chunk), place(values, i, j & 1));
+      const uint32_t k = (uint32_t)min(4 * kReqRows * i + row, there - 1 - at) * (uint32_t)RB;
+      dma16(from, k + chunk, place(values, i, j & 1));
     }
   };
-  uint32_t k_rd[KS], v_rd[TT];
-#pragma unroll
-  for (int s = 0; s < KS; ++s) k_rd[s] = lds0 + (uint32_t)(r * RB + 16 * ((4 * s + g) ^ (r & (C - 1))));
+  // fragments in stage 0: k-step s at k_rd ^ 64 s, output tile t at v_rd ^ 32 t.  (The body keeps all of them; the steps that go one by one have no registers
+  // left for that: one that goes to memory there waits, with the memory's order, for every row on its way.)
   const int vkey = 4 * g + (r >> 2);
-#pragma unroll
-  for (int t = 0; t < TT; ++t) v_rd[t] = lds0 + (uint32_t)(kTile + vkey * RB + 32 * (t ^ (vkey & (TT - 1))) + 8 * (r & 3));
+  const uint32_t k_rd = lds0 + (uint32_t)(r * RB + 16 * (g ^ (r & (C - 1))));
+  const uint32_t v_rd = lds0 + (uint32_t)(kTile + vkey * RB + 32 * (vkey & (TT - 1)) + 8 * (r & 3));
 
   request(0, false);
   request(0, true);
   u32x4_t qf[U][KS][QH];
-  int limit[U];   // own rows that a lane's queries see
+  // own rows that query n of the walk sees
+  auto limit_of = [&](int n) __attribute__((always_inline)) {
+    int rest, unused;
+    divide(min(n, w.queries - 1), a.by_each, rest);
+    return held(w.before + divide(rest, a.by_share, unused) + 1, w.rows[1]);
+  };
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     int token;
     const long long at = query_place(a, w.key_head, w.first_sequence, min(w.first + 16 * (U * wave + u) + r, w.queries - 1), token);
-    limit[u] = held(w.before + token + 1, w.rows[1]);
 #pragma unroll
     for (int s = 0; s < KS; ++s) to_halves(load8_raw(reinterpret_cast<const QT*>(a.q) + at * HD + 32 * s + 8 * g), qf[u][s]);
   }
@@ -617,7 +629,7 @@ __device__ __forceinline__ void meet_many(const SharedAttention& a, const Walk<u
     for (int s = 0; s < KS; ++s)
 #pragma unroll
       for (int h = 0; h < QH; ++h) asm volatile("" : "+v"(qf[u][s][h]));
-  const int nearest = __builtin_amdgcn_readlane(limit[0], 0), farthest = __builtin_amdgcn_readlane(limit[U - 1], 63);  // of the wave's queries
+  const int nearest = limit_of(w.first + 16 * U * wave), farthest = limit_of(w.first + 16 * U * wave + 16 * U - 1);   // of the wave's queries
   // steps of this wave
   const int steps = w.first + 16 * U * wave >= w.queries ? 0 : farthest > 0 ? 2 * prefix_blocks + ((farthest + 31) >> 5) : (w.rows[0] + 31) >> 5;
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -626,7 +638,9 @@ __device__ __forceinline__ void meet_many(const SharedAttention& a, const Walk<u
 
   f32x4_t sn[U][2];  // products of the step ahead
   u32x4_t pf[U];     // probabilities of the step behind
-  auto key_frag = [&](int at, int i) __attribute__((always_inline)) { return pf_read128(k_rd[i >> 1] + (uint32_t)(at + (i & 1) * 16 * RB)); };
+  auto key_frag = [&](uint32_t base, int at, int i) __attribute__((always_inline)) {
+    return pf_read128((base ^ (uint32_t)(64 * (i >> 1))) + (uint32_t)(at + (i & 1) * 16 * RB));
+  };
   auto score = [&](const u32x4_t& kf, int i) __attribute__((always_inline)) {
 #pragma unroll
     for (int h = 0; h < QH; ++h)
@@ -636,6 +650,7 @@ __device__ __forceinline__ void meet_many(const SharedAttention& a, const Walk<u
   // Step t: products from the keys at k_at, values at v_at (kV: not in the very first), and req(piece)
   auto step = [&](int t, auto values, auto masked, int k_at, int v_at, auto req) __attribute__((always_inline)) {
     constexpr bool kV = decltype(values)::value;
+    constexpr int ahead = decltype(masked)::value ? 1 : kAhead;   // (the steps that go one by one have no registers for more)
     f32x4_t sc[U][2];
 #pragma unroll
     for (int u = 0; u < U; ++u)
@@ -643,22 +658,26 @@ __device__ __forceinline__ void meet_many(const SharedAttention& a, const Walk<u
       for (int jb = 0; jb < 2; ++jb) sc[u][jb] = sn[u][jb];
     u32x4_t kf[TT];
     u32x2_t vl[TT], vh[TT];
+    uint32_t k_base = k_rd, v_base = v_rd;
+    if (decltype(masked)::value) asm volatile("" : "+v"(k_base), "+v"(v_base));
     auto fetch = [&](int i) __attribute__((always_inline)) {
-      kf[i] = key_frag(k_at, i);
+      kf[i] = key_frag(k_base, k_at, i);
       if (kV) {
-        vl[i] = pf_read_tr(v_rd[i] + (uint32_t)v_at);
-        vh[i] = pf_read_tr(v_rd[i] + (uint32_t)(v_at + 16 * RB));
+        vl[i] = pf_read_tr((v_base ^ (uint32_t)(32 * i)) + (uint32_t)v_at);
+        vh[i] = pf_read_tr((v_base ^ (uint32_t)(32 * i)) + (uint32_t)(v_at + 16 * RB));
       }
     };
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) fetch(i);
+    for (int i = 0; i < ahead; ++i) fetch(i);
     if (decltype(masked)::value) {
       const bool own = (t >> 1) >= prefix_blocks;
       const int at = 32 * (t - (own ? 2 * prefix_blocks : 0));
       if (at + 32 > (own ? nearest : w.rows[0])) {
+        int l = lane;
+        asm volatile("" : "+v"(l));
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          const int last = (own ? limit[u] : w.rows[0]) - at - 4 * g;
+          const int last = (own ? limit_of(w.first + 16 * (U * wave + u) + (l & 15)) : w.rows[0]) - at - 4 * (l >> 4);
 #pragma unroll
           for (int jb = 0; jb < 2; ++jb)
 #pragma unroll
@@ -673,7 +692,7 @@ __device__ __forceinline__ void meet_many(const SharedAttention& a, const Walk<u
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int i = 0; i < TT; ++i) {
-      if (i + kAhead < TT) fetch(i + kAhead);
+      if (i + ahead < TT) fetch(i + ahead);
       req(i);
       score(kf[i], i);
 #pragma unroll
@@ -696,31 +715,9 @@ __device__ __forceinline__ void meet_many(const SharedAttention& a, const Walk<u
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (__builtin_amdgcn_ballot_w64(row[u].fresh || psum[u] > kPfTrigger) != 0) {
-        float x[8], mx = -INFINITY;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          x[e] = __builtin_fmaf(sc[u][e >> 2][e & 3], a.scale2, -row[u].m);
-          mx = fmaxf(mx, x[e]);
-        }
-        mx = quad_max(mx);
-        const bool move = row[u].fresh ? mx > -INFINITY : mx > kPfSlack;
-        const float shift = move ? mx : 0.f;
-        const float corr = move && !row[u].fresh ? exp2_hw(-shift) : 1.0f;
-        psum[u] = 0.f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          p[u][e] = exp2_hw(x[e] - shift);
-          psum[u] += p[u][e];
-        }
+      if (__builtin_amdgcn_ballot_w64(!(psum[u] <= kPfTrigger)) != 0) {
+        move_point<HD, 8, kV>(row[u], sc[u], a.scale2, p[u], psum[u]);
         pn[u] = pack8_bf16(p[u]);
-        row[u].m += shift;
-        row[u].fresh = row[u].fresh && !move;
-        row[u].l *= corr;
-        if (kV) {
-#pragma unroll
-          for (int tt = 0; tt < TT; ++tt) row[u].o[tt] *= corr;
-        }
       }
       row[u].l += psum[u];
       pf[u] = pn[u];
@@ -728,10 +725,12 @@ __device__ __forceinline__ void meet_many(const SharedAttention& a, const Walk<u
   };
   auto last_values = [&](int v_at) __attribute__((always_inline)) {
     u32x2_t vl[TT], vh[TT];
+    uint32_t v_base = v_rd;
+    asm volatile("" : "+v"(v_base));
 #pragma unroll
     for (int i = 0; i < TT; ++i) {
-      vl[i] = pf_read_tr(v_rd[i] + (uint32_t)v_at);
-      vh[i] = pf_read_tr(v_rd[i] + (uint32_t)(v_at + 16 * RB));
+      vl[i] = pf_read_tr((v_base ^ (uint32_t)(32 * i)) + (uint32_t)v_at);
+      vh[i] = pf_read_tr((v_base ^ (uint32_t)(32 * i)) + (uint32_t)(v_at + 16 * RB));
     }
 #pragma unroll
     for (int i = 0; i < TT; ++i) {
@@ -746,7 +745,7 @@ __device__ __forceinline__ void meet_many(const SharedAttention& a, const Walk<u
   if (steps > 0) {
     u32x4_t kf[TT];
 #pragma unroll
-    for (int i = 0; i < TT; ++i) kf[i] = key_frag(0, i);
+    for (int i = 0; i < TT; ++i) kf[i] = key_frag(k_rd, 0, i);
 #pragma unroll
     for (int i = 0; i < TT; ++i) score(kf[i], i);
     step(0, no, yes, 32 * RB, 0, none);
@@ -808,7 +807,7 @@ __device__ __forceinline__ void leave_part(const SharedAttention& a, const Walk<
     if (n >= w.queries) continue;
     int token;
     const long long place = query_place(a, w.key_head, w.first_sequence, n, token) + part * a.queries;
-    if (g == 0) a.part_ml[place] = float2{row[u].fresh && l == 0.f ? -INFINITY : row[u].m, l};
+    if (g == 0) a.part_ml[place] = row[u].part(l);
 #pragma unroll
     for (int t = 0; t < HD / 16; ++t) *reinterpret_cast<f32x4_t*>(a.part_sums + place * HD + 16 * t + 4 * g) = row[u].o[t];
   }
@@ -888,12 +887,12 @@ __global__ __launch_bounds__(256, 2) void shared_attention_walk_kernel(SharedAtt
   w.first_sequence = b;
   w.queries = a.tokens * share;
   w.first = 64 * U * tile;
-  w.before = a.rows[b] + (a.offset ? *a.offset : 0ll);
-  const int there = a.counts ? held(a.counts[b], a.tokens) : a.tokens;
+  w.before = read_uniform(a.rows + b) + (a.offset ? read_uniform(a.offset) : 0ll);
+  const int there = a.counts ? held(read_uniform(a.counts + b), a.tokens) : a.tokens;
   const int last = min(divide(w.first + 64 * U - 1, a.by_share, unused), there - 1);          // the tile's last token that is there
   const size_t at = (size_t)group * a.prefix_group + (size_t)hk * a.prefix_head, own = (size_t)b * a.cache_batch + (size_t)hk * a.cache_head;
   const bool none = w.first >= there * share;
-  const int prefix_rows = none ? 0 : held(a.prefix_lengths[group], a.prefix_cap), own_rows = none ? 0 : held(w.before + last + 1, a.max_len);
+  const int prefix_rows = none ? 0 : held(read_uniform(a.prefix_lengths + group), a.prefix_cap), own_rows = none ? 0 : held(w.before + last + 1, a.max_len);
   // this part's blocks: first .. first + many - 1 of the prefix's and the sequence's own
   const int prefix_blocks = (prefix_rows + 63) >> 6, blocks = prefix_blocks + ((own_rows + 63) >> 6), per = (blocks + parts - 1) / parts;
   const int first = min(blocks, part * per), many = min(blocks - first, per);
