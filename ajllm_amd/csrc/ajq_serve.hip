@@ -120,7 +120,10 @@ SharedPlan shared_plan(const ajqs_shared_attention_args* a) {
   p.queries = (long long)a->batch * a->heads * a->tokens;
   if (bf16 && mine > 64) {
     p.form = SharedForm::walk;
-    p.own_rt = a->q_dtype == AJQS_F32 ? 1 : 2;   // (two bf16 for a query component leave no registers for two tiles)
+    // Tiles of 128 queries (bf16 ones of 128 components: more do not leave registers, narrower heads' steps are too short) where there are enough of them and
+    // most rows are the prefix's; else of 64.  16 sequences of 100 tokens x 4 behind 2048 rows 74 us, 90 with tiles of 64; of 400 behind 2048 229 and 292; of 100
+    // behind 100 + 1400 74 and 47; 8 of 40 behind 1000 24 and 21; 12 heads of 64, 16 of 300 behind 2048: 68 and 58.
+    p.own_rt = a->q_dtype == AJQS_BF16 && a->dim == 128 && a->prefix_cap >= a->max_len && own_units * ceil_div(mine, 128) >= 256 ? 2 : 1;
     p.own_tiles = (int)ceil_div(mine, 64 * p.own_rt);
     p.own_parts = parts(own_units * p.own_tiles, 512, (long long)a->prefix_cap + a->max_len, 128, kMostParts);
     p.own_blocks = ceil_div(own_units, 8) * 8 * p.own_tiles * p.own_parts;
@@ -304,7 +307,13 @@ int ajqs_shared_attention(const ajqs_shared_attention_args* a, void* workspace, 
         using CacheT = decltype(cache);
         if constexpr (sizeof(CacheT) == 2) {
           if (p.form == SharedForm::walk) {
-            status = launch_walk<HD, QT, sizeof(QT) == 4 ? 1 : 2>(s, p, (hipStream_t)stream, what);
+            if constexpr (HD == 128 && sizeof(QT) == 2) {
+              if (p.own_rt == 2) {
+                status = launch_walk<HD, QT, 2>(s, p, (hipStream_t)stream, what);
+                return;
+              }
+            }
+            status = launch_walk<HD, QT, 1>(s, p, (hipStream_t)stream, what);
             return;
           }
           if (p.form == SharedForm::many) {

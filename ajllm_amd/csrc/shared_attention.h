@@ -750,48 +750,60 @@ __device__ __forceinline__ void meet_many(const SharedAttention& a, const Walk<u
     for (int i = 0; i < TT; ++i) score(kf[i], i);
     step(0, no, yes, 32 * RB, 0, none);
   }
-  // The prefix's blocks j (even) and j + 1 at places known to the compiler: the second step of j, both of j + 1, the first of j + 2, while what they ask for and
-  // multiply is whole blocks.
-  int j = 0;
-  const int whole = w.rows[0] >> 6;
-  const char* k_from = reinterpret_cast<const char*>(w.keys[0]) + 2 * kTile;
-  const char* v_from = reinterpret_cast<const char*>(w.values[0]) + kTile;
-  if (2 * j + 5 < steps && j + 4 <= whole) {
-    // lines: of the keys waves 0 and 1, of the values 2 and 3, of block j + 4 (of the last whole one, at most)
-    const uint32_t corner = lds0 + (uint32_t)(4 * kTile + 256 * wave);
-    const uint32_t line = (uint32_t)((64 * (wave & 1) + lane) * (RB / 2));
-    const char* lines = reinterpret_cast<const char*>(wave < 2 ? w.keys[0] : w.values[0]);
-    auto touch = [&](int block) __attribute__((always_inline)) { dma4(lines + (size_t)min(block, whole - 1) * kTile, line, corner); };
-    touch(4);
-    do {
+  // Blocks j (even) and j + 1 of a run at places known to the compiler: the second step of j, both of j + 1, the first of j + 2, while what they ask for and
+  // multiply is whole blocks that all of the wave's queries see.  The others one by one.
+  // (Two tiles of queries leave no registers to do so with the second run's: its steps all go one by one.)
+  constexpr int kRuns = U == 1 ? 2 : 1;
+  int t = 1;
+#pragma unroll 1
+  for (int run = 0; run < kRuns; ++run) {
+    int j = t >> 1;
+    const int ahead_of_run = run ? prefix_blocks : 0, whole = (run ? w.rows[1] : w.rows[0]) >> 6;
+    const int last = min(ahead_of_run + min(whole - 4, run ? ((nearest - 32) >> 6) - 2 : whole), (steps - 6) >> 1);   // the last such j
+    if (j <= last) {
+      const char* const keys = reinterpret_cast<const char*>(run ? w.keys[1] : w.keys[0]);
+      const char* const values = reinterpret_cast<const char*>(run ? w.values[1] : w.values[0]);
+      const char* k_from = keys + (size_t)(j - ahead_of_run + 2) * kTile;
+      const char* v_from = values + (size_t)(j - ahead_of_run + 1) * kTile;
+      // lines: of the keys waves 0 and 1, of the values 2 and 3, of block j + 4 (of the last whole one, at most)
+      const uint32_t corner = lds0 + (uint32_t)(4 * kTile + 256 * wave);
+      const uint32_t line = (uint32_t)((64 * (wave & 1) + lane) * (RB / 2));
+      auto touch = [&](int block) __attribute__((always_inline)) {
+        dma4((wave < 2 ? keys : values) + (size_t)min(block - ahead_of_run, whole - 1) * kTile, line, corner);
+      };
+      touch(j + 4);
+      do {
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        asm volatile("s_waitcnt vmcnt(1)" ::: "memory");   // (all but the touch)
-        turn_barrier();
-        step(2 * j + 2 * x + 1, yes, no, (x ^ 1) * 2 * kTile, x * 2 * kTile, [&](int i) __attribute__((always_inline)) {
-          if (i < KS) dma16(k_from + i * 4096, k_lane, place(false, i, x));
-          else dma16(v_from + (i - KS) * 4096, v_lane, place(true, i - KS, x ^ 1));
-          if (i == TT - 1) touch(j + x + 5);
-        });
-        k_from += kTile;
-        v_from += kTile;
-        step(2 * j + 2 * x + 2, yes, no, (x ^ 1) * 2 * kTile + 32 * RB, x * 2 * kTile + 32 * RB, none);
-      }
-      j += 2;
-    } while (2 * j + 5 < steps && j + 4 <= whole);
-  }
-  for (int t = 2 * j + 1; t < 2 * blocks; ++t) {
-    const int block = t >> 1;
-    if (t & 1) {
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      turn_barrier();
-      if (block + 2 < blocks) request(block + 2, false);
-      if (block + 1 < blocks) request(block + 1, true);
+        for (int x = 0; x < 2; ++x) {
+          asm volatile("s_waitcnt vmcnt(1)" ::: "memory");   // (all but the touch)
+          turn_barrier();
+          step(2 * j + 2 * x + 1, yes, no, (x ^ 1) * 2 * kTile, x * 2 * kTile, [&](int i) __attribute__((always_inline)) {
+            if (i < KS) dma16(k_from + i * 4096, k_lane, place(false, i, x));
+            else dma16(v_from + (i - KS) * 4096, v_lane, place(true, i - KS, x ^ 1));
+            if (i == TT - 1) touch(j + x + 5);
+          });
+          k_from += kTile;
+          v_from += kTile;
+          step(2 * j + 2 * x + 2, yes, no, (x ^ 1) * 2 * kTile + 32 * RB, x * 2 * kTile + 32 * RB, none);
+        }
+        j += 2;
+      } while (j <= last);
     }
-    auto half = [&](int n) { return ((n >> 1) & 1) * 2 * kTile + (n & 1) * 32 * RB; };  // where step n's keys (values) lie
-    // (the last step's products of the one behind it are of no use, whatever lies there)
-    if (t < steps) step(t, yes, yes, half(t + 1), half(t - 1), none);
-    else if (t == steps) last_values(half(t - 1));
+    // (the first run's up to where the second's whole blocks may begin, at an even block)
+    const int until = run + 1 == kRuns ? 2 * blocks : min(2 * blocks, 2 * max(j, (prefix_blocks + 1) & ~1) + 1);
+    for (t = 2 * j + 1; t < until; ++t) {
+      const int block = t >> 1;
+      if (t & 1) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        turn_barrier();
+        if (block + 2 < blocks) request(block + 2, false);
+        if (block + 1 < blocks) request(block + 1, true);
+      }
+      auto half = [&](int n) { return ((n >> 1) & 1) * 2 * kTile + (n & 1) * 32 * RB; };  // where step n's keys (values) lie
+      // (the last step's products of the one behind it are of no use, whatever lies there)
+      if (t < steps) step(t, yes, yes, half(t + 1), half(t - 1), none);
+      else if (t == steps) last_values(half(t - 1));
+    }
   }
   if (steps == 2 * blocks) last_values(((blocks - 1) & 1) * 2 * kTile + 32 * RB);
 }
