@@ -93,3 +93,31 @@ def adjust_logits(logits, tokens, lengths, prompt, prompt_lengths, repetition, f
                 if not (words[v // 32] >> (v % 32)) & 1:
                     x[b, v] = -math.inf
     return x, size
+
+
+def shared_prefix_attention_by_heads(q, prefix_keys, prefix_values, prefix_lengths, keys, values, rows, counts):
+    """The same of larger calls: (out, weight), float64 on q's device, all queries of a sequence and a key head at once."""
+    batch, heads, tokens, hd = q.shape
+    groups, kv, capacity, _ = prefix_keys.shape
+    max_len, share, each = keys.shape[2], heads // kv, batch // groups
+    out = torch.zeros(batch, tokens, heads, hd, dtype=torch.float64, device=q.device)
+    size = torch.zeros_like(out)
+    token = torch.arange(tokens, device=q.device)
+    for b in range(batch):
+        before = min(max(int(prefix_lengths[b // each]), 0), capacity)
+        many = tokens if counts is None else min(max(int(counts[b]), 0), tokens)
+        sees = (int(rows[b]) + token[:many] + 1).clamp(0, max_len)                       # own rows of each token
+        if many == 0 or before + int(sees.max()) == 0:
+            continue
+        own = int(sees.max())
+        hidden = torch.arange(before + own, device=q.device) >= before + sees[:, None]    # [many, rows]
+        nothing = (before + sees == 0)[:, None, None]
+        for k in range(kv):
+            ks = torch.cat((prefix_keys[b // each, k, :before], keys[b, k, :own])).double()
+            vs = torch.cat((prefix_values[b // each, k, :before], values[b, k, :own])).double()
+            x = q[b, k * share:(k + 1) * share, :many].double().transpose(0, 1)           # [many, share, hd]
+            score = (x.reshape(-1, hd) @ ks.t().contiguous()).view(many, share, -1) / math.sqrt(hd)
+            w = torch.softmax(score.masked_fill(hidden[:, None, :], -math.inf), dim=-1).masked_fill(nothing, 0.0).view(many * share, -1)
+            out[b, :many, k * share:(k + 1) * share] = (w @ vs).view(many, share, hd)
+            size[b, :many, k * share:(k + 1) * share] = (w @ vs.abs()).view(many, share, hd)
+    return out.view(batch, tokens, heads * hd), size.view(batch, tokens, heads * hd)

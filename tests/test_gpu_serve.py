@@ -239,6 +239,51 @@ def test_shared_attention_scores_far_apart(cuda, cache_type):
     _attention_near(got, want, size)
 
 
+def _share_by_heads(cuda, groups, batch, tokens, heads, kv, hd, prefix, max_len, q_type, cache_type, seed):
+    """Lengths, positions and counts at random, one sequence and one group full, one sequence without tokens; rows that nobody sees hold anything."""
+    gen = torch.Generator(device=cuda).manual_seed(seed)
+    randn = lambda *shape: torch.randn(shape, generator=gen, device=cuda)  # noqa: E731
+    whole = lambda low, high, n: torch.randint(low, high + 1, (n,), generator=gen, device=cuda)  # noqa: E731
+    q = randn(batch, heads, tokens, hd).to(q_type)
+    pk, pv = (randn(groups, kv, prefix, hd).to(cache_type) for _ in range(2))
+    k, v = (randn(batch, kv, max_len, hd).to(cache_type) for _ in range(2))
+    lengths, rows, counts = whole(prefix // 2, prefix, groups), whole(0, max_len - tokens, batch), whole((tokens + 1) // 2, tokens, batch)
+    lengths[-1], rows[0], counts[0] = prefix, max_len - tokens, tokens
+    if batch > 2:
+        counts[batch // 2] = 0
+    if groups > 2:
+        lengths[1] = 0
+    want, size = serve_plain.shared_prefix_attention_by_heads(q, pk, pv, lengths, k, v, rows, counts)
+    for g in range(groups):
+        pk[g, :, int(lengths[g]):], pv[g, :, int(lengths[g]):] = math.nan, math.inf
+    for b in range(batch):
+        last = int(rows[b]) + int(counts[b])
+        k[b, :, last:], v[b, :, last:] = math.inf, math.nan
+    got = attention.shared_prefix_attention(q, pk, pv, lengths, k, v, rows, counts=counts)
+    _attention_near(got, want.cpu(), size.cpu())
+
+
+FEW = [   # (groups, batch, tokens, heads, kv, prefix, max_len): one and two tiles of queries a wave, for the prefix and for own rows; one launch and two
+    (1, 2, 1, 8, 2, 900, 70), (1, 9, 1, 8, 2, 900, 70), (1, 2, 7, 8, 2, 900, 70), (3, 6, 1, 16, 4, 700, 600), (2, 4, 5, 4, 4, 1300, 9),
+    (1, 2, 1, 8, 2, 100, 70), (1, 2, 7, 8, 2, 100, 70), (1, 2, 40, 6, 1, 1000, 300),
+]
+MANY = [   # tiles of 64 and of 128 queries for the prefix, of 16 and of 32 for own rows
+    (1, 40, 1, 8, 2, 900, 70), (3, 33, 1, 24, 2, 1000, 300), (1, 9, 7, 8, 2, 1500, 200), (1, 130, 1, 8, 2, 8200, 40), (2, 64, 9, 8, 2, 8500, 60),
+]
+WALK = [   # several parts and one, most rows before or in the sequences' own, odd and even numbers of blocks
+    (1, 2, 70, 4, 2, 500, 900), (2, 6, 33, 8, 2, 1000, 40), (1, 16, 64, 32, 8, 700, 300), (1, 16, 90, 32, 8, 1290, 200), (2, 32, 70, 8, 4, 130, 1000),
+    (1, 32, 70, 8, 4, 64, 1000), (4, 32, 70, 8, 4, 700, 700), (1, 40, 150, 8, 8, 3, 777),
+]
+
+
+@pytest.mark.parametrize("hd", [128, 64, 32])
+@pytest.mark.parametrize("q_type", [F32, BF16])
+@pytest.mark.parametrize("cache_type,case", [(t, c) for c in FEW for t in (F32, BF16)] + [(BF16, c) for c in MANY + WALK])
+def test_shared_attention_tiles_and_parts(cuda, hd, q_type, cache_type, case):
+    groups, batch, tokens, heads, kv, prefix, max_len = case
+    _share_by_heads(cuda, groups, batch, tokens, heads, kv, hd, prefix, max_len, q_type, cache_type, seed=hd + batch + tokens)
+
+
 def test_shared_attention_offsets_past_32_bits(cuda):
     """A prefix of more than 2^31 elements a head, of which the last row alone weighs; caches more than 2^31 elements apart."""
     hd, rows = 32, 2 ** 31 // 32 + 100
