@@ -112,7 +112,8 @@ def norm_rope(qkv: torch.Tensor, cosine: torch.Tensor, sine: torch.Tensor, keys:
     ``rows[b] + offset + t`` of its caches and turns by position ``positions[b] + offset + t`` (``positions`` None: the row); ``rows``,
     ``positions`` and ``counts`` int64 ``[B]``, ``offset`` one int64, all on the device.  Of the tokens of sequence b the first
     ``counts[b]`` are there (None: all); the others write no row, and zeros for queries.  A row outside the caches is not written, a
-    position is held inside the tables.  Returns the queries ``[B, heads, tokens, hd]`` in ``out_dtype``
+    position is held inside the tables; heads of the caches may not overlap.  Returns the queries ``[B, heads, tokens, hd]`` in ``out_dtype``,
+    without a gradient, as all of these functions
     (RMSNorm.forward, src/ajllm/modeling/layers.py:70-74, on every head, then attention.py:36-60)."""
     what = "norm_rope"
     if not qkv.is_cuda:
@@ -146,6 +147,15 @@ def norm_rope(qkv: torch.Tensor, cosine: torch.Tensor, sine: torch.Tensor, keys:
         status = _lib.load_serve().ajqs_norm_rope(ctypes.byref(args), torch.cuda.current_stream().cuda_stream)
     _lib.check_serve(status, what)
     return q
+
+
+def shared_prefix_launches(batch: int, heads: int, tokens: int, prefix_keys: torch.Tensor, keys: torch.Tensor, q_dtype: torch.dtype = torch.float32) -> int:
+    """Kernel launches of ``shared_prefix_attention`` on such caches: two where what its workgroups make of a query is put together by a second."""
+    at = keys.data_ptr()
+    args = _lib.SharedAttentionArgs(at, at, at, at, at, at, at, None, None, at, prefix_keys.stride(0), prefix_keys.stride(1), keys.stride(0), keys.stride(1),
+                                    prefix_keys.shape[0], batch, tokens, heads, keys.shape[1], keys.shape[3], prefix_keys.shape[2], keys.shape[2],
+                                    _TYPES[q_dtype], _TYPES[keys.dtype])
+    return 2 if _lib.load_serve().ajqs_shared_attention_workspace(ctypes.byref(args)) else 1
 
 
 def shared_prefix_attention(q: torch.Tensor, prefix_keys: torch.Tensor, prefix_values: torch.Tensor, prefix_lengths: torch.Tensor,

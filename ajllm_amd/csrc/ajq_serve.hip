@@ -3,6 +3,7 @@
 #include <math.h>
 #include <stdarg.h>
 #include <stdio.h>
+#include <stdlib.h>
 
 #include "../../include/ajq_serve.h"
 #include "ajq_common.h"
@@ -55,6 +56,29 @@ int check_caches(const char* what, const void* keys, const void* values, long lo
     return fail(AJQ_ERR_ALIGN, "%s: caches must be 16-byte aligned, their strides multiples of 8 elements", what);
   if (outer < 0 || head < 0) return fail(AJQ_ERR_SHAPE, "%s: negative cache stride", what);
   return AJQ_OK;
+}
+
+// Whether one of the blocks of `size` numbers at i * outer + j * inner (i < n, j < m) meets one of the same blocks moved by d numbers (d 0: another one).
+bool blocks_meet(long long d, long long outer, long long n, long long inner, long long m, long long size) {
+  const bool nested = (m == 1 || inner >= size) && (n == 1 || outer >= (m - 1) * inner + size);
+  const bool crossed = (n == 1 || outer >= size) && (m == 1 || inner >= (n - 1) * outer + size);
+  if ((nested || crossed) && (d == 0 || std::abs(d) >= (n - 1) * outer + (m - 1) * inner + size)) return false;
+  for (long long j = 1 - m; j < m; ++j) {
+    const long long x = d + j * inner, near = outer ? -x / outer : 0;
+    for (long long i = near - 1; i <= near + 1; ++i) {
+      const long long k = std::max(1 - n, std::min(i, n - 1));
+      if (std::abs(x + k * outer) < size && (d != 0 || j != 0 || k != 0)) return true;
+    }
+  }
+  return false;
+}
+// The same of one row-major matrix and another.
+bool rows_meet(const void* a, long long a_pitch, long long a_bytes, const void* b, long long b_pitch, long long b_bytes, long long rows) {
+  const long long d = (long long)(reinterpret_cast<uintptr_t>(b) - reinterpret_cast<uintptr_t>(a));   // (bytes)
+  if (d >= (rows - 1) * a_pitch + a_bytes || -d >= (rows - 1) * b_pitch + b_bytes) return false;
+  if (rows == 1 || a_pitch != b_pitch) return true;   // (pitches that differ: taken to meet)
+  const long long r = (d % a_pitch + a_pitch) % a_pitch;
+  return r < a_bytes || a_pitch - r < b_bytes;
 }
 
 constexpr int kMostRows = 1 << 30;   // of a cache head
@@ -258,8 +282,13 @@ int ajqs_norm_rope(const ajqs_norm_rope_args* a, void* stream) {
   if (!aligned16(a->qkv) || !aligned16(a->q) || !aligned16(a->cosine) || !aligned16(a->sine) || !aligned16(a->q_gain) || !aligned16(a->k_gain))
     return fail(AJQ_ERR_ALIGN, "%s: qkv, q, the tables and the gains must be 16-byte aligned", what);
   if (int e = check_caches(what, a->keys, a->values, a->cache_batch, a->cache_head)) return e;
-  if ((a->kv_heads > 1 && a->cache_head < room) || (a->batch > 1 && a->cache_batch < room))
+  if (blocks_meet(0, a->cache_batch, a->batch, a->cache_head, a->kv_heads, room))
     return fail(AJQ_ERR_SHAPE, "%s: cache heads that overlap cannot be written", what);
+  const int size = a->cache_dtype == AJQS_BF16 ? 2 : 4;
+  const long long d = (long long)(reinterpret_cast<uintptr_t>(a->values) - reinterpret_cast<uintptr_t>(a->keys)) / size;
+  if (d == 0 || blocks_meet(d, a->cache_batch, a->batch, a->cache_head, a->kv_heads, room))
+    return fail(AJQ_ERR_SHAPE, "%s: keys and values that overlap cannot be written", what);
+  if (!(a->eps >= 0.f)) return fail(AJQ_ERR_SHAPE, "%s: epsilon %g", what, a->eps);
   const NormRope n{a->qkv, a->cosine, a->sine, a->q_gain, a->k_gain, int64s(a->rows), int64s(a->positions), int64s(a->counts),
                    int64s(a->offset), a->keys, a->values, a->q, a->ld, a->cache_batch, a->cache_head, a->tokens, a->heads, a->kv_heads,
                    a->max_len, a->table_rows, a->eps, divide_by(a->tokens)};
@@ -362,6 +391,9 @@ int ajqs_adjust_logits(const ajqs_adjust_logits_args* a, void* stream) {
     return fail(AJQ_ERR_SHAPE, "%s: %d masks for %d rows", what, a->masks, a->batch);
   if (!aligned4(a->out) || !aligned4(a->allowed) || (a->dtype == AJQS_F32 && !aligned4(a->logits)) || (reinterpret_cast<uintptr_t>(a->logits) & 1u))
     return fail(AJQ_ERR_ALIGN, "%s: logits, out and the masks must be aligned to their elements", what);
+  const int size = a->dtype == AJQS_BF16 ? 2 : 4;
+  if (a->logits != a->out && rows_meet(a->logits, a->ld * size, (long long)a->vocab * size, a->out, a->out_ld * 4, (long long)a->vocab * 4, a->batch))
+    return fail(AJQ_ERR_SHAPE, "%s: out overlaps the logits without being them", what);
   const bool words = (a->tokens && a->max_tokens) || (a->prompt && a->max_prompt) || (a->bias_ids && a->biases);
   // slices of 16384 tokens (two workgroups of 1024 lanes a CU then), smaller ones until there are two workgroups a CU
   int slice = 4 * kSliceThreads * kSlicePieces;

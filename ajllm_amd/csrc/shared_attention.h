@@ -882,7 +882,7 @@ __global__ __launch_bounds__(256, 2) void shared_attention_many_kernel(SharedAtt
   leave_part<HD, U>(a, walk, row, w.part);
 }
 
-// Sequences with many new tokens each: 128 queries of one sequence walk the prefix and then its own rows, and what comes out is the result.  With
+// Sequences with many new tokens each: 64 U queries of one sequence walk the prefix and then its own rows, and what comes out is the result.  With
 // own_parts > 1 the walk is cut up and leaves parts for the merge.
 template <int HD, typename QT, int U>
 __global__ __launch_bounds__(256, 2) void shared_attention_walk_kernel(SharedAttention a) {

@@ -15,7 +15,7 @@ import ctypes
 import torch
 
 from . import _lib, dense, modeling
-from .attention import norm_rope, prefill_attention, shared_prefix_attention
+from .attention import norm_rope, prefill_attention, shared_prefix_attention, shared_prefix_launches
 from .quant import QuantLinear, repack_w4, repack_w8, w4a16_matmul, w8a16_matmul
 from .sampling import adjust_logits
 
@@ -697,7 +697,7 @@ class FusedDecoder(GraphDecoder):
         return int(self.head_norm) + 1 + int(self.merge_launch)
 
     def launches_per_step(self) -> int:
-        """Kernel launches of one decode step as this decoder is configured."""
+        """Kernel launches of one decode step as this decoder is configured (without the one that ``set_penalties`` asks for)."""
         lib = _lib.load()
         if self.fuse_epilogue:
             # q|k|v, attention (+ merge), output projection, w1|w3 with the gate, w2; the first norm, head, pick
@@ -870,10 +870,9 @@ class SharedPrefixDecoder(FusedDecoder):
 
     @property
     def attention_launches(self) -> int:
-        return 3   # (norm and rotation, attention of the prefix's and the own rows, what puts them together)
+        return 1 + shared_prefix_launches(self.batch, self.heads, 1, self.prefix.keys[0], self.cache.keys[0])   # (the first: norm and rotation)
 
-    @staticmethod
-    def _padded(prompts: torch.Tensor | list[list[int]], count: int, longest: int, what: str) -> tuple[torch.Tensor, torch.Tensor]:
+    def _padded(self, prompts: torch.Tensor | list[list[int]], count: int, longest: int, what: str) -> tuple[torch.Tensor, torch.Tensor]:
         """Token lists as ``[count, T]``, padded with zeros, and their lengths."""
         if isinstance(prompts, torch.Tensor):
             if prompts.dim() != 2:
@@ -882,6 +881,8 @@ class SharedPrefixDecoder(FusedDecoder):
         lengths = [len(p) for p in prompts]
         if len(prompts) != count or min(lengths) < 1 or max(lengths) > longest:
             raise ValueError(f"{what}: {count} of 1 to {longest} tokens each expected")
+        if not all(0 <= v < self.vocab for p in prompts for v in p):
+            raise ValueError(f"{what}: tokens in [0, {self.vocab}) expected")
         return torch.tensor([list(p) + [0] * (max(lengths) - len(p)) for p in prompts]), torch.tensor(lengths)
 
     @torch.no_grad()

@@ -59,7 +59,7 @@ def adjust_logits(logits: torch.Tensor, *, tokens: torch.Tensor | None = None, l
 
     ``tokens`` and ``prompt`` are int64 ``[B, n]``, of which the first ``lengths`` (``prompt_lengths``) count: int64 on the device, one a row or
     one for all (a decoder's step counter), None: all of them.  Ids outside ``[0, V)`` are passed over.  ``repetition``, ``frequency`` and
-    ``presence`` are numbers or fp32 ``[B]``.  ``out`` may be ``logits`` itself where they are fp32; without it the rows of the result begin
+    ``presence`` are numbers or fp32 ``[B]``.  ``out`` may be ``logits`` itself where they are fp32 (and overlaps them in no other way); without it the rows of the result begin
     on 16-byte boundaries, as ``ajq_sample_pick`` wants them (fp32 logits that nothing is to happen to are returned as they are)."""
     if not logits.is_cuda:
         raise ValueError("adjust_logits needs tensors on a ROCm device (there is no CPU path)")

@@ -42,7 +42,8 @@ typedef struct {
  * key head x becomes x / sqrt(mean(x^2) + eps) * gain (q_gain, k_gain fp32 [dim]; NULL: as it is), then its pairs (x[2i], x[2i + 1])
  * turn by the tables' row positions[b] + *offset + t (positions NULL: rows; cosine, sine fp32 [table_rows, dim / 2]; held inside the
  * tables).  Queries go to q [batch, heads, tokens, dim] (zeros where a token is not there), keys and values to the token's row of the caches
- * (element strides cache_batch, cache_head); a row outside [0, max_len) is not written.  dim 128, 64 or 32.
+ * (element strides cache_batch, cache_head); a row outside [0, max_len) is not written.  dim 128, 64 or 32;
+ * no head of the caches may overlap another.
  * (RMSNorm.forward, src/ajllm/modeling/layers.py:70-74, on each head; RotaryPositionalEmbedding.forward, attention.py:36-60.) */
 int ajqs_norm_rope(const ajqs_norm_rope_args* args, void* stream);
 
@@ -77,7 +78,7 @@ typedef struct {
   int32_t batch, vocab, max_tokens, max_prompt, biases, masks, token_count_stride, prompt_count_stride;
   int32_t dtype;
 } ajqs_adjust_logits_args;
-/* out[b, v] (fp32, row stride out_ld; may be the fp32 logits themselves) from x = logits[b, v] (dtype, row stride ld):
+/* out[b, v] (fp32, row stride out_ld; may be the fp32 logits themselves, and overlap them in no other way) from x = logits[b, v] (dtype, row stride ld):
  *   x > 0 ? x / repetition[b] : x * repetition[b]   where v is among row b's prompt or tokens;
  *   x - (frequency[b] * n + presence[b])            where v is n > 0 times among its tokens;
  *   x + the sum of bias[b, i] over bias_ids[b, i] == v, in the order of i;

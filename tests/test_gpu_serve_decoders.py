@@ -86,10 +86,11 @@ def test_questions_behind_a_shared_text(cuda, kv_dtype, head_norm):
 
 def test_launches_of_a_step(cuda):
     model = _model(cuda)
-    dec = decoding.SharedPrefixDecoder(model, 1, 4, 32, 32)
-    assert dec.attention_launches == 3
     base = decoding.FusedDecoder(model, 4, 64)
-    assert dec.launches_per_step() == base.launches_per_step() + 2 * (3 - base.attention_launches)
+    for prefix_len, dtype, launches in ((32, torch.bfloat16, 2), (160, torch.float32, 3)):   # (few rows: attention in one launch)
+        dec = decoding.SharedPrefixDecoder(model, 1, 4, prefix_len, 40, dtype)
+        assert dec.attention_launches == launches
+        assert dec.launches_per_step() == base.launches_per_step() + 2 * (launches - base.attention_launches)
     assert decoding.FusedDecoder(_model(cuda, head_norm=True), 4, 64).launches_per_step() == base.launches_per_step() + 2
 
 
@@ -238,7 +239,7 @@ def test_refusals(cuda):
             decoding.SharedPrefixDecoder(**{**dict(model=model, prompts=1, completions=2, prefix_len=10, max_len=20), **bad})
     dec = decoding.SharedPrefixDecoder(model, 2, 2, 10, 20)
     for prompt, questions in ((_ids(1, 5), None), (_ids(1, 5, 11), None), (_ids(1, 5, 0), None), (_ids(1, 5, 5), _ids(2, 3, 3)), (_ids(1, 5, 5), _ids(2, 3, 3, 3, 20)),
-                              (torch.zeros(5), None)):
+                              (torch.zeros(5), None), ([[VOCAB], [1]], None), ([[1], [-1]], None), (_ids(1, 5, 5), [[1], [2], [3], [VOCAB]])):
         with pytest.raises(ValueError):
             dec.prefill(prompt, questions)
     dec.prefill(_ids(1, 5, 5), _ids(2, 3, 3, 3, 12))

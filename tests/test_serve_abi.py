@@ -88,6 +88,28 @@ def test_norm_rope_refuses(memory):
     for change in (dict(cache_head=512), dict(cache_batch=0)):
         _refused(call, _filled(_lib.NormRopeArgs, memory, **{**NORM, **change}), -2, "overlap")
     _refused(call, _filled(_lib.NormRopeArgs, memory, **{**NORM, "cache_head": -1024}), -2, "negative")
+    for change in (dict(cache_head=1024, cache_batch=1024), dict(cache_head=2048, cache_batch=2048), dict(cache_head=1032, cache_batch=1024),
+                   dict(batch=3, cache_head=4096, cache_batch=2048)):
+        _refused(call, _filled(_lib.NormRopeArgs, memory, **{**NORM, **change}), -2, "cache heads that overlap")
+
+
+def test_norm_rope_refuses_keys_and_values_that_overlap(memory):
+    """Against the definition: no element of one's heads is one of the other's.  (Layouts that are in order are refused for their epsilon's sake:
+    nothing is launched.)"""
+    call = _lib.load_serve().ajqs_norm_rope
+    heads = lambda at, b, h: {at + i * b + j * h + e for i in range(2) for j in range(2) for e in range(1024)}  # noqa: E731
+    met = set()
+    for d in (0, 8, 1016, 1024, 1032, 2048, 3064, 4096, 4104, 5120, 6144, 7160, 7168, 9000):
+        for batch, head in ((2048, 1024), (4096, 2048), (1024, 2048), (8192, 1024), (1024, 8192), (2048, 4096)):
+            meets = bool(heads(0, batch, head) & heads(d, batch, head))
+            met.add(meets)
+            args = _filled(_lib.NormRopeArgs, memory, **{**NORM, "values": memory + 4 * d, "cache_batch": batch, "cache_head": head})
+            if meets:
+                _refused(call, args, -2, "keys and values that overlap")
+            else:
+                args.eps = -1.0   # (the last check)
+                _refused(call, args, -2, "epsilon")
+    assert met == {False, True}
 
 
 SHARED = dict(prefix_group=2048, prefix_head=1024, cache_batch=2048, cache_head=1024, groups=2, batch=4, tokens=1, heads=4, kv_heads=2, dim=64,
@@ -139,3 +161,13 @@ def test_adjust_logits_refuses(memory):
         _refused(call, _filled(_lib.AdjustLogitsArgs, memory, **{**good, **change}), -2, message)
     for name, by in (("logits", 2), ("out", 1), ("allowed", 1)):
         _refused(call, _filled(_lib.AdjustLogitsArgs, memory, **{**good, name: memory + 512 + by}), -3, "aligned")
+
+
+def test_adjust_logits_refuses_an_overlapping_out(memory):
+    call = _lib.load_serve().ajqs_adjust_logits
+    good = {**LOGITS, "ld": 128, "out_ld": 128, "batch": 2}
+    for by in (4, 252, -4, -252, 512, 508, 516, 764):   # bytes; rows of 256 in a pitch of 512
+        args = _filled(_lib.AdjustLogitsArgs, memory + 1024, **{**good, "out": memory + 1024 + by})
+        _refused(call, args, -2, "out overlaps")
+    for change in (dict(out=memory + 1024 + 256, out_ld=64), dict(out=memory + 1024 + 64, dtype=1, ld=256), dict(out=memory + 1024 + 64, batch=1)):
+        _refused(call, _filled(_lib.AdjustLogitsArgs, memory + 1024, **{**good, **change}), -2, "out overlaps")
