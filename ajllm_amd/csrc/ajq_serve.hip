@@ -119,6 +119,7 @@ enum class SharedForm { few, many, walk, each };   // (the prefix by meet_few, b
 struct SharedPlan {
   SharedForm form;
   int prefix_rt, own_rt;            // tiles of 16 queries a wave
+  bool own_alone;                   // a wave a tile of own queries, not a workgroup
   int prefix_tiles, own_tiles, prefix_parts, own_parts;
   long long prefix_blocks, own_blocks, queries;
   size_t bytes;
@@ -128,10 +129,16 @@ constexpr int kMostParts = 64;      // a lane each in the merge
 // bf16, rows of prefix + own): 8 sequences of 64 rows 4.7 and 9.0 us, of 512 6.7 and 9.4, of 768 7.7 and 9.2, of 1536 11.5 and 11.5; 128 sequences of 64 9.0 and
 // 14.2, of 768 22.3 and 23.5, of 1536 49 and 39.  fp32 rows take longer in fp32: 8 of 64 6.3 and 11.2, of 192 8.5 and 11.5, of 512 14.4 and 12.9; 128 of 192 27.0
 // and 28.8.
-bool shared_each(const ajqs_shared_attention_args* a, long long workgroups) {
+// With more of them than 1024, each to a wave (below): 4096 of 50 rows 12.6 and 17.1, 1536 of 130 10.1 and 11.8, of 260 14.1 and 12.9.
+bool shared_each(const ajqs_shared_attention_args* a, long long tiles) {
   const long long rows = (long long)a->prefix_cap + a->max_len;
-  return workgroups <= 1024 && rows <= (a->cache_dtype == AJQS_BF16 ? 768 : 192);
+  if (a->cache_dtype == AJQS_BF16) return rows <= (tiles <= 1024 ? 768 : 128);
+  return rows <= (tiles <= 1024 ? 192 : 64);
 }
+// Whether a wave takes a tile of a sequence's queries by itself, with the `rows` rows that they meet: no join, four times as many at once, but the longest is one
+// wave's.  Behind a prefix, 1536 heads (128 sequences of 12 heads of 64) of 60 rows 9.9 and 13.5 us, of 200 16.6 and 17.4; of 128, of 300 rows 49.4 and 44.6;
+// 512 (64 of 8) of 60 18.4 and 18.7.  Everything in one walk: 768 of 130 rows 7.7 and 9.6, of 430 14.9 and 14.7; 512 of 130 7.7 and 6.5.
+bool shared_alone(long long tiles, long long rows, long long most) { return tiles >= 768 && rows <= most; }
 SharedPlan shared_plan(const ajqs_shared_attention_args* a) {
   SharedPlan p{};
   const long long share = a->heads / a->kv_heads, mine = a->tokens * share, all = a->batch / a->groups * mine;
@@ -156,7 +163,8 @@ SharedPlan shared_plan(const ajqs_shared_attention_args* a) {
     p.own_rt = mine > 16 ? 2 : 1;
     p.own_tiles = (int)ceil_div(mine, 16 * p.own_rt);
     p.own_parts = 1;
-    p.own_blocks = ceil_div(own_units, 8) * 8 * p.own_tiles;
+    p.own_alone = shared_alone(own_units * p.own_tiles, (long long)a->prefix_cap + a->max_len, 384);
+    p.own_blocks = p.own_alone ? ceil_div(own_units * p.own_tiles, 4) : ceil_div(own_units, 8) * 8 * p.own_tiles;
   } else {
     p.form = bf16 && all > 64 ? SharedForm::many : SharedForm::few;
     p.own_rt = mine > 16 ? 2 : 1;
@@ -169,7 +177,8 @@ SharedPlan shared_plan(const ajqs_shared_attention_args* a) {
     const long long others = std::min(256ll, prefix_units * p.prefix_tiles * p.prefix_parts);
     p.own_parts = parts(own_units * p.own_tiles, 512 - others, a->max_len, bf16 || p.own_rt > 1 ? 128 : 64, 16);
     p.prefix_blocks = ceil_div(prefix_units * p.prefix_parts, 8) * 8 * p.prefix_tiles;
-    p.own_blocks = ceil_div(own_units * p.own_parts, 8) * 8 * p.own_tiles;
+    p.own_alone = p.own_parts == 1 && shared_alone(own_units * p.own_tiles, a->max_len, 256);
+    p.own_blocks = p.own_alone ? ceil_div(own_units * p.own_tiles, 4) : ceil_div(own_units * p.own_parts, 8) * 8 * p.own_tiles;
   }
   const int all_parts = p.prefix_parts + p.own_parts;
   p.bytes = all_parts > 1 ? (size_t)all_parts * p.queries * (8 + 4 * (size_t)a->dim) : 0;
@@ -207,6 +216,7 @@ SharedAttention shared_of(const ajqs_shared_attention_args* a, const SharedPlan&
   s.prefix_tiles = p.prefix_tiles;
   s.own_parts = p.own_parts;
   s.own_tiles = p.own_tiles;
+  s.own_alone = p.own_alone;
   s.scale2 = kLog2e / sqrtf((float)a->dim);
   s.by_share = divide_by(a->heads / a->kv_heads);
   s.by_each = divide_by((long long)a->tokens * (a->heads / a->kv_heads));

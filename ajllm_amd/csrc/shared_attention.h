@@ -31,6 +31,7 @@ struct SharedAttention {
   long long queries;    // batch * heads * tokens, in the order of q
   int groups, batch, tokens, heads, kv_heads, prefix_cap, max_len;
   int prefix_blocks, prefix_parts, prefix_tiles, own_parts, own_tiles;
+  int own_alone;        // a wave has a tile of a sequence's queries and its rows to itself, a workgroup four such
   float scale2;         // log2(e) / sqrt(HD)
   Divide by_share, by_each, by_tokens, by_heads, by_kv_heads, by_group;   // heads / kv_heads, that times tokens, .., batch / groups
   Divide by_prefix_tiles, by_prefix_parts, by_own_tiles, by_own_parts;
@@ -54,7 +55,7 @@ template <typename CacheT> struct Meeting {
   int begin, end;                // rows
   const CacheT *own_keys, *own_values;   // a second run of rows, from its first on (only where a workgroup walks both: `own` is then false and
   int own_end;                           // the queries are one sequence's)
-  bool own;
+  bool own, alone;               // (alone: a wave's, not a workgroup's)
   long long before;              // own rows a sequence's first new token sees ahead of its own row
 };
 
@@ -142,10 +143,12 @@ __device__ __forceinline__ void to_probabilities(RunningRow<HD>& row, const f32x
 template <typename CacheT, int HD>
 __device__ __forceinline__ bool find_meeting(const SharedAttention& a, int tile_queries_prefix, int tile_queries_own, Meeting<CacheT>& w) {
   w.own = (int)blockIdx.x >= a.prefix_blocks;
+  w.alone = w.own && a.own_alone;
   const int id = (int)blockIdx.x - (w.own ? a.prefix_blocks : 0);
   w.parts = w.own ? a.own_parts : a.prefix_parts;
   int tile;
-  const int run = (id & 7) + 8 * divide(id >> 3, w.own ? a.by_own_tiles : a.by_prefix_tiles, tile);
+  const int run = w.alone ? divide(4 * id + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), a.by_own_tiles, tile)
+                          : (id & 7) + 8 * divide(id >> 3, w.own ? a.by_own_tiles : a.by_prefix_tiles, tile);
   if (run >= (w.own ? a.batch : a.groups) * a.kv_heads * w.parts) return false;
   const int unit = divide(run, w.own ? a.by_own_parts : a.by_prefix_parts, w.part);
   w.outer = divide(unit, a.by_kv_heads, w.key_head);
@@ -193,7 +196,7 @@ __device__ __forceinline__ void find_both(const SharedAttention& a, Meeting<Cach
 }
 
 // ---- Few queries: the four waves of a workgroup take blocks of 32 rows in turn, each for itself (no barrier until the end), and RT tiles of 16
-// queries meet every row fetched.  What bounds it is memory: a wave asks for the next block's keys as soon as it has used this block's, and for
+// queries meet every row fetched.  Where there are sequences enough, each wave takes all rows of its own tile instead, and has nobody to join.  What bounds it is memory: a wave asks for the next block's keys as soon as it has used this block's, and for
 // its values likewise; eight waves a CU (bf16) then have 64 to 128 KB on their way.
 // LDS of a wave: keys, then values, 32 rows each; fp32 rows as two planes of bf16, through registers.
 template <int HD, typename CacheT> constexpr int few_wave_bytes() { return 2 * 32 * 2 * HD * kHalves<CacheT>; }
@@ -203,8 +206,52 @@ template <int HD, typename CacheT, int RT> constexpr int few_lds_bytes() {
   return walk > join ? walk : join;
 }
 
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
+// Components of a query's result as they are summed up, or as bf16 times scale (0: zeros, whatever they are).
+__device__ __forceinline__ void store_run(float* to, f32x4_t x, float) { *reinterpret_cast<f32x4_t*>(to) = x; }
+__device__ __forceinline__ void store_run(float* to, f32x2_t x, float) { *reinterpret_cast<f32x2_t*>(to) = x; }
+__device__ __forceinline__ void store_run(uint16_t* to, f32x4_t x, float scale) {
+  *reinterpret_cast<u32x2_t*>(to) = scale == 0.f ? u32x2_t{0u, 0u} : u32x2_t{pack2_bf16(x[0] * scale, x[1] * scale), pack2_bf16(x[2] * scale, x[3] * scale)};
+}
+__device__ __forceinline__ void store_run(uint16_t* to, f32x2_t x, float scale) {
+  *reinterpret_cast<uint32_t*>(to) = scale == 0.f ? 0u : pack2_bf16(x[0] * scale, x[1] * scale);
+}
+// Where a query of a workgroup (or wave) that meets all of its rows goes, and one over its weights' sum (0 where a token is not there or saw nothing).
+template <int HD, typename CacheT>
+__device__ __forceinline__ uint16_t* result_place(const SharedAttention& a, const Meeting<CacheT>& w, int n, int token, float l, float& scale) {
+  int rest, share;
+  divide(n, a.by_each, rest);
+  divide(rest, a.by_share, share);
+  const bool there = a.counts == nullptr || token < a.counts[w.outer];
+  scale = there && (l > 0.f || l != l) ? 1.f / l : 0.f;
+  return a.out + (((size_t)w.outer * a.tokens + token) * a.heads + (w.key_head * (int)a.by_share.d + share)) * HD;
+}
+
+// A wave's results are the workgroup's (Meeting::alone).  put(u, to, scale): a lane's sums of its query of tile u, to the query's row.
+template <int HD, int RT, bool kWhole, typename CacheT, typename Put>
+__device__ __forceinline__ void leave_alone(const SharedAttention& a, const Meeting<CacheT>& w, const RunningRow<HD> (&row)[RT], Put put) {
+  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+#pragma unroll
+  for (int u = 0; u < RT; ++u) {
+    const float l = quad_sum(row[u].l);
+    const int n = w.first + 16 * u + r;
+    if (n >= w.queries) continue;
+    int token;
+    const long long in_q = query_place(a, w.key_head, w.first_sequence, n, token);
+    if constexpr (kWhole) {
+      float scale;
+      uint16_t* out = result_place<HD>(a, w, n, token, l, scale);
+      put(u, out, scale);
+    } else {
+      const long long place = in_q + a.prefix_parts * a.queries;
+      if (g == 0) a.part_ml[place] = row[u].part(l);
+      put(u, a.part_sums + place * HD, 1.f);
+    }
+  }
+}
+
 // The four waves' results meet in LDS (rows of HD + 4 numbers: sixteen queries' pieces fall on different banks) and become the workgroup's part, or
-// (kWhole) the result.  put(u, to): a lane's sums of its query of tile u, to the query's row.
+// (kWhole) the result.
 template <int HD, int RT, int kMl, bool kWhole, typename CacheT, typename Put>
 __device__ __forceinline__ void join_waves(const SharedAttention& a, const Meeting<CacheT>& w, unsigned char* lds, const RunningRow<HD> (&row)[RT], Put put) {
   constexpr int kJoin = RT * 16, kPitch = HD + 4, kHelpers = 256 / kJoin;   // queries, lanes that put one together
@@ -216,7 +263,7 @@ __device__ __forceinline__ void join_waves(const SharedAttention& a, const Meeti
   for (int u = 0; u < RT; ++u) {
     const float l = quad_sum(row[u].l);
     if (g == 0) ml[wave * kJoin + 16 * u + r] = row[u].part(l);
-    put(u, sums + (wave * kJoin + 16 * u + r) * kPitch);
+    put(u, sums + (wave * kJoin + 16 * u + r) * kPitch, 1.f);
   }
   __syncthreads();
   const int n = (int)threadIdx.x / kHelpers, d0 = 4 * ((int)threadIdx.x % kHelpers);
@@ -237,26 +284,17 @@ __device__ __forceinline__ void join_waves(const SharedAttention& a, const Meeti
   const long long in_q = query_place(a, w.key_head, w.first_sequence, w.first + n, token);
   const long long place = in_q + (kWhole ? 0 : (w.part + (w.own ? a.prefix_parts : 0)) * a.queries);
   if (!kWhole && d0 == 0) a.part_ml[place] = float2{m, l};
-  float scale = 1.f;   // (zeros where a token is not there or saw nothing)
+  float scale = 1.f;
   uint16_t* out = nullptr;
-  if constexpr (kWhole) {
-    int rest, share;
-    divide(w.first + n, a.by_each, rest);
-    divide(rest, a.by_share, share);
-    const bool there = a.counts == nullptr || token < a.counts[w.outer];
-    scale = there && (l > 0.f || l != l) ? 1.f / l : 0.f;
-    out = a.out + (((size_t)w.outer * a.tokens + token) * a.heads + (w.key_head * (int)a.by_share.d + share)) * HD;
-  }
+  if constexpr (kWhole) out = result_place<HD>(a, w, w.first + n, token, l, scale);
 #pragma unroll
   for (int d = 0; d < HD; d += 4 * kHelpers) {
     if (d + d0 >= HD) break;
     f32x4_t o = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int k = 0; k < 4; ++k) o += *reinterpret_cast<const f32x4_t*>(sums + (k * kJoin + n) * kPitch + d + d0) * weight[k];
-    if constexpr (kWhole)
-      *reinterpret_cast<u32x2_t*>(out + d + d0) =
-          scale == 0.f ? u32x2_t{0u, 0u} : u32x2_t{pack2_bf16(o[0] * scale, o[1] * scale), pack2_bf16(o[2] * scale, o[3] * scale)};
-    else *reinterpret_cast<f32x4_t*>(a.part_sums + place * HD + d + d0) = o;
+    if constexpr (kWhole) store_run(out + d + d0, o, scale);
+    else store_run(a.part_sums + place * HD + d + d0, o, 1.f);
   }
 }
 
@@ -358,9 +396,9 @@ __device__ __forceinline__ void meet_few(const SharedAttention& a, Meeting<Cache
 #pragma unroll
   for (int t = 0; t < TT; ++t) v_rd[t] = values0 + (uint32_t)(vkey * RB + 32 * (t ^ (vkey & (TT - 1))) + 8 * (r & 3));
 
-  const int blocks = wave < W ? blocks_of<32, kBoth>(w) : 0;
-  if (wave < blocks) {
-    const Rows first(w, wave);
+  const int blocks = w.alone || wave < W ? blocks_of<32, kBoth>(w) : 0, begin = w.alone ? 0 : wave, by = w.alone ? 1 : W;
+  if (begin < blocks) {
+    const Rows first(w, begin);
     if constexpr (kDma) {
       ask(first.keys, first.rows, mine, false);
       ask(first.values, first.rows, values0, true);
@@ -373,9 +411,9 @@ __device__ __forceinline__ void meet_few(const SharedAttention& a, Meeting<Cache
   for (int u = 0; u < RT; ++u)
 #pragma unroll
     for (int s = 0; s < KS; ++s) to_halves(raw[u][s], qf[u][s]);
-  for (int n = wave; n < blocks; n += W) {
-    const bool more = n + W < blocks;
-    const Rows now(w, n), next(w, more ? n + W : n);
+  for (int n = begin; n < blocks; n += by) {
+    const bool more = n + by < blocks;
+    const Rows now(w, n), next(w, more ? n + by : n);
     if constexpr (kDma) {
       // (behind this block's keys only its values are on their way)
       asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kAsk) : "memory");
@@ -447,10 +485,12 @@ __device__ __forceinline__ void meet_few(const SharedAttention& a, Meeting<Cache
     }
   }
 
-  join_waves<HD, RT, few_join_bytes<HD, RT>(), kBoth>(a, w, lds, row, [&](int u, float* to) {
+  auto put = [&](int u, auto* to, float scale) __attribute__((always_inline)) {
 #pragma unroll
-    for (int t = 0; t < TT; ++t) *reinterpret_cast<f32x4_t*>(to + 16 * t + 4 * g) = row[u].o[t];
-  });
+    for (int t = 0; t < TT; ++t) store_run(to + 16 * t + 4 * g, row[u].o[t], scale);
+  };
+  if (w.alone) leave_alone<HD, RT, kBoth>(a, w, row, put);
+  else join_waves<HD, RT, few_join_bytes<HD, RT>(), kBoth>(a, w, lds, row, put);
 }
 
 // ---- At most 16 queries on fp32 rows, in fp32 throughout (v_mfma_f32_16x16x4_f32: 32 cycles for 16 rows x 4 components, where the memory's share of a CU
@@ -525,18 +565,18 @@ __device__ __forceinline__ void meet_few_f32(const SharedAttention& a, Meeting<f
         for (int e = 0; e < P; ++e) row[0].o[c * P + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(rows.v[i][c][e], p[i], row[0].o[c * P + e], 0, 0, 0);
   };
   // two blocks' registers in turn, the next one's rows on their way while one is worked on
-  const int blocks = blocks_of<16, kBoth>(w);
+  const int blocks = blocks_of<16, kBoth>(w), begin = w.alone ? 0 : wave, by = w.alone ? 1 : 4;
   Fetched even_rows, odd_rows;
-  if (wave < blocks) ask(Rows(w, wave), even_rows);
-  for (int n = wave; n < blocks; n += 8) {
-    if (n + 4 < blocks) ask(Rows(w, n + 4), odd_rows);
+  if (begin < blocks) ask(Rows(w, begin), even_rows);
+  for (int n = begin; n < blocks; n += 2 * by) {
+    if (n + by < blocks) ask(Rows(w, n + by), odd_rows);
     meet(n, even_rows);
-    if (n + 4 >= blocks) break;
-    if (n + 8 < blocks) ask(Rows(w, n + 8), even_rows);
-    meet(n + 4, odd_rows);
+    if (n + by >= blocks) break;
+    if (n + 2 * by < blocks) ask(Rows(w, n + 2 * by), even_rows);
+    meet(n + by, odd_rows);
   }
   // a lane has components 16 P v + P (4 g + i) + e of query r: of each v 4 P of them one behind the other
-  join_waves<HD, 1, few_join_bytes<HD, 1>(), kBoth>(a, w, lds, row, [&](int, float* to) {
+  auto put = [&](int, auto* to, float scale) __attribute__((always_inline)) {
 #pragma unroll
     for (int c = 0; c < VC; ++c)
 #pragma unroll
@@ -544,9 +584,11 @@ __device__ __forceinline__ void meet_few_f32(const SharedAttention& a, Meeting<f
         part_t x;
 #pragma unroll
         for (int e = 0; e < P; ++e) x[e] = row[0].o[c * P + e][i];
-        *reinterpret_cast<part_t*>(to + 16 * P * c + P * (4 * g + i)) = x;
+        store_run(to + 16 * P * c + P * (4 * g + i), x, scale);
       }
-  });
+  };
+  if (w.alone) leave_alone<HD, 1, kBoth>(a, w, row, put);
+  else join_waves<HD, 1, few_join_bytes<HD, 1>(), kBoth>(a, w, lds, row, put);
 }
 
 // ---- Many queries on bf16 rows: 64 U to a workgroup, 16 U to each wave, all four walking the same blocks of 64 rows (LDS, two stages of a key and a
