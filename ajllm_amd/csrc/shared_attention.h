@@ -608,6 +608,17 @@ template <typename CacheT> struct Walk {
 };
 template <int HD> constexpr int many_lds_bytes() { return 4 * 64 * 2 * HD + 4 * 256; }
 
+// Two requests of 1 KiB each for 4096 bytes ahead of lds_addr (from 4096 bytes ahead of base) and for lds_addr: the instruction's offset moves both sides.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"  // (m0, as dma16)
+__device__ __forceinline__ void dma16_pair(const void* base, uint32_t voff, uint32_t lds_addr) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 offset:-4096\n\tglobal_load_lds_dwordx4 %1, %2"
+               :
+               : "s"(lds_addr), "v"(voff), "s"(base)
+               : "memory", "m0");
+}
+#pragma clang diagnostic pop
+
 template <int HD, typename QT, int U>
 __device__ __forceinline__ void meet_many(const SharedAttention& a, const Walk<uint16_t>& w, RunningRow<HD> (&row)[U], uint32_t lds0) {
   constexpr int RB = 2 * HD, C = HD / 8, KS = HD / 32, TT = HD / 16, QH = kHalves<QT>, kAhead = TT < 3 ? TT : 3;
@@ -703,11 +714,11 @@ __device__ __forceinline__ void meet_many(const SharedAttention& a, const Walk<u
     uint32_t k_base = k_rd, v_base = v_rd;
     if (decltype(masked)::value) asm volatile("" : "+v"(k_base), "+v"(v_base));
     auto fetch = [&](int i) __attribute__((always_inline)) {
-      kf[i] = key_frag(k_base, k_at, i);
-      if (kV) {
+      if (kV) {   // (first: what waits for the keys then waits for them too)
         vl[i] = pf_read_tr((v_base ^ (uint32_t)(32 * i)) + (uint32_t)v_at);
         vh[i] = pf_read_tr((v_base ^ (uint32_t)(32 * i)) + (uint32_t)(v_at + 16 * RB));
       }
+      kf[i] = key_frag(k_base, k_at, i);
     };
 #pragma unroll
     for (int i = 0; i < ahead; ++i) fetch(i);
@@ -729,8 +740,13 @@ __device__ __forceinline__ void meet_many(const SharedAttention& a, const Walk<u
       }
     }
     u32x4_t pn[U];
-    float p[U][8], psum[U] = {};
-    constexpr int kPer = 8 * U / TT;  // exponentials of a piece
+    float p[U][8], psum[U];
+    // exponentials of a piece: beside their exponents of the next piece's and the sum of the last one's, so that none waits for what is just being made
+    constexpr int kPer = 8 * U / TT;
+    auto exponent = [&](int n) __attribute__((always_inline)) { return __builtin_fmaf(sc[n >> 3][(n & 7) >> 2][n & 3], a.scale2, -row[n >> 3].m); };
+    auto add = [&](int n) __attribute__((always_inline)) { psum[n >> 3] = (n & 7) == 0 ? p[n >> 3][0] : psum[n >> 3] + p[n >> 3][n & 7]; };
+#pragma unroll
+    for (int x = 0; x < kPer; ++x) p[x >> 3][x & 7] = exponent(x);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int i = 0; i < TT; ++i) {
@@ -739,14 +755,19 @@ __device__ __forceinline__ void meet_many(const SharedAttention& a, const Walk<u
       score(kf[i], i);
 #pragma unroll
       for (int x = 0; x < kPer; ++x) {
-        const int u = (i * kPer + x) >> 3, e = (i * kPer + x) & 7;
-        p[u][e] = exp2_hw(__builtin_fmaf(sc[u][e >> 2][e & 3], a.scale2, -row[u].m));
-        psum[u] += p[u][e];
+        const int n = i * kPer + x, u = n >> 3, e = n & 7;
+        p[u][e] = exp2_hw(p[u][e]);
+        if (n + kPer < 8 * U) p[(n + kPer) >> 3][(n + kPer) & 7] = exponent(n + kPer);
+        if (i > 0) add(n - kPer);
+        if (i == TT - 1) add(n);
       }
       if (U * (i + 1) % TT == 0) {  // a group of rows is through (pinned: the compiler would sink it behind the branches below)
         const int u = U * i / TT;
         pn[u] = pack8_bf16(p[u]);
-        asm volatile("" : "+v"(pn[u]), "+v"(psum[u]));
+        asm volatile("" : "+v"(pn[u]));
+        if (i == TT - 1)
+#pragma unroll
+          for (int v = 0; v < U; ++v) asm volatile("" : "+v"(psum[v]));
       }
       if (kV) {
         const u32x4_t vf = {vl[i].x, vl[i].y, vh[i].x, vh[i].y};
@@ -820,8 +841,11 @@ __device__ __forceinline__ void meet_many(const SharedAttention& a, const Walk<u
           asm volatile("s_waitcnt vmcnt(1)" ::: "memory");   // (all but the touch)
           turn_barrier();
           step(2 * j + 2 * x + 1, yes, no, (x ^ 1) * 2 * kTile, x * 2 * kTile, [&](int i) __attribute__((always_inline)) {
-            if (i < KS) dma16(k_from + i * 4096, k_lane, place(false, i, x));
-            else dma16(v_from + (i - KS) * 4096, v_lane, place(true, i - KS, x ^ 1));
+            const int n = i % KS;   // request of the wave: of the keys', then of the values'
+            const char* const from = (i < KS ? k_from : v_from) + n * 4096;
+            const uint32_t at = i < KS ? k_lane : v_lane, to = place(i >= KS, n, i < KS ? x : x ^ 1);
+            if (KS == 1) dma16(from, at, to);
+            else if (n % 2 == 0) dma16_pair(from + 4096, at, to + 4096);
             if (i == TT - 1) touch(j + x + 5);
           });
           k_from += kTile;
