@@ -4,7 +4,8 @@
 //   bits 0 .. 19  how often the token is among the row's tokens,   bit 20  whether it is in the prompt,   bits 21 .. 31  its bias slot + 1,
 // fills them from the row's lists (whole numbers: no result depends on the order of the atomics) while the logits are on their way, and
 // puts both together, four tokens a lane at a time.  What bounds it is memory: a row is read and written once; its lists are read by
-// every slice, from L2 (slices of a row run next to each other on one XCD).
+// every slice, from L2 (slices of a row run next to each other on one XCD).  256 rows of 128256 fp32 logits with 9216 listed tokens and a mask each (281 MB)
+// 65.7 us = 4.3 TB/s, 32 rows with 2560 11.7 us, one of 32000 4.2: a launch and two round trips, the lists' and the logits'.
 #pragma once
 #include "lane_rows.h"
 
