@@ -259,6 +259,7 @@ def _share_by_heads(cuda, groups, batch, tokens, heads, kv, hd, prefix, max_len,
     for b in range(batch):
         last = int(rows[b]) + int(counts[b])
         k[b, :, last:], v[b, :, last:] = math.inf, math.nan
+        q[b, :, int(counts[b]):] = math.nan   # (a token that is not there: zeros, and nobody else's business)
     got = attention.shared_prefix_attention(q, pk, pv, lengths, k, v, rows, counts=counts)
     _attention_near(got, want.cpu(), size.cpu())
 

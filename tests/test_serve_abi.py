@@ -7,8 +7,9 @@ import subprocess
 from pathlib import Path
 
 import pytest
+import torch
 
-from ajllm_amd import _lib
+from ajllm_amd import _lib, attention, sampling
 
 HEADER = Path(__file__).resolve().parents[1] / "include" / "ajq_serve.h"
 STRUCTS = {"ajqs_norm_rope_args": _lib.NormRopeArgs, "ajqs_shared_attention_args": _lib.SharedAttentionArgs,
@@ -37,6 +38,16 @@ def test_structures_have_the_header_layout(tmp_path):
         name, field, at = line.split()
         struct = STRUCTS[name]
         assert int(at) == (ctypes.sizeof(struct) if field == "." else getattr(struct, field).offset), line
+
+
+def test_functions_need_a_gpu():
+    q, cache, whole = torch.zeros(2, 4, 1, 64), torch.zeros(2, 2, 8, 64), torch.zeros(2, dtype=torch.long)
+    with pytest.raises(ValueError, match="norm_rope needs tensors on a ROCm device"):
+        attention.norm_rope(torch.zeros(2, 512), torch.zeros(8, 32), torch.zeros(8, 32), cache, cache.clone(), whole, heads=4)
+    with pytest.raises(ValueError, match="shared_prefix_attention needs tensors on a ROCm device"):
+        attention.shared_prefix_attention(q, cache, cache, whole, cache, cache, whole)
+    with pytest.raises(ValueError, match="adjust_logits needs tensors on a ROCm device"):
+        sampling.adjust_logits(torch.zeros(2, 100), repetition=1.5)
 
 
 @pytest.fixture()
