@@ -158,19 +158,24 @@ SharedPlan shared_plan(const ajqs_shared_attention_args* a) {
     p.own_tiles = (int)ceil_div(mine, 64 * p.own_rt);
     p.own_parts = parts(own_units * p.own_tiles, 512, (long long)a->prefix_cap + a->max_len, 128, kMostParts);
     p.own_blocks = ceil_div(own_units, 8) * 8 * p.own_tiles * p.own_parts;
-  } else if (shared_each(a, own_units * ceil_div(mine, mine > 16 ? 32 : 16))) {
-    p.form = SharedForm::each;
-    p.own_rt = mine > 16 ? 2 : 1;
-    p.own_tiles = (int)ceil_div(mine, 16 * p.own_rt);
+  } else if (shared_each(a, own_units * ceil_div(mine, 16))) {
+    p.form = SharedForm::each;   // (always tiles of 16: 8 sequences of 7 tokens x 4 behind 500 rows with 250 8.9 us, of 32 13.1)
+    p.own_rt = 1;
+    p.own_tiles = (int)ceil_div(mine, 16);
     p.own_parts = 1;
     p.own_alone = shared_alone(own_units * p.own_tiles, (long long)a->prefix_cap + a->max_len, 384);
     p.own_blocks = p.own_alone ? ceil_div(own_units * p.own_tiles, 4) : ceil_div(own_units, 8) * 8 * p.own_tiles;
   } else {
-    p.form = bf16 && all > 64 ? SharedForm::many : SharedForm::few;
-    p.own_rt = mine > 16 ? 2 : 1;
-    p.prefix_rt = all > 16 ? 2 : 1;
-    // tiles of 128 queries, 64 where those times 128 rows are less than two a CU
-    if (p.form == SharedForm::many) p.prefix_rt = prefix_units * ceil_div(all, 128) * ceil_div(a->prefix_cap, 128) < 512 ? 1 : 2;
+    // (128 queries a head behind 8192 rows: few 21.9, many 22.3 us; 120 of 16 heads behind 4096 25.6 and 27.6; 256 behind 8192 31.0 and 27.9)
+    p.form = bf16 && all > 128 ? SharedForm::many : SharedForm::few;
+    // Own rows by tiles of 16 queries (28 a head behind 4000 rows 11.3 us, of 32 12.5), of 32 where fp32 rows meet many (24 are better off with 32 by a
+    // fourteenth, 28 with 16 by an eighth).  The prefix by tiles of 32 where 16 would fetch the rows too often, from L2 even: bf16 rows, 28 queries 8.2 and
+    // 10.2 with 32, 64 10.1 and 11.0, 128 behind 8192 20.1 and 18.0; fp32 rows, 28 15.7 and 17.3, 64 21.5 and 19.6.
+    p.own_rt = !bf16 && mine > 32 ? 2 : 1;
+    p.prefix_rt = all > (bf16 ? 64 : 32) ? 2 : 1;
+    // Many: tiles of 128 queries, 64 where those times 128 rows are less than four a CU (400 queries of 8 heads behind 4096 rows 23.5 us and, with 64, 23.1, 512
+    // behind 2048 20.5 and 18.3, behind 16384 59.6 and 71.2).
+    if (p.form == SharedForm::many) p.prefix_rt = prefix_units * ceil_div(all, 128) * ceil_div(a->prefix_cap, 128) < 1024 ? 1 : 2;
     p.own_tiles = (int)ceil_div(mine, 16 * p.own_rt);
     p.prefix_tiles = (int)ceil_div(all, (p.form == SharedForm::many ? 64 : 16) * p.prefix_rt);
     p.prefix_parts = parts(prefix_units * p.prefix_tiles, 256, a->prefix_cap, bf16 || p.prefix_rt > 1 ? 128 : 64, kMostParts - 16);
@@ -245,18 +250,18 @@ int launch_few(const SharedAttention& s, const SharedPlan& p, hipStream_t stream
   hipLaunchKernelGGL(kernel, dim3((unsigned)(p.prefix_blocks + p.own_blocks)), dim3(256), bytes, stream, s);
   return merge_parts<HD>(s, p, stream, what);
 }
-template <int HD, typename QT, typename CacheT, int RT>
+template <int HD, typename QT, typename CacheT>
 int launch_each(const SharedAttention& s, const SharedPlan& p, hipStream_t stream, const char* what) {
-  constexpr int bytes = some_lds_bytes<HD, CacheT, RT>();
-  auto kernel = shared_attention_each_kernel<HD, QT, CacheT, RT>;
+  constexpr int bytes = some_lds_bytes<HD, CacheT, 1>();
+  auto kernel = shared_attention_each_kernel<HD, QT, CacheT>;
   if (int e = allow_lds(kernel, bytes, what)) return e;
   hipLaunchKernelGGL(kernel, dim3((unsigned)p.own_blocks), dim3(256), bytes, stream, s);
   return check_launch(what);
 }
-template <int HD, typename QT, int U, int RTO>
+template <int HD, typename QT, int U>
 int launch_many(const SharedAttention& s, const SharedPlan& p, hipStream_t stream, const char* what) {
-  constexpr int bytes = std::max(many_lds_bytes<HD>(), few_lds_bytes<HD, uint16_t, RTO>());
-  auto kernel = shared_attention_many_kernel<HD, QT, U, RTO>;
+  constexpr int bytes = std::max(many_lds_bytes<HD>(), few_lds_bytes<HD, uint16_t, 1>());
+  auto kernel = shared_attention_many_kernel<HD, QT, U>;
   if (int e = allow_lds(kernel, bytes, what)) return e;
   hipLaunchKernelGGL(kernel, dim3((unsigned)(p.prefix_blocks + p.own_blocks)), dim3(256), bytes, stream, s);
   return merge_parts<HD>(s, p, stream, what);
@@ -314,11 +319,12 @@ int ajqs_norm_rope(const ajqs_norm_rope_args* a, void* stream) {
           };
           const std::integral_constant<bool, true> yes;
           const std::integral_constant<bool, false> no;
-          // one head a team until there are workgroups enough, then as many as a token has for its sixteen teams
+          // one head a team until there are workgroups enough, then two or three, whichever leaves fewer of a token's teams idle (16 prompts of 333 tokens, one, two and
+          // three: 48 heads 33.3, 31.2 and 28.5 us, 96 63.6, 52.5 and 50.5, 32 23.9, 20.9 and 21.4, 36 of 64 18.3, 17.0 and 14.6; 2 of 333, 48 6.7, 6.6 and 6.8)
           const bool full = (long long)a->batch * a->tokens >= 1024;
           if (a->tokens == 1) full && all > 16 ? launch(Size<2>{}, no) : launch(Size<1>{}, no);
           else if (!full || all <= 16) launch(Size<1>{}, yes);
-          else all <= 32 || all > 48 ? launch(Size<2>{}, yes) : launch(Size<3>{}, yes);
+          else ceil_div(all, 48) * 48 > ceil_div(all, 32) * 32 ? launch(Size<2>{}, yes) : launch(Size<3>{}, yes);
         });
       });
     });
@@ -356,20 +362,21 @@ int ajqs_shared_attention(const ajqs_shared_attention_args* a, void* workspace, 
             return;
           }
           if (p.form == SharedForm::many) {
-            const auto launch = p.prefix_rt == 2 ? (p.own_rt == 2 ? launch_many<HD, QT, 2, 2> : launch_many<HD, QT, 2, 1>)
-                                                 : (p.own_rt == 2 ? launch_many<HD, QT, 1, 2> : launch_many<HD, QT, 1, 1>);
-            status = launch(s, p, (hipStream_t)stream, what);
+            status = p.prefix_rt == 2 ? launch_many<HD, QT, 2>(s, p, (hipStream_t)stream, what) : launch_many<HD, QT, 1>(s, p, (hipStream_t)stream, what);
             return;
           }
         }
         if (p.form == SharedForm::each) {
-          const auto launch = p.own_rt == 2 ? launch_each<HD, QT, CacheT, 2> : launch_each<HD, QT, CacheT, 1>;
-          status = launch(s, p, (hipStream_t)stream, what);
+          status = launch_each<HD, QT, CacheT>(s, p, (hipStream_t)stream, what);
           return;
         }
-        const auto launch = p.own_rt == 2      ? launch_few<HD, QT, CacheT, 2, 2>
-                            : p.prefix_rt == 2 ? launch_few<HD, QT, CacheT, 2, 1>
-                                               : launch_few<HD, QT, CacheT, 1, 1>;
+        if constexpr (sizeof(CacheT) == 4) {
+          if (p.own_rt == 2) {
+            status = launch_few<HD, QT, CacheT, 2, 2>(s, p, (hipStream_t)stream, what);
+            return;
+          }
+        }
+        const auto launch = p.prefix_rt == 2 ? launch_few<HD, QT, CacheT, 2, 1> : launch_few<HD, QT, CacheT, 1, 1>;
         status = launch(s, p, (hipStream_t)stream, what);
       });
     });
@@ -405,7 +412,8 @@ int ajqs_adjust_logits(const ajqs_adjust_logits_args* a, void* stream) {
   if (a->logits != a->out && rows_meet(a->logits, a->ld * size, (long long)a->vocab * size, a->out, a->out_ld * 4, (long long)a->vocab * 4, a->batch))
     return fail(AJQ_ERR_SHAPE, "%s: out overlaps the logits without being them", what);
   const bool words = (a->tokens && a->max_tokens) || (a->prompt && a->max_prompt) || (a->bias_ids && a->biases);
-  // slices of 16384 tokens (two workgroups of 1024 lanes a CU then), smaller ones until there are two workgroups a CU
+  // Slices of 16384 tokens (two workgroups of 1024 lanes a CU then; 256 rows of 128256 66 us, 75 in slices of 8192, whose rows' lists are read twice as often),
+  // smaller ones until there are two workgroups a CU (8 rows 6.2 us, 8.2 with one a CU, 6.4 with four; 64 rows 15.7, 16.0 and 20.0).
   int slice = 4 * kSliceThreads * kSlicePieces;
   while (slice > 1024 && (long long)a->batch * ceil_div(a->vocab, slice) < 512) slice /= 2;
   const int threads = std::min(slice / 4, std::max(256, slice / (4 * kSlicePieces))), slices = (int)ceil_div(a->vocab, slice);

@@ -196,8 +196,9 @@ __device__ __forceinline__ void find_both(const SharedAttention& a, Meeting<Cach
 }
 
 // ---- Few queries: the four waves of a workgroup take blocks of 32 rows in turn, each for itself (no barrier until the end), and RT tiles of 16
-// queries meet every row fetched.  Where there are sequences enough, each wave takes all rows of its own tile instead, and has nobody to join.  What bounds it is memory: a wave asks for the next block's keys as soon as it has used this block's, and for
-// its values likewise; eight waves a CU (bf16) then have 64 to 128 KB on their way.
+// queries meet every row fetched.  Where there are sequences enough, each wave takes all rows of its own tile instead, and has nobody to join.  What bounds
+// it is memory: a wave asks for the next block's keys as soon as it has used this block's, and for its values likewise; eight waves a CU (bf16) then have 64 to
+// 128 KB on their way.  8 prompts of 1500 rows with 8 sequences of 300 each (12 heads of 64, 59 MB) 12.8 us = 4.6 TB/s.
 // LDS of a wave: keys, then values, 32 rows each; fp32 rows as two planes of bf16, through registers.
 template <int HD, typename CacheT> constexpr int few_wave_bytes() { return 2 * 32 * 2 * HD * kHalves<CacheT>; }
 template <int HD, int RT> constexpr int few_join_bytes() { return 4 * RT * 16 * (HD + 4) * 4; }
@@ -318,6 +319,7 @@ __device__ __forceinline__ int blocks_of(const Meeting<CacheT>& w) {
   return (w.end - w.begin + N - 1) / N + (kBoth ? (w.own_end + N - 1) / N : 0);
 }
 
+// W: how many of the waves work.
 template <int HD, typename QT, typename CacheT, int RT, int W = 4, bool kBoth = false>
 __device__ __forceinline__ void meet_few(const SharedAttention& a, Meeting<CacheT>& w, unsigned char* lds, uint32_t lds0) {
   constexpr int RB = 2 * HD, C = HD / 8, KS = HD / 32, TT = HD / 16, KH = kHalves<CacheT>, QH = kHalves<QT>;
@@ -592,7 +594,7 @@ __device__ __forceinline__ void meet_few_f32(const SharedAttention& a, Meeting<f
 }
 
 // ---- Many queries on bf16 rows: 64 U to a workgroup, 16 U to each wave, all four walking the same blocks of 64 rows (LDS, two stages of a key and a
-// value tile, one barrier a block).  Bound by MFMA.  The walk goes over a run of the group's prefix and, behind it, of one sequence's own
+// value tile, one barrier a block).  Bound by what a wave issues beside its MFMAs.  The walk goes over a run of the group's prefix and, behind it, of one sequence's own
 // rows; either may be empty.  It goes in steps of 32 rows; step t holds the exponents of step t + 1, the softmax of step t and the values of step t - 1
 // times their probabilities, laid out in HD / 16 pieces of either product with their share of the exponentials, in that order for good, so that a
 // wave has MFMAs and vector work to issue side by side (attn_prefill_steps_kernel).
@@ -911,24 +913,26 @@ __global__ __launch_bounds__(256, sizeof(CacheT) == 4 && RTP == 2 ? 1 : 2) void 
 
 // Few rows in all: a workgroup walks the prefix and then a sequence's own rows with that sequence's queries alone, and what comes out is the result, in
 // one launch.  Each sequence reads the prefix again (from L2), which two launches cost more than.
-template <int HD, typename QT, typename CacheT, int RT>
-__global__ __launch_bounds__(256, sizeof(CacheT) == 4 && RT == 2 ? 1 : 2) void shared_attention_each_kernel(SharedAttention a) {
+template <int HD, typename QT, typename CacheT>
+__global__ __launch_bounds__(256, 2) void shared_attention_each_kernel(SharedAttention a) {
   extern __shared__ __attribute__((aligned(1024))) unsigned char shared_lds[];
   const uint32_t lds0 = (uint32_t)(uintptr_t)(pf_lds_char_t*)shared_lds;
   Meeting<CacheT> w;
-  if (!find_meeting<CacheT, HD>(a, 16 * RT, 16 * RT, w)) return;
-  meet_some<HD, QT, CacheT, RT, true>(a, w, shared_lds, lds0);
+  if (!find_meeting<CacheT, HD>(a, 16, 16, w)) return;
+  meet_some<HD, QT, CacheT, 1, true>(a, w, shared_lds, lds0);
 }
 
-// The prefix by meet_many, the sequences' own rows by meet_few.
-template <int HD, typename QT, int U, int RTO>
+// The prefix by meet_many, the sequences' own rows by meet_few: beside a long prefix (U 2) by two waves a workgroup, which leave more of the memory to the prefix
+// (128 sequences of 8 heads x 4 behind 32768 rows with 1000, 399 MB and 70 GFLOP, 110 us; by one wave 118, by four 115; the prefix alone 82 us = 850 TFLOP/s, own rows
+// alone 55).
+template <int HD, typename QT, int U>
 __global__ __launch_bounds__(256, 2) void shared_attention_many_kernel(SharedAttention a) {
   extern __shared__ __attribute__((aligned(1024))) unsigned char shared_lds[];
   const uint32_t lds0 = (uint32_t)(uintptr_t)(pf_lds_char_t*)shared_lds;
   Meeting<uint16_t> w;
-  if (!find_meeting<uint16_t, HD>(a, 64 * U, 16 * RTO, w)) return;
+  if (!find_meeting<uint16_t, HD>(a, 64 * U, 16, w)) return;
   if (w.own) {
-    meet_few<HD, QT, uint16_t, RTO, U == 2 ? 2 : 4>(a, w, shared_lds, lds0);
+    meet_few<HD, QT, uint16_t, 1, U == 2 ? 2 : 4>(a, w, shared_lds, lds0);
     return;
   }
   find_rows(a, w);
@@ -949,7 +953,8 @@ __global__ __launch_bounds__(256, 2) void shared_attention_many_kernel(SharedAtt
 }
 
 // Sequences with many new tokens each: 64 U queries of one sequence walk the prefix and then its own rows, and what comes out is the result.  With
-// own_parts > 1 the walk is cut up and leaves parts for the merge.
+// own_parts > 1 the walk is cut up and leaves parts for the merge.  16 sequences of 100 tokens x 4 of 8 heads behind 2048 rows 71 us = 590 TFLOP/s (358 tiles on 256 CUs), 24 of 50
+// behind 8000 203 us = 775.
 template <int HD, typename QT, int U>
 __global__ __launch_bounds__(256, 2) void shared_attention_walk_kernel(SharedAttention a) {
   extern __shared__ __attribute__((aligned(1024))) unsigned char shared_lds[];

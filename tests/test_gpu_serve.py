@@ -268,10 +268,10 @@ FEW = [   # (groups, batch, tokens, heads, kv, prefix, max_len): one and two til
     (1, 2, 1, 8, 2, 900, 70), (1, 9, 1, 8, 2, 900, 70), (1, 2, 7, 8, 2, 900, 70), (3, 6, 1, 16, 4, 700, 600), (2, 4, 5, 4, 4, 1300, 9),
     (1, 2, 1, 8, 2, 100, 70), (1, 2, 7, 8, 2, 100, 70), (1, 2, 40, 6, 1, 1000, 300),
     (1, 66, 1, 12, 12, 900, 120), (3, 33, 3, 26, 26, 700, 250), (2, 50, 20, 8, 8, 840, 33),   # a wave for itself
-    (1, 66, 1, 12, 12, 100, 200), (3, 33, 20, 13, 13, 30, 90), (2, 50, 40, 8, 8, 20, 44), (1, 130, 1, 16, 16, 1, 1),
+    (1, 66, 1, 12, 12, 100, 200), (3, 33, 20, 13, 13, 30, 90), (2, 50, 40, 8, 8, 20, 44), (1, 130, 1, 16, 16, 1, 1), (1, 20, 1, 8, 2, 900, 70), (1, 3, 12, 8, 2, 900, 70),
 ]
 MANY = [   # tiles of 64 and of 128 queries for the prefix, of 16 and of 32 for own rows
-    (1, 40, 1, 8, 2, 900, 70), (3, 33, 1, 24, 2, 1000, 300), (1, 9, 7, 8, 2, 1500, 200), (1, 130, 1, 8, 2, 8200, 40), (2, 64, 9, 8, 2, 8500, 60), (1, 97, 1, 9, 9, 900, 256),
+    (1, 40, 1, 8, 2, 900, 70), (3, 33, 1, 24, 2, 1000, 300), (1, 9, 7, 8, 2, 1500, 200), (1, 130, 1, 8, 2, 8200, 40), (2, 64, 9, 8, 2, 8500, 60), (1, 97, 1, 9, 9, 900, 256), (1, 130, 1, 8, 2, 14000, 40),
 ]
 WALK = [   # several parts and one, most rows before or in the sequences' own, odd and even numbers of blocks
     (1, 2, 70, 4, 2, 500, 900), (2, 6, 33, 8, 2, 1000, 40), (1, 16, 64, 32, 8, 700, 300), (1, 16, 90, 32, 8, 1290, 200), (2, 32, 70, 8, 4, 130, 1000),
