@@ -168,11 +168,15 @@ SharedPlan shared_plan(const ajqs_shared_attention_args* a) {
   } else {
     // (128 queries a head behind 8192 rows: few 21.9, many 22.3 us; 120 of 16 heads behind 4096 25.6 and 27.6; 256 behind 8192 31.0 and 27.9)
     p.form = bf16 && all > 128 ? SharedForm::many : SharedForm::few;
-    // Own rows by tiles of 16 queries (28 a head behind 4000 rows 11.3 us, of 32 12.5), of 32 where fp32 rows meet many (24 are better off with 32 by a
-    // fourteenth, 28 with 16 by an eighth).  The prefix by tiles of 32 where 16 would fetch the rows too often, from L2 even: bf16 rows, 28 queries 8.2 and
-    // 10.2 with 32, 64 10.1 and 11.0, 128 behind 8192 20.1 and 18.0; fp32 rows, 28 15.7 and 17.3, 64 21.5 and 19.6.
-    p.own_rt = !bf16 && mine > 32 ? 2 : 1;
-    p.prefix_rt = all > (bf16 ? 64 : 32) ? 2 : 1;
+    // Tiles of 32 queries fetch rows half as often as tiles of 16, which are twice as many and wait less: 16 it is while rows come from L2 and workgroups are few.  The
+    // prefix (32 heads in five groups of 30 queries, 4672 fp32 rows: 137 us with 32, 221 with 16; 16 heads, 30 queries, 4000 rows 29.6 and 26.4; 8 heads, 64 queries,
+    // 4000 bf16 rows 11.0 and 10.1, 64 fp32 19.6 and 21.5); own rows that are fp32 (64 sequences of 28 queries, 1000 rows 128 and 142 us; 2 of 28, 300 rows 23.4 and
+    // 20.4).  bf16 own rows gain either way (8 of 24, 600 rows 15.9 and 13.6; 64 of 28, 1000 rows 53.6 and 54.2; 128 of 20, 1000 rows 72 and 79): always 16.
+    auto tiles_of = [&](long long queries, long long units, long long rows, long long from_l2) {
+      return queries > (units * ceil_div(rows, 128) > 512 ? 16 : from_l2) ? 2 : 1;
+    };
+    p.own_rt = bf16 ? 1 : tiles_of(mine, own_units, a->max_len, 32);
+    p.prefix_rt = std::max(p.own_rt, tiles_of(all, prefix_units, a->prefix_cap, bf16 ? 64 : 32));
     // Many: tiles of 128 queries, 64 where those times 128 rows are less than four a CU (400 queries of 8 heads behind 4096 rows 23.5 us and, with 64, 23.1, 512
     // behind 2048 20.5 and 18.3, behind 16384 59.6 and 71.2).
     if (p.form == SharedForm::many) p.prefix_rt = prefix_units * ceil_div(all, 128) * ceil_div(a->prefix_cap, 128) < 1024 ? 1 : 2;

@@ -269,6 +269,7 @@ FEW = [   # (groups, batch, tokens, heads, kv, prefix, max_len): one and two til
     (1, 2, 1, 8, 2, 100, 70), (1, 2, 7, 8, 2, 100, 70), (1, 2, 40, 6, 1, 1000, 300),
     (1, 66, 1, 12, 12, 900, 120), (3, 33, 3, 26, 26, 700, 250), (2, 50, 20, 8, 8, 840, 33),   # a wave for itself
     (1, 66, 1, 12, 12, 100, 200), (3, 33, 20, 13, 13, 30, 90), (2, 50, 40, 8, 8, 20, 44), (1, 130, 1, 16, 16, 1, 1), (1, 20, 1, 8, 2, 900, 70), (1, 3, 12, 8, 2, 900, 70),
+    (5, 60, 3, 26, 26, 700, 40), (1, 24, 9, 10, 10, 300, 500),
 ]
 MANY = [   # tiles of 64 and of 128 queries for the prefix, of 16 and of 32 for own rows
     (1, 40, 1, 8, 2, 900, 70), (3, 33, 1, 24, 2, 1000, 300), (1, 9, 7, 8, 2, 1500, 200), (1, 130, 1, 8, 2, 8200, 40), (2, 64, 9, 8, 2, 8500, 60), (1, 97, 1, 9, 9, 900, 256), (1, 130, 1, 8, 2, 14000, 40),
