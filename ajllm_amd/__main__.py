@@ -29,6 +29,8 @@ def main(argv: list[str] | None = None) -> int:
     prompts = [[int(t) for t in text.split(",")] for text in args.tokens]
     if len({len(p) for p in prompts}) != 1:
         ap.error("the prompts of a batch must have equal length")
+    if not args.repetition_penalty > 0:
+        ap.error("the repetition penalty must be positive")
 
     import torch
 

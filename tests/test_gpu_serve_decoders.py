@@ -2,11 +2,13 @@
 adjusted logits, each against the model's own code."""
 
 import copy
+import json
 
 import pytest
 import torch
+from safetensors.torch import save_file
 
-from ajllm_amd import decoding, modeling, quantize_model_
+from ajllm_amd import checkpoint, decoding, modeling, quantize_model_
 from tests.helpers import errors
 
 pytestmark = pytest.mark.gpu
@@ -230,6 +232,36 @@ def test_dense_decoder_with_penalties(cuda):
         dec.set_penalties(allowed=allowed)
         dec.prefill(prompt)
         assert dec.generate(8).unique().tolist() == [96]
+
+
+def test_penalties_from_the_command_line(cuda, tmp_path, capsys):
+    from ajllm_amd.__main__ import main as command
+
+    torch.manual_seed(3)
+    mixer = {"heads": 4, "dim": 32, "rot_dim": 16, "vdim": 48, "kv_rank": 64, "scale": 0.15, "mask": {"size": 9}, "rot": {"base": 1000.0, "dims": 16}}
+    cfg = {"architecture": "Dorutar", "vocab": 97, "width": 80, "max_positions": 64, "norm": {"eps": 1e-5},
+           "layers": [{"type": "latent_attention", "mixer": mixer, "mlp": {"kind": "dense", "ff": 96}}] * 2}
+    (tmp_path / "config.json").write_text(json.dumps(cfg))
+    model = modeling.build_model(cfg)
+    names = model.checkpoint_names()
+    save_file({names[k]: v.contiguous() for k, v in model.state_dict().items()}, str(tmp_path / "model.safetensors"))
+    run = ["generate", "--model", str(tmp_path), "--tokens", "1,2,3,4", "--max-new-tokens", "40"]
+
+    def tokens(*more):
+        assert command(run + list(more)) == 0
+        return [int(t) for t in capsys.readouterr().out.strip().splitlines()[-1].split(",")]
+
+    model = checkpoint.load_model(tmp_path, cuda, torch.bfloat16)
+    for more, penalties in (((), None), (("--presence-penalty", "1e4"), dict(presence=1e4)),
+                            (("--repetition-penalty", "1.5", "--frequency-penalty", "0.5"), dict(repetition=1.5, frequency=0.5))):
+        dec = decoding.DenseDecoder(model, 1, 44)
+        if penalties:
+            dec.set_penalties(**penalties)
+        dec.prefill(torch.tensor([[1, 2, 3, 4]]))
+        assert tokens(*more) == dec.generate(40)[0].tolist()
+    assert len(set(tokens("--presence-penalty", "1e4"))) == 40
+    with pytest.raises(SystemExit):
+        command(run + ["--repetition-penalty", "0"])
 
 
 def test_refusals(cuda):
