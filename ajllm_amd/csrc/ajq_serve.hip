@@ -166,8 +166,9 @@ SharedPlan shared_plan(const ajqs_shared_attention_args* a) {
     p.own_alone = shared_alone(own_units * p.own_tiles, (long long)a->prefix_cap + a->max_len, 384);
     p.own_blocks = p.own_alone ? ceil_div(own_units * p.own_tiles, 4) : ceil_div(own_units, 8) * 8 * p.own_tiles;
   } else {
-    // (128 queries a head behind 8192 rows: few 21.9, many 22.3 us; 120 of 16 heads behind 4096 25.6 and 27.6; 256 behind 8192 31.0 and 27.9)
-    p.form = bf16 && all > 128 ? SharedForm::many : SharedForm::few;
+    // 128 queries a head behind 8192 rows of 8 heads: few 21.9, many 22.3 us; 120 of 16 heads behind 4096 25.6 and 27.6; 256 behind 8192 31.0 and 27.9.  Behind 32768
+    // rows of 8 heads, 64 queries 37.3 and 36.4, 96 50.2 and 43.7, 128 56.4 and 49.5; 96 of 16 heads behind 8192 44.1 and 47.4.
+    p.form = bf16 && (all > 128 || (all > 64 && prefix_units * ceil_div(a->prefix_cap, 128) > 1024)) ? SharedForm::many : SharedForm::few;
     // Tiles of 32 queries fetch rows half as often as tiles of 16, which are twice as many and wait less: 16 it is while rows come from L2 and workgroups are few.  The
     // prefix (32 heads in five groups of 30 queries, 4672 fp32 rows: 137 us with 32, 221 with 16; 16 heads, 30 queries, 4000 rows 29.6 and 26.4; 8 heads, 64 queries,
     // 4000 bf16 rows 11.0 and 10.1, 64 fp32 19.6 and 21.5); own rows that are fp32 (64 sequences of 28 queries, 1000 rows 128 and 142 us; 2 of 28, 300 rows 23.4 and

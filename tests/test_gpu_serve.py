@@ -273,6 +273,7 @@ FEW = [   # (groups, batch, tokens, heads, kv, prefix, max_len): one and two til
 ]
 MANY = [   # tiles of 64 and of 128 queries for the prefix, of 16 and of 32 for own rows
     (1, 40, 1, 8, 2, 900, 70), (3, 33, 1, 24, 2, 1000, 300), (1, 9, 7, 8, 2, 1500, 200), (1, 130, 1, 8, 2, 8200, 40), (2, 64, 9, 8, 2, 8500, 60), (1, 97, 1, 9, 9, 900, 256), (1, 130, 1, 8, 2, 14000, 40),
+    (1, 70, 1, 12, 12, 11200, 40),
 ]
 WALK = [   # several parts and one, most rows before or in the sequences' own, odd and even numbers of blocks
     (1, 2, 70, 4, 2, 500, 900), (2, 6, 33, 8, 2, 1000, 40), (1, 16, 64, 32, 8, 700, 300), (1, 16, 90, 32, 8, 1290, 200), (2, 32, 70, 8, 4, 130, 1000),
