@@ -37,7 +37,7 @@ def _of_rows(name: str, value: torch.Tensor | float | None, batch: int, device: 
     if value is None:
         return None
     if not isinstance(value, torch.Tensor):
-        return torch.full((batch,), float(value), device=device)
+        return torch.full((batch,), float(value), dtype=torch.float32, device=device)   # (the kernel reads fp32, whatever the default dtype)
     if value.dtype != torch.float32 or tuple(value.shape) != (batch,) or not value.is_contiguous() or value.device != device:
         raise ValueError(f"adjust_logits: {name} must be a number or contiguous float32 [B] on the device of the logits")
     return value
