@@ -87,7 +87,7 @@ class GraphDecoder:
             raise ValueError("allowed_rows without allowed")
         if bias and not all(0 <= v < self.model.vocab_size for v in bias):
             raise ValueError(f"biased tokens must be in [0, {self.model.vocab_size})")
-        rows = lambda value: torch.full((self.batch,), float(value), device=self.device)  # noqa: E731
+        rows = lambda value: torch.full((self.batch,), float(value), dtype=torch.float32, device=self.device)  # noqa: E731
         self.adjustments = {}
         if repetition != 1.0:
             self.adjustments["repetition"] = rows(repetition)

@@ -1,11 +1,12 @@
 """Numbers that kernels read as fp32 are fp32 whatever torch's default dtype is."""
 
 import contextlib
+from types import SimpleNamespace
 
 import pytest
 import torch
 
-from ajllm_amd import sampling
+from ajllm_amd import decoding, modeling, sampling
 from tests import serve_plain
 
 DEFAULTS = [torch.bfloat16, torch.float64]
@@ -26,6 +27,44 @@ def test_numbers_become_fp32_rows(dtype):
     with _default(dtype):
         rows = sampling._of_rows("repetition", 1.25, 4, torch.device("cpu"))
     assert rows.dtype == torch.float32 and rows.tolist() == [1.25] * 4
+
+
+def _stub(**more):
+    """What the setters of a decoder look at, without a device."""
+    return SimpleNamespace(batch=3, max_len=5, device=torch.device("cpu"), model=SimpleNamespace(vocab_size=11), _drop_graphs=lambda: None, **more)
+
+
+@pytest.mark.parametrize("dtype", DEFAULTS)
+def test_penalties_become_fp32_rows(dtype):
+    stub = _stub()
+    with _default(dtype):
+        decoding.GraphDecoder.set_penalties(stub, repetition=1.25, frequency=0.5, presence=0.25, bias={4: 1.5})
+    for name, value in (("repetition", [1.25] * 3), ("frequency", [0.5] * 3), ("presence", [0.25] * 3), ("bias", [[1.5]] * 3)):
+        assert stub.adjustments[name].dtype == torch.float32 and stub.adjustments[name].tolist() == value, name
+
+
+def _small_model(dtype=torch.float32):
+    torch.manual_seed(0)
+    with _default(torch.float32):
+        return modeling.TransformerLM(vocab_size=101, context_length=64, d_model=64, num_layers=1, num_heads=2, d_ff=64).to(dtype)
+
+
+def _decoded(model, cuda, **sampling_of):
+    decoder = decoding.GraphDecoder(model, 3, 24)
+    if sampling_of:
+        decoder.set_sampling(**sampling_of)
+    decoder.set_penalties(repetition=1.5, frequency=0.5, presence=0.25, bias={7: 1.5})
+    decoder.prefill(torch.arange(12).view(3, 4))
+    return decoder.generate(16)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DEFAULTS)
+def test_a_decoder_takes_penalties_under_any_default(cuda, dtype):
+    model = _small_model().to(cuda)
+    want = _decoded(model, cuda)
+    with _default(dtype):
+        assert torch.equal(_decoded(model, cuda), want)
 
 
 @pytest.mark.gpu
