@@ -66,7 +66,7 @@ class GraphDecoder:
         self.uniforms = None
         if self.temperature > 0:
             generator = torch.Generator(device=self.device).manual_seed(int(seed))
-            self.uniforms = torch.rand((self.max_len, self.batch), generator=generator, device=self.device)
+            self.uniforms = torch.rand((self.max_len, self.batch), generator=generator, dtype=torch.float32, device=self.device)
         self._drop_graphs()
 
     def _drop_graphs(self) -> None:

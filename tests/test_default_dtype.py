@@ -43,6 +43,15 @@ def test_penalties_become_fp32_rows(dtype):
         assert stub.adjustments[name].dtype == torch.float32 and stub.adjustments[name].tolist() == value, name
 
 
+@pytest.mark.parametrize("dtype", DEFAULTS)
+def test_random_numbers_of_a_draw_are_fp32(dtype):
+    want, stub = _stub(), _stub()
+    decoding.GraphDecoder.set_sampling(want, 0.8, seed=5)
+    with _default(dtype):
+        decoding.GraphDecoder.set_sampling(stub, 0.8, seed=5)
+    assert stub.uniforms.dtype == torch.float32 and torch.equal(stub.uniforms, want.uniforms)
+
+
 def _small_model(dtype=torch.float32):
     torch.manual_seed(0)
     with _default(torch.float32):
@@ -65,6 +74,15 @@ def test_a_decoder_takes_penalties_under_any_default(cuda, dtype):
     want = _decoded(model, cuda)
     with _default(dtype):
         assert torch.equal(_decoded(model, cuda), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DEFAULTS)
+def test_a_decoder_draws_under_any_default(cuda, dtype):
+    model = _small_model().to(cuda)
+    want = _decoded(model, cuda, temperature=0.9, top_p=0.9, seed=4)
+    with _default(dtype):
+        assert torch.equal(_decoded(model, cuda, temperature=0.9, top_p=0.9, seed=4), want)
 
 
 @pytest.mark.gpu
