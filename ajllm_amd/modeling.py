@@ -274,7 +274,7 @@ class RingCache:
         self.rings = [torch.zeros((batch, rows, width) if g is None else (batch, g, rows, width), device=device, dtype=dtype)
                       for rows, width, g in zip(capacities, widths, groups)]
         self.kept = kept or [0] * runs
-        self.states = [torch.zeros((batch, *shape), device=device) if shape is not None else None
+        self.states = [torch.zeros((batch, *shape), dtype=torch.float32, device=device) if shape is not None else None
                        for shape in states or [None] * runs]
         self.batch = batch
         self.length = 0

@@ -101,3 +101,10 @@ def test_adjust_logits_takes_numbers_under_any_default(cuda, dtype):
     assert got.dtype == torch.float32 and torch.equal(got, same)
     # 4 roundings (quotient, count times frequency, sum with presence, difference) and the numbers' own to fp32: 5 steps of 2^-24 of what is added up
     assert bool(((got.double().cpu() - want).abs() <= 5 * 2.0 ** -24 * size).all())
+
+
+@pytest.mark.parametrize("dtype", DEFAULTS)
+def test_states_of_a_cache_are_fp32(dtype):
+    with _default(dtype):
+        cache = modeling.RingCache([4], [16], 2, 8, torch.device("cpu"), torch.bfloat16, states=[(4, 16, 4)])
+    assert cache.states[0].dtype == torch.float32 and cache.rings[0].dtype == torch.bfloat16
