@@ -88,7 +88,19 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(NormRope a) {
       float ss = 0.f;
 #pragma unroll
       for (int i = 0; i < DPL; ++i) ss += x[u].v[i] * x[u].v[i];
-      const Divisor by_rms(sqrtf(team_sum16(ss) / (float)HD + a.eps));
+      float mean = team_sum16(ss) / (float)HD + a.eps;
+      if (!(mean >= 0x1p-100f && mean <= 0x1.fffffep127f)) {
+        // squares past what fp32 holds (components above 1.6e18), or lost at its lower end (no epsilon, components below 1e-15): the same of x times a power of two
+        const float by = mean > 1.f ? 0x1p-100f : 0x1p100f;
+        ss = 0.f;
+#pragma unroll
+        for (int i = 0; i < DPL; ++i) {
+          x[u].v[i] *= by;
+          ss += x[u].v[i] * x[u].v[i];
+        }
+        mean = team_sum16(ss) / (float)HD + a.eps * by * by;
+      }
+      const Divisor by_rms(sqrtf(mean));
 #pragma unroll
       for (int i = 0; i < DPL; ++i) x[u].v[i] = by_rms.divide(x[u].v[i]) * (query ? gain[0].v[i] : gain[1].v[i]);
     }
