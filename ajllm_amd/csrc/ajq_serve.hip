@@ -399,15 +399,17 @@ int ajqs_adjust_logits(const ajqs_adjust_logits_args* a, void* stream) {
   if (!known(a->dtype)) return fail(AJQ_ERR_UNSUPPORTED, "%s: unknown element type", what);
   if (a->logits == a->out && (a->dtype != AJQS_F32 || a->ld != a->out_ld))
     return fail(AJQ_ERR_UNSUPPORTED, "%s: only fp32 logits can be adjusted in place, row by row", what);
-  if (a->tokens && (a->max_tokens < 0 || a->max_tokens > kMaxHistory || a->tokens_ld < a->max_tokens))
+  // (read only: a stride of 0 is one list, or mask, for all rows)
+  auto rows_of = [](long long stride, long long width) { return stride == 0 || stride >= width; };
+  if (a->tokens && (a->max_tokens < 0 || a->max_tokens > kMaxHistory || !rows_of(a->tokens_ld, a->max_tokens)))
     return fail(AJQ_ERR_SHAPE, "%s: %d tokens a row (at most %d, and the rows' stride %lld)", what, a->max_tokens, kMaxHistory,
                 (long long)a->tokens_ld);
-  if (a->prompt && (a->max_prompt < 0 || a->max_prompt > kMaxHistory || a->prompt_ld < a->max_prompt))
+  if (a->prompt && (a->max_prompt < 0 || a->max_prompt > kMaxHistory || !rows_of(a->prompt_ld, a->max_prompt)))
     return fail(AJQ_ERR_SHAPE, "%s: %d prompt tokens a row (at most %d, and the rows' stride %lld)", what, a->max_prompt, kMaxHistory,
                 (long long)a->prompt_ld);
   if (a->bias_ids && (a->biases < 0 || a->biases > kMaxBiases || a->bias_ld < a->biases))
     return fail(AJQ_ERR_SHAPE, "%s: %d biases a row (at most %d, and the rows' stride %lld)", what, a->biases, kMaxBiases, (long long)a->bias_ld);
-  if (a->allowed && (a->masks < 1 || a->allowed_ld < ((long long)a->vocab + 31) / 32))
+  if (a->allowed && (a->masks < 1 || !rows_of(a->allowed_ld, ((long long)a->vocab + 31) / 32)))
     return fail(AJQ_ERR_SHAPE, "%s: masks of %lld words for a vocabulary of %d", what, (long long)a->allowed_ld, a->vocab);
   if (a->allowed && !a->allowed_rows && a->masks < a->batch)
     return fail(AJQ_ERR_SHAPE, "%s: %d masks for %d rows", what, a->masks, a->batch);

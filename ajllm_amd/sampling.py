@@ -58,7 +58,7 @@ def adjust_logits(logits: torch.Tensor, *, tokens: torch.Tensor | None = None, l
       ``allowed_rows[b]`` (int64 ``[B]``; a number outside ``[0, masks)``: none), or mask b without it.  A row whose mask leaves nothing is ``-inf``.
 
     ``tokens`` and ``prompt`` are int64 ``[B, n]``, of which the first ``lengths`` (``prompt_lengths``) count: int64 on the device, one a row or
-    one for all (a decoder's step counter), None: all of them.  Ids outside ``[0, V)`` are passed over.  ``repetition``, ``frequency`` and
+    one for all (a decoder's step counter), None: all of them; lists and masks that all rows share may be expanded (a stride of 0).  Ids outside ``[0, V)`` are passed over.  ``repetition``, ``frequency`` and
     ``presence`` are numbers or fp32 ``[B]``.  ``out`` may be ``logits`` itself where they are fp32 (and overlaps them in no other way); without it the rows of the result begin
     on 16-byte boundaries, as ``ajq_sample_pick`` wants them (fp32 logits that nothing is to happen to are returned as they are)."""
     if not logits.is_cuda:

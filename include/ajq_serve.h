@@ -86,7 +86,8 @@ typedef struct {
  * The first min(token_counts[b * token_count_stride], max_tokens) of row b's tokens count (stride 0: one number for all; token_counts
  * NULL: all), prompt likewise.  Ids outside [0, vocab) are passed over.  Mask of row b: row allowed_rows[b] of allowed [masks, allowed_ld] (NULL: row b),
  * none where that is not in [0, masks).  Each of repetition, frequency and presence may be NULL (1, 0, 0), as may
- * tokens, prompt, bias_ids and allowed.  Up to 1024 biases a row, 1048575 tokens a row. */
+ * tokens, prompt, bias_ids and allowed.  Row strides of tokens, prompt and allowed may be 0: one list, or mask, for all rows.  Up to 1024 biases a
+ * row, 1048575 tokens a row. */
 int ajqs_adjust_logits(const ajqs_adjust_logits_args* args, void* stream);
 
 #ifdef __cplusplus

@@ -3,7 +3,7 @@
 import pytest
 import torch
 
-from ajllm_amd import attention
+from ajllm_amd import attention, sampling
 from tests import serve_plain
 
 pytestmark = pytest.mark.gpu
@@ -37,3 +37,23 @@ def test_norm_rope_heads_whose_squares_pass_fp32(cuda, hd, in_type, tokens, size
         assert bool(torch.isfinite(got).all()), what
         assert bool(((got.double().cpu() - exact).abs() <= 16 * 2.0 ** -24 * magnitude + 2.0 ** -149).all()), what
     assert torch.equal(on[4].double().cpu(), want[2])
+
+
+@pytest.mark.parametrize("type", [F32, BF16])
+def test_adjust_logits_takes_lists_and_masks_that_rows_share(cuda, type):
+    """Expanded lists and masks are the same as copies of them for every row, down to the bit."""
+    gen = torch.Generator().manual_seed(9)
+    batch, vocab = 5, 1500
+    logits = (torch.randn((batch, vocab), generator=gen) * 4).to(type).to(cuda)
+    prompt, tokens = (torch.randint(-3, 200, (1, n), generator=gen).to(cuda) for n in (90, 33))
+    allowed = torch.randint(-2 ** 31, 2 ** 31, (1, 47), generator=gen).int().to(cuda)
+    more = dict(lengths=torch.tensor([33, 0, 7, 20, 1], device=cuda), prompt_lengths=torch.tensor([60], device=cuda), repetition=1.5, frequency=0.25, presence=0.5)
+    shared = dict(tokens=tokens.expand(batch, 33), prompt=prompt.expand(batch, 90), allowed=allowed.expand(batch, 47))
+    assert all(t.stride(0) == 0 for t in shared.values())
+    got = sampling.adjust_logits(logits, **shared, **more)
+    assert torch.equal(got, sampling.adjust_logits(logits, **{k: t.contiguous() for k, t in shared.items()}, **more))
+    want, size = serve_plain.adjust_logits(logits.cpu(), shared["tokens"].cpu(), more["lengths"].cpu(), shared["prompt"].cpu(), more["prompt_lengths"].cpu(), 1.5, 0.25, 0.5, None,
+                                           None, shared["allowed"].cpu(), None)
+    got = got.double().cpu()
+    assert torch.equal(torch.isinf(got), torch.isinf(want))
+    assert bool((torch.where(torch.isinf(want), 0.0, (got - want).abs()) <= 4 * 2.0 ** -24 * size).all())   # (four roundings, each 2^-24 of what is added up)
