@@ -112,6 +112,7 @@ int allow_lds(K kernel, int bytes, const char* what) {
 }
 
 long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
+constexpr long long kMostLanes = 0xFFFFFFFFLL;   // of a grid in a dimension: HIP launches no more
 
 // How an attention call is cut up: tiles of queries, parts of the rows.  The device's lengths are not known here; the capacities are what they
 // can be.
@@ -295,6 +296,8 @@ int ajqs_norm_rope(const ajqs_norm_rope_args* a, void* stream) {
       (long long)a->batch * a->tokens > 0x7FFFFFFFLL)
     return fail(AJQ_ERR_SHAPE, "%s: unsupported shape (batch=%d tokens=%d heads=%d kv_heads=%d max_len=%d table_rows=%d)", what, a->batch,
                 a->tokens, a->heads, a->kv_heads, a->max_len, a->table_rows);
+  if ((long long)a->batch * a->tokens > kMostLanes / 256)
+    return fail(AJQ_ERR_SHAPE, "%s: %d x %d tokens in a launch", what, a->batch, a->tokens);
   const long long all = (long long)a->heads + 2ll * a->kv_heads, room = (long long)a->max_len * a->dim;
   if (all > 1 << 20 || a->ld < all * a->dim || a->ld % 4 != 0)
     return fail(AJQ_ERR_SHAPE, "%s: rows of %lld elements (a multiple of 4, at least %lld)", what, (long long)a->ld, all * a->dim);
@@ -343,7 +346,8 @@ int ajqs_shared_attention(const ajqs_shared_attention_args* a, void* workspace, 
   const char* what = "ajqs_shared_attention";
   if (int e = check_shared(a)) return e;
   const SharedPlan p = shared_plan(a);
-  if (p.prefix_blocks + p.own_blocks > 0x7FFFFFFFLL) return fail(AJQ_ERR_SHAPE, "%s: too many tiles of queries", what);
+  if (p.prefix_blocks + p.own_blocks > kMostLanes / 256) return fail(AJQ_ERR_SHAPE, "%s: too many tiles of queries", what);
+  if (p.bytes && ceil_div(p.queries, 4) > kMostLanes / 256) return fail(AJQ_ERR_SHAPE, "%s: too many queries (%lld)", what, p.queries);
   if (p.bytes && (!workspace || workspace_bytes < p.bytes))
     return fail(AJQ_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, %zu given", what, p.bytes, workspace_bytes);
   if (!aligned16(workspace)) return fail(AJQ_ERR_ALIGN, "%s: the workspace must be 16-byte aligned", what);
@@ -425,7 +429,7 @@ int ajqs_adjust_logits(const ajqs_adjust_logits_args* a, void* stream) {
   while (slice > 1024 && (long long)a->batch * ceil_div(a->vocab, slice) < 512) slice /= 2;
   const int threads = std::min(slice / 4, std::max(256, slice / (4 * kSlicePieces))), slices = (int)ceil_div(a->vocab, slice);
   const long long blocks = ceil_div(a->batch, 8) * 8 * slices;
-  if (blocks > 0x7FFFFFFFLL) return fail(AJQ_ERR_SHAPE, "%s: %d rows of %d", what, a->batch, a->vocab);
+  if (blocks > kMostLanes / threads) return fail(AJQ_ERR_SHAPE, "%s: %d rows of %d", what, a->batch, a->vocab);
   const AdjustLogits n{a->logits, a->out, a->max_tokens ? int64s(a->tokens) : nullptr, int64s(a->token_counts), a->max_prompt ? int64s(a->prompt) : nullptr, int64s(a->prompt_counts),
                        a->repetition, a->frequency, a->presence, int64s(a->bias_ids), a->bias, a->allowed, int64s(a->allowed_rows), a->ld, a->out_ld, a->tokens_ld,
                        a->prompt_ld, a->bias_ld, a->allowed_ld, a->vocab, a->max_tokens, a->max_prompt, a->bias_ids ? a->biases : 0, a->masks,

@@ -5,7 +5,7 @@ import ctypes
 import pytest
 
 from ajllm_amd import _lib
-from tests.test_serve_abi import LOGITS, _filled, _refused, memory  # noqa: F401
+from tests.test_serve_abi import LOGITS, NORM, SHARED, _filled, _refused, memory  # noqa: F401
 
 
 @pytest.mark.parametrize("change", [dict(tokens_ld=0), dict(prompt_ld=0), dict(allowed_ld=0), dict(tokens_ld=0, prompt_ld=0, allowed_ld=0)])
@@ -19,3 +19,20 @@ def test_lists_and_masks_may_be_shared_by_all_rows(memory, change):  # noqa: F81
 def test_other_strides_are_refused(memory, change, message):  # noqa: F811
     args = _filled(_lib.AdjustLogitsArgs, memory, **{**LOGITS, "out": memory + 1024, **change})
     _refused(_lib.load_serve().ajqs_adjust_logits, args, -2, message)
+
+
+def test_launches_of_2_to_the_32_lanes_are_refused(memory):  # noqa: F811
+    """A grid has fewer than 2^32 lanes in a dimension.  (One less is let through, to a later check.)"""
+    lib = _lib.load_serve()
+    many = 2 ** 24   # workgroups of 256 lanes
+    for batch, tokens in ((many, 1), (2 ** 12, 2 ** 12), (3, many // 3 + 1)):
+        _refused(lib.ajqs_norm_rope, _filled(_lib.NormRopeArgs, memory, **{**NORM, "batch": batch, "tokens": tokens, "values": memory + 2 ** 38}), -2, "tokens in a launch")
+    _refused(lib.ajqs_norm_rope, _filled(_lib.NormRopeArgs, memory, **{**NORM, "batch": 1, "tokens": many - 1, "eps": -1.0, "values": memory + 2 ** 38}), -2, "epsilon")
+    one = {**SHARED, "heads": 1, "kv_heads": 1, "groups": 1}
+    # everything in one launch, four sequences a workgroup, or more tokens; parts, whose merge takes four queries a workgroup
+    for change in (dict(batch=4 * many), dict(batch=4 * many, prefix_cap=4096), dict(batch=2, tokens=2 * many, prefix_cap=4096)):
+        args = _filled(_lib.SharedAttentionArgs, memory, **{**one, **change})
+        _refused(lib.ajqs_shared_attention, args, -2, "too many", memory, 1 << 62)
+    for batch, vocab in ((2 ** 22, 16384), (2 ** 22, 3), (2 ** 19, 128256)):
+        args = _filled(_lib.AdjustLogitsArgs, memory, **{**LOGITS, "out": memory + 4 * 2 ** 19, "batch": batch, "vocab": vocab, "ld": 2 ** 20, "out_ld": 2 ** 20, "allowed": None})
+        _refused(lib.ajqs_adjust_logits, args, -2, f"{batch} rows of {vocab}")
