@@ -90,6 +90,8 @@ def adjust_logits(logits: torch.Tensor, *, tokens: torch.Tensor | None = None, l
     if allowed_rows is not None and (allowed is None or allowed_rows.dtype != torch.int64 or tuple(allowed_rows.shape) != (batch,)
                                      or not allowed_rows.is_contiguous() or allowed_rows.device != device):
         raise ValueError("adjust_logits: allowed_rows must be contiguous int64 [B] on the device of the logits, beside masks")
+    if max(batch, vocab, most, most_before, 0 if bias is None else bias.shape[1], 0 if allowed is None else allowed.shape[0]) >= 2 ** 31:
+        raise ValueError("adjust_logits: fewer than 2^31 rows, tokens, listed tokens, biases and masks expected")
     if out is None:
         out = torch.empty((batch, vocab + -vocab % 4), dtype=torch.float32, device=device)[:, :vocab]
     elif out.shape != logits.shape or out.dtype != torch.float32 or out.stride(1) != 1 or out.device != device:

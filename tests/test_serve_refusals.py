@@ -3,8 +3,10 @@
 import ctypes
 
 import pytest
+import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
 
-from ajllm_amd import _lib
+from ajllm_amd import _lib, sampling
 from tests.test_serve_abi import LOGITS, NORM, SHARED, _filled, _refused, memory  # noqa: F401
 
 
@@ -36,3 +38,17 @@ def test_launches_of_2_to_the_32_lanes_are_refused(memory):  # noqa: F811
     for batch, vocab in ((2 ** 22, 16384), (2 ** 22, 3), (2 ** 19, 128256)):
         args = _filled(_lib.AdjustLogitsArgs, memory, **{**LOGITS, "out": memory + 4 * 2 ** 19, "batch": batch, "vocab": vocab, "ld": 2 ** 20, "out_ld": 2 ** 20, "allowed": None})
         _refused(lib.ajqs_adjust_logits, args, -2, f"{batch} rows of {vocab}")
+
+
+@pytest.mark.parametrize("name", ["rows", "vocabulary", "tokens", "prompt", "biases", "masks"])
+def test_adjust_logits_refuses_sizes_past_32_bits(name):
+    """A size handed on as 32 bits of it would be another size: 2^32 + 5 tokens are not 5.  (Tensors without memory.)"""
+    size = lambda this, other: 2 ** 32 + 5 if name == this else other  # noqa: E731
+    with FakeTensorMode():
+        whole = lambda *shape: torch.empty(shape, dtype=torch.long, device="cuda")  # noqa: E731
+        batch, vocab = size("rows", 1), size("vocabulary", 64)
+        args = dict(tokens=whole(batch, size("tokens", 3)), prompt=whole(batch, size("prompt", 3)), bias_ids=whole(batch, size("biases", 3)),
+                    bias=torch.empty((batch, size("biases", 3)), dtype=torch.float32, device="cuda"),
+                    allowed=torch.empty((size("masks", batch), (vocab + 31) // 32), dtype=torch.int32, device="cuda"))
+        with pytest.raises(ValueError, match="2\\^31"):
+            sampling.adjust_logits(torch.empty((batch, vocab), dtype=torch.float32, device="cuda"), **args)
