@@ -52,3 +52,15 @@ def test_adjust_logits_refuses_sizes_past_32_bits(name):
                     allowed=torch.empty((size("masks", batch), (vocab + 31) // 32), dtype=torch.int32, device="cuda"))
         with pytest.raises(ValueError, match="2\\^31"):
             sampling.adjust_logits(torch.empty((batch, vocab), dtype=torch.float32, device="cuda"), **args)
+
+
+@pytest.mark.parametrize("shape", [dict(prefix_cap=1024, max_len=512, prefix_group=131072, prefix_head=65536, cache_batch=65536, cache_head=32768),   # parts of either
+                                   dict(prefix_cap=1024, max_len=16, tokens=40, cache_dtype=1, prefix_group=131072, prefix_head=65536)])             # a walk in parts
+def test_workspaces_that_do_not_do_are_refused(memory, shape):  # noqa: F811
+    lib = _lib.load_serve()
+    args = _filled(_lib.SharedAttentionArgs, memory, **{**SHARED, **shape})
+    need = lib.ajqs_shared_attention_workspace(ctypes.byref(args))
+    assert need > 0 and need % (4 * 4 * args.tokens * (8 + 4 * 64)) == 0   # [parts, queries] of (maximum, sum) and 64 components, fp32
+    for at, size, status, message in ((memory, need - 1, -6, "bytes needed"), (None, need, -6, "bytes needed"), (memory, 0, -6, "bytes needed"),
+                                      (memory + 8, need, -3, "workspace must be")):
+        _refused(lib.ajqs_shared_attention, args, status, message, at, size)
