@@ -168,7 +168,9 @@ def shared_prefix_attention(q: torch.Tensor, prefix_keys: torch.Tensor, prefix_v
     rows, the T new tokens' (``norm_rope`` writes them) included.  Token t of sequence b sees its group's prefix and its own rows up to ``rows[b]
     + offset + t``.  Caches fp32 or bf16; ``prefix_lengths`` int64 ``[G]``, ``rows`` and ``counts`` int64 ``[B]``, ``offset`` one int64, on
     the device, as in ``norm_rope``.  Returns bf16 ``[B, T, H * hd]`` (what the output projection takes); zeros for a token that is not there
-    or sees nothing."""
+    or sees nothing.  Rows that nobody sees may hold anything; values that a token of the sequence sees must be finite.  The launches are chosen by the
+    capacities (``shared_prefix_launches``), not by the lengths: slices of the caches down to what can be filled are the faster.  Precision, and the memory that a call
+    takes for itself: include/ajq_serve.h."""
     what = "shared_prefix_attention"
     if not q.is_cuda:
         raise ValueError("shared_prefix_attention needs tensors on a ROCm device (there is no CPU path)")

@@ -153,7 +153,7 @@ SharedPlan shared_plan(const ajqs_shared_attention_args* a) {
   if (bf16 && mine > 64) {
     p.form = SharedForm::walk;
     // Tiles of 128 queries (bf16 ones of 128 components: more do not leave registers, narrower heads' steps are too short) where there are enough of them and
-    // most rows are the prefix's; else of 64.  16 sequences of 100 tokens x 4 behind 2048 rows 74 us, 90 with tiles of 64; of 400 behind 2048 229 and 292; of 100
+    // most rows are the prefix's; else of 64.  (Both sides in first calls after a pause, whose clock is some 10 % lower.)  16 sequences of 100 tokens x 4 behind 2048 rows 74 us, 90 with tiles of 64; of 400 behind 2048 229 and 292; of 100
     // behind 100 + 1400 74 and 47; 8 of 40 behind 1000 24 and 21; 12 heads of 64, 16 of 300 behind 2048: 68 and 58.
     p.own_rt = a->q_dtype == AJQS_BF16 && a->dim == 128 && a->prefix_cap >= a->max_len && own_units * ceil_div(mine, 128) >= 256 ? 2 : 1;
     p.own_tiles = (int)ceil_div(mine, 64 * p.own_rt);

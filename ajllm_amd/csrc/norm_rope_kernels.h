@@ -5,7 +5,7 @@
 //
 // Sixteen lanes hold a head (dim / 16 components each, in the places LaneDims gives them), so the sum of squares is four DPP adds and
 // a pair never leaves its lane.  Everything is read once and written once, which is what bounds it: 16 prompts of 333 tokens (32 + 16 heads of 128, fp32 in,
-// bf16 out, 160 MB) 28.2 us = 5.7 TB/s; a token of each of 96 sequences 3.3 us, of 8 2.8, of which a launch takes 2.6.
+// bf16 out, 160 MB) 28.2 to 30.0 us = 5.3 to 5.7 TB/s; a token of each of 96 sequences 3.3 us, of 8 2.8, of which a launch takes 2.6.
 #pragma once
 #include "lane_rows.h"
 

@@ -197,9 +197,11 @@ __device__ __forceinline__ void find_both(const SharedAttention& a, Meeting<Cach
 
 // ---- Few queries: the four waves of a workgroup take blocks of 32 rows in turn, each for itself (no barrier until the end), and RT tiles of 16
 // queries meet every row fetched.  Where there are sequences enough, each wave takes all rows of its own tile instead, and has nobody to join.  What bounds
-// it is memory: a wave asks for the next block's keys as soon as it has used this block's, and for its values likewise; eight waves a CU (bf16) then have 64 to
-// 128 KB on their way.  8 prompts of 1500 rows with 8 sequences of 300 each (12 heads of 64, 59 MB) 12.8 us = 4.6 TB/s.
-// LDS of a wave: keys, then values, 32 rows each; fp32 rows as two planes of bf16, through registers.
+// it (but for tiles of 32 on fp32 rows) is memory: a wave asks for the next block's keys as soon as it has used this block's, and for its values likewise; eight
+// waves a CU (bf16) then have 64 to 128 KB on their way.  8 prompts of 1500 rows with 8 sequences of 300 each (12 heads of 64, 59 MB) 12.8 us = 4.6 TB/s.
+// LDS of a wave: keys, then values, 32 rows each; fp32 rows as two planes of bf16, through registers.  Tiles of 32 queries on fp32 rows are bound by that: each wave splits its
+// rows for its 32 queries alone, and one wave a SIMD (212 registers) has nothing to run beside it.  16 sequences of 100 tokens x 4 of 8 heads behind 2048 rows 386 us: 39 % of a SIMD's
+// cycles are vector instructions, 16 % MFMAs.
 template <int HD, typename CacheT> constexpr int few_wave_bytes() { return 2 * 32 * 2 * HD * kHalves<CacheT>; }
 template <int HD, int RT> constexpr int few_join_bytes() { return 4 * RT * 16 * (HD + 4) * 4; }
 template <int HD, typename CacheT, int RT> constexpr int few_lds_bytes() {
@@ -953,8 +955,9 @@ __global__ __launch_bounds__(256, 2) void shared_attention_many_kernel(SharedAtt
 }
 
 // Sequences with many new tokens each: 64 U queries of one sequence walk the prefix and then its own rows, and what comes out is the result.  With
-// own_parts > 1 the walk is cut up and leaves parts for the merge.  16 sequences of 100 tokens x 4 of 8 heads behind 2048 rows 71 us = 590 TFLOP/s (358 tiles on 256 CUs), 24 of 50
-// behind 8000 203 us = 775.
+// own_parts > 1 the walk is cut up and leaves parts for the merge.  16 sequences of 100 tokens x 4 of 8 heads behind 2048 rows 66 us = 630 TFLOP/s (71 in the first calls after
+// a pause), 24 of 50 behind 8000 203 us = 775.  Of the former's cycles a CU is busy for 63 % (358 tiles on 256 CUs: some have two, some one), and a SIMD for 45 % of those with MFMAs,
+// 36 % with other vector instructions; its LDS is no limit (no bank conflicts).
 template <int HD, typename QT, int U>
 __global__ __launch_bounds__(256, 2) void shared_attention_walk_kernel(SharedAttention a) {
   extern __shared__ __attribute__((aligned(1024))) unsigned char shared_lds[];

@@ -850,7 +850,8 @@ class SharedPrefixDecoder(FusedDecoder):
 
     A prompt's rows (up to ``prefix_len``) are in caches ``[prompts, Hkv, prefix_len, hd]``; every sequence has ``max_len`` rows of its own behind them, at
     positions of its own.  A step is FusedDecoder's with ``attention.norm_rope`` and ``attention.shared_prefix_attention`` in the attention's place,
-    replayed from a graph like it.  Sequence ``b`` continues prompt ``b // completions``."""
+    replayed from a graph like it.  Sequence ``b`` continues prompt ``b // completions``.  Attention's launches are chosen by ``prefix_len`` and ``max_len``, not by
+    what is filled: give what the prompts and continuations need.  Long questions are read several times faster behind bf16 caches (``kv_dtype``) than behind fp32 ones."""
 
     def __init__(self, model: modeling.TransformerLM, prompts: int, completions: int, prefix_len: int, max_len: int,
                  kv_dtype: torch.dtype | None = None, activation_rounding: str = "reference") -> None:

@@ -57,10 +57,15 @@ typedef struct {
 } ajqs_shared_attention_args;
 /* out bf16 [batch, tokens, heads * dim] = softmax(q . k / sqrt(dim)) v of q [batch, heads, tokens, dim]: token t of sequence b sees the
  * first prefix_lengths[g] rows (at most prefix_cap; g = b / (batch / groups)) of its group's prefix caches and its own rows 0 ..
- * rows[b] + *offset + t (at most max_len), which hold the new tokens already.  Zeros where a token is not there or sees nothing.  The
- * rows that a new token of the call makes must be finite; rows that no token of a sequence sees may hold anything.  heads a
+ * rows[b] + *offset + t (at most max_len), which hold the new tokens already.  Zeros where a token is not there or sees nothing.  Values
+ * that a token of the sequence sees must be finite (one that is not may make its component NaN for all tokens of the call, earlier ones too);
+ * rows that no token of a sequence sees may hold anything.  heads a
  * multiple of kv_heads; dim 128, 64 or 32; caches fp32 or bf16, strides in elements, multiples of 8; q fp32 or bf16.
- * Products carry bf16's eight bits of the caches and of bf16 queries, sixteen of fp32 ones; sums, maxima and denominators are fp32.
+ * Products carry all bits of bf16 caches and queries and sixteen at least of fp32 ones; a weight is rounded to bf16 for its product with the values, but
+ * for fp32 rows that tiles of 16 queries meet (short runs; at most 16, or 32, queries of a key head), which are in fp32 throughout; sums, maxima and denominators are fp32.
+ * How the call is cut up goes by the capacities prefix_cap and max_len, since the lengths are on the device: choose them near to what will be filled.  The
+ * workspace holds [parts, batch * heads * tokens] of dim + 2 fp32 numbers; on fp32 caches two parts at least of all but short runs, whatever the number of
+ * tokens (1.06 GB for 16 x 2000 tokens of 32 heads of 128 behind 2048 rows), on bf16 ones none where more than 64 queries of a sequence and key head make tiles enough.
  * (scaled_dot_product_attention, src/ajllm/modeling/attention.py:20-33.) */
 size_t ajqs_shared_attention_workspace(const ajqs_shared_attention_args* args);
 int ajqs_shared_attention(const ajqs_shared_attention_args* args, void* workspace, size_t workspace_bytes, void* stream);

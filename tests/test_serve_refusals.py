@@ -40,6 +40,7 @@ def test_launches_of_2_to_the_32_lanes_are_refused(memory):  # noqa: F811
         _refused(lib.ajqs_adjust_logits, args, -2, f"{batch} rows of {vocab}")
 
 
+@pytest.mark.filterwarnings("ignore:Accessing the data pointer")
 @pytest.mark.parametrize("name", ["rows", "vocabulary", "tokens", "prompt", "biases", "masks"])
 def test_adjust_logits_refuses_sizes_past_32_bits(name):
     """A size handed on as 32 bits of it would be another size: 2^32 + 5 tokens are not 5.  (Tensors without memory.)"""
