@@ -316,7 +316,51 @@ SERVE_SIGNATURES: dict[str, tuple] = {
     "ajqs_adjust_logits": (c_int, [ctypes.POINTER(AdjustLogitsArgs), _P]),
 }
 
+DRAFT_LIBRARY_PATH = LIBRARY_PATH.with_name("libajq_draft.so")
+
+
+class TreeAttentionArgs(ctypes.Structure):
+    """``ajqt_tree_attention_args``"""
+
+    _fields_ = ([(n, c_void_p) for n in ("q", "keys", "values", "masks", "rows", "counts", "offset", "out")]
+                + [(n, c_int64) for n in ("cache_batch", "cache_head", "mask_batch", "mask_token")]
+                + [(n, c_int) for n in ("batch", "tokens", "heads", "kv_heads", "dim", "max_len", "q_dtype", "cache_dtype")])
+
+
+class KeepRowsArgs(ctypes.Structure):
+    """``ajqt_keep_rows_args``"""
+
+    _fields_ = ([(n, c_void_p) for n in ("keys", "values", "rows", "index", "counts", "offset")]
+                + [(n, c_int64) for n in ("cache_layer", "cache_batch", "cache_head", "index_ld")]
+                + [(n, c_int) for n in ("layers", "batch", "kv_heads", "dim", "max_len", "width", "dtype")])
+
+
+class LogProbsArgs(ctypes.Structure):
+    """``ajqt_log_probs_args``"""
+
+    _fields_ = ([(n, c_void_p) for n in ("logits", "targets", "log_probs", "entropy", "top_log_probs", "ranks", "top_ids")]
+                + [("ld", c_int64)] + [(n, c_int) for n in ("rows", "vocab", "top", "dtype")])
+
+
+class FollowDraftsArgs(ctypes.Structure):
+    """``ajqt_follow_drafts_args``"""
+
+    _fields_ = ([(n, c_void_p) for n in ("tokens", "parents", "choices", "counts", "path", "accepted", "chosen")]
+                + [(n, c_int64) for n in ("tokens_ld", "parents_ld", "choices_ld", "choices_step")] + [(n, c_int) for n in ("batch", "nodes")])
+
+
+DRAFT_SIGNATURES: dict[str, tuple] = {
+    "ajqt_last_error": (c_char_p, []),
+    "ajqt_tree_attention_workspace": (c_size_t, [ctypes.POINTER(TreeAttentionArgs)]),
+    "ajqt_tree_attention": (c_int, [ctypes.POINTER(TreeAttentionArgs), _P, c_size_t, _P]),
+    "ajqt_keep_rows": (c_int, [ctypes.POINTER(KeepRowsArgs), _P]),
+    "ajqt_log_probs_workspace": (c_size_t, [ctypes.POINTER(LogProbsArgs)]),
+    "ajqt_log_probs": (c_int, [ctypes.POINTER(LogProbsArgs), _P, c_size_t, _P]),
+    "ajqt_follow_drafts": (c_int, [ctypes.POINTER(FollowDraftsArgs), _P]),
+}
+
 _lib: ctypes.CDLL | None = None
+_draft_lib: ctypes.CDLL | None = None
 _serve_lib: ctypes.CDLL | None = None
 _dense_lib: ctypes.CDLL | None = None
 _bench_lib: ctypes.CDLL | None = None
@@ -437,6 +481,31 @@ def load_serve() -> ctypes.CDLL:
         fn.argtypes = argtypes
     _serve_lib = lib
     return lib
+
+
+def load_draft() -> ctypes.CDLL:
+    """The operators of checking drafted tokens, bound on first use (built by ``python -m ajllm_amd.build``)."""
+    global _draft_lib
+    if _draft_lib is not None:
+        return _draft_lib
+    if not DRAFT_LIBRARY_PATH.exists():
+        raise RuntimeError(f"{DRAFT_LIBRARY_PATH} is missing: build it with `python -m ajllm_amd.build` "
+                           "(these operators have no fallback path)")
+    lib = ctypes.CDLL(str(DRAFT_LIBRARY_PATH))
+    for name, (restype, argtypes) in DRAFT_SIGNATURES.items():
+        fn = getattr(lib, name)
+        fn.restype = restype
+        fn.argtypes = argtypes
+    _draft_lib = lib
+    return lib
+
+
+def check_draft(status: int, what: str) -> None:
+    """``check`` for a status of libajq_draft.so."""
+    if status == 0:
+        return
+    message = f"{what}: {load_draft().ajqt_last_error().decode()}"
+    raise ValueError(message) if status in _ARGUMENT_ERRORS else RuntimeError(message)
 
 
 def check_serve(status: int, what: str) -> None:

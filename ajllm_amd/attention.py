@@ -1,5 +1,5 @@
-"""Host side of the library's causal prefill attention (``ajq_attn_prefill``), and of attention for sequences that share a prefix
-(``norm_rope``, ``shared_prefix_attention``).
+"""Host side of the library's causal prefill attention (``ajq_attn_prefill``), of attention for sequences that share a prefix
+(``norm_rope``, ``shared_prefix_attention``), and of that for trees of drafted tokens (``tree_masks``, ``tree_attention``, ``keep_rows``).
 
 The first stands where the reference switches to its FlashAttention under ``use_flash_attention``
 (src/ajllm/modeling/attention.py:106-117; its own kernels, flash_attention.py:44-108,194-298, need
@@ -203,3 +203,110 @@ def shared_prefix_attention(q: torch.Tensor, prefix_keys: torch.Tensor, prefix_v
         status = lib.ajqs_shared_attention(ctypes.byref(args), _pointer(room), size, torch.cuda.current_stream().cuda_stream)
     _lib.check_serve(status, what)
     return out
+
+
+def tree_masks(parents: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """What a tree of drafted tokens is laid out as: ``masks`` int32 ``[.., T, ceil(T / 32)]``, bit u % 32 of word u // 32 set where u is t or one of its
+    ancestors (what ``tree_attention`` takes), and ``depths`` int64 ``[.., T]``, the number of its ancestors (what ``norm_rope`` takes).
+
+    ``parents`` int64 ``[T]`` (one tree for all sequences) or ``[B, T]``: node t > 0 hangs on ``parents[t]``, in ``[0, t)``; one with another parent, as the
+    root's, has no ancestors.  A few torch operators on the device of ``parents``: a tree that stays the same is laid out once."""
+    if parents.dtype != torch.int64 or parents.dim() not in (1, 2) or 0 in parents.shape:
+        raise ValueError("tree_masks: parents int64 [T] or [B, T] expected")
+    flat = parents if parents.dim() == 2 else parents[None]
+    batch, nodes = flat.shape
+    place = torch.arange(nodes, device=parents.device)
+    # pointers twice as far in each round; one place behind the nodes for what is above a root
+    up = torch.where((flat >= 0) & (flat < place), flat, nodes)
+    up = torch.nn.functional.pad(up, (0, 1), value=nodes)
+    sees = torch.nn.functional.pad(torch.eye(nodes, dtype=torch.bool, device=parents.device), (0, 0, 0, 1)).repeat(batch, 1, 1)
+    for _ in range((nodes - 1).bit_length()):
+        sees = sees | sees.gather(1, up[:, :, None].expand(batch, nodes + 1, nodes))
+        up = up.gather(1, up)
+    sees = sees[:, :nodes]
+    bits = torch.nn.functional.pad(sees, (0, -nodes % 32)).view(batch, nodes, -1, 32).long()
+    words = (bits << torch.arange(32, device=parents.device)).sum(-1)
+    masks = torch.where(words >= 2 ** 31, words - 2 ** 32, words).int()
+    depths = sees.sum(-1) - 1
+    return (masks, depths) if parents.dim() == 2 else (masks[0], depths[0])
+
+
+def tree_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, rows: torch.Tensor, masks: torch.Tensor, *,
+                   counts: torch.Tensor | None = None, offset: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of a tree of ``T`` drafted tokens a sequence over its cache: each sees the committed rows and, of the tokens' own, those that its mask has.
+
+    ``q`` fp32 or bf16 ``[B, H, T, hd]`` (rotated, each by its depth); ``keys`` / ``values`` ``[B, Hkv, max_len, hd]`` fp32 or bf16, the first ``rows[b] +
+    offset`` rows committed, token u's own in row ``rows[b] + offset + u`` (``norm_rope`` writes them).  ``masks`` int32 ``[B, T, >= T / 32]``, or ``[T, >= T /
+    32]`` for all sequences: token t sees token u where bit u % 32 of word u // 32 is set (``tree_masks``; any other set of bits as well).  ``rows`` and
+    ``counts`` int64 ``[B]``, ``offset`` one int64, on the device; of the tokens of sequence b the first ``counts[b]`` are there (None: all), for queries as for
+    rows.  Returns bf16 ``[B, T, H * hd]``; zeros for a token that is not there or sees nothing.  Rows behind the tokens that are there may hold anything; the
+    values of the others must be finite.  Precision, and the memory that a call takes for itself: include/ajq_draft.h."""
+    what = "tree_attention"
+    if not q.is_cuda:
+        raise ValueError("tree_attention needs tensors on a ROCm device (there is no CPU path)")
+    device = q.device
+    _check_caches(what, keys, values, device)
+    if q.dim() != 4 or q.dtype not in _TYPES:
+        raise ValueError("tree_attention: q [B, H, T, hd] in float32 or bfloat16 expected")
+    batch, heads, nodes, hd = q.shape
+    if 0 in q.shape or 0 in keys.shape:
+        raise ValueError("tree_attention: unsupported shape: q and caches with elements expected")
+    if keys.shape[0] != batch or keys.shape[3] != hd:
+        raise ValueError("tree_attention: caches [B, Hkv, max_len, hd] expected")
+    if (masks.dtype != torch.int32 or masks.dim() not in (2, 3) or masks.shape[-2] != nodes or masks.shape[-1] * 32 < nodes or masks.stride(-1) != 1
+            or (masks.dim() == 3 and masks.shape[0] != batch) or masks.device != device):
+        raise ValueError("tree_attention: masks int32 [B, T, words] or [T, words], a bit for every token, on the device of the others expected")
+    _whole_numbers(what, "rows", rows, batch, device)
+    _whole_numbers(what, "counts", counts, batch, device)
+    _whole_numbers(what, "offset", offset, 1, device)
+    q = q.contiguous()
+    out = torch.empty((batch, nodes, heads * hd), dtype=torch.bfloat16, device=device)
+    args = _lib.TreeAttentionArgs(
+        q.data_ptr(), keys.data_ptr(), values.data_ptr(), masks.data_ptr(), rows.data_ptr(), _pointer(counts), _pointer(offset), out.data_ptr(),
+        keys.stride(0), keys.stride(1), masks.stride(0) if masks.dim() == 3 else 0, masks.stride(-2), batch, nodes, heads, keys.shape[1], hd, keys.shape[2],
+        _TYPES[q.dtype], _TYPES[keys.dtype])
+    lib = _lib.load_draft()
+    with _on(device):
+        size = lib.ajqt_tree_attention_workspace(ctypes.byref(args))
+        room = torch.empty(size, dtype=torch.uint8, device=device) if size else None
+        status = lib.ajqt_tree_attention(ctypes.byref(args), _pointer(room), size, torch.cuda.current_stream().cuda_stream)
+    _lib.check_draft(status, what)
+    return out
+
+
+def keep_rows(keys: torch.Tensor, values: torch.Tensor, rows: torch.Tensor, index: torch.Tensor, counts: torch.Tensor | None = None, *,
+              offset: torch.Tensor | None = None) -> None:
+    """Moves the rows that stay together, in place: row ``rows[b] + offset + i`` becomes what row ``rows[b] + offset + index[b, i]`` was.
+
+    ``keys`` / ``values`` fp32 or bf16 ``[B, Hkv, max_len, hd]``, or ``[layers, B, Hkv, max_len, hd]`` for all layers at once; ``rows`` and ``counts`` int64 ``[B]``,
+    ``offset`` one int64, ``index`` int64 ``[B, n]`` (or ``[n]`` for all sequences), on the device.  The first ``counts[b]`` numbers of a list count (None: all).  They ascend
+    from 0 or more, and their rows are in the cache: a list ends ahead of the first number that does not.  No other row is written; heads of the caches may not overlap.
+    ``follow_drafts``' path and length make the accepted drafts of ``tree_attention``'s rows follow the committed ones; a list of any rows, with ``rows`` of 0, gives up the
+    others."""
+    what = "keep_rows"
+    if not keys.is_cuda:
+        raise ValueError("keep_rows needs tensors on a ROCm device (there is no CPU path)")
+    device = keys.device
+    if keys.dim() == 5 and values.dim() == 5:
+        layers, apart = keys.shape[0], keys.stride(0)
+        if keys.shape[0] != values.shape[0] or keys.stride(0) != values.stride(0) or 0 in keys.shape:
+            raise ValueError("keep_rows: caches [layers, B, Hkv, max_len, hd] of one shape and layout expected")
+        first_keys, first_values = keys[0], values[0]
+    else:
+        layers, apart, first_keys, first_values = 1, 0, keys, values
+    _check_caches(what, first_keys, first_values, device)
+    batch, kv_heads, max_len, hd = first_keys.shape
+    _whole_numbers(what, "rows", rows, batch, device)
+    _whole_numbers(what, "counts", counts, batch, device)
+    _whole_numbers(what, "offset", offset, 1, device)
+    if (index.dtype != torch.int64 or index.dim() not in (1, 2) or (index.dim() == 2 and index.shape[0] != batch) or index.device != device
+            or (index.shape[-1] > 1 and index.stride(-1) != 1)):
+        raise ValueError("keep_rows: index int64 [B, n] or [n] on the device of the others expected")
+    if 0 in keys.shape or index.shape[-1] == 0:
+        return
+    args = _lib.KeepRowsArgs(
+        keys.data_ptr(), values.data_ptr(), rows.data_ptr(), index.data_ptr(), _pointer(counts), _pointer(offset), apart, first_keys.stride(0),
+        first_keys.stride(1), index.stride(0) if index.dim() == 2 else 0, layers, batch, kv_heads, hd, max_len, index.shape[-1], _TYPES[keys.dtype])
+    with _on(device):
+        status = _lib.load_draft().ajqt_keep_rows(ctypes.byref(args), torch.cuda.current_stream().cuda_stream)
+    _lib.check_draft(status, what)

@@ -1,4 +1,4 @@
-"""Compile the HIP sources in ``csrc/`` into ``libajq.so``, ``libajq_dense.so`` and ``libajq_serve.so`` next to this file, and the
+"""Compile the HIP sources in ``csrc/`` into ``libajq.so``, ``libajq_dense.so``, ``libajq_serve.so`` and ``libajq_draft.so`` next to this file, and the
 extension module ``_native.so``.
 
 Cross-compiles for gfx950 with hipcc; needs no GPU.  Run as
@@ -24,6 +24,9 @@ DENSE_LIBRARY = PACKAGE_DIR / "libajq_dense.so"
 # operators of decoding many continuations of one prompt (include/ajq_serve.h)
 SERVE_SOURCE = PACKAGE_DIR / "csrc" / "ajq_serve.hip"
 SERVE_LIBRARY = PACKAGE_DIR / "libajq_serve.so"
+# operators of checking drafted tokens (include/ajq_draft.h)
+DRAFT_SOURCE = PACKAGE_DIR / "csrc" / "ajq_draft.hip"
+DRAFT_LIBRARY = PACKAGE_DIR / "libajq_draft.so"
 # a quantized layer's forward (and the operators above) without the interpreter: an extension module that calls the libraries
 NATIVE_SOURCES = [PACKAGE_DIR / "csrc" / "native_linear.cpp", PACKAGE_DIR / "csrc" / "native_serve.cpp"]
 NATIVE_MODULE = PACKAGE_DIR / "_native.so"
@@ -71,6 +74,10 @@ def build_serve_library(verbose: bool = False) -> Path:
     return build_library(verbose, SERVE_SOURCE, SERVE_LIBRARY)
 
 
+def build_draft_library(verbose: bool = False) -> Path:
+    return build_library(verbose, DRAFT_SOURCE, DRAFT_LIBRARY)
+
+
 def ensure_dense_library() -> Path:
     """The dense library, compiled now if it is not there yet."""
     if not DENSE_LIBRARY.exists():
@@ -110,5 +117,6 @@ if __name__ == "__main__":
     print(build_library(verbose=True))
     print(build_dense_library(verbose=True))
     print(build_serve_library(verbose=True))
+    print(build_draft_library(verbose=True))
     print(build_native_module(verbose=True))
     print(build_bench_library(verbose=True))

@@ -1,15 +1,19 @@
 """What a program does to logits ahead of the choice of a token: penalties for repeated tokens, biases, masks of allowed tokens
-(``ajqs_adjust_logits``).  The choice itself is ``decoding``'s (the reference's ``sample_next_token``,
-src/ajllm/generation/sampling.py:8-22, has neither)."""
+(``ajqs_adjust_logits``); what it reads off them: log probabilities, entropies, the most probable alternatives (``ajqt_log_probs``); and what the
+choices behind drafted tokens come to (``ajqt_follow_drafts``).  The choice itself is ``decoding``'s (the reference's ``sample_next_token``,
+src/ajllm/generation/sampling.py:8-22, has none of these)."""
 
 from __future__ import annotations
 
 import ctypes
+from typing import NamedTuple
 
 import torch
 
 from . import _lib
 from .attention import _TYPES, _on, _pointer
+
+MOST_TOP = 64   # alternatives of token_log_probs
 
 
 def _list(name: str, ids: torch.Tensor | None, lengths: torch.Tensor | None, batch: int, device: torch.device) -> tuple:
@@ -106,4 +110,92 @@ def adjust_logits(logits: torch.Tensor, *, tokens: torch.Tensor | None = None, l
     with _on(device):
         status = _lib.load_serve().ajqs_adjust_logits(ctypes.byref(args), torch.cuda.current_stream().cuda_stream)
     _lib.check_serve(status, "adjust_logits")
+    return out
+
+
+class TokenLogProbs(NamedTuple):
+    """``token_log_probs``' results; None for what was not asked for."""
+
+    log_probs: torch.Tensor | None       # fp32 [R]: of the targets
+    ranks: torch.Tensor | None           # int64 [R]: how many tokens come ahead of the target (0: it is the most probable one)
+    entropy: torch.Tensor                # fp32 [R]
+    top_log_probs: torch.Tensor | None   # fp32 [R, top]: of the most probable tokens, the first one first
+    top_ids: torch.Tensor | None         # int64 [R, top]
+
+
+def token_log_probs(logits: torch.Tensor, targets: torch.Tensor | None = None, *, top: int = 0) -> TokenLogProbs:
+    """Log probabilities of given tokens under ``softmax(logits)``, ranks, entropies (in nats) and the ``top`` most probable tokens, in one pass over the logits.
+
+    ``logits`` ``[R, V]`` fp32 or bf16 (rows may be further apart), ``targets`` int64 ``[R]`` (None: neither log probabilities nor ranks; a target
+    outside ``[0, V)`` asks for nothing: log probability 0, rank -1), ``top`` up to 64 and V.  Tokens of equal logits come in the order of their ids,
+    for ranks as for the alternatives: ``top_ids[r, ranks[r]]`` is the target where it is among them, and ``top=1`` is the greedy choice.  A token that a mask has set to -inf has
+    the log probability -inf and adds nothing to the entropy; a row of which nothing is left has -inf for every token, and an entropy of 0.  A row with NaN or +inf gives NaN,
+    and ids and ranks that are some tokens'.  Without a gradient."""
+    what = "token_log_probs"
+    if not logits.is_cuda:
+        raise ValueError("token_log_probs needs tensors on a ROCm device (there is no CPU path)")
+    device = logits.device
+    if logits.dim() != 2 or logits.dtype not in _TYPES or logits.shape[1] == 0 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise ValueError("token_log_probs: logits [R, V] in float32 or bfloat16 expected")
+    rows, vocab = logits.shape
+    if max(rows, vocab) >= 2 ** 31:
+        raise ValueError("token_log_probs: fewer than 2^31 rows and tokens expected")
+    if targets is not None and (targets.dtype != torch.int64 or tuple(targets.shape) != (rows,) or not targets.is_contiguous() or targets.device != device):
+        raise ValueError("token_log_probs: targets must be contiguous int64 [R] on the device of the logits")
+    if not 0 <= top <= min(MOST_TOP, vocab):
+        raise ValueError(f"token_log_probs: top must be in [0, {min(MOST_TOP, vocab)}]")
+    floats = lambda *shape: torch.empty(shape, dtype=torch.float32, device=device)  # noqa: E731
+    whole = lambda *shape: torch.empty(shape, dtype=torch.int64, device=device)     # noqa: E731
+    out = TokenLogProbs(floats(rows) if targets is not None else None, whole(rows) if targets is not None else None, floats(rows),
+                        floats(rows, top) if top else None, whole(rows, top) if top else None)
+    if rows == 0:
+        return out
+    args = _lib.LogProbsArgs(logits.data_ptr(), _pointer(targets), _pointer(out.log_probs), out.entropy.data_ptr(), _pointer(out.top_log_probs),
+                             _pointer(out.ranks), _pointer(out.top_ids), _apart(logits), rows, vocab, top, _TYPES[logits.dtype])
+    lib = _lib.load_draft()
+    with _on(device):
+        size = lib.ajqt_log_probs_workspace(ctypes.byref(args))
+        room = torch.empty(size, dtype=torch.uint8, device=device) if size else None
+        status = lib.ajqt_log_probs(ctypes.byref(args), _pointer(room), size, torch.cuda.current_stream().cuda_stream)
+    _lib.check_draft(status, what)
+    return out
+
+
+class FollowedDrafts(NamedTuple):
+    """``follow_drafts``' results."""
+
+    path: torch.Tensor       # int64 [B, T]: the nodes that were right, from the root on, ascending; then -1
+    accepted: torch.Tensor   # int64 [B]: how many there are (the root is one)
+    chosen: torch.Tensor     # int64 [B, T]: the choices behind them, which is what the step has produced; then -1
+
+
+def follow_drafts(tokens: torch.Tensor, parents: torch.Tensor, choices: torch.Tensor, *, counts: torch.Tensor | None = None) -> FollowedDrafts:
+    """The drafts that are what the model chose: from the root of each tree on, to the first child that guesses the choice behind the node it hangs on.
+
+    ``tokens`` int64 ``[B, T]``: node 0 is the root (its token is not looked at), node t guesses ``tokens[b, t]`` behind node ``parents[t]``; ``parents`` int64 ``[T]``
+    or ``[B, T]`` as in ``tree_masks`` (a node whose parent is not in ``[0, t)`` is never reached); ``choices`` int64 ``[B, T]``, the model's choice behind each node,
+    greedy or drawn (a view such as ``top_ids[:, :1].view(B, T)`` will do): what is accepted has the distribution that decoding a token at a time has.  The first ``counts[b]``
+    nodes are there (None: all).  T up to 4096."""
+    what = "follow_drafts"
+    if not tokens.is_cuda:
+        raise ValueError("follow_drafts needs tensors on a ROCm device (there is no CPU path)")
+    device = tokens.device
+    if tokens.dim() != 2 or tokens.dtype != torch.int64 or (tokens.shape[1] > 1 and tokens.stride(1) != 1):
+        raise ValueError("follow_drafts: tokens int64 [B, T] expected")
+    batch, nodes = tokens.shape
+    if parents.dtype != torch.int64 or tuple(parents.shape) not in ((nodes,), (batch, nodes)) or parents.device != device or (nodes > 1 and parents.stride(-1) != 1):
+        raise ValueError("follow_drafts: parents int64 [T] or [B, T] on the device of the tokens expected")
+    if choices.dtype != torch.int64 or choices.shape != tokens.shape or choices.device != device:
+        raise ValueError("follow_drafts: choices int64 [B, T] on the device of the tokens expected")
+    if counts is not None and (counts.dtype != torch.int64 or tuple(counts.shape) != (batch,) or not counts.is_contiguous() or counts.device != device):
+        raise ValueError("follow_drafts: counts must be contiguous int64 [B] on the device of the tokens")
+    whole = lambda *shape: torch.empty(shape, dtype=torch.int64, device=device)  # noqa: E731
+    out = FollowedDrafts(whole(batch, nodes), whole(batch), whole(batch, nodes))
+    if 0 in tokens.shape:
+        return out._replace(accepted=out.accepted.zero_())
+    args = _lib.FollowDraftsArgs(tokens.data_ptr(), parents.data_ptr(), choices.data_ptr(), _pointer(counts), *(t.data_ptr() for t in out), tokens.stride(0),
+                                 parents.stride(0) if parents.dim() == 2 else 0, choices.stride(0), choices.stride(1), batch, nodes)
+    with _on(device):
+        status = _lib.load_draft().ajqt_follow_drafts(ctypes.byref(args), torch.cuda.current_stream().cuda_stream)
+    _lib.check_draft(status, what)
     return out
