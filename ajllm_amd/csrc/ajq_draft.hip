@@ -28,6 +28,73 @@ int check_tree(const ajqt_tree_attention_args* a) {
   return check_caches(what, a->keys, a->values, a->cache_batch, a->cache_head);
 }
 
+// How a call is cut up: tiles of a sequence's queries of a key head, parts of its rows.  The lengths are on the device: max_len is what they can be.
+struct TreePlan {
+  bool walk;     // tiles of 64 rt queries, by meet_many; else of 16 rt, by meet_few
+  int rt, tiles, parts;
+  bool alone;    // a wave a tile, not a workgroup
+  long long blocks, queries;
+  size_t bytes;
+};
+constexpr int kMostParts = 64;      // a lane each in the merge
+TreePlan tree_plan(const ajqt_tree_attention_args* a) {
+  TreePlan p{};
+  const long long share = a->heads / a->kv_heads, mine = a->tokens * share, units = (long long)a->batch * a->kv_heads;
+  const bool bf16 = a->cache_dtype == AJQS_BF16;
+  p.queries = (long long)a->batch * a->heads * a->tokens;
+  p.walk = bf16 && mine > 64;
+  if (p.walk) {
+    p.rt = a->q_dtype == AJQS_BF16 && a->dim == 128 && units * ceil_div(mine, 128) >= 256 ? 2 : 1;
+    p.tiles = (int)ceil_div(mine, 64 * p.rt);
+  } else {
+    p.rt = mine > 16 ? 2 : 1;
+    p.tiles = (int)ceil_div(mine, 16 * p.rt);
+  }
+  const long long workgroups = units * p.tiles;
+  p.parts = (int)std::max(1ll, std::min({512 / workgroups, ceil_div(a->max_len, bf16 || p.rt > 1 ? 128 : 64), (long long)kMostParts}));
+  p.blocks = p.walk ? ceil_div(units, 8) * 8 * p.tiles * p.parts : ceil_div(units * p.parts, 8) * 8 * p.tiles;
+  p.bytes = p.parts > 1 ? (size_t)p.parts * p.queries * (8 + 4 * (size_t)a->dim) : 0;
+  return p;
+}
+
+TreeAttention tree_of(const ajqt_tree_attention_args* a, const TreePlan& p, void* workspace) {
+  TreeAttention s{};
+  s.q = a->q;
+  s.prefix_keys = s.keys = a->keys;
+  s.prefix_values = s.values = a->values;
+  s.rows = int64s(a->rows);
+  s.counts = int64s(a->counts);
+  s.offset = int64s(a->offset);
+  s.out = reinterpret_cast<uint16_t*>(a->out);
+  s.part_sums = reinterpret_cast<float*>(workspace);
+  s.part_ml = reinterpret_cast<float2*>(s.part_sums + (size_t)p.parts * p.queries * a->dim);
+  s.prefix_group = s.cache_batch = a->cache_batch;
+  s.prefix_head = s.cache_head = a->cache_head;
+  s.queries = p.queries;
+  s.groups = s.batch = a->batch;
+  s.tokens = a->tokens;
+  s.heads = a->heads;
+  s.kv_heads = a->kv_heads;
+  s.prefix_cap = s.max_len = a->max_len;
+  s.own_parts = p.parts;
+  s.own_tiles = p.tiles;
+  s.own_alone = p.alone;
+  s.scale2 = kLog2e / sqrtf((float)a->dim);
+  s.by_share = divide_by(a->heads / a->kv_heads);
+  s.by_each = divide_by((long long)a->tokens * (a->heads / a->kv_heads));
+  s.by_tokens = divide_by(a->tokens);
+  s.by_heads = divide_by(a->heads);
+  s.by_kv_heads = divide_by(a->kv_heads);
+  s.by_group = divide_by(1);
+  s.by_prefix_tiles = s.by_prefix_parts = divide_by(1);
+  s.by_own_tiles = divide_by(p.tiles);
+  s.by_own_parts = divide_by(p.parts);
+  s.masks = a->masks;
+  s.mask_batch = a->mask_batch;
+  s.mask_token = a->mask_token;
+  return s;
+}
+
 // Whether the blocks of `size` bytes at the sums of the dimensions' multiples lie apart, one dimension inside the other (any other order is taken to meet).
 struct Dimension {
   long long count, stride;   // (bytes)
@@ -49,24 +116,50 @@ extern "C" {
 
 const char* ajqt_last_error(void) { return g_error; }
 
-size_t ajqt_tree_attention_workspace(const ajqt_tree_attention_args* a) { return check_tree(a) ? 0 : 0; }
+size_t ajqt_tree_attention_workspace(const ajqt_tree_attention_args* a) { return check_tree(a) ? 0 : tree_plan(a).bytes; }
 
 int ajqt_tree_attention(const ajqt_tree_attention_args* a, void* workspace, size_t workspace_bytes, void* stream) {
   const char* what = "ajqt_tree_attention";
   if (int e = check_tree(a)) return e;
-  if (a->heads > 0xFFFF || a->batch > 0xFFFF) return fail(AJQ_ERR_SHAPE, "%s: %d heads of %d sequences", what, a->heads, a->batch);
-  const TreeAttention s{a->q, a->keys, a->values, a->masks, int64s(a->rows), int64s(a->counts), int64s(a->offset), reinterpret_cast<uint16_t*>(a->out),
-                        a->cache_batch, a->cache_head, a->mask_batch, a->mask_token, a->batch, a->tokens, a->heads, a->kv_heads, a->max_len,
-                        kLog2e / sqrtf((float)a->dim)};
+  const TreePlan p = tree_plan(a);
+  if (p.blocks > kMostLanes / 256) return fail(AJQ_ERR_SHAPE, "%s: too many tiles of queries", what);
+  if (p.bytes && ceil_div(p.queries, 4) > kMostLanes / 256) return fail(AJQ_ERR_SHAPE, "%s: too many queries (%lld)", what, p.queries);
+  if (p.bytes && (!workspace || workspace_bytes < p.bytes))
+    return fail(AJQ_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, %zu given", what, p.bytes, workspace_bytes);
+  if (!aligned16(workspace)) return fail(AJQ_ERR_ALIGN, "%s: the workspace must be 16-byte aligned", what);
+  const TreeAttention s = tree_of(a, p, workspace);
+  int status = AJQ_OK;
   with_dim(a->dim, [&](auto dim) {
     with_type(a->q_dtype, [&](auto q) {
       with_type(a->cache_dtype, [&](auto cache) {
-        hipLaunchKernelGGL((tree_attention_kernel<decltype(dim)::value, decltype(q), decltype(cache)>),
-                           dim3((unsigned)a->tokens, (unsigned)a->heads, (unsigned)a->batch), dim3(64), 0, (hipStream_t)stream, s);
+        constexpr int HD = decltype(dim)::value;
+        using QT = decltype(q);
+        using CacheT = decltype(cache);
+        auto launch = [&](auto kernel, int lds) {
+          if ((status = allow_lds(kernel, lds, what)) != AJQ_OK) return;
+          hipLaunchKernelGGL(kernel, dim3((unsigned)p.blocks), dim3(256), lds, (hipStream_t)stream, s);
+          if ((status = check_launch(what)) != AJQ_OK || p.parts == 1) return;
+          hipLaunchKernelGGL(shared_attention_merge_kernel<HD>, dim3((unsigned)ceil_div(p.queries, 4)), dim3(256), 0, (hipStream_t)stream,
+                             static_cast<const SharedAttention&>(s));
+          status = check_launch(what);
+        };
+        if constexpr (sizeof(CacheT) == 2) {
+          if (p.walk) {
+            if constexpr (HD == 128 && sizeof(QT) == 2) {
+              if (p.rt == 2) return launch(tree_attention_walk_kernel<HD, QT, 2>, many_lds_bytes<HD>());
+            }
+            return launch(tree_attention_walk_kernel<HD, QT, 1>, many_lds_bytes<HD>());
+          }
+        }
+        auto few = [&](auto tiles) {
+          constexpr int RT = decltype(tiles)::value, lds = some_lds_bytes<HD, CacheT, RT>();
+          p.parts == 1 ? launch(tree_attention_few_kernel<HD, QT, CacheT, RT, true>, lds) : launch(tree_attention_few_kernel<HD, QT, CacheT, RT, false>, lds);
+        };
+        p.rt == 2 ? few(Size<2>{}) : few(Size<1>{});
       });
     });
   });
-  return check_launch(what);
+  return status;
 }
 
 int ajqt_keep_rows(const ajqt_keep_rows_args* a, void* stream) {

@@ -35,6 +35,7 @@ struct SharedAttention {
   float scale2;         // log2(e) / sqrt(HD)
   Divide by_share, by_each, by_tokens, by_heads, by_kv_heads, by_group;   // heads / kv_heads, that times tokens, .., batch / groups
   Divide by_prefix_tiles, by_prefix_parts, by_own_tiles, by_own_parts;
+  static constexpr bool kTree = false;   // (TreeAttention: which rows of its own a token sees is a matter of bits)
 };
 
 // a number that every lane of a workgroup reads, kept where such numbers are
@@ -87,6 +88,12 @@ __device__ __forceinline__ void to_halves(const Raw8F32& x, u32x4_t* to) {
   split8(v, to[0], to[1]);
 }
 __device__ __forceinline__ void to_halves(const u32x4_t& x, u32x4_t* to) { to[0] = x; }
+
+// Which of 32 rows from row `at` of a token's own (below 0: rows ahead of them, which all see) it sees: nothing to say but in a tree.
+template <typename A> struct SeenBits {
+  __device__ __forceinline__ void ask(const A&, int, int) {}
+};
+__device__ __forceinline__ int held_place(long long n) { return (int)min(max(n, -(1ll << 30)), 1ll << 30); }
 
 // The running softmax of 16 queries, one a lane & 15: m, the lane's own part of the sum, and HD / 16 accumulators of O^T.
 template <int HD> struct RunningRow {
@@ -321,9 +328,9 @@ __device__ __forceinline__ int blocks_of(const Meeting<CacheT>& w) {
   return (w.end - w.begin + N - 1) / N + (kBoth ? (w.own_end + N - 1) / N : 0);
 }
 
-// W: how many of the waves work.
-template <int HD, typename QT, typename CacheT, int RT, int W = 4, bool kBoth = false>
-__device__ __forceinline__ void meet_few(const SharedAttention& a, Meeting<CacheT>& w, unsigned char* lds, uint32_t lds0) {
+// W: how many of the waves work.  kWhole: they meet all rows, and what comes out is the result.
+template <int HD, typename QT, typename CacheT, int RT, int W = 4, bool kBoth = false, bool kWhole = kBoth, typename A>
+__device__ __forceinline__ void meet_few(const A& a, Meeting<CacheT>& w, unsigned char* lds, uint32_t lds0) {
   constexpr int RB = 2 * HD, C = HD / 8, KS = HD / 32, TT = HD / 16, KH = kHalves<CacheT>, QH = kHalves<QT>;
   constexpr int kPlane = 32 * RB;                 // 32 rows of bf16
   constexpr bool kDma = KH == 1;
@@ -343,15 +350,19 @@ __device__ __forceinline__ void meet_few(const SharedAttention& a, Meeting<Cache
 #pragma unroll
     for (int s = 0; s < KS; ++s) raw[u][s] = load8_raw(reinterpret_cast<const QT*>(a.q) + place * HD + 32 * s + 8 * g);
   }
+  SeenBits<A> bits[RT];
+#pragma unroll
+  for (int u = 0; u < RT; ++u) bits[u].ask(a, w.outer, token[u]);
   __builtin_amdgcn_sched_barrier(0);
   kBoth ? find_both<HD>(a, w) : find_rows(a, w);
   RunningRow<HD> row[RT];
   int limit[RT];   // how many of the meeting's rows (kBoth: of the second run's) a lane's queries see
 #pragma unroll
   for (int u = 0; u < RT; ++u) {
-    limit[u] = kBoth ? held(w.before + token[u] + 1, w.own_end) : w.own ? held(w.before + token[u] + 1, w.end) : w.end;
+    limit[u] = kBoth ? held(w.before + token[u] + 1, w.own_end) : w.own && !A::kTree ? held(w.before + token[u] + 1, w.end) : w.end;
     row[u].clear();
   }
+  const int before = A::kTree ? held_place(w.before) : 0;
 
   // ---- rows on their way (past the last: the last again, which is there and finite)
   const int ask_row = lane / C, slot = lane % C;
@@ -461,6 +472,16 @@ __device__ __forceinline__ void meet_few(const SharedAttention& a, Meeting<Cache
           for (int i = 0; i < 4; ++i)
             if (16 * jb + 4 * g + i >= seen) sc[u][jb][i] = -INFINITY;
       }
+      if constexpr (A::kTree) {
+        if (now.at + 32 > before) {
+          const uint32_t word = bits[u].of(a, now.at - before) >> (4 * g);
+#pragma unroll
+          for (int jb = 0; jb < 2; ++jb)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if ((word >> (16 * jb + i) & 1) == 0) sc[u][jb][i] = -INFINITY;
+        }
+      }
       float p[8];
       to_probabilities<HD, 2>(row[u], sc[u], a.scale2, p);
       pf[u] = pack8_bf16(p);
@@ -493,8 +514,8 @@ __device__ __forceinline__ void meet_few(const SharedAttention& a, Meeting<Cache
 #pragma unroll
     for (int t = 0; t < TT; ++t) store_run(to + 16 * t + 4 * g, row[u].o[t], scale);
   };
-  if (w.alone) leave_alone<HD, RT, kBoth>(a, w, row, put);
-  else join_waves<HD, RT, few_join_bytes<HD, RT>(), kBoth>(a, w, lds, row, put);
+  if (w.alone) leave_alone<HD, RT, kWhole>(a, w, row, put);
+  else join_waves<HD, RT, few_join_bytes<HD, RT>(), kWhole>(a, w, lds, row, put);
 }
 
 // ---- At most 16 queries on fp32 rows, in fp32 throughout (v_mfma_f32_16x16x4_f32: 32 cycles for 16 rows x 4 components, where the memory's share of a CU
@@ -511,8 +532,8 @@ __device__ __forceinline__ float4 query4(const uint16_t* p) {
   return v;
 }
 template <int HD> constexpr int few_f32_lds_bytes() { return few_join_bytes<HD, 1>() + 4 * 16 * 8; }
-template <int HD, typename QT, bool kBoth = false>
-__device__ __forceinline__ void meet_few_f32(const SharedAttention& a, Meeting<float>& w, unsigned char* lds) {
+template <int HD, typename QT, bool kBoth = false, bool kWhole = kBoth, typename A>
+__device__ __forceinline__ void meet_few_f32(const A& a, Meeting<float>& w, unsigned char* lds) {
   constexpr int KC = HD / 16, P = HD == 32 ? 2 : 4, VC = HD / (16 * P);
   typedef float part_t __attribute__((ext_vector_type(P)));
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -522,9 +543,12 @@ __device__ __forceinline__ void meet_few_f32(const SharedAttention& a, Meeting<f
   float4 q[KC];
 #pragma unroll
   for (int c = 0; c < KC; ++c) q[c] = query4(from + 16 * c);
+  SeenBits<A> bits;
+  bits.ask(a, w.outer, token);
   __builtin_amdgcn_sched_barrier(0);
   kBoth ? find_both<HD>(a, w) : find_rows(a, w);
-  const int limit = kBoth ? held(w.before + token + 1, w.own_end) : w.own ? held(w.before + token + 1, w.end) : w.end;
+  const int limit = kBoth ? held(w.before + token + 1, w.own_end) : w.own && !A::kTree ? held(w.before + token + 1, w.end) : w.end;
+  const int before = A::kTree ? held_place(w.before) : 0;
   using Rows = Block<HD, 16, kBoth, float>;
   RunningRow<HD> row[1];
   row[0].clear();
@@ -559,6 +583,14 @@ __device__ __forceinline__ void meet_few_f32(const SharedAttention& a, Meeting<f
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       if (4 * g + i >= seen) sc[0][i] = -INFINITY;
+    if constexpr (A::kTree) {
+      if (now.at + 16 > before) {
+        const uint32_t word = bits.of(a, now.at - before) >> (4 * g);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if ((word >> i & 1) == 0) sc[0][i] = -INFINITY;
+      }
+    }
     float p[4];
     to_probabilities<HD, 1>(row[0], sc, a.scale2, p);
 #pragma unroll
@@ -591,8 +623,8 @@ __device__ __forceinline__ void meet_few_f32(const SharedAttention& a, Meeting<f
         store_run(to + 16 * P * c + P * (4 * g + i), x, scale);
       }
   };
-  if (w.alone) leave_alone<HD, 1, kBoth>(a, w, row, put);
-  else join_waves<HD, 1, few_join_bytes<HD, 1>(), kBoth>(a, w, lds, row, put);
+  if (w.alone) leave_alone<HD, 1, kWhole>(a, w, row, put);
+  else join_waves<HD, 1, few_join_bytes<HD, 1>(), kWhole>(a, w, lds, row, put);
 }
 
 // ---- Many queries on bf16 rows: 64 U to a workgroup, 16 U to each wave, all four walking the same blocks of 64 rows (LDS, two stages of a key and a
@@ -623,8 +655,8 @@ __device__ __forceinline__ void dma16_pair(const void* base, uint32_t voff, uint
 }
 #pragma clang diagnostic pop
 
-template <int HD, typename QT, int U>
-__device__ __forceinline__ void meet_many(const SharedAttention& a, const Walk<uint16_t>& w, RunningRow<HD> (&row)[U], uint32_t lds0) {
+template <int HD, typename QT, int U, typename A>
+__device__ __forceinline__ void meet_many(const A& a, const Walk<uint16_t>& w, RunningRow<HD> (&row)[U], uint32_t lds0) {
   constexpr int RB = 2 * HD, C = HD / 8, KS = HD / 32, TT = HD / 16, QH = kHalves<QT>, kAhead = TT < 3 ? TT : 3;
   constexpr int kTile = 64 * RB;
   constexpr int kReqRows = 1024 / RB;
@@ -669,6 +701,7 @@ __device__ __forceinline__ void meet_many(const SharedAttention& a, const Walk<u
   u32x4_t qf[U][KS][QH];
   // own rows that query n of the walk sees
   auto limit_of = [&](int n) __attribute__((always_inline)) {
+    if constexpr (A::kTree) return held(w.before, w.rows[1]);
     int rest, unused;
     divide(min(n, w.queries - 1), a.by_each, rest);
     return held(w.before + divide(rest, a.by_share, unused) + 1, w.rows[1]);
@@ -686,7 +719,8 @@ __device__ __forceinline__ void meet_many(const SharedAttention& a, const Walk<u
     for (int s = 0; s < KS; ++s)
 #pragma unroll
       for (int h = 0; h < QH; ++h) asm volatile("" : "+v"(qf[u][s][h]));
-  const int nearest = limit_of(w.first + 16 * U * wave), farthest = limit_of(w.first + 16 * U * wave + 16 * U - 1);   // of the wave's queries
+  const int nearest = limit_of(w.first + 16 * U * wave);   // of the wave's queries
+  const int farthest = A::kTree ? w.rows[1] : limit_of(w.first + 16 * U * wave + 16 * U - 1);
   // steps of this wave
   const int steps = w.first + 16 * U * wave >= w.queries ? 0 : farthest > 0 ? 2 * prefix_blocks + ((farthest + 31) >> 5) : (w.rows[0] + 31) >> 5;
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -734,6 +768,22 @@ __device__ __forceinline__ void meet_many(const SharedAttention& a, const Walk<u
         asm volatile("" : "+v"(l));
 #pragma unroll
         for (int u = 0; u < U; ++u) {
+          if constexpr (A::kTree) {
+            if (own) {
+              int rest, unused;
+              divide(min(w.first + 16 * (U * wave + u) + (l & 15), w.queries - 1), a.by_each, rest);
+              SeenBits<A> bits;
+              bits.ask(a, w.first_sequence, divide(rest, a.by_share, unused));
+              const int there = w.rows[1] - at;
+              const uint32_t word = (bits.of(a, at - (int)w.before) & (there < 32 ? (1u << max(there, 0)) - 1u : ~0u)) >> (4 * (l >> 4));
+#pragma unroll
+              for (int jb = 0; jb < 2; ++jb)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                  if ((word >> (16 * jb + i) & 1) == 0) sc[u][jb][i] = -INFINITY;
+              continue;
+            }
+          }
           const int last = (own ? limit_of(w.first + 16 * (U * wave + u) + (l & 15)) : w.rows[0]) - at - 4 * (l >> 4);
 #pragma unroll
           for (int jb = 0; jb < 2; ++jb)
@@ -895,10 +945,10 @@ __device__ __forceinline__ void leave_part(const SharedAttention& a, const Walk<
   }
 }
 
-template <int HD, typename QT, typename CacheT, int RT, bool kBoth = false>
-__device__ __forceinline__ void meet_some(const SharedAttention& a, Meeting<CacheT>& w, unsigned char* lds, uint32_t lds0) {
-  if constexpr (sizeof(CacheT) == 4 && RT == 1) meet_few_f32<HD, QT, kBoth>(a, w, lds);
-  else meet_few<HD, QT, CacheT, RT, 4, kBoth>(a, w, lds, lds0);
+template <int HD, typename QT, typename CacheT, int RT, bool kBoth = false, bool kWhole = kBoth, typename A>
+__device__ __forceinline__ void meet_some(const A& a, Meeting<CacheT>& w, unsigned char* lds, uint32_t lds0) {
+  if constexpr (sizeof(CacheT) == 4 && RT == 1) meet_few_f32<HD, QT, kBoth, kWhole>(a, w, lds);
+  else meet_few<HD, QT, CacheT, RT, 4, kBoth, kWhole>(a, w, lds, lds0);
 }
 template <int HD, typename CacheT, int RT> constexpr int some_lds_bytes() {
   return sizeof(CacheT) == 4 && RT == 1 ? few_f32_lds_bytes<HD>() : few_lds_bytes<HD, CacheT, RT>();
@@ -958,10 +1008,8 @@ __global__ __launch_bounds__(256, 2) void shared_attention_many_kernel(SharedAtt
 // own_parts > 1 the walk is cut up and leaves parts for the merge.  16 sequences of 100 tokens x 4 of 8 heads behind 2048 rows 66 us = 630 TFLOP/s (71 in the first calls after
 // a pause), 24 of 50 behind 8000 203 us = 775.  Of the former's cycles a CU is busy for 63 % (358 tiles on 256 CUs: some have two, some one), and a SIMD for 45 % of those with MFMAs,
 // 36 % with other vector instructions; its LDS is no limit (no bank conflicts).
-template <int HD, typename QT, int U>
-__global__ __launch_bounds__(256, 2) void shared_attention_walk_kernel(SharedAttention a) {
-  extern __shared__ __attribute__((aligned(1024))) unsigned char shared_lds[];
-  const uint32_t lds0 = (uint32_t)(uintptr_t)(pf_lds_char_t*)shared_lds;
+template <int HD, typename QT, int U, typename A>
+__device__ __forceinline__ void walk_own(const A& a, uint32_t lds0) {
   const int share = (int)a.by_share.d, parts = a.own_parts;
   int part, hk, unused, tile;
   const int id = (int)blockIdx.x, run = (id & 7) + 8 * divide(divide(id >> 3, a.by_own_parts, part), a.by_own_tiles, tile);
@@ -976,9 +1024,21 @@ __global__ __launch_bounds__(256, 2) void shared_attention_walk_kernel(SharedAtt
   w.before = read_uniform(a.rows + b) + (a.offset ? read_uniform(a.offset) : 0ll);
   const int there = a.counts ? held(read_uniform(a.counts + b), a.tokens) : a.tokens;
   const int last = min(divide(w.first + 64 * U - 1, a.by_share, unused), there - 1);          // the tile's last token that is there
-  const size_t at = (size_t)group * a.prefix_group + (size_t)hk * a.prefix_head, own = (size_t)b * a.cache_batch + (size_t)hk * a.cache_head;
+  const size_t at = (size_t)group * a.prefix_group + (size_t)hk * a.prefix_head;
+  size_t own = (size_t)b * a.cache_batch + (size_t)hk * a.cache_head;
   const bool none = w.first >= there * share;
-  const int prefix_rows = none ? 0 : held(read_uniform(a.prefix_lengths + group), a.prefix_cap), own_rows = none ? 0 : held(w.before + last + 1, a.max_len);
+  int prefix_rows, own_rows;
+  if constexpr (A::kTree) {
+    // whole blocks of committed rows are the first run (its caches are the sequence's own), the others and the tree's the second
+    const int rows = none ? 0 : held(w.before + there, a.max_len);
+    prefix_rows = held(w.before, rows) & ~63;
+    own_rows = rows - prefix_rows;
+    own += (size_t)prefix_rows * HD;
+    w.before = held_place(w.before) - prefix_rows;
+  } else {
+    prefix_rows = none ? 0 : held(read_uniform(a.prefix_lengths + group), a.prefix_cap);
+    own_rows = none ? 0 : held(w.before + last + 1, a.max_len);
+  }
   // this part's blocks: first .. first + many - 1 of the prefix's and the sequence's own
   const int prefix_blocks = (prefix_rows + 63) >> 6, blocks = prefix_blocks + ((own_rows + 63) >> 6), per = (blocks + parts - 1) / parts;
   const int first = min(blocks, part * per), many = min(blocks - first, per);
@@ -1016,6 +1076,11 @@ __global__ __launch_bounds__(256, 2) void shared_attention_walk_kernel(SharedAtt
           zero ? u32x2_t{0u, 0u} : u32x2_t{pack2_bf16(o[0] * inv, o[1] * inv), pack2_bf16(o[2] * inv, o[3] * inv)};
     }
   }
+}
+template <int HD, typename QT, int U>
+__global__ __launch_bounds__(256, 2) void shared_attention_walk_kernel(SharedAttention a) {
+  extern __shared__ __attribute__((aligned(1024))) unsigned char shared_lds[];
+  walk_own<HD, QT, U>(a, (uint32_t)(uintptr_t)(pf_lds_char_t*)shared_lds);
 }
 
 // ---- the parts of a query put together: a wave a query, lane p holding part p's (m, sum).  The first kFirst parts' sums are asked for beside them.
