@@ -390,6 +390,29 @@ def serve_native(name: str):
     return function
 
 
+_draft_native: dict = {}
+
+
+def draft_native(name: str):
+    """``serve_native`` for ``tree_attention``, ``keep_rows``, ``token_log_probs`` and ``follow_drafts``."""
+    function = _draft_native.get(name)
+    if function is None:
+        lib = load_draft()
+        try:
+            module = load_native()
+        except NativeModuleMissing as error:
+            warnings.warn(f"{error}; until then these calls take the longer way through the interpreter", RuntimeWarning, stacklevel=3)
+            module = None
+        else:
+            module.bind_draft(*(ctypes.cast(getattr(lib, entry), c_void_p).value for entry in (
+                "ajqt_tree_attention_workspace", "ajqt_tree_attention", "ajqt_keep_rows", "ajqt_log_probs_workspace", "ajqt_log_probs",
+                "ajqt_follow_drafts")))
+        for each in ("tree_attention", "keep_rows", "token_log_probs", "follow_drafts"):
+            _draft_native[each] = getattr(module, each, _leave)
+        function = _draft_native[name]
+    return function
+
+
 def _leave(*args) -> None:
     """In a native function's place."""
 

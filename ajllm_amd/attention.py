@@ -244,6 +244,10 @@ def tree_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, ro
     what = "tree_attention"
     if not q.is_cuda:
         raise ValueError("tree_attention needs tensors on a ROCm device (there is no CPU path)")
+    # tensors as the kernel takes them: one call of native code, which leaves everything else to the lines below it
+    out = (_lib._draft_native.get(what) or _lib.draft_native(what))(q, keys, values, rows, masks, counts, offset)
+    if out is not None:
+        return out
     device = q.device
     _check_caches(what, keys, values, device)
     if q.dim() != 4 or q.dtype not in _TYPES:
@@ -286,6 +290,8 @@ def keep_rows(keys: torch.Tensor, values: torch.Tensor, rows: torch.Tensor, inde
     what = "keep_rows"
     if not keys.is_cuda:
         raise ValueError("keep_rows needs tensors on a ROCm device (there is no CPU path)")
+    if (_lib._draft_native.get(what) or _lib.draft_native(what))(keys, values, rows, index, counts, offset):
+        return
     device = keys.device
     if keys.dim() == 5 and values.dim() == 5:
         layers, apart = keys.shape[0], keys.stride(0)

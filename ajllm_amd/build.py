@@ -28,7 +28,8 @@ SERVE_LIBRARY = PACKAGE_DIR / "libajq_serve.so"
 DRAFT_SOURCE = PACKAGE_DIR / "csrc" / "ajq_draft.hip"
 DRAFT_LIBRARY = PACKAGE_DIR / "libajq_draft.so"
 # a quantized layer's forward (and the operators above) without the interpreter: an extension module that calls the libraries
-NATIVE_SOURCES = [PACKAGE_DIR / "csrc" / "native_linear.cpp", PACKAGE_DIR / "csrc" / "native_serve.cpp"]
+NATIVE_SOURCES = [PACKAGE_DIR / "csrc" / "native_linear.cpp", PACKAGE_DIR / "csrc" / "native_serve.cpp",
+                  PACKAGE_DIR / "csrc" / "native_draft.cpp"]
 NATIVE_MODULE = PACKAGE_DIR / "_native.so"
 # measurement probes for bench.py (include/ajq_bench.h); the operator library does not depend on it
 BENCH_SOURCE = PACKAGE_DIR / "csrc" / "ajq_bench.hip"

@@ -110,6 +110,41 @@ bool nested(Dimension (&dims)[N], long long size) {
   return true;
 }
 
+int check_log_probs(const ajqt_log_probs_args* a) {
+  const char* what = "ajqt_log_probs";
+  if (!a) return fail(AJQ_ERR_NULL, "%s: null arguments", what);
+  if (!a->logits || !a->entropy || (a->targets && (!a->log_probs || !a->ranks)) || (a->top && (!a->top_log_probs || !a->top_ids)))
+    return fail(AJQ_ERR_NULL, "%s: null pointer argument", what);
+  if (!known(a->dtype)) return fail(AJQ_ERR_UNSUPPORTED, "%s: unknown element type", what);
+  if (a->rows < 1 || a->vocab < 1 || a->ld < 0 || a->top < 0 || a->top > kMostTop || a->top > a->vocab)
+    return fail(AJQ_ERR_SHAPE, "%s: unsupported shape (rows=%d vocab=%d ld=%lld top=%d)", what, a->rows, a->vocab, (long long)a->ld, a->top);
+  if (!aligned4(a->log_probs) || !aligned4(a->entropy) || !aligned4(a->top_log_probs) || (a->dtype == AJQS_F32 && !aligned4(a->logits)) ||
+      (reinterpret_cast<uintptr_t>(a->logits) & 1u))
+    return fail(AJQ_ERR_ALIGN, "%s: logits and results must be aligned to their elements", what);
+  if (a->rows > kMostLanes / 256) return fail(AJQ_ERR_SHAPE, "%s: %d rows in a launch", what, a->rows);
+  return AJQ_OK;
+}
+
+// How rows are cut up: slices of about one size, at most what a workgroup's registers hold.
+struct LogProbsPlan {
+  int lanes, slice;
+  long long slices;
+  size_t bytes;
+};
+#ifndef LP_WANT
+#define LP_WANT 128
+#endif
+LogProbsPlan log_probs_plan(const ajqt_log_probs_args* a) {
+  LogProbsPlan p{};
+  const long long piece = kLogPieces * (a->dtype == AJQS_BF16 ? 8 : 4);
+  p.lanes = a->vocab <= 256 * piece || (a->vocab > 1024 * piece && a->rows * ceil_div(a->vocab, 1024 * piece) < LP_WANT) ? 256 : 1024;
+  p.slices = ceil_div(a->vocab, p.lanes * piece);
+  p.slice = (int)std::min((long long)a->vocab, ceil_div(ceil_div(a->vocab, p.slices), 64) * 64);
+  p.slices = ceil_div(a->vocab, p.slice);
+  p.bytes = p.slices > 1 ? (size_t)a->rows * p.slices * (sizeof(f32x4_t) + 8 * (size_t)a->top) : 0;
+  return p;
+}
+
 }  // namespace
 
 extern "C" {
@@ -186,24 +221,37 @@ int ajqt_keep_rows(const ajqt_keep_rows_args* a, void* stream) {
   return check_launch(what);
 }
 
-size_t ajqt_log_probs_workspace(const ajqt_log_probs_args*) { return 0; }
+size_t ajqt_log_probs_workspace(const ajqt_log_probs_args* a) { return check_log_probs(a) ? 0 : log_probs_plan(a).bytes; }
 
 int ajqt_log_probs(const ajqt_log_probs_args* a, void* workspace, size_t workspace_bytes, void* stream) {
   const char* what = "ajqt_log_probs";
-  if (!a) return fail(AJQ_ERR_NULL, "%s: null arguments", what);
-  if (!a->logits || (a->targets && (!a->log_probs || !a->ranks)) || (a->top && (!a->top_log_probs || !a->top_ids)))
-    return fail(AJQ_ERR_NULL, "%s: null pointer argument", what);
-  if (!known(a->dtype)) return fail(AJQ_ERR_UNSUPPORTED, "%s: unknown element type", what);
-  if (a->rows < 1 || a->vocab < 1 || a->ld < 0 || a->top < 0 || a->top > kMostTop || a->top > a->vocab)
-    return fail(AJQ_ERR_SHAPE, "%s: unsupported shape (rows=%d vocab=%d ld=%lld top=%d)", what, a->rows, a->vocab, (long long)a->ld, a->top);
-  if (!aligned4(a->log_probs) || !aligned4(a->entropy) || !aligned4(a->top_log_probs) || (a->dtype == AJQS_F32 && !aligned4(a->logits)) ||
-      (reinterpret_cast<uintptr_t>(a->logits) & 1u))
-    return fail(AJQ_ERR_ALIGN, "%s: logits and results must be aligned to their elements", what);
-  if (a->rows > kMostLanes / 256) return fail(AJQ_ERR_SHAPE, "%s: %d rows in a launch", what, a->rows);
+  if (int e = check_log_probs(a)) return e;
+  const LogProbsPlan p = log_probs_plan(a);
+  if (a->rows * p.slices > kMostLanes / p.lanes) return fail(AJQ_ERR_SHAPE, "%s: %d rows of %d", what, a->rows, a->vocab);
+  if (p.bytes && (!workspace || workspace_bytes < p.bytes))
+    return fail(AJQ_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, %zu given", what, p.bytes, workspace_bytes);
+  if (!aligned16(workspace)) return fail(AJQ_ERR_ALIGN, "%s: the workspace must be 16-byte aligned", what);
+  f32x4_t* parts = reinterpret_cast<f32x4_t*>(workspace);
   const LogProbs n{a->logits, int64s(a->targets), a->log_probs, a->entropy, a->top_log_probs, reinterpret_cast<long long*>(a->ranks),
-                   reinterpret_cast<long long*>(a->top_ids), a->ld, a->rows, a->vocab, a->top};
+                   reinterpret_cast<long long*>(a->top_ids), parts, reinterpret_cast<unsigned long long*>(parts + (size_t)a->rows * p.slices), a->ld, a->rows, a->vocab,
+                   a->top, p.slice, (int)p.slices};
   with_type(a->dtype, [&](auto type) {
-    hipLaunchKernelGGL(log_probs_kernel<decltype(type)>, dim3((unsigned)a->rows), dim3(256), 0, (hipStream_t)stream, n);
+    using T = decltype(type);
+    auto launch = [&](auto lanes, auto rank, auto top) {
+      constexpr int LANES = decltype(lanes)::value;
+      hipLaunchKernelGGL((log_probs_kernel<T, LANES, decltype(rank)::value, decltype(top)::value>), dim3((unsigned)(a->rows * p.slices)), dim3(LANES), 0,
+                         (hipStream_t)stream, n);
+    };
+    const std::integral_constant<bool, true> yes;
+    const std::integral_constant<bool, false> no;
+    auto with_top = [&](auto lanes, auto rank) { a->top ? launch(lanes, rank, yes) : launch(lanes, rank, no); };
+    auto with_rank = [&](auto lanes) { a->targets ? with_top(lanes, yes) : with_top(lanes, no); };
+    p.lanes == 1024 ? with_rank(Size<1024>{}) : with_rank(Size<256>{});
+  });
+  if (int e = check_launch(what)) return e;
+  if (p.slices == 1) return AJQ_OK;
+  with_type(a->dtype, [&](auto type) {
+    hipLaunchKernelGGL(log_probs_merge_kernel<decltype(type)>, dim3((unsigned)a->rows), dim3(a->top ? 256 : 64), 0, (hipStream_t)stream, n);
   });
   return check_launch(what);
 }

@@ -1,92 +1,354 @@
 // Log probabilities of given tokens, entropies, and the first tokens in the order of their logits.
 //
 //   log p_t = (x_t - m) - log s,   H = log s - u / s,   m = max x_v,   s = sum e^(x_v - m),   u = sum e^(x_v - m) (x_v - m)
+//
+// A workgroup takes a slice of one row, up to 128 KiB, into its registers at once, so that everything behind the maximum is worked out of them and memory
+// is read once.  Slices' (m, s, u, tokens ahead) and first tokens are put together by a second launch where a row has several.
+//
+// The first `top` of a slice: lanes 128 apart are a group, and every group knows its first token.  The top-th of these 128 is a border that at least `top` tokens
+// reach, and only the groups that lead it have others that do: some top * (1 + top / 256) of them in a row without order, 16 bytes' worth of tokens for each of `top` in
+// one that is all alike or sorted.  They gather in LDS, each counts those ahead of itself, and that is its place.  Where they are more than LDS is set aside for (a
+// row made to be so), `top` rounds over the slice find them instead.
 #pragma once
 #include "lane_rows.h"
 
 namespace ajq {
 
-constexpr int kMostTop = 64;
+constexpr int kMostTop = 64, kLogPieces = 8, kGroups = 128, kGathered = 2048;
 struct LogProbs {
   const void* logits;
   const long long* targets;
   float *log_probs, *entropy, *top_log_probs;
   long long *ranks, *top_ids;
+  f32x4_t* parts;               // [rows, slices] m, s, u, tokens ahead of the target (a whole number's bits)
+  unsigned long long* firsts;   // [rows, slices, top]
   long long ld;
-  int rows, vocab, top;
+  int rows, vocab, top, slice, slices;
 };
 
-// The order of the tokens as whole numbers: larger logits first (NaN ahead of all, -0 as 0), then smaller ids.
-__device__ __forceinline__ uint32_t order_of(float x) {
+// The order of the tokens as whole numbers: larger logits first (NaN ahead of all, -0 as 0), then smaller ids.  0 is no token's.
+__device__ __forceinline__ unsigned long long key_of(float x, int id) {
   const uint32_t bits = __float_as_uint(x + 0.f);
-  return x != x ? 0xFFFFFFFFu : bits ^ ((uint32_t)((int)bits >> 31) | 0x80000000u);
+  const uint32_t order = x != x ? 0xFFFFFFFFu : bits ^ ((uint32_t)((int)bits >> 31) | 0x80000000u);
+  return (unsigned long long)order << 32 | (uint32_t)~id;
 }
-__device__ __forceinline__ unsigned long long key_of(float x, int id) { return (unsigned long long)order_of(x) << 32 | (uint32_t)~id; }
+__device__ __forceinline__ int id_of(unsigned long long key) { return (int)~(uint32_t)key; }
+__device__ __forceinline__ float logit_of(unsigned long long key) {
+  const uint32_t order = (uint32_t)(key >> 32);
+  return __uint_as_float(order & 0x80000000u ? order ^ 0x80000000u : ~order);
+}
+__device__ __forceinline__ unsigned long long larger(unsigned long long x, unsigned long long y) { return x > y ? x : y; }
+
 __device__ __forceinline__ float logit(const float* p) { return *p; }
 __device__ __forceinline__ float logit(const uint16_t* p) { return __uint_as_float((uint32_t)*p << 16); }
-
-// fn over a workgroup of 256 lanes; every lane gets the result
-template <typename T, typename F>
-__device__ __forceinline__ T over_group(T v, T* room, F&& fn) {
-  __syncthreads();
-  room[threadIdx.x] = v;
-  for (int n = 128; n > 0; n >>= 1) {
-    __syncthreads();
-    if ((int)threadIdx.x < n) room[threadIdx.x] = fn(room[threadIdx.x], room[threadIdx.x + n]);
-  }
-  __syncthreads();
-  return room[0];
+template <typename T> constexpr int kPiece = 16 / (int)sizeof(T);   // logits of 16 bytes
+template <typename T>
+__device__ __forceinline__ float logit(const u32x4_t& raw, int e) {
+  if constexpr (sizeof(T) == 4) return __uint_as_float(raw[e]);
+  return __uint_as_float(e & 1 ? raw[e >> 1] & 0xFFFF0000u : raw[e >> 1] << 16);
+}
+// Sixteen bytes of a row wherever they lie (rows of an odd vocabulary begin anywhere; the hardware takes any address); behind its end -inf.
+typedef uint32_t u32x4f_t __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t u32x4h_t __attribute__((ext_vector_type(4), aligned(2)));
+__device__ __forceinline__ u32x4_t load_piece(const float* p, int there) {
+  if (there >= 4) return __builtin_nontemporal_load(reinterpret_cast<const u32x4f_t*>(p));
+  constexpr uint32_t kNone = 0xFF800000u;
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(p);
+  return u32x4_t{w[0], there > 1 ? w[1] : kNone, there > 2 ? w[2] : kNone, kNone};
+}
+__device__ __forceinline__ u32x4_t load_piece(const uint16_t* p, int there) {
+  if (there >= 8) return __builtin_nontemporal_load(reinterpret_cast<const u32x4h_t*>(p));
+  u32x4_t v;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = (2 * i < there ? p[2 * i] : 0xFF80u) | (2 * i + 1 < there ? (uint32_t)p[2 * i + 1] : 0xFF80u) << 16;
+  return v;
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void log_probs_kernel(LogProbs a) {
-  __shared__ unsigned long long keys[256];
-  __shared__ float numbers[256];
-  __shared__ int counts[256];
-  const int r = blockIdx.x;
+__device__ __forceinline__ float wave_most(float v) {
+  v = quad_max(v);   // over lanes l, l ^ 16, l ^ 32, l ^ 48
+  v = fmaxf(v, row_ror<8>(v));
+  v = fmaxf(v, row_ror<4>(v));
+  v = fmaxf(v, row_ror<2>(v));
+  return fmaxf(v, row_ror<1>(v));
+}
+
+// What is known of a row, or of a slice of it.
+struct RowSums {
+  float m, s, u;   // (m: 0 where everything is -inf)
+  int ahead;
+  bool nothing;
+};
+__device__ __forceinline__ float log_prob(float x, const RowSums& r, float log_s) { return r.nothing ? -INFINITY : (x - r.m) - log_s; }
+__device__ __forceinline__ void leave_row(const LogProbs& a, int row, const RowSums& r, float log_s, bool asked, float mine) {
+  a.entropy[row] = r.nothing ? 0.f : log_s - r.u / r.s;
+  if (a.targets) {
+    a.log_probs[row] = asked ? log_prob(mine, r, log_s) : 0.f;
+    a.ranks[row] = asked ? min(r.ahead, a.vocab - 1) : -1;
+  }
+}
+
+template <typename T, int LANES, bool kRank, bool kTop>
+__global__ __launch_bounds__(LANES, 8) void log_probs_kernel(LogProbs a) {
+  constexpr int E = kPiece<T>, W = LANES / 64, kRound = LANES * E;
+  __shared__ __attribute__((aligned(16))) float most[W], sums[W], spreads[W];
+  __shared__ int aheads[W], gathered;
+  __shared__ __attribute__((aligned(16))) unsigned long long groups[kTop ? kGroups : 1], border, found[kTop ? kGathered : 1];   // (found: at first the lanes' own)
+  const int t = threadIdx.x, wave = t >> 6;
+  const int r = (int)blockIdx.x / a.slices, part = (int)blockIdx.x - r * a.slices, base = part * a.slice;
   const T* row = reinterpret_cast<const T*>(a.logits) + (size_t)r * a.ld;
-  float m = -INFINITY;
-  for (int v = threadIdx.x; v < a.vocab; v += 256) m = fmaxf(m, logit(row + v));
-  m = over_group(m, numbers, [](float x, float y) { return fmaxf(x, y); });
-  const bool nothing = m == -INFINITY;
-  const long long target = a.targets ? a.targets[r] : -1;
-  const bool asked = target >= 0 && target < a.vocab;
-  const float mine = asked ? logit(row + target) : 0.f;
-  const unsigned long long my_key = asked ? key_of(mine, (int)target) : ~0ull;
+  const T* mine_from = row;
+  row += base;
+  const int count = min(a.slice, a.vocab - base);
+  u32x4_t x[kLogPieces];
+#pragma unroll
+  for (int i = 0; i < kLogPieces; ++i) {
+    const int at = t * E + i * kRound;
+    constexpr uint32_t kNone = sizeof(T) == 4 ? 0xFF800000u : 0xFF80FF80u;
+    x[i] = u32x4_t{kNone, kNone, kNone, kNone};
+    if (at < count) x[i] = load_piece(row + at, count - at);
+  }
+  bool asked = false;
+  float mine = 0.f;
+  int ahead = 0, target = 0;
+  if constexpr (kRank) {
+    const long long given = a.targets[r];
+    asked = given >= 0 && given < a.vocab;
+    target = (int)min(max(given - base, -1ll), (long long)count);   // its place in the slice, or one beside it
+    if (asked) mine = logit(mine_from + given);
+    // of the target's own piece the tokens in front of it that have the same logit
+    if (asked && target >= 0 && target < count && t < E - 1) {
+      const int at = target / E * E + t;
+      if (at < target) ahead = logit(row + at) == mine;
+    }
+  }
+  if (kTop && t == 0) gathered = 0;
+
+  // ---- the maximum
+  float top = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < kLogPieces; ++i)
+    if (i * kRound < count) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) top = fmaxf(top, logit<T>(x[i], e));
+    }
+  const float lane_top = top;
+  top = wave_most(top);
+  if ((t & 63) == 0) most[wave] = top;
+  unsigned long long own_first = 0ull;
+  if constexpr (kTop) {
+    // the lane's first token
+    int first = 0x7FFFFFFF;
+#pragma unroll
+    for (int i = kLogPieces - 1; i >= 0; --i)
+      if (i * kRound < count) {
+#pragma unroll
+        for (int e = E - 1; e >= 0; --e) {
+          const float v = logit<T>(x[i], e);
+          first = !(v < lane_top) ? t * E + i * kRound + e : first;
+        }
+      }
+    // (where there is NaN the first of it or of the largest: the border is then one that some NaN reaches)
+    own_first = first < count ? key_of(lane_top, base + first) : 0ull;
+    found[t] = own_first;
+  }
+  __syncthreads();
+  if constexpr (kTop) {
+    if (t < kGroups) {
+      unsigned long long key = found[t];
+#pragma unroll
+      for (int i = kGroups; i < LANES; i += kGroups) key = larger(key, found[t + i]);
+      groups[t] = key;
+    }
+  }
+  RowSums sum;
+#pragma unroll
+  for (int w = 0; w < W; ++w) top = fmaxf(top, most[w]);
+  sum.m = top == -INFINITY ? 0.f : top;
+
+  // ---- sums
+  const float lower = asked ? mine : 0.f;
+  const uint32_t bits = __float_as_uint(lower + 0.f);
+  // the number just below the target's logit (of -inf none: no number is not above it)
+  const float below = __uint_as_float(bits == 0u ? 0x80000001u : (int)bits > 0 ? bits - 1u : bits + 1u);
   float s = 0.f, u = 0.f;
-  int ahead = 0;
-  for (int v = threadIdx.x; v < a.vocab; v += 256) {
-    const float x = logit(row + v), d = x - (nothing ? 0.f : m), p = exp2_hw(d * kLog2e);
-    s += p;
-    u += p != 0.f ? p * d : 0.f;
-    ahead += key_of(x, v) > my_key;
+#pragma unroll
+  for (int i = 0; i < kLogPieces; ++i)
+    if (i * kRound < count) {
+      const float than = t * E + i * kRound + E - 1 < target ? below : lower;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const float v = logit<T>(x[i], e), d = v - sum.m, p = exp2_hw(d * kLog2e);
+        s += p;
+        u = __builtin_fmaf(p, fmaxf(d, -1e30f), u);   // (nothing of -inf)
+        if constexpr (kRank) ahead += !(v <= than);
+      }
+    }
+  s = wave_sum(s);
+  u = wave_sum(u);
+  if constexpr (kRank) {
+#pragma unroll
+    for (int n = 32; n > 0; n >>= 1) ahead += __shfl_xor(ahead, n);
   }
-  const auto add = [](auto x, auto y) { return x + y; };
-  s = over_group(s, numbers, add);
-  u = over_group(u, numbers, add);
-  ahead = over_group(ahead, counts, add);
-  const bool empty = nothing && s == 0.f;
-  const float log_s = logf(s);
-  if (threadIdx.x == 0) {
-    if (a.entropy) a.entropy[r] = empty ? 0.f : log_s - u / s;
-    if (a.targets) {
-      a.log_probs[r] = !asked ? 0.f : empty ? -INFINITY : (mine - m) - log_s;
-      a.ranks[r] = asked ? ahead : -1;
+  if ((t & 63) == 0) {
+    sums[wave] = s;
+    spreads[wave] = u;
+    aheads[wave] = ahead;
+  }
+  // ---- the border: the top-th of the groups' first tokens
+  if constexpr (kTop) {
+    __syncthreads();
+    if (t < kGroups) {
+      const unsigned long long key = groups[t];
+      int before = 0;
+#pragma unroll 16
+      for (int i = 0; i < kGroups; ++i) before += groups[i] > key;
+      // (no token: 0, which several groups may have; the first of them speaks)
+      if (key == 0ull) {
+        for (int i = 0; i < t; ++i) before += groups[i] == 0ull;
+      }
+      if (before == a.top - 1) border = key;
     }
   }
-  unsigned long long last = ~0ull;
-  for (int k = 0; k < a.top; ++k) {
-    unsigned long long best = 0;
-    for (int v = threadIdx.x; v < a.vocab; v += 256) {
-      const unsigned long long key = key_of(logit(row + v), v);
-      if (key < last && key > best) best = key;
+  __syncthreads();
+  sum.s = sum.u = 0.f;
+  sum.ahead = 0;
+#pragma unroll
+  for (int w = 0; w < W; ++w) {
+    sum.s += sums[w];
+    sum.u += spreads[w];
+    sum.ahead += aheads[w];
+  }
+  sum.nothing = top == -INFINITY && sum.s == 0.f;
+  const bool whole = a.slices == 1;
+  const float log_s = logf(sum.s);
+  if (t == 0) {
+    if (whole) leave_row(a, r, sum, log_s, asked, mine);
+    else a.parts[blockIdx.x] = f32x4_t{top, sum.s, sum.u, __int_as_float(sum.ahead)};
+  }
+  if constexpr (kTop) {
+    const unsigned long long least = border;
+    const size_t to = (size_t)blockIdx.x * a.top;
+    auto leave = [&](int place, unsigned long long key) {
+      if (whole) {
+        a.top_ids[to + place] = id_of(key);
+        a.top_log_probs[to + place] = log_prob(logit_of(key), sum, log_s);
+      } else {
+        a.firsts[to + place] = key;
+      }
+    };
+    const float least_logit = least == 0ull ? -INFINITY : logit_of(least);
+#pragma unroll
+    for (int i = 0; i < kLogPieces; ++i)
+      if (i * kRound < count && own_first >= least) {   // (few lanes)
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const float v = logit<T>(x[i], e);
+          const int id = t * E + i * kRound + e;
+          if (!(v < least_logit) && id < count) {
+            const unsigned long long key = key_of(v, base + id);
+            if (key >= least) {
+              const int n = atomicAdd(&gathered, 1);
+              if (n < kGathered) found[n] = key;
+            }
+          }
+        }
+      }
+    __syncthreads();
+    const int many = gathered;
+    if (many <= kGathered) {
+      for (int n = t; n < many; n += LANES) {
+        const unsigned long long key = found[n];
+        int place = 0;
+        for (int i = 0; i < many; ++i) place += found[i] > key;
+        if (place < a.top) leave(place, key);
+      }
+      if (!whole)   // (a slice that has fewer tokens)
+        for (int n = many + t; n < a.top; n += LANES) a.firsts[to + n] = 0ull;
+    } else {
+      unsigned long long last = ~0ull;
+      for (int k = 0; k < a.top; ++k) {
+        unsigned long long best = 0ull;
+        for (int i = 0; i < kLogPieces; ++i)
+          if (i * kRound < count) {
+            for (int e = 0; e < E; ++e) {
+              const int id = t * E + i * kRound + e;
+              const unsigned long long key = id < count ? key_of(logit(row + id), base + id) : 0ull;
+              if (key < last) best = larger(best, key);
+            }
+          }
+        __syncthreads();
+        found[t] = best;
+        for (int n = LANES / 2; n > 0; n >>= 1) {
+          __syncthreads();
+          if (t < n) found[t] = larger(found[t], found[t + n]);
+        }
+        __syncthreads();
+        last = found[0];
+        if (t == 0) leave(k, last);
+      }
     }
-    last = over_group(best, keys, [](unsigned long long x, unsigned long long y) { return x > y ? x : y; });
-    if (threadIdx.x == 0) {
-      const int id = (int)~(uint32_t)last;
-      a.top_ids[(size_t)r * a.top + k] = id;
-      a.top_log_probs[(size_t)r * a.top + k] = empty ? -INFINITY : (logit(row + id) - m) - log_s;
+  }
+}
+
+// ---- a row's slices put together, a workgroup a row.  A token's place is its place in its slice and, of every other slice, how many are ahead of it.
+constexpr int kMergeKeys = 2048;
+template <typename T>
+__global__ __launch_bounds__(256) void log_probs_merge_kernel(LogProbs a) {
+  __shared__ unsigned long long keys[kMergeKeys];
+  const int r = blockIdx.x, t = threadIdx.x, lane = t & 63;
+  const f32x4_t* parts = a.parts + (size_t)r * a.slices;
+  const unsigned long long* from = a.firsts + (size_t)r * a.slices * a.top;
+  const int many = a.slices * a.top;
+  const bool held = many <= kMergeKeys;
+  if (held)
+    for (int n = t; n < many; n += blockDim.x) keys[n] = from[n];
+  // (every wave the same)
+  float top = -INFINITY;
+  for (int n = lane; n < a.slices; n += 64) top = fmaxf(top, parts[n][0]);
+  top = wave_most(top);
+  RowSums sum;
+  sum.m = top == -INFINITY ? 0.f : top;
+  sum.s = sum.u = 0.f;
+  sum.ahead = 0;
+  for (int n = lane; n < a.slices; n += 64) {
+    const f32x4_t p = parts[n];
+    const float d = p[0] - sum.m, w = exp2_hw(d * kLog2e);
+    sum.s += p[1] * w;
+    sum.u += w == 0.f ? 0.f : w * (p[2] + p[1] * d);
+    sum.ahead += __float_as_int(p[3]);
+  }
+  sum.s = wave_sum(sum.s);
+  sum.u = wave_sum(sum.u);
+#pragma unroll
+  for (int n = 32; n > 0; n >>= 1) sum.ahead += __shfl_xor(sum.ahead, n);
+  sum.nothing = top == -INFINITY && sum.s == 0.f;
+  const float log_s = logf(sum.s);
+  if (t == 0) {
+    const long long target = a.targets ? a.targets[r] : -1;
+    const bool asked = target >= 0 && target < a.vocab;
+    leave_row(a, r, sum, log_s, asked, asked ? logit(reinterpret_cast<const T*>(a.logits) + (size_t)r * a.ld + target) : 0.f);
+  }
+  if (a.top == 0) return;
+  __syncthreads();
+  const unsigned long long* list = held ? keys : from;
+  for (int n = t; n < many; n += blockDim.x) {
+    const unsigned long long key = list[n];
+    if (key == 0ull) continue;
+    const int own = n / a.top;
+    int place = n - own * a.top;
+    for (int other = 0; other < a.slices && place < a.top; ++other) {
+      if (other == own) continue;
+      int low = 0, high = a.top;   // the first of its places that is not ahead
+      while (low < high) {
+        const int middle = (low + high) >> 1;
+        if (list[other * a.top + middle] > key) low = middle + 1;
+        else high = middle;
+      }
+      place += low;
     }
+    if (place >= a.top) continue;
+    a.top_ids[(size_t)r * a.top + place] = id_of(key);
+    a.top_log_probs[(size_t)r * a.top + place] = log_prob(logit_of(key), sum, log_s);
   }
 }
 

@@ -105,6 +105,11 @@ PyMethodDef methods[] = {{"linear", reinterpret_cast<PyCFunction>(reinterpret_ca
                          {"shared_prefix_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&native::shared_prefix_attention)),
                           METH_FASTCALL, nullptr},
                          {"adjust_logits", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&native::adjust_logits)), METH_FASTCALL, nullptr},
+                         {"tree_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&native::tree_attention)), METH_FASTCALL, nullptr},
+                         {"keep_rows", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&native::keep_rows)), METH_FASTCALL, nullptr},
+                         {"token_log_probs", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&native::token_log_probs)), METH_FASTCALL, nullptr},
+                         {"follow_drafts", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&native::follow_drafts)), METH_FASTCALL, nullptr},
+                         {"bind_draft", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&native::bind_draft)), METH_FASTCALL, nullptr},
                          {"bind_serve", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&native::bind_serve)), METH_FASTCALL, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -134,6 +134,9 @@ def token_log_probs(logits: torch.Tensor, targets: torch.Tensor | None = None, *
     what = "token_log_probs"
     if not logits.is_cuda:
         raise ValueError("token_log_probs needs tensors on a ROCm device (there is no CPU path)")
+    made = (_lib._draft_native.get(what) or _lib.draft_native(what))(logits, targets, top)
+    if made is not None:
+        return TokenLogProbs._make(made)
     device = logits.device
     if logits.dim() != 2 or logits.dtype not in _TYPES or logits.shape[1] == 0 or (logits.shape[1] > 1 and logits.stride(1) != 1):
         raise ValueError("token_log_probs: logits [R, V] in float32 or bfloat16 expected")
@@ -179,6 +182,9 @@ def follow_drafts(tokens: torch.Tensor, parents: torch.Tensor, choices: torch.Te
     what = "follow_drafts"
     if not tokens.is_cuda:
         raise ValueError("follow_drafts needs tensors on a ROCm device (there is no CPU path)")
+    made = (_lib._draft_native.get(what) or _lib.draft_native(what))(tokens, parents, choices, counts)
+    if made is not None:
+        return FollowedDrafts._make(made)
     device = tokens.device
     if tokens.dim() != 2 or tokens.dtype != torch.int64 or (tokens.shape[1] > 1 and tokens.stride(1) != 1):
         raise ValueError("follow_drafts: tokens int64 [B, T] expected")
