@@ -91,8 +91,8 @@ template <typename T, int LANES, bool kRank, bool kTop>
 __global__ __launch_bounds__(LANES, 8) void log_probs_kernel(LogProbs a) {
   constexpr int E = kPiece<T>, W = LANES / 64, kRound = LANES * E;
   __shared__ __attribute__((aligned(16))) float most[W], sums[W], spreads[W];
-  __shared__ int aheads[W], gathered;
-  __shared__ __attribute__((aligned(16))) unsigned long long groups[kTop ? kGroups : 1], border, found[kTop ? kGathered : 1];   // (found: at first the lanes' own)
+  __shared__ int aheads[W], gathered, places[kTop ? kGroups : 1];
+  __shared__ __attribute__((aligned(16))) unsigned long long groups[kTop ? kGroups : 1], found[kTop ? kGathered : 1];   // (found: at first the lanes' own)
   const int t = threadIdx.x, wave = t >> 6;
   const int r = (int)blockIdx.x / a.slices, part = (int)blockIdx.x - r * a.slices, base = part * a.slice;
   const T* row = reinterpret_cast<const T*>(a.logits) + (size_t)r * a.ld;
@@ -121,7 +121,10 @@ __global__ __launch_bounds__(LANES, 8) void log_probs_kernel(LogProbs a) {
       if (at < target) ahead = logit(row + at) == mine;
     }
   }
-  if (kTop && t == 0) gathered = 0;
+  if constexpr (kTop) {
+    if (t == 0) gathered = 0;
+    if (t < kGroups) places[t] = 0;
+  }
 
   // ---- the maximum
   float top = -INFINITY;
@@ -136,17 +139,15 @@ __global__ __launch_bounds__(LANES, 8) void log_probs_kernel(LogProbs a) {
   if ((t & 63) == 0) most[wave] = top;
   unsigned long long own_first = 0ull;
   if constexpr (kTop) {
-    // the lane's first token
-    int first = 0x7FFFFFFF;
+    // the lane's first token (its number among the lane's own: a constant that the instruction holds)
+    int first = 0;
 #pragma unroll
     for (int i = kLogPieces - 1; i >= 0; --i)
       if (i * kRound < count) {
 #pragma unroll
-        for (int e = E - 1; e >= 0; --e) {
-          const float v = logit<T>(x[i], e);
-          first = !(v < lane_top) ? t * E + i * kRound + e : first;
-        }
+        for (int e = E - 1; e >= 0; --e) first = !(logit<T>(x[i], e) < lane_top) ? i * E + e : first;
       }
+    first = t * E + first / E * kRound + first % E;
     // (where there is NaN the first of it or of the largest: the border is then one that some NaN reaches)
     own_first = first < count ? key_of(lane_top, base + first) : 0ull;
     found[t] = own_first;
@@ -154,11 +155,12 @@ __global__ __launch_bounds__(LANES, 8) void log_probs_kernel(LogProbs a) {
   __syncthreads();
   if constexpr (kTop) {
     if (t < kGroups) {
-      unsigned long long key = found[t];
+      unsigned long long key = larger(found[t], kGroups - t);   // (of an empty group a number below every token's, its own)
 #pragma unroll
       for (int i = kGroups; i < LANES; i += kGroups) key = larger(key, found[t + i]);
       groups[t] = key;
     }
+    __syncthreads();
   }
   RowSums sum;
 #pragma unroll
@@ -194,20 +196,14 @@ __global__ __launch_bounds__(LANES, 8) void log_probs_kernel(LogProbs a) {
     spreads[wave] = u;
     aheads[wave] = ahead;
   }
-  // ---- the border: the top-th of the groups' first tokens
+  // ---- a group's place among the others: a lane counts a share of them
   if constexpr (kTop) {
-    __syncthreads();
-    if (t < kGroups) {
-      const unsigned long long key = groups[t];
-      int before = 0;
-#pragma unroll 16
-      for (int i = 0; i < kGroups; ++i) before += groups[i] > key;
-      // (no token: 0, which several groups may have; the first of them speaks)
-      if (key == 0ull) {
-        for (int i = 0; i < t; ++i) before += groups[i] == 0ull;
-      }
-      if (before == a.top - 1) border = key;
-    }
+    constexpr int kShare = kGroups * kGroups / LANES;
+    const unsigned long long key = groups[t % kGroups];
+    int before = 0;
+#pragma unroll
+    for (int i = 0; i < kShare; ++i) before += groups[t / kGroups * kShare + i] > key;
+    atomicAdd(&places[t % kGroups], before);
   }
   __syncthreads();
   sum.s = sum.u = 0.f;
@@ -226,7 +222,10 @@ __global__ __launch_bounds__(LANES, 8) void log_probs_kernel(LogProbs a) {
     else a.parts[blockIdx.x] = f32x4_t{top, sum.s, sum.u, __int_as_float(sum.ahead)};
   }
   if constexpr (kTop) {
-    const unsigned long long least = border;
+    // the border: the group in place top - 1
+    const int lane = t & 63;
+    const unsigned long long low = __builtin_amdgcn_ballot_w64(places[lane] == a.top - 1), high = __builtin_amdgcn_ballot_w64(places[64 + lane] == a.top - 1);
+    const unsigned long long least = groups[low ? __builtin_ctzll(low) : 64 + __builtin_ctzll(high)];
     const size_t to = (size_t)blockIdx.x * a.top;
     auto leave = [&](int place, unsigned long long key) {
       if (whole) {
@@ -236,33 +235,50 @@ __global__ __launch_bounds__(LANES, 8) void log_probs_kernel(LogProbs a) {
         a.firsts[to + place] = key;
       }
     };
-    const float least_logit = least == 0ull ? -INFINITY : logit_of(least);
+    // A lane's own first reaches it in some `top` lanes, others of its tokens in hardly any.
+    auto gather = [&](bool is, unsigned long long key) __attribute__((always_inline)) {
+      const unsigned long long who = __builtin_amdgcn_ballot_w64(is);
+      if (who == 0) return;
+      int at = 0;
+      if (lane == 0) at = atomicAdd(&gathered, __builtin_popcountll(who));
+      at = __builtin_amdgcn_readfirstlane(at) + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0));
+      if (is && at < kGathered) found[at] = key;
+    };
+    gather(own_first >= least, own_first);
+    const float least_logit = least <= kGroups ? -INFINITY : logit_of(least);
+    int reach = 0;
 #pragma unroll
     for (int i = 0; i < kLogPieces; ++i)
-      if (i * kRound < count && own_first >= least) {   // (few lanes)
+      if (i * kRound < count) {
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const float v = logit<T>(x[i], e);
-          const int id = t * E + i * kRound + e;
-          if (!(v < least_logit) && id < count) {
+        for (int e = 0; e < E; ++e) reach += !(logit<T>(x[i], e) < least_logit);
+      }
+    if (__builtin_amdgcn_ballot_w64(own_first >= least && reach > 1) != 0) {
+#pragma unroll
+      for (int i = 0; i < kLogPieces; ++i)
+        if (i * kRound < count) {
+#pragma unroll
+          for (int e = 0; e < E; ++e) {
+            const float v = logit<T>(x[i], e);
+            const int id = t * E + i * kRound + e;
+            bool is = own_first >= least && id < count && !(v < least_logit);
+            if (__builtin_amdgcn_ballot_w64(is) == 0) continue;
             const unsigned long long key = key_of(v, base + id);
-            if (key >= least) {
-              const int n = atomicAdd(&gathered, 1);
-              if (n < kGathered) found[n] = key;
-            }
+            gather(is && key >= least && (uint32_t)key != (uint32_t)own_first, key);
           }
         }
-      }
+    }
     __syncthreads();
     const int many = gathered;
     if (many <= kGathered) {
       for (int n = t; n < many; n += LANES) {
         const unsigned long long key = found[n];
         int place = 0;
+#pragma unroll 8
         for (int i = 0; i < many; ++i) place += found[i] > key;
         if (place < a.top) leave(place, key);
       }
-      if (!whole)   // (a slice that has fewer tokens)
+      if (!whole)   // (a slice that has fewer tokens than that)
         for (int n = many + t; n < a.top; n += LANES) a.firsts[to + n] = 0ull;
     } else {
       unsigned long long last = ~0ull;
