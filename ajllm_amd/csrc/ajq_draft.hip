@@ -136,10 +136,13 @@ struct LogProbsPlan {
 #endif
 LogProbsPlan log_probs_plan(const ajqt_log_probs_args* a) {
   LogProbsPlan p{};
-  const long long piece = kLogPieces * (a->dtype == AJQS_BF16 ? 8 : 4);
-  p.lanes = a->vocab <= 256 * piece || (a->vocab > 1024 * piece && a->rows * ceil_div(a->vocab, 1024 * piece) < LP_WANT) ? 256 : 1024;
-  p.slices = ceil_div(a->vocab, p.lanes * piece);
-  p.slice = (int)std::min((long long)a->vocab, ceil_div(ceil_div(a->vocab, p.slices), 64) * 64);
+  const long long size = a->dtype == AJQS_BF16 ? 2 : 4, piece = 16 / size;
+  // (rows that do not begin on 16 bytes fill up the piece they begin in)
+  const bool even = aligned16(a->logits) && (a->rows == 1 || a->ld * size % 16 == 0);
+  auto most = [&](long long lanes) { return lanes * kLogPieces * piece - (even ? 0 : piece); };
+  p.lanes = a->vocab <= most(256) || (a->vocab > most(1024) && a->rows * ceil_div(a->vocab, most(1024)) < LP_WANT) ? 256 : 1024;
+  p.slices = ceil_div(a->vocab, most(p.lanes));
+  p.slice = (int)std::min((long long)a->vocab, std::min(ceil_div(ceil_div(a->vocab, p.slices), 64) * 64, most(p.lanes)));
   p.slices = ceil_div(a->vocab, p.slice);
   p.bytes = p.slices > 1 ? (size_t)a->rows * p.slices * (sizeof(f32x4_t) + 8 * (size_t)a->top) : 0;
   return p;

@@ -5,16 +5,17 @@
 // A workgroup takes a slice of one row, up to 128 KiB, into its registers at once, so that everything behind the maximum is worked out of them and memory
 // is read once.  Slices' (m, s, u, tokens ahead) and first tokens are put together by a second launch where a row has several.
 //
-// The first `top` of a slice: lanes 128 apart are a group, and every group knows its first token.  The top-th of these 128 is a border that at least `top` tokens
-// reach, and only the groups that lead it have others that do: some top * (1 + top / 256) of them in a row without order, 16 bytes' worth of tokens for each of `top` in
-// one that is all alike or sorted.  They gather in LDS, each counts those ahead of itself, and that is its place.  Where they are more than LDS is set aside for (a
-// row made to be so), `top` rounds over the slice find them instead.
+// The first `top` of a slice: lanes 128 apart are a group, and every group knows its largest logit and the 16 bytes that it first has it in.  The top-th of these 128 is
+// a border that at least `top` tokens reach, and only the groups that lead it have others that do: some top * (1 + top / 256) of them in a row without order, 16 bytes'
+// worth of tokens for each of `top` in one that is all alike or sorted.  Their pieces gather in LDS, a lane takes a token, each counts those ahead of itself, and
+// that is its place.  Where they are more than LDS is set aside for (a row made to be so), `top` rounds over the slice find them instead.
 #pragma once
 #include "lane_rows.h"
+#include <type_traits>
 
 namespace ajq {
 
-constexpr int kMostTop = 64, kLogPieces = 8, kGroups = 128, kGathered = 2048;
+constexpr int kMostTop = 64, kLogPieces = 8, kGroups = 128, kHits = 512, kGathered = 1024;   // (at least the lanes of a workgroup)
 struct LogProbs {
   const void* logits;
   const long long* targets;
@@ -47,21 +48,14 @@ __device__ __forceinline__ float logit(const u32x4_t& raw, int e) {
   if constexpr (sizeof(T) == 4) return __uint_as_float(raw[e]);
   return __uint_as_float(e & 1 ? raw[e >> 1] & 0xFFFF0000u : raw[e >> 1] << 16);
 }
-// Sixteen bytes of a row wherever they lie (rows of an odd vocabulary begin anywhere; the hardware takes any address); behind its end -inf.
-typedef uint32_t u32x4f_t __attribute__((ext_vector_type(4), aligned(4)));
-typedef uint32_t u32x4h_t __attribute__((ext_vector_type(4), aligned(2)));
-__device__ __forceinline__ u32x4_t load_piece(const float* p, int there) {
-  if (there >= 4) return __builtin_nontemporal_load(reinterpret_cast<const u32x4f_t*>(p));
-  constexpr uint32_t kNone = 0xFF800000u;
-  const uint32_t* w = reinterpret_cast<const uint32_t*>(p);
-  return u32x4_t{w[0], there > 1 ? w[1] : kNone, there > 2 ? w[2] : kNone, kNone};
-}
-__device__ __forceinline__ u32x4_t load_piece(const uint16_t* p, int there) {
-  if (there >= 8) return __builtin_nontemporal_load(reinterpret_cast<const u32x4h_t*>(p));
-  u32x4_t v;
+// the logits of a piece from `first` to `last`, -inf for the others
+template <typename T>
+__device__ __forceinline__ u32x4_t load_some(const T* p, int first, int last) {
+  uint32_t w[kPiece<T>];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = (2 * i < there ? p[2 * i] : 0xFF80u) | (2 * i + 1 < there ? (uint32_t)p[2 * i + 1] : 0xFF80u) << 16;
-  return v;
+  for (int e = 0; e < kPiece<T>; ++e) w[e] = e >= first && e <= last ? reinterpret_cast<const std::conditional_t<sizeof(T) == 4, uint32_t, uint16_t>*>(p)[e] : sizeof(T) == 4 ? 0xFF800000u : 0xFF80u;
+  if constexpr (sizeof(T) == 4) return u32x4_t{w[0], w[1], w[2], w[3]};
+  else return u32x4_t{w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16};
 }
 
 __device__ __forceinline__ float wave_most(float v) {
@@ -70,6 +64,12 @@ __device__ __forceinline__ float wave_most(float v) {
   v = fmaxf(v, row_ror<4>(v));
   v = fmaxf(v, row_ror<2>(v));
   return fmaxf(v, row_ror<1>(v));
+}
+
+// numbers that all lanes have, kept where such numbers are (the logits leave no registers for them)
+__device__ __forceinline__ float uniform(float v) { return __uint_as_float((uint32_t)__builtin_amdgcn_readfirstlane(__float_as_int(v))); }
+__device__ __forceinline__ unsigned long long uniform(unsigned long long v) {
+  return (unsigned long long)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)v) | (unsigned long long)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(v >> 32)) << 32;
 }
 
 // What is known of a row, or of a slice of it.
@@ -91,21 +91,34 @@ template <typename T, int LANES, bool kRank, bool kTop>
 __global__ __launch_bounds__(LANES, 8) void log_probs_kernel(LogProbs a) {
   constexpr int E = kPiece<T>, W = LANES / 64, kRound = LANES * E;
   __shared__ __attribute__((aligned(16))) float most[W], sums[W], spreads[W];
-  __shared__ int aheads[W], gathered, places[kTop ? kGroups : 1];
+  __shared__ int aheads[W], hits, gathered, places[kTop ? kGroups : 1], hit_places[kTop ? kHits : 1];
+  __shared__ __attribute__((aligned(16))) u32x4_t hit_pieces[kTop ? kHits : 1];
   __shared__ __attribute__((aligned(16))) unsigned long long groups[kTop ? kGroups : 1], found[kTop ? kGathered : 1];   // (found: at first the lanes' own)
   const int t = threadIdx.x, wave = t >> 6;
   const int r = (int)blockIdx.x / a.slices, part = (int)blockIdx.x - r * a.slices, base = part * a.slice;
   const T* row = reinterpret_cast<const T*>(a.logits) + (size_t)r * a.ld;
-  const T* mine_from = row;
-  row += base;
+  const T* slice = row + base;
   const int count = min(a.slice, a.vocab - base);
+  // Places go by 16 bytes, wherever the slice begins (a row of an odd vocabulary begins anywhere; pieces across such borders take a quarter longer): token base + n is in
+  // place shift + n.
+  const int shift = (int)((reinterpret_cast<uintptr_t>(slice) & 15u) / sizeof(T)), places_end = shift + count;
+  slice -= shift;
+  constexpr uint32_t kNone = sizeof(T) == 4 ? 0xFF800000u : 0xFF80FF80u;
   u32x4_t x[kLogPieces];
 #pragma unroll
   for (int i = 0; i < kLogPieces; ++i) {
     const int at = t * E + i * kRound;
-    constexpr uint32_t kNone = sizeof(T) == 4 ? 0xFF800000u : 0xFF80FF80u;
     x[i] = u32x4_t{kNone, kNone, kNone, kNone};
-    if (at < count) x[i] = load_piece(row + at, count - at);
+    if (at >= shift && at + E <= places_end) x[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(slice + at));
+  }
+  // the piece that the slice begins in, and that it ends in
+  if (t == 0 && shift > 0) x[0] = load_some(slice, shift, places_end - 1);
+  const int last = (places_end - 1) / E;
+  if (places_end % E != 0 && t == last % LANES && last * E >= shift) {
+    const u32x4_t v = load_some(slice + last * E, 0, (places_end - 1) % E);
+#pragma unroll
+    for (int i = 0; i < kLogPieces; ++i)
+      if (i == last / LANES) x[i] = v;
   }
   bool asked = false;
   float mine = 0.f;
@@ -113,50 +126,53 @@ __global__ __launch_bounds__(LANES, 8) void log_probs_kernel(LogProbs a) {
   if constexpr (kRank) {
     const long long given = a.targets[r];
     asked = given >= 0 && given < a.vocab;
-    target = (int)min(max(given - base, -1ll), (long long)count);   // its place in the slice, or one beside it
-    if (asked) mine = logit(mine_from + given);
+    const long long off = given - base;
+    const bool here = off >= 0 && off < count;
+    // its place, or one in front of all the slice's pieces or behind them
+    target = here ? shift + (int)off : off < 0 ? 0 : (last + 1) * E;
+    if (asked) mine = uniform(logit(row + given));
     // of the target's own piece the tokens in front of it that have the same logit
-    if (asked && target >= 0 && target < count && t < E - 1) {
+    if (asked && here && t < E - 1) {
       const int at = target / E * E + t;
-      if (at < target) ahead = logit(row + at) == mine;
+      if (at >= shift && at < target) ahead = logit(slice + at) == mine;
     }
+    // (what fills up the pieces that the slice begins and ends in counts below where they are in front of a target that is -inf itself)
+    if (asked && t == 0 && mine == -INFINITY) ahead -= (target >= E ? shift : 0) + (target >= places_end ? (last + 1) * E - places_end : 0);
   }
   if constexpr (kTop) {
-    if (t == 0) gathered = 0;
+    if (t == 0) hits = gathered = 0;
     if (t < kGroups) places[t] = 0;
   }
 
   // ---- the maximum
+  auto piece_top = [&](int i) __attribute__((always_inline)) {
+    float v = logit<T>(x[i], 0);
+#pragma unroll
+    for (int e = 1; e < E; ++e) v = fmaxf(v, logit<T>(x[i], e));
+    return v;
+  };
   float top = -INFINITY;
+  int first = 0;   // the piece of the lane's that first has its largest logit (none: NaN in its first, which is ahead of all)
 #pragma unroll
   for (int i = 0; i < kLogPieces; ++i)
-    if (i * kRound < count) {
-#pragma unroll
-      for (int e = 0; e < E; ++e) top = fmaxf(top, logit<T>(x[i], e));
+    if (i * kRound < places_end) {
+      const float v = piece_top(i);
+      if (kTop) first = v > top ? i : first;
+      top = fmaxf(top, v);
     }
   const float lane_top = top;
   top = wave_most(top);
   if ((t & 63) == 0) most[wave] = top;
-  unsigned long long own_first = 0ull;
   if constexpr (kTop) {
-    // the lane's first token (its number among the lane's own: a constant that the instruction holds)
-    int first = 0;
-#pragma unroll
-    for (int i = kLogPieces - 1; i >= 0; --i)
-      if (i * kRound < count) {
-#pragma unroll
-        for (int e = E - 1; e >= 0; --e) first = !(logit<T>(x[i], e) < lane_top) ? i * E + e : first;
-      }
-    first = t * E + first / E * kRound + first % E;
-    // (where there is NaN the first of it or of the largest: the border is then one that some NaN reaches)
-    own_first = first < count ? key_of(lane_top, base + first) : 0ull;
-    found[t] = own_first;
+    // of the lane's tokens one at least is not behind the last of that piece, and none is ahead of its first
+    const int at = t * E + first * kRound;
+    found[t] = at < places_end ? key_of(lane_top, base - shift + at + E - 1) : 0ull;
   }
   __syncthreads();
   if constexpr (kTop) {
     if (t < kGroups) {
       unsigned long long key = larger(found[t], kGroups - t);   // (of an empty group a number below every token's, its own)
-#pragma unroll
+#pragma unroll 2
       for (int i = kGroups; i < LANES; i += kGroups) key = larger(key, found[t + i]);
       groups[t] = key;
     }
@@ -165,6 +181,7 @@ __global__ __launch_bounds__(LANES, 8) void log_probs_kernel(LogProbs a) {
   RowSums sum;
 #pragma unroll
   for (int w = 0; w < W; ++w) top = fmaxf(top, most[w]);
+  top = uniform(top);
   sum.m = top == -INFINITY ? 0.f : top;
 
   // ---- sums
@@ -175,7 +192,7 @@ __global__ __launch_bounds__(LANES, 8) void log_probs_kernel(LogProbs a) {
   float s = 0.f, u = 0.f;
 #pragma unroll
   for (int i = 0; i < kLogPieces; ++i)
-    if (i * kRound < count) {
+    if (i * kRound < places_end) {
       const float than = t * E + i * kRound + E - 1 < target ? below : lower;
 #pragma unroll
       for (int e = 0; e < E; ++e) {
@@ -201,7 +218,7 @@ __global__ __launch_bounds__(LANES, 8) void log_probs_kernel(LogProbs a) {
     constexpr int kShare = kGroups * kGroups / LANES;
     const unsigned long long key = groups[t % kGroups];
     int before = 0;
-#pragma unroll
+#pragma unroll 4   // (more would not leave the logits their registers)
     for (int i = 0; i < kShare; ++i) before += groups[t / kGroups * kShare + i] > key;
     atomicAdd(&places[t % kGroups], before);
   }
@@ -214,9 +231,10 @@ __global__ __launch_bounds__(LANES, 8) void log_probs_kernel(LogProbs a) {
     sum.u += spreads[w];
     sum.ahead += aheads[w];
   }
+  sum.s = uniform(sum.s);
   sum.nothing = top == -INFINITY && sum.s == 0.f;
   const bool whole = a.slices == 1;
-  const float log_s = logf(sum.s);
+  const float log_s = uniform(logf(sum.s));
   if (t == 0) {
     if (whole) leave_row(a, r, sum, log_s, asked, mine);
     else a.parts[blockIdx.x] = f32x4_t{top, sum.s, sum.u, __int_as_float(sum.ahead)};
@@ -225,7 +243,7 @@ __global__ __launch_bounds__(LANES, 8) void log_probs_kernel(LogProbs a) {
     // the border: the group in place top - 1
     const int lane = t & 63;
     const unsigned long long low = __builtin_amdgcn_ballot_w64(places[lane] == a.top - 1), high = __builtin_amdgcn_ballot_w64(places[64 + lane] == a.top - 1);
-    const unsigned long long least = groups[low ? __builtin_ctzll(low) : 64 + __builtin_ctzll(high)];
+    const unsigned long long least = uniform(groups[low ? __builtin_ctzll(low) : 64 + __builtin_ctzll(high)]);
     const size_t to = (size_t)blockIdx.x * a.top;
     auto leave = [&](int place, unsigned long long key) {
       if (whole) {
@@ -235,42 +253,34 @@ __global__ __launch_bounds__(LANES, 8) void log_probs_kernel(LogProbs a) {
         a.firsts[to + place] = key;
       }
     };
-    // A lane's own first reaches it in some `top` lanes, others of its tokens in hardly any.
-    auto gather = [&](bool is, unsigned long long key) __attribute__((always_inline)) {
-      const unsigned long long who = __builtin_amdgcn_ballot_w64(is);
-      if (who == 0) return;
-      int at = 0;
-      if (lane == 0) at = atomicAdd(&gathered, __builtin_popcountll(who));
-      at = __builtin_amdgcn_readfirstlane(at) + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0));
-      if (is && at < kGathered) found[at] = key;
-    };
-    gather(own_first >= least, own_first);
-    const float least_logit = least <= kGroups ? -INFINITY : logit_of(least);
-    int reach = 0;
-#pragma unroll
-    for (int i = 0; i < kLogPieces; ++i)
-      if (i * kRound < count) {
-#pragma unroll
-        for (int e = 0; e < E; ++e) reach += !(logit<T>(x[i], e) < least_logit);
-      }
-    if (__builtin_amdgcn_ballot_w64(own_first >= least && reach > 1) != 0) {
+    // the lanes, and their pieces, that may hold such tokens: the largest logit with the first id reaches it
+    int l = t;
+    asm volatile("" : "+v"(l));   // (places are formed again: nothing of them is kept beside the logits)
+    auto reaches = [&](float v, int at) { return at < places_end && key_of(v, base + max(at - shift, 0)) >= least; };
+    if (reaches(lane_top, l * E + first * kRound)) {
 #pragma unroll
       for (int i = 0; i < kLogPieces; ++i)
-        if (i * kRound < count) {
-#pragma unroll
-          for (int e = 0; e < E; ++e) {
-            const float v = logit<T>(x[i], e);
-            const int id = t * E + i * kRound + e;
-            bool is = own_first >= least && id < count && !(v < least_logit);
-            if (__builtin_amdgcn_ballot_w64(is) == 0) continue;
-            const unsigned long long key = key_of(v, base + id);
-            gather(is && key >= least && (uint32_t)key != (uint32_t)own_first, key);
+        if (i * kRound < places_end && reaches(piece_top(i), l * E + i * kRound)) {
+          const int n = atomicAdd(&hits, 1);
+          if (n < kHits) {
+            hit_pieces[n] = x[i];
+            hit_places[n] = l * E + i * kRound;
           }
         }
     }
     __syncthreads();
+    const int some = hits;
+    for (int n = t; n < min(some, kHits) * E; n += LANES) {
+      const int id = hit_places[n / E] + n % E - shift;
+      const unsigned long long key = key_of(logit(reinterpret_cast<const T*>(hit_pieces) + n), base + id);
+      if (id >= 0 && id < count && key >= least) {
+        const int to = atomicAdd(&gathered, 1);
+        if (to < kGathered) found[to] = key;
+      }
+    }
+    __syncthreads();
     const int many = gathered;
-    if (many <= kGathered) {
+    if (some <= kHits && many <= kGathered) {
       for (int n = t; n < many; n += LANES) {
         const unsigned long long key = found[n];
         int place = 0;
@@ -281,17 +291,15 @@ __global__ __launch_bounds__(LANES, 8) void log_probs_kernel(LogProbs a) {
       if (!whole)   // (a slice that has fewer tokens than that)
         for (int n = many + t; n < a.top; n += LANES) a.firsts[to + n] = 0ull;
     } else {
-      unsigned long long last = ~0ull;
+      unsigned long long before = ~0ull;
+#pragma unroll 1
       for (int k = 0; k < a.top; ++k) {
         unsigned long long best = 0ull;
-        for (int i = 0; i < kLogPieces; ++i)
-          if (i * kRound < count) {
-            for (int e = 0; e < E; ++e) {
-              const int id = t * E + i * kRound + e;
-              const unsigned long long key = id < count ? key_of(logit(row + id), base + id) : 0ull;
-              if (key < last) best = larger(best, key);
-            }
-          }
+#pragma unroll 1
+        for (int id = t; id < count; id += LANES) {
+          const unsigned long long key = key_of(logit(row + base + id), base + id);
+          if (key < before) best = larger(best, key);
+        }
         __syncthreads();
         found[t] = best;
         for (int n = LANES / 2; n > 0; n >>= 1) {
@@ -299,8 +307,8 @@ __global__ __launch_bounds__(LANES, 8) void log_probs_kernel(LogProbs a) {
           if (t < n) found[t] = larger(found[t], found[t + n]);
         }
         __syncthreads();
-        last = found[0];
-        if (t == 0) leave(k, last);
+        before = found[0];
+        if (t == 0) leave(k, before);
       }
     }
   }
