@@ -131,20 +131,17 @@ struct LogProbsPlan {
   long long slices;
   size_t bytes;
 };
-#ifndef LP_WANT
-#define LP_WANT 128
-#endif
 LogProbsPlan log_probs_plan(const ajqt_log_probs_args* a) {
   LogProbsPlan p{};
   const long long size = a->dtype == AJQS_BF16 ? 2 : 4, piece = 16 / size;
   // (rows that do not begin on 16 bytes fill up the piece they begin in)
   const bool even = aligned16(a->logits) && (a->rows == 1 || a->ld * size % 16 == 0);
   auto most = [&](long long lanes) { return lanes * kLogPieces * piece - (even ? 0 : piece); };
-  p.lanes = a->vocab <= most(256) || (a->vocab > most(1024) && a->rows * ceil_div(a->vocab, most(1024)) < LP_WANT) ? 256 : 1024;
+  p.lanes = a->vocab <= most(256) || (a->vocab > most(1024) && a->rows * ceil_div(a->vocab, most(1024)) < 256) ? 256 : 1024;
   p.slices = ceil_div(a->vocab, most(p.lanes));
   p.slice = (int)std::min((long long)a->vocab, std::min(ceil_div(ceil_div(a->vocab, p.slices), 64) * 64, most(p.lanes)));
   p.slices = ceil_div(a->vocab, p.slice);
-  p.bytes = p.slices > 1 ? (size_t)a->rows * p.slices * (sizeof(f32x4_t) + 8 * (size_t)a->top) : 0;
+  p.bytes = p.slices > 1 ? (size_t)a->rows * p.slices * (sizeof(f32x4_t) + 8 * (size_t)a->top) + 4 * (size_t)a->rows : 0;
   return p;
 }
 
@@ -235,8 +232,9 @@ int ajqt_log_probs(const ajqt_log_probs_args* a, void* workspace, size_t workspa
     return fail(AJQ_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, %zu given", what, p.bytes, workspace_bytes);
   if (!aligned16(workspace)) return fail(AJQ_ERR_ALIGN, "%s: the workspace must be 16-byte aligned", what);
   f32x4_t* parts = reinterpret_cast<f32x4_t*>(workspace);
+  unsigned long long* firsts = reinterpret_cast<unsigned long long*>(parts + (size_t)a->rows * p.slices);
   const LogProbs n{a->logits, int64s(a->targets), a->log_probs, a->entropy, a->top_log_probs, reinterpret_cast<long long*>(a->ranks),
-                   reinterpret_cast<long long*>(a->top_ids), parts, reinterpret_cast<unsigned long long*>(parts + (size_t)a->rows * p.slices), a->ld, a->rows, a->vocab,
+                   reinterpret_cast<long long*>(a->top_ids), parts, reinterpret_cast<float*>(firsts + (size_t)a->rows * p.slices * a->top), firsts, a->ld, a->rows, a->vocab,
                    a->top, p.slice, (int)p.slices};
   with_type(a->dtype, [&](auto type) {
     using T = decltype(type);
@@ -253,9 +251,7 @@ int ajqt_log_probs(const ajqt_log_probs_args* a, void* workspace, size_t workspa
   });
   if (int e = check_launch(what)) return e;
   if (p.slices == 1) return AJQ_OK;
-  with_type(a->dtype, [&](auto type) {
-    hipLaunchKernelGGL(log_probs_merge_kernel<decltype(type)>, dim3((unsigned)a->rows), dim3(a->top ? 256 : 64), 0, (hipStream_t)stream, n);
-  });
+  hipLaunchKernelGGL(log_probs_merge_kernel, dim3((unsigned)a->rows), dim3(a->top ? 256 : 64), 0, (hipStream_t)stream, n);
   return check_launch(what);
 }
 

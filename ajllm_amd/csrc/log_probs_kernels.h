@@ -22,6 +22,7 @@ struct LogProbs {
   float *log_probs, *entropy, *top_log_probs;
   long long *ranks, *top_ids;
   f32x4_t* parts;               // [rows, slices] m, s, u, tokens ahead of the target (a whole number's bits)
+  float* mine;                  // [rows] the target's logit
   unsigned long long* firsts;   // [rows, slices, top]
   long long ld;
   int rows, vocab, top, slice, slices;
@@ -238,6 +239,7 @@ __global__ __launch_bounds__(LANES, 8) void log_probs_kernel(LogProbs a) {
   if (t == 0) {
     if (whole) leave_row(a, r, sum, log_s, asked, mine);
     else a.parts[blockIdx.x] = f32x4_t{top, sum.s, sum.u, __int_as_float(sum.ahead)};
+    if (kRank && !whole && part == 0) a.mine[r] = mine;
   }
   if constexpr (kTop) {
     // the border: the group in place top - 1
@@ -314,21 +316,30 @@ __global__ __launch_bounds__(LANES, 8) void log_probs_kernel(LogProbs a) {
   }
 }
 
-// ---- a row's slices put together, a workgroup a row.  A token's place is its place in its slice and, of every other slice, how many are ahead of it.
+// ---- a row's slices put together, a workgroup a row.  With S slices, the least of the tokens in place ceil(top / S) of theirs is a border that `top` tokens reach;
+// those that do (twice as many or so) gather, and each counts the ones ahead of itself.
 constexpr int kMergeKeys = 2048;
-template <typename T>
 __global__ __launch_bounds__(256) void log_probs_merge_kernel(LogProbs a) {
-  __shared__ unsigned long long keys[kMergeKeys];
+  __shared__ __attribute__((aligned(16))) unsigned long long keys[kMergeKeys];
+  __shared__ int gathered;
   const int r = blockIdx.x, t = threadIdx.x, lane = t & 63;
   const f32x4_t* parts = a.parts + (size_t)r * a.slices;
   const unsigned long long* from = a.firsts + (size_t)r * a.slices * a.top;
   const int many = a.slices * a.top;
-  const bool held = many <= kMergeKeys;
-  if (held)
-    for (int n = t; n < many; n += blockDim.x) keys[n] = from[n];
+  if (t == 0) gathered = 0;
+  const long long target = a.targets ? a.targets[r] : -1;
+  const float mine = a.targets ? a.mine[r] : 0.f;
   // (every wave the same)
   float top = -INFINITY;
-  for (int n = lane; n < a.slices; n += 64) top = fmaxf(top, parts[n][0]);
+  unsigned long long least = ~0ull;
+  const int place_of_all = (a.top + a.slices - 1) / a.slices - 1;
+  for (int n = lane; n < a.slices; n += 64) {
+    top = fmaxf(top, parts[n][0]);
+    if (a.top) {
+      const unsigned long long key = from[n * a.top + place_of_all];
+      least = key < least ? key : least;
+    }
+  }
   top = wave_most(top);
   RowSums sum;
   sum.m = top == -INFINITY ? 0.f : top;
@@ -347,17 +358,41 @@ __global__ __launch_bounds__(256) void log_probs_merge_kernel(LogProbs a) {
   for (int n = 32; n > 0; n >>= 1) sum.ahead += __shfl_xor(sum.ahead, n);
   sum.nothing = top == -INFINITY && sum.s == 0.f;
   const float log_s = logf(sum.s);
-  if (t == 0) {
-    const long long target = a.targets ? a.targets[r] : -1;
-    const bool asked = target >= 0 && target < a.vocab;
-    leave_row(a, r, sum, log_s, asked, asked ? logit(reinterpret_cast<const T*>(a.logits) + (size_t)r * a.ld + target) : 0.f);
-  }
+  if (t == 0) leave_row(a, r, sum, log_s, target >= 0 && target < a.vocab, mine);
   if (a.top == 0) return;
+#pragma unroll
+  for (int n = 32; n > 0; n >>= 1) {
+    const unsigned long long other = __shfl_xor(least, n);
+    least = other < least ? other : least;
+  }
+  auto leave = [&](int place, unsigned long long key) {
+    if (place >= a.top) return;
+    a.top_ids[(size_t)r * a.top + place] = id_of(key);
+    a.top_log_probs[(size_t)r * a.top + place] = log_prob(logit_of(key), sum, log_s);
+  };
   __syncthreads();
-  const unsigned long long* list = held ? keys : from;
   for (int n = t; n < many; n += blockDim.x) {
-    const unsigned long long key = list[n];
-    if (key == 0ull) continue;
+    const unsigned long long key = from[n];
+    if (key < least || key == 0ull) continue;
+    const int to = atomicAdd(&gathered, 1);
+    if (to < kMergeKeys) keys[to] = key;
+  }
+  __syncthreads();
+  const int some = gathered;
+  if (some <= kMergeKeys) {
+    for (int n = t; n < some; n += blockDim.x) {
+      const unsigned long long key = keys[n];
+      int place = 0;
+#pragma unroll 8
+      for (int i = 0; i < some; ++i) place += keys[i] > key;
+      leave(place, key);
+    }
+    return;
+  }
+  // (many slices with much the same tokens) a token's place in its slice and, of every other slice, how many are ahead of it
+  for (int n = t; n < many; n += blockDim.x) {
+    const unsigned long long key = from[n];
+    if (key < least || key == 0ull) continue;
     const int own = n / a.top;
     int place = n - own * a.top;
     for (int other = 0; other < a.slices && place < a.top; ++other) {
@@ -365,14 +400,12 @@ __global__ __launch_bounds__(256) void log_probs_merge_kernel(LogProbs a) {
       int low = 0, high = a.top;   // the first of its places that is not ahead
       while (low < high) {
         const int middle = (low + high) >> 1;
-        if (list[other * a.top + middle] > key) low = middle + 1;
+        if (from[other * a.top + middle] > key) low = middle + 1;
         else high = middle;
       }
       place += low;
     }
-    if (place >= a.top) continue;
-    a.top_ids[(size_t)r * a.top + place] = id_of(key);
-    a.top_log_probs[(size_t)r * a.top + place] = log_prob(logit_of(key), sum, log_s);
+    leave(place, key);
   }
 }
 
