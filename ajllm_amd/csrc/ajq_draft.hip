@@ -31,29 +31,37 @@ int check_tree(const ajqt_tree_attention_args* a) {
 // How a call is cut up: tiles of a sequence's queries of a key head, parts of its rows.  The lengths are on the device: max_len is what they can be.
 struct TreePlan {
   bool walk;     // tiles of 64 rt queries, by meet_many; else of 16 rt, by meet_few
-  int rt, tiles, parts;
-  bool alone;    // a wave a tile, not a workgroup
+  int rt, waves, tiles;
+  int runs;      // 0: every sequence's rows are one part
   long long blocks, queries;
   size_t bytes;
 };
-constexpr int kMostParts = 64;      // a lane each in the merge
+constexpr int kMostParts = 64;      // of a sequence: a lane each in the merge
+#ifndef TREE_ENV
+#define env(name, value) (value)
+#endif
 TreePlan tree_plan(const ajqt_tree_attention_args* a) {
   TreePlan p{};
   const long long share = a->heads / a->kv_heads, mine = a->tokens * share, units = (long long)a->batch * a->kv_heads;
   const bool bf16 = a->cache_dtype == AJQS_BF16;
   p.queries = (long long)a->batch * a->heads * a->tokens;
-  p.walk = bf16 && mine > 64;
+  p.walk = bf16 && env("T_WALK", mine > 64);
+  p.waves = 4;
   if (p.walk) {
-    p.rt = a->q_dtype == AJQS_BF16 && a->dim == 128 && units * ceil_div(mine, 128) >= 256 ? 2 : 1;
-    p.tiles = (int)ceil_div(mine, 64 * p.rt);
+    p.rt = a->q_dtype == AJQS_BF16 && a->dim == 128 && env("T_RT", mine >= 128 ? 2 : 1) == 2 ? 2 : 1;
+    p.waves = a->dim >= 64 && env("T_WV", mine > 128 ? 8 : 4) == 8 ? 8 : 4;
+    p.tiles = (int)ceil_div(mine, 16 * p.waves * p.rt);
   } else {
-    p.rt = mine > 16 ? 2 : 1;
+    p.rt = (int)env("T_RT", mine > 16 ? 2 : 1);
     p.tiles = (int)ceil_div(mine, 16 * p.rt);
+    p.waves = (int)env("T_WV", 4);
+    if (!bf16 && p.rt == 2 && a->dim == 128) p.waves = 4;
   }
-  const long long workgroups = units * p.tiles;
-  p.parts = (int)std::max(1ll, std::min({512 / workgroups, ceil_div(a->max_len, bf16 || p.rt > 1 ? 128 : 64), (long long)kMostParts}));
-  p.blocks = p.walk ? ceil_div(units, 8) * 8 * p.tiles * p.parts : ceil_div(units * p.parts, 8) * 8 * p.tiles;
-  p.bytes = p.parts > 1 ? (size_t)p.parts * p.queries * (8 + 4 * (size_t)a->dim) : 0;
+  const long long workgroups = units * p.tiles, slots = env("T_WANT", p.waves == 8 ? 256 : 512), least = env("T_LEAST", bf16 || p.rt > 1 ? 128 : 64);
+  const long long runs = env("T_RUNS", std::min({slots / (a->kv_heads * (long long)p.tiles), a->batch * ceil_div(a->max_len, least), (long long)a->batch * kMostParts}));
+  p.runs = a->batch <= kMostDealt && runs > a->batch ? (int)runs : 0;
+  p.blocks = ceil_div(p.runs ? (long long)p.runs * a->kv_heads : units, 8) * 8 * p.tiles;
+  p.bytes = p.runs ? ((size_t)p.runs * a->kv_heads * mine * (8 + 4 * (size_t)a->dim) + 8 * (size_t)a->batch) : 0;
   return p;
 }
 
@@ -67,7 +75,10 @@ TreeAttention tree_of(const ajqt_tree_attention_args* a, const TreePlan& p, void
   s.offset = int64s(a->offset);
   s.out = reinterpret_cast<uint16_t*>(a->out);
   s.part_sums = reinterpret_cast<float*>(workspace);
-  s.part_ml = reinterpret_cast<float2*>(s.part_sums + (size_t)p.parts * p.queries * a->dim);
+  const size_t partial = (size_t)p.runs * a->kv_heads * a->tokens * (a->heads / a->kv_heads);
+  s.part_ml = reinterpret_cast<float2*>(s.part_sums + partial * a->dim);
+  s.dealt = reinterpret_cast<int2*>(s.part_ml + partial);
+  s.runs = p.runs;
   s.prefix_group = s.cache_batch = a->cache_batch;
   s.prefix_head = s.cache_head = a->cache_head;
   s.queries = p.queries;
@@ -76,9 +87,8 @@ TreeAttention tree_of(const ajqt_tree_attention_args* a, const TreePlan& p, void
   s.heads = a->heads;
   s.kv_heads = a->kv_heads;
   s.prefix_cap = s.max_len = a->max_len;
-  s.own_parts = p.parts;
+  s.own_parts = 1;
   s.own_tiles = p.tiles;
-  s.own_alone = p.alone;
   s.scale2 = kLog2e / sqrtf((float)a->dim);
   s.by_share = divide_by(a->heads / a->kv_heads);
   s.by_each = divide_by((long long)a->tokens * (a->heads / a->kv_heads));
@@ -88,7 +98,7 @@ TreeAttention tree_of(const ajqt_tree_attention_args* a, const TreePlan& p, void
   s.by_group = divide_by(1);
   s.by_prefix_tiles = s.by_prefix_parts = divide_by(1);
   s.by_own_tiles = divide_by(p.tiles);
-  s.by_own_parts = divide_by(p.parts);
+  s.by_own_parts = divide_by(1);
   s.masks = a->masks;
   s.mask_batch = a->mask_batch;
   s.mask_token = a->mask_token;
@@ -157,7 +167,7 @@ int ajqt_tree_attention(const ajqt_tree_attention_args* a, void* workspace, size
   const char* what = "ajqt_tree_attention";
   if (int e = check_tree(a)) return e;
   const TreePlan p = tree_plan(a);
-  if (p.blocks > kMostLanes / 256) return fail(AJQ_ERR_SHAPE, "%s: too many tiles of queries", what);
+  if (p.blocks > kMostLanes / (64 * p.waves)) return fail(AJQ_ERR_SHAPE, "%s: too many tiles of queries", what);
   if (p.bytes && ceil_div(p.queries, 4) > kMostLanes / 256) return fail(AJQ_ERR_SHAPE, "%s: too many queries (%lld)", what, p.queries);
   if (p.bytes && (!workspace || workspace_bytes < p.bytes))
     return fail(AJQ_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, %zu given", what, p.bytes, workspace_bytes);
@@ -172,25 +182,35 @@ int ajqt_tree_attention(const ajqt_tree_attention_args* a, void* workspace, size
         using CacheT = decltype(cache);
         auto launch = [&](auto kernel, int lds) {
           if ((status = allow_lds(kernel, lds, what)) != AJQ_OK) return;
-          hipLaunchKernelGGL(kernel, dim3((unsigned)p.blocks), dim3(256), lds, (hipStream_t)stream, s);
-          if ((status = check_launch(what)) != AJQ_OK || p.parts == 1) return;
-          hipLaunchKernelGGL(shared_attention_merge_kernel<HD>, dim3((unsigned)ceil_div(p.queries, 4)), dim3(256), 0, (hipStream_t)stream,
-                             static_cast<const SharedAttention&>(s));
+          hipLaunchKernelGGL(kernel, dim3((unsigned)p.blocks), dim3(64 * p.waves), lds, (hipStream_t)stream, s);
+          if ((status = check_launch(what)) != AJQ_OK || p.runs == 0) return;
+          hipLaunchKernelGGL(tree_attention_merge_kernel<HD>, dim3((unsigned)ceil_div(p.queries, 4)), dim3(256), 0, (hipStream_t)stream, s);
           status = check_launch(what);
         };
         if constexpr (sizeof(CacheT) == 2) {
           if (p.walk) {
+            auto walk = [&](auto tiles) {
+              constexpr int U = decltype(tiles)::value;
+              if constexpr (HD >= 64) {
+                if (p.waves == 8) return launch(tree_attention_walk_kernel<HD, QT, U, 8>, many_lds_bytes<HD, 8>());
+              }
+              launch(tree_attention_walk_kernel<HD, QT, U, 4>, many_lds_bytes<HD, 4>());
+            };
             if constexpr (HD == 128 && sizeof(QT) == 2) {
-              if (p.rt == 2) return launch(tree_attention_walk_kernel<HD, QT, 2>, many_lds_bytes<HD>());
+              if (p.rt == 2) return walk(Size<2>{});
             }
-            return launch(tree_attention_walk_kernel<HD, QT, 1>, many_lds_bytes<HD>());
+            return walk(Size<1>{});
           }
         }
-        auto few = [&](auto tiles) {
-          constexpr int RT = decltype(tiles)::value, lds = some_lds_bytes<HD, CacheT, RT>();
-          p.parts == 1 ? launch(tree_attention_few_kernel<HD, QT, CacheT, RT, true>, lds) : launch(tree_attention_few_kernel<HD, QT, CacheT, RT, false>, lds);
+        auto few = [&](auto tiles, auto waves) {
+          constexpr int RT = decltype(tiles)::value, WV = decltype(waves)::value, lds = some_lds_bytes<HD, CacheT, RT, WV>();
+          p.runs ? launch(tree_attention_few_kernel<HD, QT, CacheT, RT, WV, false>, lds) : launch(tree_attention_few_kernel<HD, QT, CacheT, RT, WV, true>, lds);
         };
-        p.rt == 2 ? few(Size<2>{}) : few(Size<1>{});
+        if constexpr (sizeof(CacheT) == 2 || HD < 128) {
+          if (p.rt == 2 && p.waves == 8) return few(Size<2>{}, Size<8>{});
+        }
+        if (p.rt == 2) return few(Size<2>{}, Size<4>{});
+        p.waves == 8 ? few(Size<1>{}, Size<8>{}) : few(Size<1>{}, Size<4>{});
       });
     });
   });

@@ -68,6 +68,12 @@ __device__ __forceinline__ long long query_place(const SharedAttention& a, int k
   return ((long long)(first_sequence + sequence) * a.heads + (key_head * (int)a.by_share.d + head)) * a.tokens + token;
 }
 
+// where a query's partial result goes (n: its number in the meeting, in_q: its place in q)
+template <typename CacheT>
+__device__ __forceinline__ long long part_place(const SharedAttention& a, const Meeting<CacheT>& w, long long in_q, int) {
+  return in_q + (w.part + (w.own ? a.prefix_parts : 0)) * a.queries;
+}
+
 // 8 query components at p as bf16: hi (and lo, what fp32 has beyond it)
 __device__ __forceinline__ void split8(const float* v, u32x4_t& hi, u32x4_t& lo) {
   hi = pack8_bf16(v);
@@ -210,9 +216,9 @@ __device__ __forceinline__ void find_both(const SharedAttention& a, Meeting<Cach
 // rows for its 32 queries alone, and one wave a SIMD (212 registers) has nothing to run beside it.  16 sequences of 100 tokens x 4 of 8 heads behind 2048 rows 386 us: 39 % of a SIMD's
 // cycles are vector instructions, 16 % MFMAs.
 template <int HD, typename CacheT> constexpr int few_wave_bytes() { return 2 * 32 * 2 * HD * kHalves<CacheT>; }
-template <int HD, int RT> constexpr int few_join_bytes() { return 4 * RT * 16 * (HD + 4) * 4; }
-template <int HD, typename CacheT, int RT> constexpr int few_lds_bytes() {
-  constexpr int walk = 4 * few_wave_bytes<HD, CacheT>(), join = few_join_bytes<HD, RT>() + 4 * RT * 16 * 8;
+template <int HD, int RT, int WV = 4> constexpr int few_join_bytes() { return WV * RT * 16 * (HD + 4) * 4; }   // (of WV waves)
+template <int HD, typename CacheT, int RT, int WV = 4> constexpr int few_lds_bytes() {
+  constexpr int walk = WV * few_wave_bytes<HD, CacheT>(), join = few_join_bytes<HD, RT, WV>() + WV * RT * 16 * 8;
   return walk > join ? walk : join;
 }
 
@@ -260,11 +266,11 @@ __device__ __forceinline__ void leave_alone(const SharedAttention& a, const Meet
   }
 }
 
-// The four waves' results meet in LDS (rows of HD + 4 numbers: sixteen queries' pieces fall on different banks) and become the workgroup's part, or
+// The waves' results meet in LDS (rows of HD + 4 numbers: sixteen queries' pieces fall on different banks) and become the workgroup's part, or
 // (kWhole) the result.
-template <int HD, int RT, int kMl, bool kWhole, typename CacheT, typename Put>
-__device__ __forceinline__ void join_waves(const SharedAttention& a, const Meeting<CacheT>& w, unsigned char* lds, const RunningRow<HD> (&row)[RT], Put put) {
-  constexpr int kJoin = RT * 16, kPitch = HD + 4, kHelpers = 256 / kJoin;   // queries, lanes that put one together
+template <int HD, int RT, int kMl, bool kWhole, int WV = 4, typename A, typename CacheT, typename Put>
+__device__ __forceinline__ void join_waves(const A& a, const Meeting<CacheT>& w, unsigned char* lds, const RunningRow<HD> (&row)[RT], Put put) {
+  constexpr int kJoin = RT * 16, kPitch = HD + 4, kHelpers = 64 * WV / kJoin;   // queries, lanes that put one together
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
   float* sums = reinterpret_cast<float*>(lds);
   float2* ml = reinterpret_cast<float2*>(lds + kMl);
@@ -278,21 +284,21 @@ __device__ __forceinline__ void join_waves(const SharedAttention& a, const Meeti
   __syncthreads();
   const int n = (int)threadIdx.x / kHelpers, d0 = 4 * ((int)threadIdx.x % kHelpers);
   if (w.first + n >= w.queries) return;
-  float2 e[4];
-  float m = -INFINITY, l = 0.f, weight[4];
+  float2 e[WV];
+  float m = -INFINITY, l = 0.f, weight[WV];
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
+  for (int k = 0; k < WV; ++k) {
     e[k] = ml[k * kJoin + n];
     m = fmaxf(m, e[k].x);
   }
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
+  for (int k = 0; k < WV; ++k) {
     weight[k] = e[k].x == -INFINITY ? 0.f : exp2_hw(e[k].x - m);
     l += e[k].y * weight[k];
   }
   int token;
   const long long in_q = query_place(a, w.key_head, w.first_sequence, w.first + n, token);
-  const long long place = in_q + (kWhole ? 0 : (w.part + (w.own ? a.prefix_parts : 0)) * a.queries);
+  const long long place = kWhole ? in_q : part_place(a, w, in_q, w.first + n);
   if (!kWhole && d0 == 0) a.part_ml[place] = float2{m, l};
   float scale = 1.f;
   uint16_t* out = nullptr;
@@ -302,7 +308,7 @@ __device__ __forceinline__ void join_waves(const SharedAttention& a, const Meeti
     if (d + d0 >= HD) break;
     f32x4_t o = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int k = 0; k < 4; ++k) o += *reinterpret_cast<const f32x4_t*>(sums + (k * kJoin + n) * kPitch + d + d0) * weight[k];
+    for (int k = 0; k < WV; ++k) o += *reinterpret_cast<const f32x4_t*>(sums + (k * kJoin + n) * kPitch + d + d0) * weight[k];
     if constexpr (kWhole) store_run(out + d + d0, o, scale);
     else store_run(a.part_sums + place * HD + d + d0, o, 1.f);
   }
@@ -328,8 +334,8 @@ __device__ __forceinline__ int blocks_of(const Meeting<CacheT>& w) {
   return (w.end - w.begin + N - 1) / N + (kBoth ? (w.own_end + N - 1) / N : 0);
 }
 
-// W: how many of the waves work.  kWhole: they meet all rows, and what comes out is the result.
-template <int HD, typename QT, typename CacheT, int RT, int W = 4, bool kBoth = false, bool kWhole = kBoth, typename A>
+// W: how many of the WV waves work.  kWhole: they meet all rows, and what comes out is the result.
+template <int HD, typename QT, typename CacheT, int RT, int W = 4, bool kBoth = false, bool kWhole = kBoth, int WV = 4, typename A>
 __device__ __forceinline__ void meet_few(const A& a, Meeting<CacheT>& w, unsigned char* lds, uint32_t lds0) {
   constexpr int RB = 2 * HD, C = HD / 8, KS = HD / 32, TT = HD / 16, KH = kHalves<CacheT>, QH = kHalves<QT>;
   constexpr int kPlane = 32 * RB;                 // 32 rows of bf16
@@ -515,7 +521,7 @@ __device__ __forceinline__ void meet_few(const A& a, Meeting<CacheT>& w, unsigne
     for (int t = 0; t < TT; ++t) store_run(to + 16 * t + 4 * g, row[u].o[t], scale);
   };
   if (w.alone) leave_alone<HD, RT, kWhole>(a, w, row, put);
-  else join_waves<HD, RT, few_join_bytes<HD, RT>(), kWhole>(a, w, lds, row, put);
+  else join_waves<HD, RT, few_join_bytes<HD, RT, WV>(), kWhole, WV>(a, w, lds, row, put);
 }
 
 // ---- At most 16 queries on fp32 rows, in fp32 throughout (v_mfma_f32_16x16x4_f32: 32 cycles for 16 rows x 4 components, where the memory's share of a CU
@@ -531,8 +537,8 @@ __device__ __forceinline__ float4 query4(const uint16_t* p) {
   widen2(w.y, v.z, v.w);
   return v;
 }
-template <int HD> constexpr int few_f32_lds_bytes() { return few_join_bytes<HD, 1>() + 4 * 16 * 8; }
-template <int HD, typename QT, bool kBoth = false, bool kWhole = kBoth, typename A>
+template <int HD, int WV = 4> constexpr int few_f32_lds_bytes() { return few_join_bytes<HD, 1, WV>() + WV * 16 * 8; }
+template <int HD, typename QT, bool kBoth = false, bool kWhole = kBoth, int WV = 4, typename A>
 __device__ __forceinline__ void meet_few_f32(const A& a, Meeting<float>& w, unsigned char* lds) {
   constexpr int KC = HD / 16, P = HD == 32 ? 2 : 4, VC = HD / (16 * P);
   typedef float part_t __attribute__((ext_vector_type(P)));
@@ -601,7 +607,7 @@ __device__ __forceinline__ void meet_few_f32(const A& a, Meeting<float>& w, unsi
         for (int e = 0; e < P; ++e) row[0].o[c * P + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(rows.v[i][c][e], p[i], row[0].o[c * P + e], 0, 0, 0);
   };
   // two blocks' registers in turn, the next one's rows on their way while one is worked on
-  const int blocks = blocks_of<16, kBoth>(w), begin = w.alone ? 0 : wave, by = w.alone ? 1 : 4;
+  const int blocks = blocks_of<16, kBoth>(w), begin = w.alone ? 0 : wave, by = w.alone ? 1 : WV;
   Fetched even_rows, odd_rows;
   if (begin < blocks) ask(Rows(w, begin), even_rows);
   for (int n = begin; n < blocks; n += 2 * by) {
@@ -624,7 +630,7 @@ __device__ __forceinline__ void meet_few_f32(const A& a, Meeting<float>& w, unsi
       }
   };
   if (w.alone) leave_alone<HD, 1, kWhole>(a, w, row, put);
-  else join_waves<HD, 1, few_join_bytes<HD, 1>(), kWhole>(a, w, lds, row, put);
+  else join_waves<HD, 1, few_join_bytes<HD, 1, WV>(), kWhole, WV>(a, w, lds, row, put);
 }
 
 // ---- Many queries on bf16 rows: 64 U to a workgroup, 16 U to each wave, all four walking the same blocks of 64 rows (LDS, two stages of a key and a
@@ -640,9 +646,10 @@ template <typename CacheT> struct Walk {
   const CacheT *keys[2], *values[2];   // the part's first rows: prefix, own
   int rows[2];                         // how many there are
   int key_head, first_sequence, queries, first;
+  int there;                           // in a tree: how many of the queries are
   long long before;                    // own rows ahead of a sequence's first new token, counted from the part's first own row
 };
-template <int HD> constexpr int many_lds_bytes() { return 4 * 64 * 2 * HD + 4 * 256; }
+template <int HD, int WV = 4> constexpr int many_lds_bytes() { return 4 * 64 * 2 * HD + WV * 256; }
 
 // Two requests of 1 KiB each for 4096 bytes ahead of lds_addr (from 4096 bytes ahead of base) and for lds_addr: the instruction's offset moves both sides.
 #pragma clang diagnostic push
@@ -655,9 +662,11 @@ __device__ __forceinline__ void dma16_pair(const void* base, uint32_t voff, uint
 }
 #pragma clang diagnostic pop
 
-template <int HD, typename QT, int U, typename A>
+template <int HD, typename QT, int U, int WV = 4, typename A>
 __device__ __forceinline__ void meet_many(const A& a, const Walk<uint16_t>& w, RunningRow<HD> (&row)[U], uint32_t lds0) {
   constexpr int RB = 2 * HD, C = HD / 8, KS = HD / 32, TT = HD / 16, QH = kHalves<QT>, kAhead = TT < 3 ? TT : 3;
+  constexpr int KQ = KS * 4 / WV;   // requests of a wave for a block's keys (or values)
+  static_assert((WV == 4 || WV == 8) && KQ > 0, "four waves, or eight where there are requests enough");
   constexpr int kTile = 64 * RB;
   constexpr int kReqRows = 1024 / RB;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -669,12 +678,14 @@ __device__ __forceinline__ void meet_many(const A& a, const Walk<uint16_t>& w, R
   const int prefix_blocks = (w.rows[0] + 63) >> 6, blocks = prefix_blocks + ((w.rows[1] + 63) >> 6);
   if (blocks == 0) return;
 
-  // ---- requests: 1 KiB of rows each; wave w takes rows kReqRows w .. of every group of 4 kReqRows.  Rows past a run's last: that one again.
-  const int krow = kReqRows * wave + lane / C, slot = lane % C;
+  // ---- requests: 1 KiB of rows each; wave w takes rows kReqRows w .. of every group of 4 kReqRows (of eight waves the last four those of the second half).  Rows past a
+  // run's last: that one again.
+  const int turn = WV == 4 ? wave : (wave & 3) + 4 * KQ * (wave >> 2);   // the wave's first request
+  const int krow = kReqRows * turn + lane / C, slot = lane % C;
   const uint32_t k_lane = (uint32_t)(krow * RB) + (uint32_t)(slot ^ (krow & (C - 1))) * 16u;
   const uint32_t v_lane = (uint32_t)(krow * RB) + (uint32_t)((((slot >> 1) ^ (krow & (TT - 1))) << 1) | (slot & 1)) * 16u;
   auto place = [&](bool values, int i, int stage) __attribute__((always_inline)) {
-    return lds0 + (uint32_t)(stage * 2 * kTile + (values ? kTile : 0) + (wave + 4 * i) * 1024);
+    return lds0 + (uint32_t)(stage * 2 * kTile + (values ? kTile : 0) + (turn + 4 * i) * 1024);
   };
   auto request = [&](int j, bool values) __attribute__((always_inline)) {
     const bool own = j >= prefix_blocks;
@@ -682,10 +693,10 @@ __device__ __forceinline__ void meet_many(const A& a, const Walk<uint16_t>& w, R
     const uint16_t* from = (values ? (own ? w.values[1] : w.values[0]) : (own ? w.keys[1] : w.keys[0])) + (size_t)at * HD;
     int l = lane;   // (formed again from the lane's number: no register of its own beside the steps)
     asm volatile("" : "+v"(l));
-    const int row = kReqRows * wave + l / C, to = l % C;
+    const int row = kReqRows * turn + l / C, to = l % C;
     const uint32_t chunk = values ? (uint32_t)((((to >> 1) ^ (row & (TT - 1))) << 1) | (to & 1)) * 16u : (uint32_t)(to ^ (row & (C - 1))) * 16u;
 #pragma unroll
-    for (int i = 0; i < KS; ++i) {
+    for (int i = 0; i < KQ; ++i) {
       const uint32_t k = (uint32_t)min(4 * kReqRows * i + row, there - 1 - at) * (uint32_t)RB;
       dma16(from, k + chunk, place(values, i, j & 1));
     }
@@ -722,7 +733,7 @@ __device__ __forceinline__ void meet_many(const A& a, const Walk<uint16_t>& w, R
   const int nearest = limit_of(w.first + 16 * U * wave);   // of the wave's queries
   const int farthest = A::kTree ? w.rows[1] : limit_of(w.first + 16 * U * wave + 16 * U - 1);
   // steps of this wave
-  const int steps = w.first + 16 * U * wave >= w.queries ? 0 : farthest > 0 ? 2 * prefix_blocks + ((farthest + 31) >> 5) : (w.rows[0] + 31) >> 5;
+  const int steps = w.first + 16 * U * wave >= (A::kTree ? w.there : w.queries) ? 0 : farthest > 0 ? 2 * prefix_blocks + ((farthest + 31) >> 5) : (w.rows[0] + 31) >> 5;
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   if (blocks > 1) request(1, false);
   turn_barrier();
@@ -882,11 +893,11 @@ __device__ __forceinline__ void meet_many(const A& a, const Walk<uint16_t>& w, R
       const char* const values = reinterpret_cast<const char*>(run ? w.values[1] : w.values[0]);
       const char* k_from = keys + (size_t)(j - ahead_of_run + 2) * kTile;
       const char* v_from = values + (size_t)(j - ahead_of_run + 1) * kTile;
-      // lines: of the keys waves 0 and 1, of the values 2 and 3, of block j + 4 (of the last whole one, at most)
+      // lines: of the keys waves 0 and 1, of the values 2 and 3, of block j + 4 (of the last whole one, at most); waves 4 .. 7 the same ones again
       const uint32_t corner = lds0 + (uint32_t)(4 * kTile + 256 * wave);
       const uint32_t line = (uint32_t)((64 * (wave & 1) + lane) * (RB / 2));
       auto touch = [&](int block) __attribute__((always_inline)) {
-        dma4((wave < 2 ? keys : values) + (size_t)min(block - ahead_of_run, whole - 1) * kTile, line, corner);
+        dma4(((WV == 4 ? wave < 2 : (wave & 2) == 0) ? keys : values) + (size_t)min(block - ahead_of_run, whole - 1) * kTile, line, corner);
       };
       touch(j + 4);
       do {
@@ -898,8 +909,8 @@ __device__ __forceinline__ void meet_many(const A& a, const Walk<uint16_t>& w, R
             const int n = i % KS;   // request of the wave: of the keys', then of the values'
             const char* const from = (i < KS ? k_from : v_from) + n * 4096;
             const uint32_t at = i < KS ? k_lane : v_lane, to = place(i >= KS, n, i < KS ? x : x ^ 1);
-            if (KS == 1) dma16(from, at, to);
-            else if (n % 2 == 0) dma16_pair(from + 4096, at, to + 4096);
+            if (KQ == 1 && n == 0) dma16(from, at, to);
+            else if (n % 2 == 0 && n < KQ) dma16_pair(from + 4096, at, to + 4096);
             if (i == TT - 1) touch(j + x + 5);
           });
           k_from += kTile;
@@ -929,8 +940,9 @@ __device__ __forceinline__ void meet_many(const A& a, const Walk<uint16_t>& w, R
 }
 
 // a lane's queries of meet_many as partial results
-template <int HD, int U>
-__device__ __forceinline__ void leave_part(const SharedAttention& a, const Walk<uint16_t>& w, const RunningRow<HD> (&row)[U], int part) {
+__device__ __forceinline__ long long part_place(const SharedAttention& a, const Walk<uint16_t>&, long long in_q, int, int part) { return in_q + part * a.queries; }
+template <int HD, int U, typename A>
+__device__ __forceinline__ void leave_part(const A& a, const Walk<uint16_t>& w, const RunningRow<HD> (&row)[U], int part) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
 #pragma unroll
   for (int u = 0; u < U; ++u) {
@@ -938,20 +950,20 @@ __device__ __forceinline__ void leave_part(const SharedAttention& a, const Walk<
     const int n = w.first + 16 * (U * wave + u) + r;
     if (n >= w.queries) continue;
     int token;
-    const long long place = query_place(a, w.key_head, w.first_sequence, n, token) + part * a.queries;
+    const long long place = part_place(a, w, query_place(a, w.key_head, w.first_sequence, n, token), n, part);
     if (g == 0) a.part_ml[place] = row[u].part(l);
 #pragma unroll
     for (int t = 0; t < HD / 16; ++t) *reinterpret_cast<f32x4_t*>(a.part_sums + place * HD + 16 * t + 4 * g) = row[u].o[t];
   }
 }
 
-template <int HD, typename QT, typename CacheT, int RT, bool kBoth = false, bool kWhole = kBoth, typename A>
+template <int HD, typename QT, typename CacheT, int RT, bool kBoth = false, bool kWhole = kBoth, int WV = 4, typename A>
 __device__ __forceinline__ void meet_some(const A& a, Meeting<CacheT>& w, unsigned char* lds, uint32_t lds0) {
-  if constexpr (sizeof(CacheT) == 4 && RT == 1) meet_few_f32<HD, QT, kBoth, kWhole>(a, w, lds);
-  else meet_few<HD, QT, CacheT, RT, 4, kBoth, kWhole>(a, w, lds, lds0);
+  if constexpr (sizeof(CacheT) == 4 && RT == 1) meet_few_f32<HD, QT, kBoth, kWhole, WV>(a, w, lds);
+  else meet_few<HD, QT, CacheT, RT, WV, kBoth, kWhole, WV>(a, w, lds, lds0);
 }
-template <int HD, typename CacheT, int RT> constexpr int some_lds_bytes() {
-  return sizeof(CacheT) == 4 && RT == 1 ? few_f32_lds_bytes<HD>() : few_lds_bytes<HD, CacheT, RT>();
+template <int HD, typename CacheT, int RT, int WV = 4> constexpr int some_lds_bytes() {
+  return sizeof(CacheT) == 4 && RT == 1 ? few_f32_lds_bytes<HD, WV>() : few_lds_bytes<HD, CacheT, RT, WV>();
 }
 template <int HD, typename QT, typename CacheT, int RTP, int RTO>
 __global__ __launch_bounds__(256, sizeof(CacheT) == 4 && RTP == 2 ? 1 : 2) void shared_attention_few_kernel(SharedAttention a) {
@@ -1008,27 +1020,29 @@ __global__ __launch_bounds__(256, 2) void shared_attention_many_kernel(SharedAtt
 // own_parts > 1 the walk is cut up and leaves parts for the merge.  16 sequences of 100 tokens x 4 of 8 heads behind 2048 rows 66 us = 630 TFLOP/s (71 in the first calls after
 // a pause), 24 of 50 behind 8000 203 us = 775.  Of the former's cycles a CU is busy for 63 % (358 tiles on 256 CUs: some have two, some one), and a SIMD for 45 % of those with MFMAs,
 // 36 % with other vector instructions; its LDS is no limit (no bank conflicts).
-template <int HD, typename QT, int U, typename A>
-__device__ __forceinline__ void walk_own(const A& a, uint32_t lds0) {
-  const int share = (int)a.by_share.d, parts = a.own_parts;
-  int part, hk, unused, tile;
-  const int id = (int)blockIdx.x, run = (id & 7) + 8 * divide(divide(id >> 3, a.by_own_parts, part), a.by_own_tiles, tile);
-  if (run >= a.batch * a.kv_heads) return;
-  tile = a.own_tiles - 1 - tile;
-  const int b = divide(run, a.by_kv_heads, hk), group = divide(b, a.by_group, unused);
+struct WalkTurn {
+  int sequence, key_head, tile, part, parts;
+  int left_at;   // the part's number among the partial results
+};
+template <int HD, typename QT, int U, int WV = 4, typename A>
+__device__ __forceinline__ void walk_own(const A& a, const WalkTurn& turn, bool leaves_parts, uint32_t lds0) {
+  const int share = (int)a.by_share.d, parts = turn.parts, part = turn.part, hk = turn.key_head, b = turn.sequence, tile = turn.tile;
+  int unused;
+  const int group = divide(b, a.by_group, unused);
   Walk<uint16_t> w;
   w.key_head = hk;
   w.first_sequence = b;
   w.queries = a.tokens * share;
-  w.first = 64 * U * tile;
+  w.first = 16 * WV * U * tile;
   w.before = read_uniform(a.rows + b) + (a.offset ? read_uniform(a.offset) : 0ll);
   const int there = a.counts ? held(read_uniform(a.counts + b), a.tokens) : a.tokens;
-  const int last = min(divide(w.first + 64 * U - 1, a.by_share, unused), there - 1);          // the tile's last token that is there
+  const int last = min(divide(w.first + 16 * WV * U - 1, a.by_share, unused), there - 1);          // the tile's last token that is there
   const size_t at = (size_t)group * a.prefix_group + (size_t)hk * a.prefix_head;
   size_t own = (size_t)b * a.cache_batch + (size_t)hk * a.cache_head;
   const bool none = w.first >= there * share;
   int prefix_rows, own_rows;
   if constexpr (A::kTree) {
+    w.there = there * share;
     // whole blocks of committed rows are the first run (its caches are the sequence's own), the others and the tree's the second
     const int rows = none ? 0 : held(w.before + there, a.max_len);
     prefix_rows = held(w.before, rows) & ~63;
@@ -1052,9 +1066,9 @@ __device__ __forceinline__ void walk_own(const A& a, uint32_t lds0) {
   w.rows[1] = max(min(own_rows - own_skip * 64, (many - of_prefix) * 64), 0);
   w.before -= (long long)own_skip * 64;
   RunningRow<HD> row[U];
-  meet_many<HD, QT, U>(a, w, row, lds0);
-  if (parts > 1) {
-    leave_part<HD, U>(a, w, row, part);
+  meet_many<HD, QT, U, WV>(a, w, row, lds0);
+  if (leaves_parts) {
+    leave_part<HD, U>(a, w, row, turn.left_at);
     return;
   }
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
@@ -1080,7 +1094,14 @@ __device__ __forceinline__ void walk_own(const A& a, uint32_t lds0) {
 template <int HD, typename QT, int U>
 __global__ __launch_bounds__(256, 2) void shared_attention_walk_kernel(SharedAttention a) {
   extern __shared__ __attribute__((aligned(1024))) unsigned char shared_lds[];
-  walk_own<HD, QT, U>(a, (uint32_t)(uintptr_t)(pf_lds_char_t*)shared_lds);
+  WalkTurn turn;
+  const int id = (int)blockIdx.x, run = (id & 7) + 8 * divide(divide(id >> 3, a.by_own_parts, turn.part), a.by_own_tiles, turn.tile);
+  if (run >= a.batch * a.kv_heads) return;
+  turn.tile = a.own_tiles - 1 - turn.tile;
+  turn.sequence = divide(run, a.by_kv_heads, turn.key_head);
+  turn.parts = a.own_parts;
+  turn.left_at = turn.part;
+  walk_own<HD, QT, U>(a, turn, a.own_parts > 1, (uint32_t)(uintptr_t)(pf_lds_char_t*)shared_lds);
 }
 
 // ---- the parts of a query put together: a wave a query, lane p holding part p's (m, sum).  The first kFirst parts' sums are asked for beside them.
@@ -1091,20 +1112,18 @@ __device__ __forceinline__ float wave_max(float v) {
   v = fmaxf(v, row_ror<2>(v));
   return fmaxf(v, row_ror<1>(v));
 }
-template <int HD>
-__global__ __launch_bounds__(256) void shared_attention_merge_kernel(SharedAttention a) {
+// ml, sums: the query's first part's; the others `apart` queries behind.  late(there, to): whether the token is there, and where the result goes.
+template <int HD, typename Late>
+__device__ __forceinline__ void put_together(const float2* ml_from, const float* sums, size_t apart, int parts, Late late) {
   constexpr int kEach = HD == 128 ? 2 : 1, kLanes = HD / kEach, kFirst = 8;   // components of a lane, lanes that hold some
-  const long long place = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (place >= a.queries) return;
-  const int lane = threadIdx.x & 63, parts = a.prefix_parts + a.own_parts;
-  const float2 ml = a.part_ml[min(lane, parts - 1) * a.queries + place];
-  const float* from = a.part_sums + place * HD + kEach * min(lane, kLanes - 1);
-  const size_t apart = (size_t)a.queries * HD;
+  const int lane = threadIdx.x & 63;
+  const float2 ml = ml_from[min(lane, parts - 1) * apart];
+  const float* from = sums + kEach * min(lane, kLanes - 1);
   float x[kFirst][kEach];
   auto ask = [&](int first) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < kFirst; ++i) {
-      const float* at = from + min(first + i, parts - 1) * apart;
+      const float* at = from + min(first + i, parts - 1) * (apart * HD);
       if constexpr (kEach == 2) {
         const float2 v = *reinterpret_cast<const float2*>(at);
         x[i][0] = v.x;
@@ -1115,9 +1134,9 @@ __global__ __launch_bounds__(256) void shared_attention_merge_kernel(SharedAtten
     }
   };
   ask(0);
-  int t, h;
-  const int b = divide(divide((int)place, a.by_tokens, t), a.by_heads, h);
-  const bool there = a.counts == nullptr || t < a.counts[b];
+  bool there;
+  uint16_t* to;
+  late(there, to);
   const float mine = lane < parts && there ? ml.x : -INFINITY;
   const float top = wave_max(mine);
   const float weight = mine == -INFINITY ? 0.f : exp2_hw(mine - top);
@@ -1135,9 +1154,20 @@ __global__ __launch_bounds__(256) void shared_attention_merge_kernel(SharedAtten
   }
   if (lane >= kLanes) return;
   const bool some = l > 0.f || l != l;
-  uint16_t* to = a.out + (((size_t)b * a.tokens + t) * a.heads + h) * HD + kEach * lane;
+  to += kEach * lane;
   if constexpr (kEach == 2) *reinterpret_cast<uint32_t*>(to) = some ? pack2_bf16(o[0] / l, o[kEach - 1] / l) : 0u;
   else *to = some ? f32_to_bf16_rne(o[0] / l) : (uint16_t)0;
+}
+template <int HD>
+__global__ __launch_bounds__(256) void shared_attention_merge_kernel(SharedAttention a) {
+  const long long place = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (place >= a.queries) return;
+  put_together<HD>(a.part_ml + place, a.part_sums + place * HD, (size_t)a.queries, a.prefix_parts + a.own_parts, [&](bool& there, uint16_t*& to) __attribute__((always_inline)) {
+    int t, h;
+    const int b = divide(divide((int)place, a.by_tokens, t), a.by_heads, h);
+    there = a.counts == nullptr || t < a.counts[b];
+    to = a.out + (((size_t)b * a.tokens + t) * a.heads + h) * HD;
+  });
 }
 
 }  // namespace ajq
