@@ -311,6 +311,7 @@ class AdjustLogitsArgs(ctypes.Structure):
 SERVE_SIGNATURES: dict[str, tuple] = {
     "ajqs_last_error": (c_char_p, []),
     "ajqs_norm_rope": (c_int, [ctypes.POINTER(NormRopeArgs), _P]),
+    "ajqs_norm_rope_at": (c_int, [ctypes.POINTER(NormRopeArgs), _P, c_int64, _P]),
     "ajqs_shared_attention_workspace": (c_size_t, [ctypes.POINTER(SharedAttentionArgs)]),
     "ajqs_shared_attention": (c_int, [ctypes.POINTER(SharedAttentionArgs), _P, c_size_t, _P]),
     "ajqs_adjust_logits": (c_int, [ctypes.POINTER(AdjustLogitsArgs), _P]),

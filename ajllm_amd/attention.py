@@ -103,14 +103,15 @@ def _floats(what: str, name: str, t: torch.Tensor | None, shape: tuple, device: 
 def norm_rope(qkv: torch.Tensor, cosine: torch.Tensor, sine: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, rows: torch.Tensor, *,
               heads: int, tokens: int = 1, q_gain: torch.Tensor | None = None, k_gain: torch.Tensor | None = None, epsilon: float = 1e-5,
               positions: torch.Tensor | None = None, counts: torch.Tensor | None = None, offset: torch.Tensor | None = None,
-              out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
+              out_dtype: torch.dtype = torch.float32, depths: torch.Tensor | None = None) -> torch.Tensor:
     """Queries and keys of a projection's output, each head RMS-normed (``q_gain``, ``k_gain`` fp32 ``[hd]``; None: as it is) and rotated,
     keys and values written into the caches, in one launch: for sequences at positions of their own.
 
     ``qkv`` fp32 or bf16 ``[B * tokens, (heads + 2 Hkv) * hd]`` (query heads, key heads, value heads; rows may be further apart); ``cosine`` /
     ``sine`` fp32 ``[positions, hd / 2]``; ``keys`` / ``values`` ``[B, Hkv, max_len, hd]`` fp32 or bf16.  Token t of sequence b goes to row
     ``rows[b] + offset + t`` of its caches and turns by position ``positions[b] + offset + t`` (``positions`` None: the row); ``rows``,
-    ``positions`` and ``counts`` int64 ``[B]``, ``offset`` one int64, all on the device.  Of the tokens of sequence b the first
+    ``positions`` and ``counts`` int64 ``[B]``, ``offset`` one int64, all on the device.  Tokens that do not follow each other (a tree's, ``tree_masks``) turn by
+    ``depths[t]`` (int64 ``[tokens]``, or ``[B, tokens]``) in t's place.  Of the tokens of sequence b the first
     ``counts[b]`` are there (None: all); the others write no row, and zeros for queries.  A row outside the caches is not written, a
     position is held inside the tables; heads of the caches may not overlap.  Returns the queries ``[B, heads, tokens, hd]`` in ``out_dtype``,
     without a gradient, as all of these functions
@@ -119,10 +120,11 @@ def norm_rope(qkv: torch.Tensor, cosine: torch.Tensor, sine: torch.Tensor, keys:
     if not qkv.is_cuda:
         raise ValueError("norm_rope needs tensors on a ROCm device (there is no CPU path)")
     # tensors as the kernel takes them: one call of native code, which leaves everything else to the lines below it
-    q = (_lib._serve_native.get(what) or _lib.serve_native(what))(
-        qkv, cosine, sine, keys, values, rows, heads, tokens, q_gain, k_gain, epsilon, positions, counts, offset, out_dtype)
-    if q is not None:
-        return q
+    if depths is None:
+        q = (_lib._serve_native.get(what) or _lib.serve_native(what))(
+            qkv, cosine, sine, keys, values, rows, heads, tokens, q_gain, k_gain, epsilon, positions, counts, offset, out_dtype)
+        if q is not None:
+            return q
     device = qkv.device
     _check_caches(what, keys, values, device)
     batch, kv_heads, max_len, hd = keys.shape
@@ -138,13 +140,17 @@ def norm_rope(qkv: torch.Tensor, cosine: torch.Tensor, sine: torch.Tensor, keys:
     _whole_numbers(what, "positions", positions, batch, device)
     _whole_numbers(what, "counts", counts, batch, device)
     _whole_numbers(what, "offset", offset, 1, device)
+    if depths is not None and (depths.dtype != torch.int64 or tuple(depths.shape) not in ((tokens,), (batch, tokens)) or depths.device != device
+                               or (tokens > 1 and depths.stride(-1) != 1)):
+        raise ValueError("norm_rope: depths int64 [tokens] or [B, tokens] on the device of the others expected")
     q = torch.empty((batch, heads, tokens, hd), dtype=out_dtype, device=device)
     args = _lib.NormRopeArgs(
         qkv.data_ptr(), cosine.data_ptr(), sine.data_ptr(), _pointer(q_gain), _pointer(k_gain), rows.data_ptr(), _pointer(positions),
         _pointer(counts), _pointer(offset), keys.data_ptr(), values.data_ptr(), q.data_ptr(), qkv.stride(0), keys.stride(0), keys.stride(1),
         batch, tokens, heads, kv_heads, hd, max_len, cosine.shape[0], _TYPES[qkv.dtype], _TYPES[out_dtype], _TYPES[keys.dtype], epsilon)
     with _on(device):
-        status = _lib.load_serve().ajqs_norm_rope(ctypes.byref(args), torch.cuda.current_stream().cuda_stream)
+        status = _lib.load_serve().ajqs_norm_rope_at(ctypes.byref(args), _pointer(depths), depths.stride(0) if depths is not None and depths.dim() == 2 else 0,
+                                                     torch.cuda.current_stream().cuda_stream)
     _lib.check_serve(status, what)
     return q
 

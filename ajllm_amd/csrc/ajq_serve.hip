@@ -198,7 +198,9 @@ extern "C" {
 
 const char* ajqs_last_error(void) { return g_error; }
 
-int ajqs_norm_rope(const ajqs_norm_rope_args* a, void* stream) {
+int ajqs_norm_rope(const ajqs_norm_rope_args* a, void* stream) { return ajqs_norm_rope_at(a, nullptr, 0, stream); }
+
+int ajqs_norm_rope_at(const ajqs_norm_rope_args* a, const int64_t* depths, int64_t depths_ld, void* stream) {
   const char* what = "ajqs_norm_rope";
   if (!a) return fail(AJQ_ERR_NULL, "%s: null arguments", what);
   if (!a->qkv || !a->cosine || !a->sine || !a->rows || !a->keys || !a->values || !a->q)
@@ -223,9 +225,10 @@ int ajqs_norm_rope(const ajqs_norm_rope_args* a, void* stream) {
   const long long d = (long long)(reinterpret_cast<uintptr_t>(a->values) - reinterpret_cast<uintptr_t>(a->keys)) / size;
   if (d == 0 || blocks_meet(d, a->cache_batch, a->batch, a->cache_head, a->kv_heads, room))
     return fail(AJQ_ERR_SHAPE, "%s: keys and values that overlap cannot be written", what);
+  if (depths && depths_ld < 0) return fail(AJQ_ERR_SHAPE, "%s: negative stride of the depths", what);
   if (!(a->eps >= 0.f)) return fail(AJQ_ERR_SHAPE, "%s: epsilon %g", what, a->eps);
   const NormRope n{a->qkv, a->cosine, a->sine, a->q_gain, a->k_gain, int64s(a->rows), int64s(a->positions), int64s(a->counts),
-                   int64s(a->offset), a->keys, a->values, a->q, a->ld, a->cache_batch, a->cache_head, a->tokens, a->heads, a->kv_heads,
+                   int64s(a->offset), int64s(depths), a->keys, a->values, a->q, a->ld, a->cache_batch, a->cache_head, depths_ld, a->tokens, a->heads, a->kv_heads,
                    a->max_len, a->table_rows, a->eps, divide_by(a->tokens)};
   with_dim(a->dim, [&](auto dim) {
     with_type(a->in_dtype, [&](auto in) {

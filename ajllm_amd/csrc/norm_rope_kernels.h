@@ -14,9 +14,9 @@ namespace ajq {
 struct NormRope {
   const void* qkv;
   const float *cosine, *sine, *q_gain, *k_gain;
-  const long long *rows, *positions, *counts, *offset;
+  const long long *rows, *positions, *counts, *offset, *depths;
   void *keys, *values, *q;
-  long long ld, cache_batch, cache_head;
+  long long ld, cache_batch, cache_head, depths_ld;
   int tokens, heads, kv_heads, max_len, table_rows;
   float eps;
   Divide by_tokens;
@@ -67,7 +67,7 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(NormRope a) {
   }
   const long long off = a.offset ? *a.offset : 0ll;
   const long long at = a.rows[b] + off + t;
-  const long long p = min(max((a.positions ? a.positions[b] + off : a.rows[b] + off) + t, 0ll), (long long)a.table_rows - 1);
+  const long long p = min(max((a.positions ? a.positions[b] + off : a.rows[b] + off) + (a.depths ? a.depths[b * a.depths_ld + t] : t), 0ll), (long long)a.table_rows - 1);
   float cs[DPL / 2], sn[DPL / 2];
 #pragma unroll
   for (int i = 0; i < DPL / 2; ++i) {

@@ -15,9 +15,10 @@ import ctypes
 import torch
 
 from . import _lib, dense, modeling
-from .attention import norm_rope, prefill_attention, shared_prefix_attention, shared_prefix_launches
+from .attention import (keep_rows, norm_rope, prefill_attention, shared_prefix_attention, shared_prefix_launches, tree_attention,
+                        tree_masks)
 from .quant import QuantLinear, repack_w4, repack_w8, w4a16_matmul, w8a16_matmul
-from .sampling import adjust_logits
+from .sampling import MOST_TOP, FollowedDrafts, TokenLogProbs, adjust_logits, follow_drafts, token_log_probs
 
 
 class GraphDecoder:
@@ -52,6 +53,8 @@ class GraphDecoder:
         self.adjustments: dict[str, torch.Tensor] = {}
         self.prompt_ids = torch.full((batch, max_len), -1, dtype=torch.long, device=device)
         self.prompt_count = torch.zeros(1, dtype=torch.long, device=device)
+        # what ``set_log_probs`` asks for: a column a token
+        self.records: TokenLogProbs | None = None
 
     def set_sampling(self, temperature: float, top_p: float | None = None, seed: int = 0) -> None:
         """Choose tokens as the reference's ``sample_next_token`` does (src/ajllm/generation/sampling.py:8-22):
@@ -103,6 +106,38 @@ class GraphDecoder:
                 self.adjustments["allowed_rows"] = allowed_rows
         self._drop_graphs()
 
+    def set_log_probs(self, alternatives: int | None = 0) -> None:
+        """Keep, beside every token that is produced, its log probability, its rank and the entropy, and the ``alternatives`` most probable tokens
+        (``sampling.token_log_probs``) under the logits that it was chosen from: as ``set_penalties`` left them, at a temperature of 1.  ``log_probs`` gives what
+        has been kept.  Call it before ``prefill``; graphs recorded so far are dropped.  None: keep nothing any more."""
+        if alternatives is not None and not 0 <= alternatives <= min(MOST_TOP, self.model.vocab_size):
+            raise ValueError(f"alternatives must be in [0, {min(MOST_TOP, self.model.vocab_size)}]")
+        self.records = None
+        if alternatives is not None:
+            shape = (self.batch, self.out.shape[1])
+            floats = lambda *s: torch.zeros(s, dtype=torch.float32, device=self.device)  # noqa: E731
+            whole = lambda *s: torch.zeros(s, dtype=torch.int64, device=self.device)     # noqa: E731
+            self.records = TokenLogProbs(floats(*shape), whole(*shape), floats(*shape), floats(*shape, alternatives) if alternatives else None,
+                                         whole(*shape, alternatives) if alternatives else None)
+        self._drop_graphs()
+
+    def log_probs(self, new_tokens: int) -> TokenLogProbs:
+        """What ``set_log_probs`` has kept of the first ``new_tokens`` tokens since ``prefill``: ``[B, new_tokens]`` each, alternatives ``[B, new_tokens, n]``."""
+        if self.records is None:
+            raise ValueError("set_log_probs says what to keep")
+        if not 0 <= new_tokens <= self.produced:
+            raise ValueError(f"{new_tokens} of {self.produced} tokens")
+        return TokenLogProbs(*(None if kept is None else kept[:, :new_tokens].clone() for kept in self.records))
+
+    def _record(self, logits: torch.Tensor, column: torch.Tensor) -> None:
+        """``self.token`` has been chosen from ``logits`` ``[B, V]`` for column ``column`` (one int64 on the device) of the output."""
+        if self.records is None:
+            return
+        top = 0 if self.records.top_ids is None else self.records.top_ids.shape[2]
+        for kept, now in zip(self.records, token_log_probs(logits, self.token.view(-1), top=top)):
+            if kept is not None:
+                kept.index_copy_(1, column, now[:, None])
+
     def _adjusted(self, logits: torch.Tensor, in_place: bool = False) -> torch.Tensor:
         """``logits`` ``[B, V]`` as ``set_penalties`` asks for them (``in_place``: fp32 ones that nobody else reads)."""
         if not self.adjustments:
@@ -134,10 +169,11 @@ class GraphDecoder:
         if self.temperature > 0:
             vocab = logits.shape[1]
             self._sample(torch.nn.functional.pad(logits.float(), (0, -vocab % 4)).contiguous(), vocab=vocab)
-            return
-        nxt = torch.argmax(logits, dim=-1, keepdim=True)
-        self.out.index_copy_(1, self.step_index, nxt)
-        self.token.copy_(nxt)
+        else:
+            nxt = torch.argmax(logits, dim=-1, keepdim=True)
+            self.out.index_copy_(1, self.step_index, nxt)
+            self.token.copy_(nxt)
+        self._record(logits, self.step_index)
 
     def _logits(self) -> torch.Tensor:
         """Logits ``[B, V]`` of the token in ``self.token`` at cache row ``cache.position``."""
@@ -632,9 +668,9 @@ class FusedDecoder(GraphDecoder):
 
         return self._layers(prompt, attend, last)
 
-    def _layers(self, tokens: torch.Tensor, attend, last: torch.Tensor | None = None) -> torch.Tensor:
+    def _layers(self, tokens: torch.Tensor, attend, last: torch.Tensor | None = None, every: bool = False) -> torch.Tensor:
         """``tokens`` ``[rows, T]`` through the layer stack on library kernels, ``attend(layer's number, its weights, normed rows)`` for q|k|v and
-        attention; the logits ``[rows, V]`` of the last position, or of position ``last[row]``."""
+        attention; the logits ``[rows, V]`` of the last position, or of position ``last[row]``, or ``[rows * T, V]`` of ``every`` position."""
         lib, st = _lib.load(), _stream()
         rows, seq = tokens.shape
         d, m = self.model.d_model, rows * seq
@@ -657,6 +693,10 @@ class FusedDecoder(GraphDecoder):
                 _lib.check(lib.ajq_swiglu(ab.data_ptr(), gated.data_ptr(), m, self.d_ff, st), "swiglu")
                 del ab
             delta = w["w2"](gated)
+        if every:
+            _lib.check(lib.ajq_add_rmsnorm(hidden.data_ptr(), delta.data_ptr(), self.final_gain.data_ptr(), self.final_eps, normed.data_ptr(), m, d, st),
+                       "add_rmsnorm")
+            return self.head(normed)[:, : self.vocab]
         if last is None:
             last_hidden = hidden.view(rows, seq, d)[:, -1, :].contiguous()
             last_delta = delta.view(rows, seq, -1)[:, -1, :d].contiguous()
@@ -677,12 +717,14 @@ class FusedDecoder(GraphDecoder):
         self._adjusted(full[:, : self.vocab], in_place=True)
         if self.temperature > 0:
             self._sample(full, self.embedding, self.embedded, self.counters, self.ticket, self.vocab)
-            return
-        _lib.check(_lib.load().ajq_greedy_pick(full.data_ptr(), self.batch, self.vocab, full.shape[1],
-                                               self.embedding.data_ptr(), self.model.d_model, self.embedded.data_ptr(),
-                                               self.token.data_ptr(), self.out.data_ptr(), self.out.shape[1],
-                                               self.step_index.data_ptr(), self.counters.data_ptr(),
-                                               self.ticket.data_ptr(), _stream()), "greedy_pick")
+        else:
+            _lib.check(_lib.load().ajq_greedy_pick(full.data_ptr(), self.batch, self.vocab, full.shape[1],
+                                                   self.embedding.data_ptr(), self.model.d_model, self.embedded.data_ptr(),
+                                                   self.token.data_ptr(), self.out.data_ptr(), self.out.shape[1],
+                                                   self.step_index.data_ptr(), self.counters.data_ptr(),
+                                                   self.ticket.data_ptr(), _stream()), "greedy_pick")
+        if self.records is not None:
+            self._record(full[:, : self.vocab], self.step_index - 1)   # (the choice has moved the counters)
 
     @property
     def merge_launch(self) -> bool:
@@ -937,6 +979,170 @@ class SharedPrefixDecoder(FusedDecoder):
                                                 offset=self.step_index).view(self.batch, -1)
 
 
+class DraftDecoder(FusedDecoder):
+    """FusedDecoder that looks at a whole tree of guessed tokens in one pass of the model and keeps the path through it that the model would have chosen itself: a pass
+    produces one token at least, and one more for every guess along that path that was right.  The tokens are the greedy ones, whatever is guessed.
+
+    ``parents`` is the tree (``attention.tree_masks``; node 0 its root, the last token chosen): a list of T parents, the first -1.  A pass is FusedDecoder's prompt path on
+    T tokens a sequence, with ``attention.norm_rope`` and ``attention.tree_attention`` in the attention's place, then ``sampling.token_log_probs`` (the choice behind every node),
+    ``sampling.follow_drafts`` and ``attention.keep_rows``, replayed from a graph.  Sequences go on at paces of their own; the host looks at the tokens after every pass."""
+
+    def __init__(self, model: modeling.TransformerLM, batch: int, max_len: int, parents: list[int], kv_dtype: torch.dtype | None = None) -> None:
+        nodes = len(parents)
+        if nodes < 1 or parents[0] != -1 or not all(0 <= up < t for t, up in enumerate(parents) if t):
+            raise ValueError("parents: -1, then for every node one ahead of it")
+        super().__init__(model, batch, max_len, kv_dtype)
+        self.parents, self.nodes = list(parents), nodes
+        self.tree = torch.tensor(self.parents, device=self.device)
+        self.masks, self.depths = tree_masks(self.tree)
+        # all layers' rows in one tensor, so that one launch moves them; a pass may begin at the last row that counts
+        first = self.cache.keys[0]
+        shape = (len(self.layers), batch, self.kv_heads, max_len + nodes, self.head_dim)
+        self.all_keys, self.all_values = (torch.zeros(shape, dtype=first.dtype, device=self.device) for _ in range(2))
+        self.cache.keys, self.cache.values = list(self.all_keys), list(self.all_values)
+        self.cache.max_len = max_len + nodes
+        self.rows = torch.zeros(batch, dtype=torch.long, device=self.device)      # committed
+        self.counts = torch.zeros(batch, dtype=torch.long, device=self.device)    # nodes that are there: none of a sequence that is done
+        self.drafts = torch.zeros((batch, nodes), dtype=torch.long, device=self.device)
+        # of the last pass: every node's logits [B * T, V] and choice, and the right path's length and tokens
+        self.logits: torch.Tensor | None = None
+        self.scored: TokenLogProbs | None = None
+        self.followed: FollowedDrafts | None = None
+        self._recorded: tuple | None = None        # the same of the graph's
+        self.texts: list[list[int]] = []           # prompts and what has been produced
+        self._ends: list[dict[tuple, list[int]]] = []   # of each text, where its runs of up to LONGEST tokens have ended, the latest last
+        self._indexed: list[int] = []
+
+    def set_sampling(self, temperature: float, top_p: float | None = None, seed: int = 0) -> None:
+        if temperature > 0:
+            raise ValueError("DraftDecoder makes the greedy choice")
+        super().set_sampling(temperature, top_p, seed)
+
+    def set_penalties(self, *args, **kwargs) -> None:
+        raise ValueError("DraftDecoder chooses from the logits as they are")
+
+    def set_log_probs(self, alternatives: int | None = 0) -> None:
+        raise ValueError("DraftDecoder's passes keep nothing beside their tokens")
+
+    @torch.no_grad()
+    def prefill(self, prompt: torch.Tensor, rows_per_pass: int | None = None, fused: bool = True) -> None:
+        super().prefill(prompt, rows_per_pass, fused)
+        self.rows.fill_(prompt.shape[1])
+        self.texts = [ids + new for ids, new in zip(prompt.tolist(), self.token.tolist())]
+        self._ends, self._indexed = [{} for _ in self.texts], [0] * self.batch
+
+    def _attend(self, index: int, w: dict, normed: torch.Tensor) -> torch.Tensor:
+        qkv = w["qkv"](normed)
+        keys, values = self.cache.keys[index], self.cache.values[index]
+        q = norm_rope(qkv[:, :w["qkv"].out_features], w["cos"], w["sin"], keys, values, self.rows, heads=self.heads, tokens=self.nodes,
+                      q_gain=w.get("gq"), k_gain=w.get("gk"), epsilon=w.get("eps_heads", 0.0), counts=self.counts, out_dtype=torch.bfloat16,
+                      depths=self.depths)
+        del qkv
+        return tree_attention(q, keys, values, self.rows, self.masks, counts=self.counts).view(self.batch * self.nodes, -1)
+
+    def _pass(self) -> tuple:
+        """The tree in ``self.drafts`` through the model; its right path's rows stay.  Logits, what they say, and the path."""
+        self.drafts[:, :1].copy_(self.token)
+        logits = self._layers(self.drafts, self._attend, every=True)
+        scored = token_log_probs(logits, top=1)
+        followed = follow_drafts(self.drafts, self.tree, scored.top_ids.view(self.batch, self.nodes), counts=self.counts)
+        keep_rows(self.all_keys, self.all_values, self.rows, followed.path, followed.accepted)
+        last = followed.chosen.gather(1, (followed.accepted - 1).clamp(min=0)[:, None])
+        self.token.copy_(torch.where(followed.accepted[:, None] > 0, last, self.token))
+        self.rows.add_(followed.accepted)
+        return logits, scored, followed
+
+    @torch.no_grad()
+    def check(self, guesses: list[list[int]] | torch.Tensor, going: list[bool] | None = None) -> list[list[int]]:
+        """One pass over ``guesses`` ``[B, T - 1]``, the tokens of nodes 1 .. T - 1, for the sequences that are ``going`` (None: all); the tokens that it has
+        produced, a list a sequence."""
+        if not self.texts:
+            raise ValueError("prefill comes first")
+        going = [True] * self.batch if going is None else list(going)
+        longest = max((len(text) for text, on in zip(self.texts, going) if on), default=0)
+        if longest > self.max_len:
+            raise ValueError("the KV cache is too short for this many tokens")
+        guesses = torch.as_tensor(guesses, dtype=torch.long).reshape(self.batch, -1)
+        if guesses.shape[1] != self.nodes - 1 or len(going) != self.batch or (guesses.numel() and not 0 <= int(guesses.min()) <= int(guesses.max()) < self.vocab):
+            raise ValueError(f"guesses [{self.batch}, {self.nodes - 1}] of tokens in [0, {self.vocab}), and {self.batch} truth values, expected")
+        self.stream.wait_stream(torch.cuda.current_stream(self.device))
+        with torch.cuda.stream(self.stream):
+            self.drafts[:, 1:].copy_(guesses)
+            self.counts.copy_(torch.tensor([self.nodes if on else 0 for on in going]))
+            if self.graph is None:
+                results = self._pass()   # (loads the libraries, sizes the allocator; capture does not execute)
+                self.stream.synchronize()
+                graph = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(graph, stream=self.stream):
+                    self._recorded = self._pass()
+                self.graph = graph
+            else:
+                self.graph.replay()
+                results = self._recorded
+            self.logits, self.scored, self.followed = results
+            both = torch.cat((self.followed.accepted[:, None], self.followed.chosen), dim=1).tolist()
+        produced = [row[1:1 + row[0]] for row in both]
+        for text, new in zip(self.texts, produced):
+            text += new
+        self.produced = min(map(len, self.texts)) - self.prompt_len
+        return produced
+
+    LONGEST, PLACES = 3, 32
+
+    def guess(self) -> list[list[int]]:
+        """Guesses from the texts themselves: behind each node the tokens that have followed its last ``LONGEST`` tokens (or fewer, down to one) at their latest
+        ``PLACES`` places in the text so far, the latest first, the first child the first of them; 0 where there are no more."""
+        children, turn = [0] * self.nodes, [0] * self.nodes   # (turn: a node's number among its siblings)
+        for t, up in enumerate(self.parents[1:], start=1):
+            turn[t] = children[up]
+            children[up] += 1
+        return [self._guess_of(b, children, turn) for b in range(self.batch)]
+
+    def _guess_of(self, b: int, children: list[int], turn: list[int]) -> list[int]:
+        text, ends = self.texts[b], self._ends[b]
+        for end in range(self._indexed[b], len(text)):
+            for n in range(1, min(self.LONGEST, end) + 1):
+                ends.setdefault(tuple(text[end - n:end]), []).append(end)
+        self._indexed[b] = len(text)
+        paths, followers, guesses = [text[-self.LONGEST:]], {}, []
+        for t, up in enumerate(self.parents[1:], start=1):
+            if up not in followers:
+                seen: dict[int, None] = {}
+                for n in range(len(paths[up]), 0, -1):
+                    for end in reversed(ends.get(tuple(paths[up][-n:]), [])[-self.PLACES:]):
+                        seen.setdefault(text[end])
+                    if len(seen) >= children[up]:
+                        break
+                followers[up] = list(seen)
+            token = followers[up][turn[t]] if turn[t] < len(followers[up]) else 0
+            paths.append((paths[up] + [token])[-self.LONGEST:])
+            guesses.append(token)
+        return guesses
+
+    @torch.no_grad()
+    def generate(self, new_tokens: int, eos_token_id: int | None = None, eos_check_every: int = 16, guess=None) -> torch.Tensor:
+        """As ``GraphDecoder.generate``; ``guess()`` gives the guesses ``[B, T - 1]`` of a pass (default: ``self.guess``; ``self.texts`` holds the sequences so far).
+        The host looks at every pass's tokens, so that ``eos_check_every`` has no meaning here."""
+        if self.prompt_len + new_tokens > self.max_len:
+            raise ValueError("the KV cache is too short for this many tokens")
+        guess = guess or self.guess
+
+        def new_of(text: list[int]) -> list[int]:
+            return text[self.prompt_len:self.prompt_len + new_tokens]
+
+        while True:
+            done = [len(new_of(text)) >= new_tokens or eos_token_id in new_of(text) for text in self.texts]
+            if all(done):
+                break
+            self.check(guess(), [not over for over in done])
+        got = [new_of(text) for text in self.texts]
+        length = new_tokens if eos_token_id is None or not all(eos_token_id in new for new in got) else max(new.index(eos_token_id) for new in got) + 1
+        while any(len(new) < length for new in got):   # (rows whose text ended ahead of the others': they go on, as in a batch)
+            self.check(guess(), [len(new) < length for new in got])
+            got = [new_of(text) for text in self.texts]
+        return torch.tensor([new[:length] for new in got], dtype=torch.long, device=self.device).view(self.batch, length)
+
+
 class DenseDecoder(GraphDecoder):
     """GraphDecoder for a ``dense.DenseLM``, whose step is this library's kernels already: the choice of the token
     and the step's two counters are one launch as well (``ajq_greedy_pick`` / ``ajq_sample_pick``), and eight steps make
@@ -979,11 +1185,13 @@ class DenseDecoder(GraphDecoder):
                 1.0 if self.top_p is None else float(self.top_p), self.uniforms.data_ptr(), self.uniforms.shape[0], None, 0, None,
                 self.token.data_ptr(), self.out.data_ptr(), self.out.shape[1], self.step_index.data_ptr(), self.counters.data_ptr(),
                 self.ticket.data_ptr(), None, _stream()), "sample_pick")
-            return
-        _lib.check(_lib.load().ajq_greedy_pick(
-            logits.data_ptr(), self.batch, logits.shape[1], logits.stride(0), None, 0, None, self.token.data_ptr(),
-            self.out.data_ptr(), self.out.shape[1], self.step_index.data_ptr(), self.counters.data_ptr(), self.ticket.data_ptr(),
-            _stream()), "greedy_pick")
+        else:
+            _lib.check(_lib.load().ajq_greedy_pick(
+                logits.data_ptr(), self.batch, logits.shape[1], logits.stride(0), None, 0, None, self.token.data_ptr(),
+                self.out.data_ptr(), self.out.shape[1], self.step_index.data_ptr(), self.counters.data_ptr(), self.ticket.data_ptr(),
+                _stream()), "greedy_pick")
+        if self.records is not None:
+            self._record(logits, self.step_index - 1)   # (the choice has moved the counters)
 
 
 def decoder_for(model: torch.nn.Module, fused: bool = False) -> type[GraphDecoder]:

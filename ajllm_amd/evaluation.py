@@ -18,6 +18,7 @@ import numpy as np
 import torch
 
 from .quant import quantize_model_
+from .sampling import TokenLogProbs, token_log_probs
 
 
 def cross_entropy(logits: torch.Tensor, targets: torch.Tensor) -> torch.Tensor:
@@ -66,6 +67,21 @@ def evaluate_model(model: torch.nn.Module, dataset, batches: int, batch_size: in
         total += float(cross_entropy(model(inputs), targets))
     loss = total / batches
     return {"loss": loss, "perplexity": math.exp(min(loss, 50.0)), "batches": batches}
+
+
+@torch.no_grad()
+def score_tokens(model: torch.nn.Module, tokens: torch.Tensor, alternatives: int = 0) -> TokenLogProbs:
+    """What ``model`` makes of texts ``tokens`` ``[B, T]`` on a ROCm device, token by token: log probability and rank of each token behind the ones ahead of it, the entropy there,
+    and the ``alternatives`` most probable tokens (``sampling.token_log_probs``), ``[B, T - 1]`` each for tokens 1 .. T - 1.  The mean of ``-log_probs`` is
+    ``cross_entropy``'s."""
+    if tokens.dim() != 2 or tokens.shape[1] < 2:
+        raise ValueError("tokens [B, T] with T > 1 expected")
+    batch, length = tokens.shape[0], tokens.shape[1] - 1
+    logits = model(tokens[:, :-1])
+    if logits.dtype not in (torch.float32, torch.bfloat16):
+        logits = logits.float()
+    scored = token_log_probs(logits.reshape(batch * length, -1), tokens[:, 1:].reshape(-1).long().contiguous(), top=alternatives)
+    return TokenLogProbs(*(None if part is None else part.view(batch, length, *part.shape[1:]) for part in scored))
 
 
 @torch.no_grad()

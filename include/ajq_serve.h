@@ -46,6 +46,9 @@ typedef struct {
  * no head of the caches may overlap another.
  * (RMSNorm.forward, src/ajllm/modeling/layers.py:70-74, on each head; RotaryPositionalEmbedding.forward, attention.py:36-60.) */
 int ajqs_norm_rope(const ajqs_norm_rope_args* args, void* stream);
+/* The same for tokens whose positions do not follow each other (a tree's): token t turns by depths[b * depths_ld + t] in t's place (int64; depths_ld 0: one
+ * row for all sequences; NULL: t itself).  Its row is the one it has there, rows[b] + *offset + t. */
+int ajqs_norm_rope_at(const ajqs_norm_rope_args* args, const int64_t* depths, int64_t depths_ld, void* stream);
 
 typedef struct {
   const void *q, *prefix_keys, *prefix_values, *keys, *values;

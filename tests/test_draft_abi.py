@@ -180,3 +180,11 @@ def test_follow_drafts_refuses(memory):
     for change in (dict(batch=0), dict(nodes=0), dict(nodes=4097), dict(tokens_ld=-1), dict(parents_ld=-1), dict(choices_ld=-1), dict(choices_step=-1),
                    dict(batch=2 ** 31 - 1)):
         _refused(call, _filled(struct, memory, **{**base, **change}), -2, "unsupported shape")
+
+
+def test_norm_rope_at_refuses(memory):
+    lib = _lib.load_serve()
+    args = _filled(_lib.NormRopeArgs, memory, ld=512, cache_batch=2048, cache_head=1024, batch=2, tokens=1, heads=4, kv_heads=2, dim=64, max_len=16, table_rows=8, eps=1e-5,
+                   values=memory + 2 ** 20)
+    assert lib.ajqs_norm_rope_at(None, memory, 1, None) == -1
+    assert lib.ajqs_norm_rope_at(ctypes.byref(args), memory, -1, None) == -2 and "stride of the depths" in lib.ajqs_last_error().decode()
