@@ -285,11 +285,25 @@ int ajqt_keep_rows(const ajqt_keep_rows_args* a, void* stream) {
   const long long apart = (long long)(reinterpret_cast<uintptr_t>(a->values) - reinterpret_cast<uintptr_t>(a->keys));
   Dimension dims[] = {{a->layers, a->cache_layer * size}, {a->batch, a->cache_batch * size}, {a->kv_heads, a->cache_head * size}, {2, std::abs(apart)}};
   if (!nested(dims, row * a->max_len)) return fail(AJQ_ERR_SHAPE, "%s: cache heads that overlap cannot be written", what);
-  const long long blocks = 2ll * a->layers * a->batch * a->kv_heads;
-  if (blocks > kMostLanes / 1024 || (double)a->layers * a->batch * a->kv_heads > 1e9) return fail(AJQ_ERR_SHAPE, "%s: %d x %d x %d heads", what, a->layers, a->batch, a->kv_heads);
+  const long long heads = 2ll * a->layers * a->batch * a->kv_heads;
+  // A short list's workgroup takes whole rows while they are four a lane, else a part of them.  A long list's are two a CU: where heads are fewer each takes a part of
+  // the rows, of 128 bytes at least.
+  const int all = (int)row / 16;
+  int columns = 1;
+  if (a->width > kShortList)
+    while (columns * 8 < all && heads * columns < 512) columns *= 2;
+  else
+    while (a->width * all > 4 * 256 * columns) columns *= 2;
+  const int lanes = all / columns, each = (a->width * lanes + 255) / 256;
+  if (heads > kMostLanes / 1024 / columns || (double)a->layers * a->batch * a->kv_heads > 1e9)
+    return fail(AJQ_ERR_SHAPE, "%s: %d x %d x %d heads", what, a->layers, a->batch, a->kv_heads);
   const KeepRows k{a->keys, a->values, int64s(a->rows), int64s(a->index), int64s(a->counts), int64s(a->offset), a->cache_layer, a->cache_batch,
-                   a->cache_head, a->index_ld, a->batch, a->kv_heads, a->max_len, a->width, (int)row, (int)size};
-  hipLaunchKernelGGL(keep_rows_kernel, dim3((unsigned)blocks), dim3(a->width <= 64 ? 256 : 1024), 0, (hipStream_t)stream, k);
+                   a->cache_head, a->index_ld, a->max_len, a->width, (int)row, (int)size, lanes, divide_by(columns), divide_by(a->kv_heads), divide_by(a->batch)};
+  const dim3 grid((unsigned)(heads * columns));
+  if (a->width > kShortList) hipLaunchKernelGGL(keep_rows_kernel, grid, dim3(1024), 0, (hipStream_t)stream, k);
+  else if (each > 2) hipLaunchKernelGGL(keep_path_kernel<4>, grid, dim3(256), 0, (hipStream_t)stream, k);
+  else if (each > 1) hipLaunchKernelGGL(keep_path_kernel<2>, grid, dim3(256), 0, (hipStream_t)stream, k);
+  else hipLaunchKernelGGL(keep_path_kernel<1>, grid, dim3(256), 0, (hipStream_t)stream, k);
   return check_launch(what);
 }
 
