@@ -55,6 +55,7 @@ class GraphDecoder:
         self.prompt_count = torch.zeros(1, dtype=torch.long, device=device)
         # what ``set_log_probs`` asks for: a column a token
         self.records: TokenLogProbs | None = None
+        self.produced = 0
 
     def set_sampling(self, temperature: float, top_p: float | None = None, seed: int = 0) -> None:
         """Choose tokens as the reference's ``sample_next_token`` does (src/ajllm/generation/sampling.py:8-22):
@@ -1055,7 +1056,7 @@ class DraftDecoder(FusedDecoder):
     @torch.no_grad()
     def check(self, guesses: list[list[int]] | torch.Tensor, going: list[bool] | None = None) -> list[list[int]]:
         """One pass over ``guesses`` ``[B, T - 1]``, the tokens of nodes 1 .. T - 1, for the sequences that are ``going`` (None: all); the tokens that it has
-        produced, a list a sequence."""
+        produced, a list a sequence (up to the one behind position ``max_len - 1``: a sequence that has it can't go on)."""
         if not self.texts:
             raise ValueError("prefill comes first")
         going = [True] * self.batch if going is None else list(going)
@@ -1081,7 +1082,7 @@ class DraftDecoder(FusedDecoder):
                 results = self._recorded
             self.logits, self.scored, self.followed = results
             both = torch.cat((self.followed.accepted[:, None], self.followed.chosen), dim=1).tolist()
-        produced = [row[1:1 + row[0]] for row in both]
+        produced = [row[1:1 + min(row[0], max(0, self.max_len + 1 - len(text)))] for row, text in zip(both, self.texts)]
         for text, new in zip(self.texts, produced):
             text += new
         self.produced = min(map(len, self.texts)) - self.prompt_len

@@ -80,7 +80,7 @@ def score_tokens(model: torch.nn.Module, tokens: torch.Tensor, alternatives: int
     logits = model(tokens[:, :-1])
     if logits.dtype not in (torch.float32, torch.bfloat16):
         logits = logits.float()
-    scored = token_log_probs(logits.reshape(batch * length, -1), tokens[:, 1:].reshape(-1).long().contiguous(), top=alternatives)
+    scored = token_log_probs(logits.reshape(batch * length, logits.shape[-1]), tokens[:, 1:].reshape(-1).long().contiguous(), top=alternatives)
     return TokenLogProbs(*(None if part is None else part.view(batch, length, *part.shape[1:]) for part in scored))
 
 

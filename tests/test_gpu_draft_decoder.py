@@ -9,6 +9,8 @@ import torch
 from ajllm_amd import attention, decoding, evaluation, modeling, quantize_model_, sampling
 from tests import draft_plain
 from tests.helpers import errors
+from tests.latent_models import config, random_weights
+from tests.test_gpu_latent import LOGIT_TOL, _build, _tokens
 
 pytestmark = pytest.mark.gpu
 
@@ -134,6 +136,27 @@ def test_generate_gives_the_greedy_tokens(cuda, tree):
     assert torch.equal(again.generate(60, eos_token_id=eos), got[:, :max(first)])
 
 
+def test_checks_end_with_the_cache(cuda):
+    """Where a right path leads past the last position, what is behind it is not produced (no position there is the model's)."""
+    model = _model(cuda, context=40)
+    dec = decoding.DraftDecoder(model, 2, 40, [-1, 0, 1, 2, 3, 4])
+    prompt = _prompt(14, 2, 36)
+    dec.prefill(prompt)                                               # (37 tokens: four positions are left, 36 to 39)
+    while min(map(len, dec.texts)) <= 40:                             # (what the passes say one by one: the model's first choices up to what logits are off by)
+        dec.check([[0] * 5] * 2, [len(text) <= 40 for text in dec.texts])
+    right = [list(text) for text in dec.texts]
+    for text in right:
+        own = _own(model, text[:40])[35:]
+        behind = own.max(-1).values - own.gather(1, torch.tensor(text[36:])[:, None])[:, 0]
+        assert len(text) == 41 and bool((behind <= 2 * LOGITS * own.norm(dim=-1)).all())
+    dec.prefill(prompt)
+    got = dec.check([text[37:] + [0] for text in right])
+    assert [len(new) for new in got] == [4, 4] and dec.texts == right
+    with pytest.raises(ValueError, match="too short"):
+        dec.check([[0] * 5] * 2)
+    assert dec.generate(4).tolist() == [text[36:40] for text in right]
+
+
 def test_guesses_come_from_the_text(cuda):
     dec = decoding.DraftDecoder(_model(cuda), 1, 100, [-1, 0, 1, 0, 3])
     dec.prefill(torch.tensor([[1, 2, 3, 4, 1, 2, 5, 6, 1]]))
@@ -211,6 +234,33 @@ def test_decoders_keep_log_probs(cuda, kind, temperature):
         dec.log_probs(4)
 
 
+def test_dense_decoder_keeps_log_probs(cuda):
+    cfg = config(window=[9, 14, 30], positions=256)
+    model = _build(cfg, random_weights(cfg, 21), cuda, torch.bfloat16)
+    prompts = torch.tensor([_tokens(cfg, 37, 40 + i) for i in range(3)], device=cuda)
+    dec = decoding.DenseDecoder(model, 3, 80)
+    dec.prefill(prompts)
+    plain = dec.generate(30)
+    dec.set_log_probs(4)
+    with pytest.raises(ValueError, match="31 of 30"):
+        dec.log_probs(31)
+    dec.prefill(prompts)
+    assert torch.equal(dec.generate(30), plain)
+    kept, cache = dec.log_probs(30), model.new_cache(3, 80)
+    logits = model(prompts, cache, last_token_only=True)[:, -1]
+    noise = 4 * LOGIT_TOL[torch.bfloat16]                             # (of a logit, test_gpu_latent.py; the logarithm of the sum moves by as much at most)
+    for step in range(30):
+        want = torch.log_softmax(logits.double(), dim=-1)
+        for mine, theirs in ((kept.log_probs[:, step, None], want.gather(1, plain[:, step, None])), (kept.top_log_probs[:, step], want.gather(1, kept.top_ids[:, step]))):
+            assert bool(((mine.double() - theirs).abs() <= 2 * noise).all()), step
+        logits = model(plain[:, step:step + 1], cache)[:, -1]
+    assert bool((kept.ranks == 0).all()) and torch.equal(kept.top_ids[:, :, 0], plain)
+    for fresh in (decoding.DenseDecoder(model, 1, 40), decoding.GraphDecoder(_model(cuda), 1, 40)):
+        fresh.set_log_probs()
+        with pytest.raises(ValueError, match="1 of 0"):
+            fresh.log_probs(1)
+
+
 def test_scored_texts(cuda):
     model = _model(cuda)
     tokens = _prompt(11, 3, 50).to(cuda)
@@ -223,6 +273,7 @@ def test_scored_texts(cuda):
     assert torch.equal(scored.top_ids[..., 0], logits.argmax(-1))
     with pytest.raises(ValueError, match="tokens"):
         evaluation.score_tokens(model, tokens[:, :1])
+    assert evaluation.score_tokens(model, tokens[:0], alternatives=3).top_ids.shape == (0, 49, 3)
 
 
 # ------------------------------------------------------------------ the operators of a step in turn, captured
