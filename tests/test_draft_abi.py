@@ -134,6 +134,18 @@ def test_tree_attention_refuses(memory):
     _refused(call, _filled(struct, memory, **{**TREE, "cache_head": -1024}), -2, "negative", *more)
 
 
+def test_tree_attention_refuses_workspaces_and_large_launches(memory):
+    lib = _lib.load_draft()
+    args = _filled(_lib.TreeAttentionArgs, memory, **{**TREE, "batch": 1, "max_len": 20000, "cache_dtype": 1})   # (long and alone: in parts)
+    size = lib.ajqt_tree_attention_workspace(ctypes.byref(args))
+    assert size > 0
+    call = lib.ajqt_tree_attention
+    for room, given in ((None, 0), (None, size), (memory, 0), (memory, size - 1)):
+        _refused(call, args, -6, "workspace of", room, given)
+    _refused(call, args, -3, "16-byte aligned", memory + 8, size)
+    _refused(call, _filled(_lib.TreeAttentionArgs, memory, **{**TREE, "batch": 2 ** 28, "tokens": 1, "heads": 1, "kv_heads": 1}), -2, "too many tiles", memory, 4096)
+
+
 KEEP = dict(cache_layer=4096, cache_batch=2048, cache_head=1024, index_ld=5, layers=2, batch=2, kv_heads=2, dim=64, max_len=16, width=5)
 
 
@@ -169,6 +181,19 @@ def test_log_probs_refuses(memory):
     _refused(call, _filled(struct, memory, **{**PROBS, "dtype": 2}), -4, "element type", *more)
     for change in (dict(logits=memory + 2), dict(logits=memory + 1, dtype=1), dict(log_probs=memory + 2), dict(entropy=memory + 1), dict(top_log_probs=memory + 2)):
         _refused(call, _filled(struct, memory, **{**PROBS, **change}), -3, "aligned", *more)
+
+
+def test_log_probs_refuses_workspaces_and_large_launches(memory):
+    lib = _lib.load_draft()
+    for dtype, top in ((0, 0), (0, 64), (1, 5)):
+        args = _filled(_lib.LogProbsArgs, memory, **{**PROBS, "vocab": 200000, "ld": 200000, "top": top, "dtype": dtype})
+        size = lib.ajqt_log_probs_workspace(ctypes.byref(args))
+        assert size > 0
+        for room, given in ((None, 0), (None, size), (memory, 0), (memory, size - 1)):
+            _refused(lib.ajqt_log_probs, args, -6, "workspace of", room, given)
+        _refused(lib.ajqt_log_probs, args, -3, "16-byte aligned", memory + 8, size)
+    for change in (dict(rows=2 ** 24 + 1), dict(rows=2 ** 23, vocab=40000, ld=40000)):
+        _refused(lib.ajqt_log_probs, _filled(_lib.LogProbsArgs, memory, **{**PROBS, **change}), -2, "rows", memory, 4096)
 
 
 def test_follow_drafts_refuses(memory):

@@ -123,6 +123,17 @@ def test_tree_attention_parts_and_tiles(cuda, batch, nodes, heads, kv, max_len, 
 
 
 @pytest.mark.parametrize("cache_type", [F32, BF16])
+@pytest.mark.parametrize("nodes,heads", [(3, 2), (40, 4), (90, 4)])
+def test_tree_attention_parts_of_odd_sequences(cuda, nodes, heads, cache_type):
+    """Rows in parts, dealt out to sequences that begin outside their caches, have no tokens, one row, or all of them; and one sequence alone."""
+    rows = [-2, -2 ** 40, 6000 - 2, 6000, 2 ** 40, 0, 5000, 1]
+    for counts in (None, [nodes, 2, nodes, 2, 1, 1, -5, 2 ** 40], [0] * 8, [0, 0, 0, 0, 0, 0, 0, 1]):
+        _attend(cuda, 8, nodes, heads, 1, 64, 6000, F32, cache_type, seed=9, rows=rows, counts=counts, ragged=False, garbage=False)
+    for alone in rows:
+        _attend(cuda, 1, nodes, heads, 1, 128, 6000, BF16, cache_type, seed=10, rows=[alone], ragged=False, garbage=False)
+
+
+@pytest.mark.parametrize("cache_type", [F32, BF16])
 @pytest.mark.parametrize("nodes", [4, 40])
 def test_tree_attention_scores_far_apart(cuda, nodes, cache_type):
     """Scores of hundreds: maxima move between blocks, most weights vanish.  (The queries are whole numbers that bf16 holds, and so are the keys: products are exact,
@@ -386,6 +397,21 @@ def test_log_probs_order_of_equal_logits(cuda, vocab, top):
         got = _score(cuda, x, targets, top)
         among = got.ranks < top
         assert torch.equal(got.top_ids.gather(1, got.ranks.clamp(max=top - 1)[:, None])[:, 0][among].cpu(), targets[among.cpu()])
+
+
+def test_log_probs_rows_that_are_hard_to_order(cuda):
+    """More tokens that may be among the first than there is room for: of a slice (whole groups of lanes above the border), of many slices (one of them far below the
+    others, or with next to nothing in it)."""
+    at = torch.arange(8192) // 4 % 128
+    one = torch.where(at < 63, 2.0, torch.where(at == 63, 1.0, 0.0)) + torch.linspace(0, 0.5, 8192)
+    _score(cuda, torch.stack((one, one.flip(0))), torch.tensor([5, 8000]), 64)
+    _score(cuda, torch.cat((one, one))[None].bfloat16(), torch.tensor([9000]), 64)
+    for last in (8192, 6000, 1):
+        many = torch.randn(1, 47 * 8192 + last, generator=_gen(last))
+        many[:, 46 * 8192:] -= 100.0
+        for top in (64, 63):
+            _score(cuda, many, torch.tensor([46 * 8192 + 3]), top)
+            _score(cuda, many.flip(1).contiguous(), torch.tensor([12]), top)
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
