@@ -316,8 +316,9 @@ __global__ __launch_bounds__(LANES, 8) void log_probs_kernel(LogProbs a) {
   }
 }
 
-// ---- a row's slices put together, a workgroup a row.  With S slices, the least of the tokens in place ceil(top / S) of theirs is a border that `top` tokens reach;
-// those that do (twice as many or so) gather, and each counts the ones ahead of itself.
+// ---- a row's slices put together, a workgroup a row.  With S slices, the least of the tokens in place ceil(top / S) of theirs is a border that `top` tokens reach,
+// and so is the first of those in place `top`; the tokens that reach both (twice as many or so; the second keeps out what a mask has left nothing of) gather, and each
+// counts the ones ahead of itself.
 constexpr int kMergeKeys = 2048;
 __global__ __launch_bounds__(256) void log_probs_merge_kernel(LogProbs a) {
   __shared__ __attribute__((aligned(16))) unsigned long long keys[kMergeKeys];
@@ -331,13 +332,14 @@ __global__ __launch_bounds__(256) void log_probs_merge_kernel(LogProbs a) {
   const float mine = a.targets ? a.mine[r] : 0.f;
   // (every wave the same)
   float top = -INFINITY;
-  unsigned long long least = ~0ull;
+  unsigned long long least = ~0ull, first_of_last = 0ull;
   const int place_of_all = (a.top + a.slices - 1) / a.slices - 1;
   for (int n = lane; n < a.slices; n += 64) {
     top = fmaxf(top, parts[n][0]);
     if (a.top) {
       const unsigned long long key = from[n * a.top + place_of_all];
       least = key < least ? key : least;
+      first_of_last = larger(first_of_last, from[n * a.top + a.top - 1]);
     }
   }
   top = wave_most(top);
@@ -364,7 +366,9 @@ __global__ __launch_bounds__(256) void log_probs_merge_kernel(LogProbs a) {
   for (int n = 32; n > 0; n >>= 1) {
     const unsigned long long other = __shfl_xor(least, n);
     least = other < least ? other : least;
+    first_of_last = larger(first_of_last, __shfl_xor(first_of_last, n));
   }
+  least = larger(least, first_of_last);
   auto leave = [&](int place, unsigned long long key) {
     if (place >= a.top) return;
     a.top_ids[(size_t)r * a.top + place] = id_of(key);

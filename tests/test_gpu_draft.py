@@ -406,6 +406,12 @@ def test_log_probs_rows_that_are_hard_to_order(cuda):
     one = torch.where(at < 63, 2.0, torch.where(at == 63, 1.0, 0.0)) + torch.linspace(0, 0.5, 8192)
     _score(cuda, torch.stack((one, one.flip(0))), torch.tensor([5, 8000]), 64)
     _score(cuda, torch.cat((one, one))[None].bfloat16(), torch.tensor([9000]), 64)
+    wide = torch.randn(5, 128256, generator=_gen(2))
+    keep = torch.rand((5, 128256), generator=_gen(3)) < torch.tensor([0.0, 3e-4, 3e-3, 1e-2, 1e-5])[:, None]
+    keep[3, 40000:90000] = False
+    for top in (64, 20, 1):   # (a mask leaves a slice fewer tokens than that, or none)
+        _score(cuda, wide.masked_fill(~keep, -math.inf), torch.tensor([7, 0, 128255, 50000, 3]), top)
+        _score(cuda, wide.masked_fill(~keep, -math.inf).bfloat16(), None, top)
     for last in (8192, 6000, 1):
         many = torch.randn(1, 47 * 8192 + last, generator=_gen(last))
         many[:, 46 * 8192:] -= 100.0
