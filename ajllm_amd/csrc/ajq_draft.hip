@@ -30,7 +30,7 @@ int check_tree(const ajqt_tree_attention_args* a) {
 
 // How a call is cut up: tiles of a sequence's queries of a key head, parts of its rows.  The lengths are on the device: max_len is what they can be.
 struct TreePlan {
-  bool walk;     // tiles of 16 rt queries a wave, by meet_many; else of 16 rt, by meet_few
+  bool walk;     // tiles of 16 rt queries a wave, by meet_many or (fp32 caches) tree_attention_laid_kernel; else of 16 rt, by meet_few
   int rt, waves, tiles;
   int runs;      // 0: every sequence's rows are one part
   long long blocks, queries;
@@ -45,22 +45,24 @@ constexpr int kMostParts = 64;      // of a sequence: a lane each in the merge
 // (geometric mean) than the fastest of what was tried.  Where the ways part, for instance (us; heads / key heads x size, tokens, rows): 32 / 8 x 128, 1 x 8 behind 500: tiles of 16
 // in one launch 6.3, of 32 9.1, in seven parts 7.2; 6 x 32 behind 2000: tiles of 32 and eight waves in one launch 18.5, four waves in 16 runs 22.0; 6 x 32 behind 12000: in 16
 // runs 56.7, eight waves in one launch 2.2 times that; 8 x 64 behind 32768: tiles of 256 of eight waves in 28 runs 254, of 128 of four 324.
+// fp32 rows laid down once: 1881 calls to 10 %; what is chosen with them takes 4 % longer than the fastest of 350 calls' ways.
 struct TreeCost {
   float start, per_waves, per_tiles, step, step_dim, step_tiles, crowd, memory, merge, merge_bytes, l2;
 };
 constexpr TreeCost kFewBf16{3.854f, 0.596f, 1.229f, 0.249f, 0.54f, 0.36f, 0.319f, 6.172f, 2.349f, 0.709f, 47.1f};
 constexpr TreeCost kWalkBf16{6.769f, 1.665f, 2.713f, 0.295f, 0.418f, 0.215f, 0.433f, 5.035f, 2.249f, 0.404f, 18.64f};
+constexpr TreeCost kLaidF32{4.405f, 0.f, 1.314f, 0.29f, 0.948f, 0.563f, 0.222f, 6.547f, 2.973f, 0.619f, 46.78f};
 constexpr TreeCost kFewF32{3.243f, 0.f, 1.392f, 0.156f, 3.167f, 0.f, 0.63f, 5.781f, 3.079f, 0.922f, 39.38f};
 float tree_cost(const ajqt_tree_attention_args* a, const TreePlan& p) {
   const bool bf16 = a->cache_dtype == AJQS_BF16;
-  const TreeCost& c = p.walk ? kWalkBf16 : bf16 ? kFewBf16 : kFewF32;
+  const TreeCost& c = p.walk ? (bf16 ? kWalkBf16 : kLaidF32) : bf16 ? kFewBf16 : kFewF32;
   const float dim = (float)a->dim / 128.f, batch = (float)a->batch, waves = (float)p.waves, kv = (float)a->kv_heads;
   // rows: of the longest sequence all (one run is one workgroup's), of several three quarters on average
   const float longest = (float)a->max_len, mean = a->batch == 1 ? longest : 0.75f * longest;
   const float rows = !p.runs ? longest : a->batch == 1 ? longest / (float)p.runs : batch * mean / ((float)p.runs - 0.5f * batch);
-  const float steps = ceilf(p.walk ? rows / 64.f : rows / (32.f * waves));
+  const float steps = ceilf(!p.walk ? rows / (32.f * waves) : bf16 ? rows / 64.f : rows / 32.f);
   const float workgroups = (p.runs ? (float)p.runs : batch) * kv * (float)p.tiles;
-  const float at_once = (!bf16 && p.rt == 2 ? 4.f : 8.f) / dim;   // waves a CU, by registers and LDS
+  const float at_once = (!bf16 && !p.walk && p.rt == 2 ? 4.f : 8.f) / dim;   // waves a CU, by registers and LDS
   const float rounds = fmaxf(1.f, workgroups * waves / (256.f * at_once)), crowd = fmaxf(1.f, fminf(ceilf(workgroups / 256.f) * waves, at_once) / 4.f);
   const float work = rounds * steps * (c.step + (c.step_dim + c.step_tiles * (float)(p.rt - 1)) * dim) * (1.f + c.crowd * (crowd - 1.f));
   const float megabytes = batch * kv * mean * 2.f * (float)a->dim * (bf16 ? 2e-6f : 4e-6f);
@@ -74,12 +76,13 @@ TreePlan plan_tree(const ajqt_tree_attention_args* a) {
   const bool bf16 = a->cache_dtype == AJQS_BF16;
   TreePlan best{};
   float least = INFINITY;
-  for (int walk = 0; walk <= (bf16 && mine > 64); ++walk) {
+  for (int walk = 0; walk <= (mine > (bf16 ? 64 : 16)); ++walk) {
     if (!walk && bf16 && mine > 256) continue;
     for (int rt = 1; rt <= 2; ++rt) {
-      if (walk ? rt == 2 && !(a->q_dtype == AJQS_BF16 && a->dim == 128) : rt == 2 && mine <= 16) continue;   // (what is not built, or has nothing to do)
+      // (what is not built, or has nothing to do)
+      if (!walk ? rt == 2 && mine <= 16 : rt == 2 && (bf16 ? a->q_dtype != AJQS_BF16 || a->dim != 128 : mine <= 64)) continue;
       for (int waves = 4; waves <= 8; waves += 4) {
-        if (waves == 8 && (walk ? a->dim < 64 || mine <= 64 * rt : !bf16 && rt == 2 && a->dim == 128)) continue;
+        if (waves == 8 && (walk ? !bf16 || a->dim < 64 || mine <= 64 * rt : !bf16 && rt == 2 && a->dim == 128)) continue;
         TreePlan p{};
         p.walk = walk != 0;
         p.rt = rt;
@@ -90,6 +93,7 @@ TreePlan plan_tree(const ajqt_tree_attention_args* a) {
         for (int n = 0; n < 4; ++n) {
           p.runs = (int)std::min(most, n == 0 ? 0 : n == 1 ? round / 2 : n == 2 ? round : 2 * round);
           if (n && (p.runs <= a->batch || a->batch > kMostDealt)) continue;
+          if (n && !bf16 && !walk && rt == 2 && waves == 4) continue;   // (parts of fp32 rows for so many queries: laid down once they take less, or eight waves do)
           const float cost = tree_cost(a, p);
           if (cost < least) {
             least = cost;
@@ -239,6 +243,15 @@ int ajqt_tree_attention(const ajqt_tree_attention_args* a, void* workspace, size
           hipLaunchKernelGGL(tree_attention_merge_kernel<HD>, dim3((unsigned)ceil_div(p.queries, 4)), dim3(256), 0, (hipStream_t)stream, s);
           status = check_launch(what);
         };
+        if constexpr (sizeof(CacheT) == 4) {
+          if (p.walk) {
+            auto laid = [&](auto tiles) {
+              constexpr int RT = decltype(tiles)::value, lds = laid_lds_bytes<HD>();
+              p.runs ? launch(tree_attention_laid_kernel<HD, QT, RT, false>, lds) : launch(tree_attention_laid_kernel<HD, QT, RT, true>, lds);
+            };
+            return p.rt == 2 ? laid(Size<2>{}) : laid(Size<1>{});
+          }
+        }
         if constexpr (sizeof(CacheT) == 2) {
           if (p.walk) {
             auto walk = [&](auto tiles) {
@@ -256,7 +269,10 @@ int ajqt_tree_attention(const ajqt_tree_attention_args* a, void* workspace, size
         }
         auto few = [&](auto tiles, auto waves) {
           constexpr int RT = decltype(tiles)::value, WV = decltype(waves)::value, lds = some_lds_bytes<HD, CacheT, RT, WV>();
-          p.runs ? launch(tree_attention_few_kernel<HD, QT, CacheT, RT, WV, false>, lds) : launch(tree_attention_few_kernel<HD, QT, CacheT, RT, WV, true>, lds);
+          if constexpr (sizeof(CacheT) == 2 || RT == 1 || WV == 8) {
+            if (p.runs) return launch(tree_attention_few_kernel<HD, QT, CacheT, RT, WV, false>, lds);
+          }
+          launch(tree_attention_few_kernel<HD, QT, CacheT, RT, WV, true>, lds);
         };
         if constexpr (sizeof(CacheT) == 2 || HD < 128) {
           if (p.rt == 2 && p.waves == 8) return few(Size<2>{}, Size<8>{});
