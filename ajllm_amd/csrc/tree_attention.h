@@ -141,7 +141,7 @@ __global__ __launch_bounds__(64 * WV, sizeof(CacheT) == 4 && RT == 2 && WV == 4 
 // stages of LDS (one barrier a block), while the next block's are on their way.  Products as there: scores of three (bf16 queries: two), results of two.
 // Fp32 queries, us (by meet_few's best form): 7 x 69 of 32 heads of 128 behind up to 112 rows 18 (38); 7 x 100 behind 1000 64 (119); 8 x 64 of 32 / 8 behind 8000 159 (372), in 64
 // parts; 12 x 25 of 12 heads of 64 behind 1500 22.6 (22.8).  350 calls with more than 16 queries a key head: 24 % less than without it if the faster is taken, 19 % as chosen.
-// Bound by a wave's own work still: 80 MFMAs of 16 cycles, 64 pieces of 16 bytes from LDS and some 300 vector instructions a block, nothing of one block beside another's.
+// Bound by a wave's own work still: 80 MFMAs of 16 cycles, 64 pieces of 16 bytes from LDS and some 400 vector instructions a block, nothing of one block beside another's.
 template <int HD> constexpr int laid_lds_bytes() { return 2 * 4 * 32 * 2 * HD; }   // stages; keys and values, each in halves
 template <int HD, typename QT, int RT, bool kWhole>
 __global__ __launch_bounds__(256, 2) void tree_attention_laid_kernel(TreeAttention a) {
