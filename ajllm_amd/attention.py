@@ -316,6 +316,8 @@ def keep_rows(keys: torch.Tensor, values: torch.Tensor, rows: torch.Tensor, inde
         raise ValueError("keep_rows: index int64 [B, n] or [n] on the device of the others expected")
     if 0 in keys.shape or index.shape[-1] == 0:
         return
+    if max(*keys.shape, index.shape[-1]) >= 2 ** 31:
+        raise ValueError("keep_rows: dimensions below 2^31 expected")
     args = _lib.KeepRowsArgs(
         keys.data_ptr(), values.data_ptr(), rows.data_ptr(), index.data_ptr(), _pointer(counts), _pointer(offset), apart, first_keys.stride(0),
         first_keys.stride(1), index.stride(0) if index.dim() == 2 else 0, layers, batch, kv_heads, hd, max_len, index.shape[-1], _TYPES[keys.dtype])

@@ -189,6 +189,8 @@ def follow_drafts(tokens: torch.Tensor, parents: torch.Tensor, choices: torch.Te
     if tokens.dim() != 2 or tokens.dtype != torch.int64 or (tokens.shape[1] > 1 and tokens.stride(1) != 1):
         raise ValueError("follow_drafts: tokens int64 [B, T] expected")
     batch, nodes = tokens.shape
+    if batch >= 2 ** 31:
+        raise ValueError("follow_drafts: fewer than 2^31 trees expected")
     if parents.dtype != torch.int64 or tuple(parents.shape) not in ((nodes,), (batch, nodes)) or parents.device != device or (nodes > 1 and parents.stride(-1) != 1):
         raise ValueError("follow_drafts: parents int64 [T] or [B, T] on the device of the tokens expected")
     if choices.dtype != torch.int64 or choices.shape != tokens.shape or choices.device != device:

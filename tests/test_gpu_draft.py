@@ -550,4 +550,10 @@ def test_follow_drafts_refuses(cuda):
         call(tokens, tokens, tokens, counts=torch.zeros(3, dtype=torch.long, device=cuda))
     with pytest.raises(ValueError, match="unsupported shape"):
         call(torch.zeros(1, 4097, dtype=torch.long, device=cuda), torch.zeros(4097, dtype=torch.long, device=cuda), torch.zeros(1, 4097, dtype=torch.long, device=cuda))
+    many = tokens[:1, :1].expand(2 ** 32 + 5, 1)
+    with pytest.raises(ValueError, match="2\\^31 trees"):
+        call(many, tokens[0, :1], many)
+    with pytest.raises(ValueError, match="dimensions below"):
+        cache = torch.zeros(1, 1, 4, 64, device=cuda)
+        attention.keep_rows(cache.expand(2 ** 32 + 5, 1, 1, 4, 64), cache.clone().expand(2 ** 32 + 5, 1, 1, 4, 64), tokens[0, :1], tokens[:1])
     assert call(tokens[:0], tokens[0], tokens[:0]).accepted.shape == (0,)
