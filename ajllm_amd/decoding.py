@@ -55,6 +55,7 @@ class GraphDecoder:
         self.prompt_count = torch.zeros(1, dtype=torch.long, device=device)
         # what ``set_log_probs`` asks for: a column a token
         self.records: TokenLogProbs | None = None
+        self.unrecorded = 0   # tokens since ``prefill`` that were there ahead of it
         self.produced = 0
 
     def set_sampling(self, temperature: float, top_p: float | None = None, seed: int = 0) -> None:
@@ -110,10 +111,11 @@ class GraphDecoder:
     def set_log_probs(self, alternatives: int | None = 0) -> None:
         """Keep, beside every token that is produced, its log probability, its rank and the entropy, and the ``alternatives`` most probable tokens
         (``sampling.token_log_probs``) under the logits that it was chosen from: as ``set_penalties`` left them, at a temperature of 1.  ``log_probs`` gives what
-        has been kept.  Call it before ``prefill``; graphs recorded so far are dropped.  None: keep nothing any more."""
+        has been kept.  Call it before ``prefill`` (of tokens that are there already nothing is known, and ``log_probs`` refuses them); graphs recorded so far are
+        dropped.  None: keep nothing any more."""
         if alternatives is not None and not 0 <= alternatives <= min(MOST_TOP, self.model.vocab_size):
             raise ValueError(f"alternatives must be in [0, {min(MOST_TOP, self.model.vocab_size)}]")
-        self.records = None
+        self.records, self.unrecorded = None, self.produced
         if alternatives is not None:
             shape = (self.batch, self.out.shape[1])
             floats = lambda *s: torch.zeros(s, dtype=torch.float32, device=self.device)  # noqa: E731
@@ -128,6 +130,8 @@ class GraphDecoder:
             raise ValueError("set_log_probs says what to keep")
         if not 0 <= new_tokens <= self.produced:
             raise ValueError(f"{new_tokens} of {self.produced} tokens")
+        if new_tokens and self.unrecorded:
+            raise ValueError(f"the first {self.unrecorded} tokens were produced ahead of set_log_probs")
         return TokenLogProbs(*(None if kept is None else kept[:, :new_tokens].clone() for kept in self.records))
 
     def _record(self, logits: torch.Tensor, column: torch.Tensor) -> None:
@@ -215,7 +219,7 @@ class GraphDecoder:
         self.step_index.zero_()
         self._choose(logits)
         self.step_index.add_(1)
-        self.produced = 1
+        self.produced, self.unrecorded = 1, 0
         self.prompt_len = prompt_len
 
     def _all_rows_done(self, eos_token_id: int) -> int | None:

@@ -1,0 +1,41 @@
+"""What decoders of drafted tokens and of log probabilities hold: rows, texts and records that belong together, whatever call comes first or fails."""
+
+import pytest
+import torch
+
+from ajllm_amd import decoding
+from tests.latent_models import config, random_weights
+from tests.test_gpu_draft_decoder import _model, _prompt
+from tests.test_gpu_latent import _build, _tokens
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("kind", ["graph", "fused", "shared", "dense"])
+def test_log_probs_of_tokens_that_were_not_kept_are_refused(cuda, kind):
+    """Tokens produced ahead of set_log_probs have no log probability to give; those of the next prompt have."""
+    if kind == "dense":
+        cfg = config(window=[9, 14, 30], positions=256)
+        dec = decoding.DenseDecoder(_build(cfg, random_weights(cfg, 21), cuda, torch.bfloat16), 2, 80)
+        prompt = torch.tensor([_tokens(cfg, 12, 40 + i) for i in range(2)], device=cuda)
+    else:
+        model, prompt = _model(cuda), _prompt(9, 2, 12)
+        dec = (decoding.SharedPrefixDecoder(model, 2, 1, 16, 40) if kind == "shared"
+               else (decoding.GraphDecoder if kind == "graph" else decoding.FusedDecoder)(model, 2, 64))
+    dec.prefill(prompt)
+    dec.generate(6)
+    dec.set_log_probs(2)
+    assert dec.log_probs(0).log_probs.shape == (2, 0)
+    for many in (1, 6):
+        with pytest.raises(ValueError, match="the first 6 tokens were produced ahead of set_log_probs"):
+            dec.log_probs(many)
+    dec.generate(10)
+    with pytest.raises(ValueError, match="the first 6 tokens"):
+        dec.log_probs(10)
+    dec.set_log_probs()
+    with pytest.raises(ValueError, match="the first 10 tokens"):
+        dec.log_probs(10)
+    dec.prefill(prompt)
+    dec.generate(10)
+    kept = dec.log_probs(10)
+    assert bool((kept.log_probs < 0).all()) and bool((kept.ranks == 0).all()) and bool((kept.entropy > 0).all())
