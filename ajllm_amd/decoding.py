@@ -33,7 +33,7 @@ class GraphDecoder:
         if device.type != "cuda":
             raise ValueError("GraphDecoder needs the model on a ROCm device")
         self.device = device
-        self.cache = model.new_cache(batch, max_len, dtype=kv_dtype)
+        self.cache = self._new_cache(kv_dtype)
         self.token = torch.zeros((batch, 1), dtype=torch.long, device=device)
         self.out = torch.zeros((batch, max_len), dtype=torch.long, device=device)
         self.step_index = torch.zeros(1, dtype=torch.long, device=device)
@@ -57,6 +57,9 @@ class GraphDecoder:
         self.records: TokenLogProbs | None = None
         self.unrecorded = 0   # tokens since ``prefill`` that were there ahead of it
         self.produced = 0
+
+    def _new_cache(self, kv_dtype: torch.dtype | None):
+        return self.model.new_cache(self.batch, self.max_len, dtype=kv_dtype)
 
     def set_sampling(self, temperature: float, top_p: float | None = None, seed: int = 0) -> None:
         """Choose tokens as the reference's ``sample_next_token`` does (src/ajllm/generation/sampling.py:8-22):
@@ -996,16 +999,10 @@ class DraftDecoder(FusedDecoder):
         nodes = len(parents)
         if nodes < 1 or parents[0] != -1 or not all(0 <= up < t for t, up in enumerate(parents) if t):
             raise ValueError("parents: -1, then for every node one ahead of it")
-        super().__init__(model, batch, max_len, kv_dtype)
         self.parents, self.nodes = list(parents), nodes
+        super().__init__(model, batch, max_len, kv_dtype)
         self.tree = torch.tensor(self.parents, device=self.device)
         self.masks, self.depths = tree_masks(self.tree)
-        # all layers' rows in one tensor, so that one launch moves them; a pass may begin at the last row that counts
-        first = self.cache.keys[0]
-        shape = (len(self.layers), batch, self.kv_heads, max_len + nodes, self.head_dim)
-        self.all_keys, self.all_values = (torch.zeros(shape, dtype=first.dtype, device=self.device) for _ in range(2))
-        self.cache.keys, self.cache.values = list(self.all_keys), list(self.all_values)
-        self.cache.max_len = max_len + nodes
         self.rows = torch.zeros(batch, dtype=torch.long, device=self.device)      # committed
         self.counts = torch.zeros(batch, dtype=torch.long, device=self.device)    # nodes that are there: none of a sequence that is done
         self.drafts = torch.zeros((batch, nodes), dtype=torch.long, device=self.device)
@@ -1017,6 +1014,16 @@ class DraftDecoder(FusedDecoder):
         self.texts: list[list[int]] = []           # prompts and what has been produced
         self._ends: list[dict[tuple, list[int]]] = []   # of each text, where its runs of up to LONGEST tokens have ended, the latest last
         self._indexed: list[int] = []
+
+    def _new_cache(self, kv_dtype: torch.dtype | None) -> modeling.KVCache:
+        """All layers' rows in one tensor, so that one launch moves them; a pass may begin at the last row that counts."""
+        model, max_len = self.model, self.max_len + self.nodes
+        dtype, head_dim = kv_dtype or model.token_embeddings.weight.dtype, model.d_model // model.num_heads
+        self.all_keys, self.all_values = (torch.zeros((model.num_layers, self.batch, model.num_kv_heads, max_len, head_dim), dtype=dtype, device=self.device)
+                                          for _ in range(2))
+        cache = modeling.KVCache(0, self.batch, model.num_kv_heads, max_len, head_dim, self.device, dtype)   # (without rows of its own)
+        cache.keys, cache.values = list(self.all_keys), list(self.all_values)
+        return cache
 
     def set_sampling(self, temperature: float, top_p: float | None = None, seed: int = 0) -> None:
         if temperature > 0:

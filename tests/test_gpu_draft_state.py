@@ -39,3 +39,18 @@ def test_log_probs_of_tokens_that_were_not_kept_are_refused(cuda, kind):
     dec.generate(10)
     kept = dec.log_probs(10)
     assert bool((kept.log_probs < 0).all()) and bool((kept.ranks == 0).all()) and bool((kept.entropy > 0).all())
+
+
+def test_draft_decoder_takes_its_caches_once(cuda):
+    """Never more than its own caches and little beside them, while it is made as afterwards."""
+    model = _model(cuda, context=4096)
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    torch.cuda.reset_peak_memory_stats()
+    before, reserved = torch.cuda.memory_allocated(), torch.cuda.memory_reserved()
+    dec = decoding.DraftDecoder(model, 64, 4000, [-1, 0, 1])
+    caches = dec.all_keys.nbytes + dec.all_values.nbytes
+    assert caches == 2 * 2 * 64 * 2 * 4003 * 64 * 4                    # (layers, keys and values; 524 MB)
+    assert torch.cuda.max_memory_allocated() - before < 1.2 * caches
+    assert torch.cuda.memory_reserved() - reserved < 1.2 * caches
+    assert [k.data_ptr() for k in dec.cache.keys] == [k.data_ptr() for k in dec.all_keys] and dec.cache.max_len == dec.cache.keys[0].shape[2] == len(dec.cache.slots)
