@@ -1011,6 +1011,7 @@ class DraftDecoder(FusedDecoder):
         self.scored: TokenLogProbs | None = None
         self.followed: FollowedDrafts | None = None
         self._recorded: tuple | None = None        # the same of the graph's
+        self._passed = False                       # whether there has been a pass: the next one is recorded
         self.texts: list[list[int]] = []           # prompts and what has been produced
         self._ends: list[dict[tuple, list[int]]] = []   # of each text, where its runs of up to LONGEST tokens have ended, the latest last
         self._indexed: list[int] = []
@@ -1081,14 +1082,16 @@ class DraftDecoder(FusedDecoder):
         with torch.cuda.stream(self.stream):
             self.drafts[:, 1:].copy_(guesses)
             self.counts.copy_(torch.tensor([self.nodes if on else 0 for on in going]))
-            if self.graph is None:
-                results = self._pass()   # (loads the libraries, sizes the allocator; capture does not execute)
-                self.stream.synchronize()
-                graph = torch.cuda.CUDAGraph()
-                with torch.cuda.graph(graph, stream=self.stream):
-                    self._recorded = self._pass()
-                self.graph = graph
+            if not self._passed:
+                results = self._pass()   # (loads the libraries, sizes the allocator)
+                self._passed = True
             else:
+                if self.graph is None:   # (ahead of anything that moves the state: a graph that can't be made leaves it as it is)
+                    self.stream.synchronize()
+                    graph = torch.cuda.CUDAGraph()
+                    with torch.cuda.graph(graph, stream=self.stream):
+                        self._recorded = self._pass()
+                    self.graph = graph
                 self.graph.replay()
                 results = self._recorded
             self.logits, self.scored, self.followed = results

@@ -54,3 +54,32 @@ def test_draft_decoder_takes_its_caches_once(cuda):
     assert torch.cuda.max_memory_allocated() - before < 1.2 * caches
     assert torch.cuda.memory_reserved() - reserved < 1.2 * caches
     assert [k.data_ptr() for k in dec.cache.keys] == [k.data_ptr() for k in dec.all_keys] and dec.cache.max_len == dec.cache.keys[0].shape[2] == len(dec.cache.slots)
+
+
+@pytest.mark.parametrize("failures", [1, 2])
+def test_a_pass_that_cannot_be_recorded_leaves_the_state_as_it_was(cuda, monkeypatch, failures):
+    """Rows and tokens on the device are those of the texts when a graph could not be made (memory that is not there), and the passes behind it go on from them."""
+    model, prompt = _model(cuda), _prompt(7, 2, 15)
+    want = decoding.DraftDecoder(model, 2, 60, [-1])
+    want.prefill(prompt)
+    for _ in range(8):
+        want.check([[], []])
+    assert len(set(want.texts[0][-9:])) > 4                            # (a token left out would show)
+    dec = decoding.DraftDecoder(model, 2, 60, [-1])
+    dec.prefill(prompt)
+
+    def no_memory():
+        raise RuntimeError("no memory for a graph")
+
+    with monkeypatch.context() as patch:
+        patch.setattr(torch.cuda, "CUDAGraph", no_memory)
+        failed = 0
+        while failed < failures:
+            try:
+                dec.check([[], []])
+            except RuntimeError:
+                failed += 1
+            assert [len(text) - 1 for text in dec.texts] == dec.rows.tolist() and [text[-1] for text in dec.texts] == dec.token[:, 0].tolist()
+    while len(dec.texts[0]) < len(want.texts[0]):
+        dec.check([[], []])
+    assert dec.texts == want.texts
