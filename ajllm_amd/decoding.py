@@ -1075,8 +1075,8 @@ class DraftDecoder(FusedDecoder):
         longest = max((len(text) for text, on in zip(self.texts, going) if on), default=0)
         if longest > self.max_len:
             raise ValueError("the KV cache is too short for this many tokens")
-        guesses = torch.as_tensor(guesses, dtype=torch.long).reshape(self.batch, -1)
-        if guesses.shape[1] != self.nodes - 1 or len(going) != self.batch or (guesses.numel() and not 0 <= int(guesses.min()) <= int(guesses.max()) < self.vocab):
+        guesses = torch.as_tensor(guesses, dtype=torch.long)
+        if tuple(guesses.shape) != (self.batch, self.nodes - 1) or len(going) != self.batch or (guesses.numel() and not 0 <= int(guesses.min()) <= int(guesses.max()) < self.vocab):
             raise ValueError(f"guesses [{self.batch}, {self.nodes - 1}] of tokens in [0, {self.vocab}), and {self.batch} truth values, expected")
         self.stream.wait_stream(torch.cuda.current_stream(self.device))
         with torch.cuda.stream(self.stream):

@@ -5,7 +5,7 @@ import torch
 
 from ajllm_amd import decoding
 from tests.latent_models import config, random_weights
-from tests.test_gpu_draft_decoder import _model, _prompt
+from tests.test_gpu_draft_decoder import VOCAB, _model, _prompt
 from tests.test_gpu_latent import _build, _tokens
 
 pytestmark = pytest.mark.gpu
@@ -83,3 +83,13 @@ def test_a_pass_that_cannot_be_recorded_leaves_the_state_as_it_was(cuda, monkeyp
     while len(dec.texts[0]) < len(want.texts[0]):
         dec.check([[], []])
     assert dec.texts == want.texts
+
+
+def test_guesses_of_another_shape_are_refused(cuda):
+    dec = decoding.DraftDecoder(_model(cuda), 2, 40, [-1, 0, 0, 1])
+    dec.prefill(_prompt(1, 2, 10))
+    for bad in ([1, 2, 3, 4, 5, 6], [[1, 2], [3, 4], [5, 6]], [[[1, 2, 3], [4, 5, 6]]], torch.zeros(6, dtype=torch.long), torch.zeros(1, 2, 3, dtype=torch.long)):
+        with pytest.raises(ValueError, match="guesses"):
+            dec.check(bad)
+    assert dec.rows.tolist() == [10, 10]
+    assert all(len(new) >= 1 for new in dec.check(torch.full((2, 3), VOCAB - 1, device=cuda)))
