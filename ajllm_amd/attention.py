@@ -263,6 +263,8 @@ def tree_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, ro
         raise ValueError("tree_attention: unsupported shape: q and caches with elements expected")
     if keys.shape[0] != batch or keys.shape[3] != hd:
         raise ValueError("tree_attention: caches [B, Hkv, max_len, hd] expected")
+    if max(*q.shape, *keys.shape) >= 2 ** 31:
+        raise ValueError("tree_attention: dimensions below 2^31 expected")
     if (masks.dtype != torch.int32 or masks.dim() not in (2, 3) or masks.shape[-2] != nodes or masks.shape[-1] * 32 < nodes
             or (masks.shape[-1] > 1 and masks.stride(-1) != 1)
             or (masks.dim() == 3 and masks.shape[0] != batch) or masks.device != device):

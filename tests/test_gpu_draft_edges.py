@@ -20,3 +20,10 @@ def test_masks_of_one_word_lie_anywhere(cuda):
     for same in (across, apart[:, ::2][:, :1], across[None].expand(2, -1, -1)):
         assert same.stride(-1) != 1
         assert torch.equal(attention.tree_attention(q, keys, values, rows, same), want)
+
+
+def test_more_key_heads_than_are_counted_are_refused(cuda):
+    """2^32 + 1 key heads (all the same one) are not one."""
+    q, cache = torch.zeros(1, 1, 1, 64, device=cuda), torch.zeros(1, 1, 8, 64, device=cuda).expand(1, 2 ** 32 + 1, 8, 64)
+    with pytest.raises(ValueError, match="below 2\\^31"):
+        attention.tree_attention(q, cache, cache, torch.zeros(1, dtype=torch.long, device=cuda), torch.ones((1, 1), dtype=torch.int32, device=cuda))
