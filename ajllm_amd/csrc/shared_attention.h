@@ -944,7 +944,9 @@ __device__ __forceinline__ void meet_many(const A& a, const Walk<uint16_t>& w, R
 __device__ __forceinline__ long long part_place(const SharedAttention& a, const Walk<uint16_t>&, long long in_q, int, int part) { return in_q + part * a.queries; }
 template <int HD, int U, typename A>
 __device__ __forceinline__ void leave_part(const A& a, const Walk<uint16_t>& w, const RunningRow<HD> (&row)[U], int part) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
+  int thread = threadIdx.x;
+  asm volatile("" : "+v"(thread));   // (the lane's place is formed again here: two tiles of queries leave no register to keep it beside the steps)
+  const int lane = thread & 63, wave = thread >> 6, r = lane & 15, g = lane >> 4;
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const float l = quad_sum(row[u].l);
