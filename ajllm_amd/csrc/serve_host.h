@@ -7,6 +7,7 @@
 #include <stdlib.h>
 
 #include "../../include/ajq_serve.h"
+#include "host_math.h"
 #include "lane_rows.h"
 
 using namespace ajq;
@@ -90,7 +91,6 @@ int allow_lds(K kernel, int bytes, const char* what) {
   return AJQ_OK;
 }
 
-long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 constexpr long long kMostLanes = 0xFFFFFFFFLL;   // of a grid in a dimension: HIP launches no more
 
 }  // namespace

@@ -11,6 +11,7 @@
 // works out the same).
 #pragma once
 #include "shared_attention.h"
+#include "tree_plan.h"   // kMostDealt
 
 namespace ajq {
 
@@ -40,7 +41,6 @@ template <> struct SeenBits<TreeAttention> {
 
 // ---- dealing.  With n_b blocks of rows a sequence, R runs and B sequences, parts of Q blocks are too many if sum ceil(n_b / Q) > R; Q = sum n_b / (R - B) is always
 // enough, sum n_b / R the least that can be.  Each lane tries a Q between the two, and the smallest that fits is taken.
-constexpr int kMostDealt = 64;   // sequences: a lane each
 struct Dealt {
   int sequence, part, parts, before, rows, there;   // (rows: 0 where no token is there)
 };
