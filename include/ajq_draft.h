@@ -39,12 +39,13 @@ typedef struct {
  * committed rows and of the tokens that are there must be finite (one that is not may make its component NaN for all tokens of the sequence); rows behind
  * them may hold anything.  heads a multiple of kv_heads; dim 128, 64 or 32; caches fp32 or bf16, strides in elements, multiples of 8; q fp32 or bf16.
  *
- * Precision: sums, maxima and scores are fp32.  fp32 queries and rows enter the products as two bf16 numbers each (16 bits and more of them), or whole where up to
- * 16 queries of a key head meet fp32 rows; a weight is rounded to bf16 ahead of the second product, but for those 16.  No atomics: the same bits from run to run, for one
- * shape (which of the ways a call goes, and so its last bits, is chosen by batch, tokens, heads, dim, max_len and types).
+ * Precision: sums, maxima and scores are fp32.  fp32 queries and rows enter the products as two bf16 numbers each (16 bits and more of them), and a weight is rounded
+ * to bf16 ahead of the second product; but a call on fp32 rows that goes by tiles of 16 queries is in fp32 throughout (up to 16 queries of a key head always do, more of them
+ * where that takes less time).  No atomics: the same bits from run to run, for one shape (which of the ways a call goes, and so its last bits, is chosen by batch,
+ * tokens, heads, dim, max_len and types).
  *
- * Workspace (16-byte aligned; this call's alone until it is done): 0 bytes where every sequence's rows are walked in one part; else, for up to 64 parts a sequence
- * and 2048 / waves / kv_heads or so in all, dim + 2 fp32 numbers a part and query. */
+ * Workspace (16-byte aligned; this call's alone until it is done): what the first function says.  0 bytes where every sequence's rows are walked in one part; else
+ * 8 a sequence and tokens * heads * (4 * dim + 8) a part, for up to 64 parts a sequence and 1024 / kv_heads in all. */
 size_t ajqt_tree_attention_workspace(const ajqt_tree_attention_args* args);
 int ajqt_tree_attention(const ajqt_tree_attention_args* args, void* workspace, size_t workspace_bytes, void* stream);
 
@@ -75,8 +76,8 @@ typedef struct {
  *                  0 and -1 for a t outside [0, vocab))
  *   top_ids, top_log_probs [rows, top]: the first `top` tokens in that order (0: neither; at most 64, and vocab).
  * A row of -inf only: -inf throughout, entropy 0.  A row with NaN or +inf: NaN, and some numbers inside [0, vocab).
- * All sums in fp32.  Workspace: 0 where a row is at most 32768 fp32 or 65536 bf16 logits (the 16 bytes that an unaligned row begins in less); else 16 + 8 * top bytes
- * for every slice of that size or, of few rows, a quarter of it. */
+ * All sums in fp32.  Workspace (16-byte aligned): what the first function says.  0 where a row is at most 32768 fp32 or 65536 bf16 logits (the 16 bytes that an unaligned
+ * row begins in less); else 4 bytes a row and 16 + 8 * top for each of its slices, of that size at most or, of few rows, a quarter of it. */
 size_t ajqt_log_probs_workspace(const ajqt_log_probs_args* args);
 int ajqt_log_probs(const ajqt_log_probs_args* args, void* workspace, size_t workspace_bytes, void* stream);
 
