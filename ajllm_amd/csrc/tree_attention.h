@@ -139,7 +139,7 @@ __global__ __launch_bounds__(64 * WV, sizeof(CacheT) == 4 && RT == 2 && WV == 4 
 // ---- Many queries on fp32 rows: 16 RT to each of four waves, all on the same blocks of 32 rows.  What bounds meet_few there is that every wave splits its rows
 // into two bf16 halves for its own queries; here the workgroup does so once: a block's pieces go from memory to the lanes' registers, and from there, as halves, to one of two
 // stages of LDS (one barrier a block), while the next block's are on their way.  Products as there: scores of three (bf16 queries: two), results of two.
-// Fp32 queries, us (by meet_few's best form): 7 x 69 of 32 heads of 128 behind up to 112 rows 18 (38); 7 x 100 behind 1000 64 (119); 8 x 64 of 32 / 8 behind 8000 159 (372), in 64
+// Fp32 queries, us (by meet_few's best form; sequences have from half of these tokens and rows on): 7 x 69 of 32 heads of 128 behind up to 112 rows 18 (38); 7 x 100 behind 1000 64 (119); 8 x 64 of 32 / 8 behind 8000 159 (372), in 64
 // parts; 12 x 25 of 12 heads of 64 behind 1500 22.6 (22.8).  350 calls with more than 16 queries a key head: 24 % less than without it if the faster is taken, 19 % as chosen.
 // Bound by a wave's own work still: 80 MFMAs of 16 cycles, 64 pieces of 16 bytes from LDS and some 400 vector instructions a block, nothing of one block beside another's.
 template <int HD> constexpr int laid_lds_bytes() { return 2 * 4 * 32 * 2 * HD; }   // stages; keys and values, each in halves

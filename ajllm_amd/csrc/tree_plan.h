@@ -35,7 +35,8 @@ constexpr int kMostParts = 64;      // of a sequence: a lane each in the merge
 // (geometric mean) than the fastest of what was tried.  Where the ways part, for instance (us; heads / key heads x size, tokens, rows): 32 / 8 x 128, 1 x 8 behind 500: tiles of 16
 // in one launch 6.3, of 32 9.1, in seven parts 7.2; 6 x 32 behind 2000: tiles of 32 and eight waves in one launch 18.5, four waves in 16 runs 22.0; 6 x 32 behind 12000: in 16
 // runs 56.7, eight waves in one launch 2.2 times that; 8 x 64 behind 32768: tiles of 256 of eight waves in 28 runs 254, of 128 of four 324.
-// fp32 rows laid down once: 1881 calls to 10 %; what is chosen with them takes 4 % longer than the fastest of 350 calls' ways.
+// fp32 rows laid down once: 1881 calls to 10 %; what is chosen with them takes 4 % longer than the fastest of 350 calls' ways.  Rows and tokens of all these calls, and of the
+// examples, are the largest of the batch: the others have from a half of that on.
 struct TreeCost {
   float start, per_waves, per_tiles, step, step_dim, step_tiles, crowd, memory, merge, merge_bytes, l2;
 };
@@ -47,7 +48,8 @@ float tree_cost(const ajqt_tree_attention_args* a, const TreePlan& p) {
   const bool bf16 = a->cache_dtype == AJQS_BF16;
   const TreeCost& c = p.walk ? (bf16 ? kWalkBf16 : kLaidF32) : bf16 ? kFewBf16 : kFewF32;
   const float dim = (float)a->dim / 128.f, batch = (float)a->batch, waves = (float)p.waves, kv = (float)a->kv_heads;
-  // rows: of the longest sequence all (one run is one workgroup's), of several three quarters on average
+  // rows: of the longest sequence the whole capacity (one run is one workgroup's), of several three quarters on average, as if lengths lay between a half of it and all.  What is
+  // filled is not known here: a cache of 32784 rows that holds 272 is read in 32 runs, 14.2 us instead of 5.8 (8 x 16, 32 / 8 x 128, bf16).
   const float longest = (float)a->max_len, mean = a->batch == 1 ? longest : 0.75f * longest;
   const float rows = !p.runs ? longest : a->batch == 1 ? longest / (float)p.runs : batch * mean / ((float)p.runs - 0.5f * batch);
   const float steps = ceilf(!p.walk ? rows / (32.f * waves) : bf16 ? rows / 64.f : rows / 32.f);

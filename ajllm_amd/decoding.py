@@ -993,7 +993,8 @@ class DraftDecoder(FusedDecoder):
 
     ``parents`` is the tree (``attention.tree_masks``; node 0 its root, the last token chosen): a list of T parents, the first -1.  A pass is FusedDecoder's prompt path on
     T tokens a sequence, with ``attention.norm_rope`` and ``attention.tree_attention`` in the attention's place, then ``sampling.token_log_probs`` (the choice behind every node),
-    ``sampling.follow_drafts`` and ``attention.keep_rows``, replayed from a graph.  Sequences go on at paces of their own; the host looks at the tokens after every pass."""
+    ``sampling.follow_drafts`` and ``attention.keep_rows``, replayed from a graph.  Sequences go on at paces of their own; the host looks at the tokens after every pass.  Attention's way is
+    chosen by ``max_len``, not by what is filled: give what the texts need."""
 
     def __init__(self, model: modeling.TransformerLM, batch: int, max_len: int, parents: list[int], kv_dtype: torch.dtype | None = None) -> None:
         nodes = len(parents)
