@@ -69,7 +69,7 @@ __device__ __forceinline__ KeptHead kept_head(const KeepRows& a, int lane) {
 }
 
 // Up to 64 numbers: each wave has them in its lanes, a vote says where they end, and one wait is enough for all rows.  A launch and two round trips, the list's and
-// the rows': a path through 16 nodes in twelve layers of 8 x 16 heads of 128 (fp32, 3072 heads, 20 MB read and written) 6.9 us (by pieces as below 8.5); 64 in 32
+// the rows': a path through 16 nodes in twelve layers of 8 x 16 heads of 128 (fp32, 20 MB read and written) 6.9 us (by pieces as below 8.5); 64 in 32
 // layers of 32 x 8 heads (bf16, 215 MB) 37 us (42).  Eight rows a lane took 244 registers, and 14 us for the first.
 constexpr int kShortList = 64;
 template <int kMost>   // rows a lane
